@@ -39,6 +39,9 @@ PRODUCT_UNITS = [("runtime", os.path.join(CSRC, "runtime.cu"), []),
                  ("gemm", os.path.join(CSRC, "gemm.cu"), []),
                  ("gemm_pair", os.path.join(CSRC, "gemm_pair.cu"), []),
                  ("gemm_decode", os.path.join(CSRC, "gemm_decode.cu"), []),
+                 ("linear", os.path.join(CSRC, "linear.cu"), []),
+                 ("linear_grad", os.path.join(CSRC, "linear_grad.cu"), []),
+                 ("moe", os.path.join(CSRC, "moe.cu"), []),
                  ("host_pipeline", os.path.join(CSRC, "host_pipeline.cu"), []),
                  ("capi", os.path.join(CSRC, "capi.cu"), [])]
 PRODUCT_UNITS += [(f"decode_inst_{m}", os.path.join(CSRC, "decode_inst.cu"), [f"-DNVFP4_DECODE_MPAD={m}"])

@@ -52,6 +52,11 @@ int encode_tiled_2d(CUtensorMap *map, CUtensorMapDataType dtype, const void *bas
                     uint64_t outer, uint64_t row_pitch_bytes, uint32_t box_inner, uint32_t box_outer,
                     CUtensorMapSwizzle swizzle);
 
+// The same for a tensor of rank 2 to 5: dims and box innermost first, strides in bytes of
+// every dimension but the innermost.
+int encode_tiled(CUtensorMap *map, CUtensorMapDataType dtype, int rank, const void *base, const uint64_t *dims,
+                 const uint64_t *strides, const uint32_t *box, CUtensorMapSwizzle swizzle);
+
 inline int cuda_status(cudaError_t e) { return e == cudaSuccess ? NVFP4_OK : NVFP4_ERR_CUDA; }
 
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

@@ -1,0 +1,717 @@
+// linear.cu — the persistent CTA-pair kernel of the 16-bit linear layers: forward with a
+// fused epilogue, input gradient and weight gradient, dense or grouped by expert.
+//
+// A cluster of two CTAs computes 256 features x up to 256 tokens with
+// tcgen05.mma.cta_group::2 (kind::f16, fp32 accumulators).  Each CTA stages its 128
+// features and its half of the tokens by TMA into a 6-slot ring of 64 reduction elements
+// (32 KB a slot); two accumulators of 256 columns fill the tensor memory, so the epilogue
+// of one tile runs under the MMAs of the next.
+//
+// Warps: 0 TMA producer, 1 MMA issue (leader CTA) and TMEM owner, 2-9 epilogue, 10 (wgrad)
+// clears the rows past a group's end in its last slot.
+#include <algorithm>
+#include <climits>
+#include <cstdlib>
+
+#include "linear.cuh"
+
+namespace nvfp4 {
+namespace linear {
+
+constexpr int kStages = 6;
+constexpr int kEpiWarps = 8;
+constexpr int kTailWarp = 2 + kEpiWarps;
+constexpr int kThreads = 32 * (kTailWarp + 1);
+constexpr int kMaxTokens = 256;  // of a tile
+constexpr int kAccCols = 256;
+
+constexpr int kOffA = 0;
+constexpr int kOffB = kOffA + kStages * kTileBytes;
+constexpr int kOffStage = kOffB + kStages * kTileBytes;  // per epilogue warp 2 KB: 32 tokens x 32 features
+constexpr int kStageWarp = 32 * 64;
+constexpr int kOffBar = kOffStage + kEpiWarps * kStageWarp;
+constexpr int kBarBytes = 256;
+constexpr int kOffTables = kOffBar + kBarBytes;
+constexpr int kSmem = kOffTables + 3 * (kMaxGroups + 1) * 4 + 1024;
+static_assert(kSmem <= 232448, "shared memory budget");
+
+struct Tile {
+    int group, f;     // group and feature tile (256 features)
+    int row0, rows;   // forward / dgrad: first token row and tokens of the tile; wgrad: the group's rows
+    int col;          // wgrad: column tile
+};
+
+// One 32-token x 32-feature piece of the accumulator (a warp's lane quarter): fragments to
+// outputs.  v[q][i] packs nothing yet: feature quarter q (l/4 + 8q), tokens 8i + 2(l%4), +1.
+template <typename T, int ACT>
+__device__ __forceinline__ void store_piece(const Params &p, uint32_t (&ra)[16], uint32_t (&rb)[16], uint32_t stage,
+                                            const float (&bias)[4], int row0, int n_rows, int feat0, int lane) {
+    constexpr bool kGlu = ACT == kActSwiglu;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            ra[4 * i + e] = __float_as_uint(__uint_as_float(ra[4 * i + e]) + bias[0]);
+            ra[4 * i + 2 + e] = __float_as_uint(__uint_as_float(ra[4 * i + 2 + e]) + bias[1]);
+            rb[4 * i + e] = __float_as_uint(__uint_as_float(rb[4 * i + e]) + bias[2]);
+            rb[4 * i + 2 + e] = __float_as_uint(__uint_as_float(rb[4 * i + 2 + e]) + bias[3]);
+        }
+    }
+    auto pk = [&](const uint32_t *r) { return Type16<T>::pack(__uint_as_float(r[0]), __uint_as_float(r[1])); };
+    // staging: 64 bytes a token, its 16-byte chunks permuted by the token so that the eight
+    // rows of a matrix, and the eight lanes of a read, each touch all banks once
+    const int mj = lane >> 3, mi = lane & 7;
+    auto stage64 = [&](int i) {  // matrix mj = features 8 mj.., tokens 8 i + mi
+        const int t = 8 * i + mi;
+        return stage + t * 64 + ((mj ^ ((t >> 1) & 3)) << 4);
+    };
+    auto copy_out64 = [&](void *dst, int cols, int f0) {
+        __syncwarp();
+#pragma unroll
+        for (int it = 0; it < 4; it++) {
+            const int t = it * 8 + (lane >> 2), c = lane & 3;
+            uint32_t a, b, cc, d;
+            ld_shared_v4(stage + t * 64 + ((c ^ ((t >> 1) & 3)) << 4), a, b, cc, d);
+            if (t < n_rows && f0 + c * 8 < cols)
+                *reinterpret_cast<uint4 *>(static_cast<T *>(dst) + (int64_t)(row0 + t) * cols + f0 + c * 8) =
+                    make_uint4(a, b, cc, d);
+        }
+        __syncwarp();
+    };
+    if (p.z) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            stmatrix_x4_trans(stage64(i), pk(ra + 4 * i), pk(ra + 4 * i + 2), pk(rb + 4 * i), pk(rb + 4 * i + 2));
+        copy_out64(p.z, p.features, feat0);
+    }
+    if constexpr (!kGlu) {
+        if (p.residual) {
+#pragma unroll
+            for (int it = 0; it < 4; it++) {
+                const int t = it * 8 + (lane >> 2), c = lane & 3;
+                uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                if (t < n_rows && feat0 + c * 8 < p.out_cols)
+                    v = *reinterpret_cast<const uint4 *>(static_cast<const T *>(p.residual) +
+                                                         (int64_t)(row0 + t) * p.out_cols + feat0 + c * 8);
+                st_shared_v4(stage + t * 64 + ((c ^ ((t >> 1) & 3)) << 4), v.x, v.y, v.z, v.w);
+            }
+            __syncwarp();
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            float o[8];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                o[e] = act<ACT>(__uint_as_float(ra[4 * i + e]));
+                o[4 + e] = act<ACT>(__uint_as_float(rb[4 * i + e]));
+            }
+            if (p.residual) {
+                uint32_t w[4];
+                ldmatrix_x4_trans(stage64(i), w[0], w[1], w[2], w[3]);
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const float2 f = Type16<T>::unpack(w[q]);
+                    o[2 * q] += f.x;
+                    o[2 * q + 1] += f.y;
+                }
+            }
+            stmatrix_x4_trans(stage64(i), Type16<T>::pack(o[0], o[1]), Type16<T>::pack(o[2], o[3]),
+                              Type16<T>::pack(o[4], o[5]), Type16<T>::pack(o[6], o[7]));
+        }
+        copy_out64(p.y, p.out_cols, feat0);
+    } else {
+        // lanes 0-15 of the quarter are gate features, 16-31 up: 16 output features, 32 bytes
+        // a token; two token groups a matrix instruction
+        const int f0 = feat0 >> 1;
+        auto stage32 = [&](int i) {
+            const int t = 8 * (i + (mj >> 1)) + mi;
+            return stage + t * 32 + (((mj & 1) ^ ((t >> 2) & 1)) << 4);
+        };
+        if (p.residual) {
+#pragma unroll
+            for (int it = 0; it < 2; it++) {
+                const int t = it * 16 + (lane >> 1), c = lane & 1;
+                uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                if (t < n_rows && f0 + c * 8 < p.out_cols)
+                    v = *reinterpret_cast<const uint4 *>(static_cast<const T *>(p.residual) +
+                                                         (int64_t)(row0 + t) * p.out_cols + f0 + c * 8);
+                st_shared_v4(stage + t * 32 + ((c ^ ((t >> 2) & 1)) << 4), v.x, v.y, v.z, v.w);
+            }
+            __syncwarp();
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+            float o[8];
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float g = __uint_as_float(ra[4 * (i + h) + e]), u = __uint_as_float(rb[4 * (i + h) + e]);
+                    o[4 * h + e] = g * sigma(g) * u;
+                }
+            if (p.residual) {
+                uint32_t w[4];
+                ldmatrix_x4_trans(stage32(i), w[0], w[1], w[2], w[3]);
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const float2 f = Type16<T>::unpack(w[q]);
+                    o[2 * q] += f.x;
+                    o[2 * q + 1] += f.y;
+                }
+            }
+            stmatrix_x4_trans(stage32(i), Type16<T>::pack(o[0], o[1]), Type16<T>::pack(o[2], o[3]),
+                              Type16<T>::pack(o[4], o[5]), Type16<T>::pack(o[6], o[7]));
+        }
+        __syncwarp();
+#pragma unroll
+        for (int it = 0; it < 2; it++) {
+            const int t = it * 16 + (lane >> 1), c = lane & 1;
+            uint32_t a, b, cc, d;
+            ld_shared_v4(stage + t * 32 + ((c ^ ((t >> 2) & 1)) << 4), a, b, cc, d);
+            if (t < n_rows && f0 + c * 8 < p.out_cols)
+                *reinterpret_cast<uint4 *>(static_cast<T *>(p.y) + (int64_t)(row0 + t) * p.out_cols + f0 + c * 8) =
+                    make_uint4(a, b, cc, d);
+        }
+        __syncwarp();
+    }
+}
+
+template <typename T, int FORM>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
+                       const Params p) {
+    constexpr bool kAmn = FORM != kForward, kBmn = FORM == kWgrad;
+    constexpr bool kBf16 = sizeof(T) == 2 && !std::is_same<T, __half>::value;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t *base_ptr = smem_raw + (base - smem_u32(smem_raw));
+    const uint32_t sA = base + kOffA, sB = base + kOffB;
+    const uint32_t bar_full = base + kOffBar;            // [stages], leader's used: both CTAs' data
+    const uint32_t bar_empty = bar_full + 8 * kStages;   // [stages]
+    const uint32_t bar_tail = bar_empty + 8 * kStages;   // [stages] wgrad: a group's last slot has landed
+    const uint32_t bar_acc_full = bar_tail + 8 * kStages;
+    const uint32_t bar_acc_empty = bar_acc_full + 16;
+    const uint32_t bar_drain = bar_acc_empty + 16;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(base_ptr + kOffBar + (3 * kStages + 5) * 8);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    static_assert((3 * kStages + 5) * 8 + 8 <= kBarBytes, "barrier region");
+    int *g_r0 = reinterpret_cast<int *>(base_ptr + kOffTables);
+    int *g_r1 = g_r0 + kMaxGroups + 1;
+    int *g_t0 = g_r1 + kMaxGroups + 1;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+    const int n_f = (p.features + 255) / 256;
+    const int n_c = FORM == kWgrad ? (p.out_cols + p.bt - 1) / p.bt : 0;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; s++) {
+            mbar_init(bar_full + 8 * s, 2);  // one arrival from each CTA's producer
+            mbar_init(bar_empty + 8 * s, 1);
+            mbar_init(bar_tail + 8 * s, 1);
+        }
+        for (int b = 0; b < 2; b++) {
+            mbar_init(bar_acc_full + 8 * b, 1);
+            mbar_init(bar_acc_empty + 8 * b, 2 * kEpiWarps);
+        }
+        mbar_init(bar_drain, 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+        prefetch_tmap(&tmap_a);
+        prefetch_tmap(&tmap_b);
+    }
+    if (warp == 1) {
+        tmem_alloc_pair(smem_u32(tmem_slot), 512);
+        tmem_relinquish_pair();
+    }
+    grid_dependency_wait();  // nothing of global memory is read or written before this
+    if (warp == 2)
+        build_tables(p.m_offsets, p.groups, p.m_total, FORM == kWgrad ? 0 : p.bt, FORM == kWgrad ? n_f * n_c : n_f,
+                     lane, g_r0, g_r1, g_t0);
+    tc_fence_before();
+    cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    const uint64_t tmo = p.ctl.wait_timeout_ns;
+    const int n_tiles = g_t0[p.groups];
+
+    // Strips of p.strip feature tiles sweep a group's tokens (wgrad: columns) together, the
+    // features fastest: the pairs that run at the same time share both operands in L2.
+    auto tile_at = [&](int t) {
+        Tile ti;
+        int lo = 0, hi = p.groups - 1;  // the last group with g_t0[g] <= t
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (g_t0[mid] <= t) lo = mid; else hi = mid - 1;
+        }
+        ti.group = lo;
+        const int r0 = g_r0[lo], n = g_r1[lo] - r0;
+        const int others = FORM == kWgrad ? n_c : (n + p.bt - 1) / p.bt;
+        const int local = t - g_t0[lo], per_strip = p.strip * others;
+        const int s = local / per_strip, f0 = s * p.strip, fs = min(p.strip, n_f - f0), rem = local - s * per_strip;
+        ti.f = f0 + rem % fs;
+        const int o = rem / fs;
+        ti.col = o;
+        ti.row0 = FORM == kWgrad ? r0 : r0 + o * p.bt;
+        ti.rows = FORM == kWgrad ? n : min(p.bt, n - o * p.bt);
+        return ti;
+    };
+    auto blocks_of = [&](const Tile &ti) {
+        return ((FORM == kWgrad ? ti.rows : p.red) + kBlockK - 1) / kBlockK;
+    };
+    // MMA columns of a tile: its tokens, rounded up to the instruction's step of 16 (each
+    // CTA holds half of them); the rounding's rows are loaded but never stored.
+    auto width_of = [&](const Tile &ti) { return FORM == kWgrad ? p.bt : (ti.rows + 15) & ~15; };
+    const uint32_t tx_bytes = kTileBytes + (p.bt / 2) * 128;
+    // wgrad: reduction rows past the group's end belong to the next group; the last slot's
+    // are cleared unless the MMA's 16-row steps end exactly with the group
+    auto dirty_tail = [&](const Tile &ti) { return FORM == kWgrad && (ti.rows & 15) != 0; };
+
+    if (warp == 0) {
+        // ------------------------------------------------------------ producer (both CTAs)
+        if (elect_one()) {
+            uint32_t stage = 0, phase = 0, issued_mask = 0, issued_parity = 0;
+            uint32_t tail_mask = 0, tail_parity = 0;  // tail barriers used; parity of their next phase
+            bool ok = true;
+            for (int t = pair; ok && t < n_tiles; t += num_pairs) {
+                const Tile ti = tile_at(t);
+                const int nkb = blocks_of(ti);
+                const int f0 = ti.f * 256 + (int)rank * 128;
+                const int b0 = FORM == kWgrad ? ti.col * p.bt + (int)rank * (p.bt / 2)
+                                              : ti.row0 + (int)rank * (width_of(ti) / 2);
+                for (int kb = 0; kb < nkb; kb++) {
+                    if (!wait_parity(bar_empty + 8 * stage, phase ^ 1, tmo, abort_flag)) {
+                        report_timeout(abort_flag, p.ctl.status);
+                        ok = false;
+                        break;
+                    }
+                    const bool tail = kb == nkb - 1 && dirty_tail(ti);
+                    const uint32_t bar = tail ? map_to_cta(bar_tail + 8 * stage, rank)
+                                              : map_to_cta(bar_full + 8 * stage, 0);
+                    mbar_arrive_expect_tx_cluster(bar, tx_bytes);
+                    if (tail) {
+                        tail_mask |= 1u << stage;
+                        tail_parity ^= 1u << stage;
+                        issued_mask &= ~(1u << stage);
+                    } else {
+                        issued_mask |= 1u << stage;
+                        issued_parity = (issued_parity & ~(1u << stage)) | (phase << stage);
+                    }
+                    const uint32_t dA = sA + stage * kTileBytes, dB = sB + stage * kTileBytes;
+                    const int k0 = kb * kBlockK;
+                    if constexpr (FORM == kForward) {
+                        tma_load_3d_pair(dA, &tmap_a, bar, k0, f0, ti.group);
+                        tma_load_2d_pair(dB, &tmap_b, bar, k0, b0);
+                    } else if constexpr (FORM == kDgrad) {
+                        tma_load_3d_pair(dA, &tmap_a, bar, f0, k0, ti.group);
+                        tma_load_3d_pair(dA + 8192, &tmap_a, bar, f0 + 64, k0, ti.group);
+                        tma_load_2d_pair(dB, &tmap_b, bar, k0, b0);
+                    } else {
+                        tma_load_2d_pair(dA, &tmap_a, bar, f0, ti.row0 + k0);
+                        tma_load_2d_pair(dA + 8192, &tmap_a, bar, f0 + 64, ti.row0 + k0);
+                        for (int c = 0; c < p.bt / 2; c += 64)
+                            tma_load_2d_pair(dB + c * 128, &tmap_b, bar, b0 + c, ti.row0 + k0);
+                    }
+                    if (++stage == kStages) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                }
+            }
+            grid_launch_dependents();
+            if (!ok) {  // let the copies in flight land before the memory goes
+                volatile int never = 0;
+                for (int s = 0; s < kStages; s++) {
+                    if (rank == 0 && (issued_mask & (1u << s)))
+                        wait_parity(bar_full + 8 * s, (issued_parity >> s) & 1, p.ctl.drain_timeout_ns, &never);
+                    if (tail_mask & (1u << s))
+                        wait_parity(bar_tail + 8 * s, ((tail_parity >> s) & 1) ^ 1, p.ctl.drain_timeout_ns, &never);
+                }
+            }
+        }
+    } else if (warp == 1) {
+        // ------------------------------------------------------------ MMA issue (leader)
+        if (rank == 0 && elect_one()) {
+            const uint32_t empty0 = map_to_cta(bar_empty, 0), empty1 = map_to_cta(bar_empty, 1);
+            const uint32_t accf0 = map_to_cta(bar_acc_full, 0), accf1 = map_to_cta(bar_acc_full, 1);
+            const uint64_t a_desc = operand_desc<kAmn>(sA), b_desc = operand_desc<kBmn>(sB);
+            uint32_t stage = 0, phase = 0;
+            int local = 0;
+            bool ok = true, any = false;
+            for (int t = pair; ok && t < n_tiles; t += num_pairs, local++) {
+                const Tile ti = tile_at(t);
+                const int nkb = blocks_of(ti);
+                const uint32_t idesc = idesc_f16(kBf16, kAmn, kBmn, 256, (uint32_t)width_of(ti));
+                const uint32_t buf = local & 1, use = local >> 1;
+                const uint32_t d_tmem = tmem_base + buf * kAccCols;
+                if (!spin_parity_cluster(bar_acc_empty + 8 * buf, (use & 1) ^ 1, tmo, abort_flag)) {
+                    report_timeout(abort_flag, p.ctl.status);
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const int red = FORM == kWgrad ? ti.rows : p.red;
+                for (int kb = 0; kb < nkb; kb++) {
+                    if (!spin_parity_cluster(bar_full + 8 * stage, phase, tmo, abort_flag)) {
+                        report_timeout(abort_flag, p.ctl.status);
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint64_t a = a_desc + (uint64_t)(stage * (kTileBytes >> 4));
+                    const uint64_t b = b_desc + (uint64_t)(stage * (kTileBytes >> 4));
+                    any = true;
+                    if ((kb + 1) * kBlockK <= red) {
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            mma_f16_pair(d_tmem, a + j * kStep16<kAmn>, b + j * kStep16<kBmn>, idesc,
+                                         (kb | j) != 0 ? 1u : 0u);
+                    } else {  // what is left, in steps of 16 (zeros past the end)
+                        const int steps = (red - kb * kBlockK + 15) / 16;
+                        for (int j = 0; j < steps; j++)
+                            mma_f16_pair(d_tmem, a + j * kStep16<kAmn>, b + j * kStep16<kBmn>, idesc,
+                                         (kb | j) != 0 ? 1u : 0u);
+                    }
+                    mma_commit_pair(empty0 + 8 * stage);
+                    mma_commit_pair(empty1 + 8 * stage);
+                    if (++stage == kStages) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                }
+                if (!ok) break;
+                mma_commit_pair(accf0 + 8 * buf);
+                mma_commit_pair(accf1 + 8 * buf);
+            }
+            if (!ok && any) {
+                volatile int never = 0;
+                mma_commit_pair(map_to_cta(bar_drain, 0));
+                wait_parity(bar_drain, 0, p.ctl.drain_timeout_ns, &never);
+            }
+        }
+    } else if (warp == kTailWarp) {
+        // ------------------------------------------------------------ tail of a group (wgrad)
+        // Both operands' rows past the group's end are set to zero (the next group's rows
+        // may hold anything, infinities included), up to the 16-row step the MMA reads.
+        if constexpr (FORM == kWgrad) {
+            uint32_t slots = 0, parity = 0;  // slots used so far; parity of each tail barrier
+            bool ok = true;
+            for (int t = pair; ok && t < n_tiles; t += num_pairs) {
+                const Tile ti = tile_at(t);
+                slots += (uint32_t)blocks_of(ti);
+                if (!dirty_tail(ti)) continue;
+                const uint32_t stage = (slots - 1) % kStages;
+                if (!wait_parity(bar_tail + 8 * stage, (parity >> stage) & 1, tmo, abort_flag)) {
+                    if (lane == 0) report_timeout(abort_flag, p.ctl.status);
+                    ok = false;
+                    break;
+                }
+                parity ^= 1u << stage;
+                const int valid = (ti.rows - 1) % kBlockK + 1, end = (valid + 15) & ~15;
+                const int per = (end - valid) * 8;  // 16-byte pieces of one 64-column chunk
+                for (int i = lane; i < per; i += 32) {
+                    const uint32_t at = (uint32_t)(valid * 128 + i * 16) + stage * kTileBytes;
+                    st_shared_v4(sA + at, 0u, 0u, 0u, 0u);
+                    st_shared_v4(sA + 8192 + at, 0u, 0u, 0u, 0u);
+                    for (int c = 0; c < p.bt / 2; c += 64) st_shared_v4(sB + c * 128 + at, 0u, 0u, 0u, 0u);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(map_to_cta(bar_full + 8 * stage, 0));
+            }
+        }
+    } else {
+        // ------------------------------------------------------------ epilogue (warps 2..9, both CTAs)
+        const int quarter = warp & 3, half = (warp - 2) >> 2;
+        const uint32_t lead_acc_empty = map_to_cta(bar_acc_empty, 0);
+        const uint32_t stage = base + kOffStage + (warp - 2) * kStageWarp;
+        const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+        int local = 0;
+        for (int t = pair; t < n_tiles; t += num_pairs, local++) {
+            const Tile ti = tile_at(t);
+            const uint32_t buf = local & 1, use = local >> 1;
+            const int feat0 = ti.f * 256 + (int)rank * 128 + quarter * 32;
+            float bias[4] = {0.f, 0.f, 0.f, 0.f};
+            if (FORM == kForward && p.bias) {
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const int f = feat0 + 8 * q + (lane >> 2);
+                    if (f < p.features)
+                        bias[q] = Type16<T>::load(static_cast<const T *>(p.bias) + (int64_t)ti.group * p.features + f);
+                }
+            }
+            if (!wait_parity(bar_acc_full + 8 * buf, use & 1, tmo, abort_flag)) {
+                if (lane == 0) report_timeout(abort_flag, p.ctl.status);
+                break;
+            }
+            tc_fence_after();
+            const uint32_t acc = tmem_base + lane_base + buf * kAccCols;
+            if constexpr (FORM != kWgrad) {
+                for (int c = half * 32; c < ti.rows; c += 64) {
+                    uint32_t ra[16], rb[16];
+                    tmem_ld_16x256b_x4(acc + c, ra);
+                    tmem_ld_16x256b_x4(acc + (16u << 16) + c, rb);
+                    tmem_ld_wait();
+                    const int n = ti.rows - c, row = ti.row0 + c;
+                    if (feat0 >= p.features) continue;
+                    switch (FORM == kForward ? p.act : (int)kActNone) {
+                        case kActRelu: store_piece<T, kActRelu>(p, ra, rb, stage, bias, row, n, feat0, lane); break;
+                        case kActSilu: store_piece<T, kActSilu>(p, ra, rb, stage, bias, row, n, feat0, lane); break;
+                        case kActGeluTanh:
+                            store_piece<T, kActGeluTanh>(p, ra, rb, stage, bias, row, n, feat0, lane);
+                            break;
+                        case kActSwiglu: store_piece<T, kActSwiglu>(p, ra, rb, stage, bias, row, n, feat0, lane); break;
+                        default: store_piece<T, kActNone>(p, ra, rb, stage, bias, row, n, feat0, lane);
+                    }
+                }
+            } else {
+                // a lane is a row of dW: 32 columns of it, 64 contiguous bytes, at a time
+                const int f = feat0 + lane;
+                T *out = static_cast<T *>(p.y) + ((int64_t)ti.group * p.features + f) * p.out_cols + ti.col * p.bt;
+                const int cols = min(p.bt, p.out_cols - ti.col * p.bt);
+                for (int c = half * 32; c < cols; c += 64) {
+                    uint32_t r[32];
+                    tmem_ld_32x32b_x32(acc + c, r);
+                    tmem_ld_wait();
+                    if (f >= p.features) continue;
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        if (c + q * 8 >= cols) continue;
+                        uint4 v = make_uint4(0u, 0u, 0u, 0u);  // a group without rows: its gradient is zero
+                        if (ti.rows > 0) {
+                            const uint32_t *s = r + q * 8;
+                            auto pk = [&](int i) {
+                                return Type16<T>::pack(__uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+                            };
+                            v = make_uint4(pk(0), pk(2), pk(4), pk(6));
+                        }
+                        *reinterpret_cast<uint4 *>(out + c + q * 8) = v;
+                    }
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster_cta_release(lead_acc_empty + 8 * buf);
+        }
+        if constexpr (FORM != kWgrad)
+            if (p.m_offsets) {  // rows outside every group (tokens that were not routed) are zero
+                const int lo = g_r0[0], hi = g_r1[p.groups - 1], outside = lo + p.m_total - hi;
+                for (int i = (int)blockIdx.x * kEpiWarps + warp - 2; i < outside; i += (int)gridDim.x * kEpiWarps) {
+                    const int64_t row = i < lo ? i : hi + (i - lo);
+                    auto clear = [&](void *dst, int cols) {
+                        uint4 *d = reinterpret_cast<uint4 *>(static_cast<T *>(dst) + row * cols);
+                        for (int c = lane; c < cols / 8; c += 32) d[c] = make_uint4(0u, 0u, 0u, 0u);
+                    };
+                    clear(p.y, p.out_cols);
+                    if (p.z) clear(p.z, p.features);
+                }
+            }
+        __syncwarp();
+    }
+
+    __syncwarp();
+    tc_fence_before();
+    cluster_sync();  // no CTA leaves while its peer may still signal it
+    if (warp == 1) {
+        __syncwarp();
+        tc_fence_after();
+        tmem_dealloc_pair(tmem_base, 512);
+    }
+}
+
+// ------------------------------------------------------------------------- host side
+template <typename T>
+static constexpr CUtensorMapDataType tma_type() {
+    return std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+}
+
+// [rows, cols] with a row pitch, as boxes of 64 columns (one swizzle row) by box_rows.
+template <typename T>
+static int map_rows(CUtensorMap *m, const void *base, int64_t rows, int cols, int64_t pitch, int box_rows) {
+    const uint64_t dims[2] = {(uint64_t)cols, (uint64_t)rows}, strides[1] = {(uint64_t)pitch * 2};
+    const uint32_t box[2] = {64, (uint32_t)box_rows};
+    return encode_tiled(m, tma_type<T>(), 2, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+// The weight [groups, N, K].
+template <typename T>
+static int map_weight(CUtensorMap *m, const void *base, int groups, int N, int K, int box_rows) {
+    const uint64_t dims[3] = {(uint64_t)K, (uint64_t)N, (uint64_t)groups};
+    const uint64_t strides[2] = {(uint64_t)K * 2, (uint64_t)N * (uint64_t)K * 2};
+    const uint32_t box[3] = {64, (uint32_t)box_rows, 1};
+    return encode_tiled(m, tma_type<T>(), 3, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <typename T, int FORM>
+static int launch_pair(const CUtensorMap &a, const CUtensorMap &b, const Params &p, int64_t tiles, const DeviceInfo &di,
+                       cudaStream_t stream) {
+    auto kern = linear_pair_kernel<T, FORM>;
+    static int configured[64] = {};
+    if (!configured[di.device]) {
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
+            return NVFP4_ERR_CUDA;
+        configured[di.device] = 1;
+    }
+    if (tiles > INT_MAX) return NVFP4_ERR_SHAPE;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(2 * (unsigned)std::min<int64_t>(tiles, di.sm_count / 2));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kSmem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, kern, a, b, p) != cudaSuccess) return NVFP4_ERR_CUDA;
+    count_launch();
+    return cuda_status(cudaGetLastError());
+}
+
+// Tokens of a tile.
+static int token_tile(int64_t m, int groups, int n_f, int pairs) {
+    (void)groups;
+    (void)n_f;
+    (void)pairs;
+    int bt = 32;
+    while (bt < kMaxTokens && bt < m) bt *= 2;
+    return bt;
+}
+
+template <typename T>
+static int forward_t(const void *X, int64_t ldx, const void *W, Params p, int K, const DeviceInfo &di,
+                     cudaStream_t s) {
+    const int n_f = (p.features + 255) / 256;
+    p.bt = token_tile(p.m_total, p.groups, n_f, di.sm_count / 2);
+    p.strip = 8;
+    p.red = K;
+    CUtensorMap a, b;
+    int st = map_weight<T>(&a, W, p.groups, p.features, K, 128);
+    if (!st) st = map_rows<T>(&b, X, p.m_total, K, ldx, p.bt / 2);
+    if (st) return st;
+    const int64_t token_tiles = (p.m_total + p.bt - 1) / p.bt + (p.m_offsets ? p.groups : 0);
+    return launch_pair<T, kForward>(a, b, p, token_tiles * n_f, di, s);
+}
+
+template <typename T>
+static int dgrad_t(const void *dZ, const void *W, Params p, int N, const DeviceInfo &di, cudaStream_t s) {
+    const int n_f = (p.features + 255) / 256;
+    p.bt = token_tile(p.m_total, p.groups, n_f, di.sm_count / 2);
+    p.strip = 8;
+    p.red = N;
+    CUtensorMap a, b;
+    int st = map_weight<T>(&a, W, p.groups, N, p.features, 64);
+    if (!st) st = map_rows<T>(&b, dZ, p.m_total, N, N, p.bt / 2);
+    if (st) return st;
+    const int64_t token_tiles = (p.m_total + p.bt - 1) / p.bt + (p.m_offsets ? p.groups : 0);
+    return launch_pair<T, kDgrad>(a, b, p, token_tiles * n_f, di, s);
+}
+
+template <typename T>
+static int wgrad_t(const void *dZ, const void *X, int64_t ldx, Params p, const DeviceInfo &di, cudaStream_t s) {
+    const int n_f = (p.features + 255) / 256;
+    p.bt = 256;
+    p.strip = 8;
+    CUtensorMap a, b;
+    int st = map_rows<T>(&a, dZ, std::max(p.m_total, 1), p.features, p.features, 64);
+    if (!st) st = map_rows<T>(&b, X, std::max(p.m_total, 1), p.out_cols, ldx, 64);
+    if (st) return st;
+    const int64_t tiles = (int64_t)p.groups * n_f * ((p.out_cols + p.bt - 1) / p.bt);
+    return launch_pair<T, kWgrad>(a, b, p, tiles, di, s);
+}
+
+// Sizes and pointers that the entry points have in common.
+static int check_sizes(int groups, const int *m_offsets, int M, int N, int K, int dtype) {
+    if (dtype != NVFP4_BF16 && dtype != NVFP4_F16) return NVFP4_ERR_INVALID;
+    if (groups < 1 || (groups > 1 && !m_offsets)) return NVFP4_ERR_INVALID;
+    if (groups > kMaxGroups || M < 0 || N < 8 || N % 8 || K < 8 || K % 8) return NVFP4_ERR_SHAPE;
+    if ((int64_t)N * K > ((int64_t)1 << 40) / 2) return NVFP4_ERR_SHAPE;  // a tensor map's strides are below 2^40
+    if (reinterpret_cast<uintptr_t>(m_offsets) & 3u) return NVFP4_ERR_ALIGN;
+    return NVFP4_OK;
+}
+
+}  // namespace linear
+}  // namespace nvfp4
+
+using namespace nvfp4;
+
+extern "C" {
+
+int nvfp4_linear(const void *X, int64_t ldx, const void *W, const void *bias, const void *residual, void *Y, void *Z,
+                 const int32_t *m_offsets, int groups, int M, int N, int K, int activation, int dtype, void *stream) {
+    int st = linear::check_sizes(groups, m_offsets, M, N, K, dtype);
+    if (st) return st;
+    if (activation < NVFP4_ACT_NONE || activation > NVFP4_ACT_SWIGLU) return NVFP4_ERR_INVALID;
+    if (activation == NVFP4_ACT_SWIGLU && N % 32) return NVFP4_ERR_SHAPE;
+    if (ldx < K || ldx % 8) return NVFP4_ERR_SHAPE;
+    if (!W || (M && (!X || !Y))) return NVFP4_ERR_INVALID;
+    if (!aligned16(X) || !aligned16(W) || !aligned16(Y) || !aligned16(Z) || !aligned16(residual) ||
+        (reinterpret_cast<uintptr_t>(bias) & 1u))
+        return NVFP4_ERR_ALIGN;
+    DeviceInfo di;
+    if ((st = device_info(&di))) return st;
+    if (M == 0) return NVFP4_OK;
+    linear::Params p = {};
+    p.y = Y;
+    p.z = Z;
+    p.bias = bias;
+    p.residual = residual;
+    p.m_offsets = m_offsets;
+    p.groups = groups;
+    p.m_total = M;
+    p.features = N;
+    p.out_cols = activation == NVFP4_ACT_SWIGLU ? N / 2 : N;
+    p.act = activation;
+    if ((st = kernel_ctl(&p.ctl))) return st;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return dtype == NVFP4_BF16 ? linear::forward_t<__nv_bfloat16>(X, ldx, W, p, K, di, s)
+                               : linear::forward_t<__half>(X, ldx, W, p, K, di, s);
+}
+
+int nvfp4_linear_dgrad(const void *dZ, const void *W, void *dX, const int32_t *m_offsets, int groups, int M, int N,
+                       int K, int dtype, void *stream) {
+    int st = linear::check_sizes(groups, m_offsets, M, N, K, dtype);
+    if (st) return st;
+    if (!W || (M && (!dZ || !dX))) return NVFP4_ERR_INVALID;
+    if (!aligned16(dZ) || !aligned16(W) || !aligned16(dX)) return NVFP4_ERR_ALIGN;
+    DeviceInfo di;
+    if ((st = device_info(&di))) return st;
+    if (M == 0) return NVFP4_OK;
+    linear::Params p = {};
+    p.y = dX;
+    p.m_offsets = m_offsets;
+    p.groups = groups;
+    p.m_total = M;
+    p.features = K;
+    p.out_cols = K;
+    if ((st = kernel_ctl(&p.ctl))) return st;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return dtype == NVFP4_BF16 ? linear::dgrad_t<__nv_bfloat16>(dZ, W, p, N, di, s)
+                               : linear::dgrad_t<__half>(dZ, W, p, N, di, s);
+}
+
+int nvfp4_linear_wgrad(const void *dZ, const void *X, int64_t ldx, void *dW, const int32_t *m_offsets, int groups,
+                       int M, int N, int K, int dtype, void *stream) {
+    int st = linear::check_sizes(groups, m_offsets, M, N, K, dtype);
+    if (st) return st;
+    if (ldx < K || ldx % 8) return NVFP4_ERR_SHAPE;
+    if (!dW || (M && (!dZ || !X))) return NVFP4_ERR_INVALID;
+    if (!aligned16(dZ) || !aligned16(X) || !aligned16(dW)) return NVFP4_ERR_ALIGN;
+    DeviceInfo di;
+    if ((st = device_info(&di))) return st;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (M == 0)  // no token: the gradient is zero
+        return cuda_status(cudaMemsetAsync(dW, 0, (size_t)groups * N * K * 2, s));
+    linear::Params p = {};
+    p.y = dW;
+    p.m_offsets = m_offsets;
+    p.groups = groups;
+    p.m_total = M;
+    p.features = N;
+    p.out_cols = K;
+    if ((st = kernel_ctl(&p.ctl))) return st;
+    return dtype == NVFP4_BF16 ? linear::wgrad_t<__nv_bfloat16>(dZ, X, ldx, p, di, s)
+                               : linear::wgrad_t<__half>(dZ, X, ldx, p, di, s);
+}
+
+}  // extern "C"

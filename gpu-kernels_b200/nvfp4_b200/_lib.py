@@ -25,6 +25,9 @@ class Epilogue(C.Structure):
 
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu_tanh": 3, "swiglu": 4}
 
+DTYPES = {"bf16": 0, "f16": 1, "f32": 2}
+SCORES = {"softmax": 0, "sigmoid": 1}
+
 SIGNATURES = {
     "nvfp4_status_string": (C.c_char_p, [C.c_int]),
     "nvfp4_version": (C.c_int, []),
@@ -54,6 +57,23 @@ SIGNATURES = {
                                     C.POINTER(C.c_uint64), C.c_int, C.c_int, C.c_int64, C.c_int, _vp]),
     "nvfp4_rank_barrier": (C.c_int, [C.POINTER(C.c_uint64), C.c_int, C.c_int, C.c_int, C.c_size_t, _vp]),
     "nvfp4_gemm_host": (C.c_int, [_u8p, _u8p, _u8p, _u8p, C.c_float, _u16p, C.c_int, C.c_int, C.c_int, _vp]),
+    "nvfp4_linear": (C.c_int, [_vp, C.c_int64, _vp, _vp, _vp, _vp, _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_int,
+                               C.c_int, C.c_int, _vp]),
+    "nvfp4_linear_dgrad": (C.c_int, [_vp, _vp, _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _vp]),
+    "nvfp4_linear_wgrad": (C.c_int, [_vp, _vp, C.c_int64, _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
+                                     _vp]),
+    "nvfp4_activation_backward_workspace_size": (C.c_size_t, [C.c_int, C.c_int, C.c_int]),
+    "nvfp4_activation_backward": (C.c_int, [_vp, _vp, _vp, _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _vp,
+                                            C.c_size_t, _vp]),
+    "nvfp4_moe_route_workspace_size": (C.c_size_t, [C.c_int, C.c_int]),
+    "nvfp4_moe_route": (C.c_int, [_vp, C.c_int, _vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_float, _vp, _vp,
+                                  _vp, _vp, _vp, C.c_size_t, _vp]),
+    "nvfp4_moe_route_backward": (C.c_int, [_vp, _vp, C.c_int, _vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
+                                           C.c_float, _vp, _vp]),
+    "nvfp4_moe_dispatch": (C.c_int, [_vp, _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_int, _vp, _vp]),
+    "nvfp4_moe_combine": (C.c_int, [_vp, C.c_int, _vp, _vp, _vp, C.c_int, C.c_int, C.c_int, _vp, _vp]),
+    "nvfp4_moe_combine_backward": (C.c_int, [_vp, _vp, C.c_int, _vp, _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_int,
+                                             _vp, _vp, _vp]),
     "nvfp4_gemm_decode_noalloc": (C.c_int, [_u8p, _u8p, _u8p, _u8p, C.c_float, _u16p, C.c_int, C.c_int, C.c_int,
                                             _vp]),
 }

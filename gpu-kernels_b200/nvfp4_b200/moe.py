@@ -1,0 +1,158 @@
+"""The mixture-of-experts layer around the experts' products: the top-k router, the movement
+of token rows to expert order and back, and their gradients.
+
+    r = moe_route(logits, top_k)                       # weights, experts, rows, m_offsets
+    xs = moe_dispatch(x, r)                            # token rows in expert order
+    ys = linear_grouped(..., r.m_offsets ...)          # or quantize_grouped + gemm_grouped
+    y = moe_combine(ys, r, residual=x)                 # weighted sum back in token order
+
+Asynchronous on torch's current stream; nothing of the routing passes through the host.
+"""
+from typing import NamedTuple, Optional, Tuple
+
+import torch
+
+from ._lib import SCORES, lib
+from .layers import _DTYPES, _matrix, _ptr, call
+
+
+class Routing(NamedTuple):
+    """What moe_route decides, all on the device."""
+    weights: torch.Tensor    # fp32 [T, top_k]
+    experts: torch.Tensor    # int32 [T, top_k], -1 where a token has no expert left
+    rows: torch.Tensor       # int32 [T, top_k], the choice's row in expert order, or -1
+    m_offsets: torch.Tensor  # int32 [E + 1], the experts' row offsets
+
+
+def _logits(logits: torch.Tensor) -> Tuple[int, int]:
+    if not logits.is_cuda or logits.dim() != 2 or logits.dtype not in _DTYPES or not logits.is_contiguous():
+        raise ValueError("logits must be a contiguous 2-D bf16, fp16 or fp32 CUDA tensor")
+    return logits.shape
+
+
+def _scoring(scoring: str) -> int:
+    if scoring not in SCORES:
+        raise ValueError(f"scoring must be one of {sorted(SCORES)}")
+    return SCORES[scoring]
+
+
+def moe_route(logits: torch.Tensor, top_k: int, scoring: str = "softmax", bias: Optional[torch.Tensor] = None,
+              renormalize: bool = True, scale: float = 1.0) -> Routing:
+    """The top_k experts of each token of logits [T, E] and their weights.
+
+    scoring "softmax" or "sigmoid"; the experts are taken by highest logit, or with bias
+    (fp32 [E], sigmoid only; it does not enter the weights) by highest score + bias, the
+    lowest index first among equals.  weights = scores, divided by the sum of the chosen
+    ones if renormalize, times scale.  An expert whose logit is -inf or NaN is never chosen;
+    a choice that finds none left is -1 with weight 0.  E <= 256, top_k <= 32."""
+    T, E = _logits(logits)
+    score = _scoring(scoring)
+    dev = logits.device
+    if bias is not None:
+        if score != SCORES["sigmoid"]:
+            raise ValueError("a selection bias needs sigmoid scoring")
+        if bias.dtype != torch.float32 or bias.shape != (E,) or bias.device != dev or not bias.is_contiguous():
+            raise ValueError(f"bias must be a contiguous float32 tensor of {E} entries on {dev}")
+    n = T * top_k
+    ints = torch.empty(2 * n + E + 1, dtype=torch.int32, device=dev)
+    experts, rows, m_offsets = ints[:n].view(T, top_k), ints[n:2 * n].view(T, top_k), ints[2 * n:]
+    weights = torch.empty((T, top_k), dtype=torch.float32, device=dev)
+    ws, ws_bytes = None, 0
+    if T > 128:
+        ws_bytes = lib().nvfp4_moe_route_workspace_size(T, E)
+        ws = torch.empty(ws_bytes // 4, dtype=torch.int32, device=dev)
+    call("nvfp4_moe_route", dev, logits.data_ptr(), _DTYPES[logits.dtype], _ptr(bias), T, E, top_k, score,
+         int(renormalize), scale, weights.data_ptr(), experts.data_ptr(), rows.data_ptr(), m_offsets.data_ptr(),
+         _ptr(ws), ws_bytes)
+    return Routing(weights, experts, rows, m_offsets)
+
+
+def moe_route_backward(dweights: torch.Tensor, logits: torch.Tensor, routing: Routing, scoring: str = "softmax",
+                       renormalize: bool = True, scale: float = 1.0) -> torch.Tensor:
+    """Gradient of the logits [T, E] from dweights fp32 [T, top_k]; the choice is constant."""
+    T, E = _logits(logits)
+    experts = routing.experts
+    k = experts.shape[1]
+    _check_ints(experts, "experts", (T, k), logits.device)
+    if dweights.dtype != torch.float32 or dweights.shape != (T, k) or dweights.device != logits.device or \
+            not dweights.is_contiguous():
+        raise ValueError(f"dweights must be a contiguous float32 tensor ({T}, {k}) on {logits.device}")
+    dl = torch.empty_like(logits)
+    call("nvfp4_moe_route_backward", logits.device, dweights.data_ptr(), logits.data_ptr(), _DTYPES[logits.dtype],
+         experts.data_ptr(), T, E, k, _scoring(scoring), int(renormalize), scale, dl.data_ptr())
+    return dl
+
+
+def _check_ints(t: torch.Tensor, name: str, shape, device) -> None:
+    if t.dtype != torch.int32 or t.shape != shape or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor {tuple(shape)} on {device}")
+
+
+def _routed(routing: Routing, device) -> Tuple[int, int, int]:
+    """(tokens, top_k, experts) of a routing on this device."""
+    rows, offs = routing.rows, routing.m_offsets
+    if rows.dim() != 2 or offs.dim() != 1:
+        raise ValueError("routing.rows must be 2-D and routing.m_offsets 1-D")
+    T, k = rows.shape
+    _check_ints(rows, "routing.rows", (T, k), device)
+    _check_ints(offs, "routing.m_offsets", offs.shape, device)
+    w = routing.weights
+    if w.dtype != torch.float32 or w.shape != (T, k) or w.device != device or not w.is_contiguous():
+        raise ValueError(f"routing.weights must be a contiguous float32 tensor ({T}, {k}) on {device}")
+    return T, k, offs.numel() - 1
+
+
+def _rows16(t: torch.Tensor, name: str, rows: int) -> int:
+    if not t.is_cuda or t.dim() != 2 or t.dtype not in (torch.bfloat16, torch.float16) or not t.is_contiguous() or \
+            t.shape[0] != rows:
+        raise ValueError(f"{name} must be a contiguous 2-D bf16 or fp16 CUDA tensor of {rows} rows")
+    if t.shape[1] % 8 or not t.shape[1]:
+        raise ValueError(f"{name} must have a multiple of 8 columns")
+    return t.shape[1]
+
+
+def moe_dispatch(x: torch.Tensor, routing: Routing) -> torch.Tensor:
+    """x [T, K] -> [T * top_k, K] in expert order, a copy of a token's row for each of its
+    choices; rows past m_offsets[-1] (masked choices) are zero."""
+    T, k, E = _routed(routing, x.device)
+    K = _rows16(x, "x", T)
+    out = x.new_empty((T * k, K))
+    call("nvfp4_moe_dispatch", x.device, x.data_ptr(), routing.rows.data_ptr(), routing.m_offsets.data_ptr(), T, E, k,
+         K, out.data_ptr())
+    return out
+
+
+def moe_dispatch_backward(dx_rows: torch.Tensor, routing: Routing) -> torch.Tensor:
+    """Gradient of moe_dispatch: dx[t] = the sum of the rows of t's choices."""
+    T, k, _ = _routed(routing, dx_rows.device)
+    K = _rows16(dx_rows, "dx_rows", T * k)
+    dx = dx_rows.new_empty((T, K))
+    call("nvfp4_moe_combine", dx.device, dx_rows.data_ptr(), _DTYPES[dx.dtype], routing.rows.data_ptr(), None, None, T,
+         k, K, dx.data_ptr())
+    return dx
+
+
+def moe_combine(x_rows: torch.Tensor, routing: Routing, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """y[t] = residual[t] + sum_j weights[t, j] * x_rows[rows[t, j]], summed in fp32."""
+    T, k, _ = _routed(routing, x_rows.device)
+    K = _rows16(x_rows, "x_rows", T * k)
+    if residual is not None:
+        _matrix(residual, "residual", (T, K), x_rows)
+    y = x_rows.new_empty((T, K))
+    call("nvfp4_moe_combine", y.device, x_rows.data_ptr(), _DTYPES[y.dtype], routing.rows.data_ptr(),
+         routing.weights.data_ptr(), _ptr(residual), T, k, K, y.data_ptr())
+    return y
+
+
+def moe_combine_backward(dy: torch.Tensor, x_rows: torch.Tensor, routing: Routing):
+    """Gradients (dx_rows [T * top_k, K], dweights fp32 [T, top_k]) of moe_combine; the
+    residual's gradient is dy itself."""
+    T, k, E = _routed(routing, x_rows.device)
+    K = _rows16(x_rows, "x_rows", T * k)
+    _matrix(dy, "dy", (T, K), x_rows)
+    dx_rows = torch.empty_like(x_rows)
+    dweights = torch.empty((T, k), dtype=torch.float32, device=dy.device)
+    call("nvfp4_moe_combine_backward", dy.device, dy.data_ptr(), x_rows.data_ptr(), _DTYPES[dy.dtype],
+         routing.rows.data_ptr(), routing.weights.data_ptr(), routing.m_offsets.data_ptr(), T, E, k, K,
+         dx_rows.data_ptr(), dweights.data_ptr())
+    return dx_rows, dweights

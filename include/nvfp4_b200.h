@@ -327,6 +327,94 @@ NVFP4_API int nvfp4_gemm_decode_noalloc(const uint8_t *A, const uint8_t *SFA, co
 /* Number of kernel launches this library has issued in this process. */
 NVFP4_API uint64_t nvfp4_launch_count(void);
 
+/*
+ * 16-bit layers (no counterpart in the reference): the linear layers that stay in bf16 or
+ * fp16 beside the NVFP4 ones, their experts, and the router around both.  dtype is one of
+ * NVFP4_BF16, NVFP4_F16 (and NVFP4_F32 for the router's logits).  All sums, statistics and
+ * activations are fp32; every result is rounded once, to its 16-bit type.  Results are the
+ * same bits on every call.  Nothing is allocated; workspaces come from the caller and need
+ * no initial value.  Tensors are contiguous, 16-byte aligned, unless a row pitch is given.
+ *
+ * Row groups: m_offsets (groups + 1 int32 on the device, non-decreasing, clamped to
+ * [0, M]) makes group g the rows [m_offsets[g], m_offsets[g+1]); group g uses weight rows
+ * [g*N, (g+1)*N) of W [groups * N, K] and bias row g.  m_offsets NULL with groups = 1: one
+ * dense layer over all M rows.  groups <= 256; M >= 0; N, K multiples of 8.
+ */
+enum { NVFP4_BF16 = 0, NVFP4_F16 = 1, NVFP4_F32 = 2 };
+
+/*
+ * Forward: z = X W^T + bias;  Y = act(z) + residual.
+ *   X [M, K], rows ldx >= K elements apart (ldx % 8 == 0); W [groups * N, K]; bias
+ *   [groups, N] or NULL; activation NVFP4_ACT_* (SwiGLU as for nvfp4_gemm_epilogue: gate
+ *   and up rows of W interleaved in blocks of 16, N % 32 == 0, N/2 output columns; silu
+ *   and gelu from exp, not the tanh approximation); residual [M, Nout] or NULL;
+ *   Y [M, Nout]; Z [M, N] receives z (rounded) for the backward pass, or NULL.
+ * With m_offsets, rows of Y (and Z) outside every group are set to zero.
+ */
+NVFP4_API int nvfp4_linear(const void *X, int64_t ldx, const void *W, const void *bias, const void *residual, void *Y,
+                           void *Z, const int32_t *m_offsets, int groups, int M, int N, int K, int activation,
+                           int dtype, void *stream);
+/* Input gradient: dX [M, K] = dZ [M, N] . W.  Rows outside every group are set to zero. */
+NVFP4_API int nvfp4_linear_dgrad(const void *dZ, const void *W, void *dX, const int32_t *m_offsets, int groups, int M,
+                                 int N, int K, int dtype, void *stream);
+/* Weight gradient: dW [groups * N, K] = dZ^T X by group (rows ldx apart in X); the gradient
+ * of a group without rows is zero. */
+NVFP4_API int nvfp4_linear_wgrad(const void *dZ, const void *X, int64_t ldx, void *dW, const int32_t *m_offsets,
+                                 int groups, int M, int N, int K, int dtype, void *stream);
+/*
+ * Gradient of the epilogue: dZ [M, N] = dY [M, Nout] * act'(Z), and, when dbias is given,
+ * dbias [groups, N] = the column sums of the unrounded dZ by group.  With NVFP4_ACT_NONE dZ
+ * is dY: only dbias is computed, Z and dZ may be NULL.  Rows of dZ outside every group are
+ * not written.  The workspace is needed for dbias only.
+ */
+NVFP4_API size_t nvfp4_activation_backward_workspace_size(int groups, int M, int N);
+NVFP4_API int nvfp4_activation_backward(const void *dY, const void *Z, void *dZ, void *dbias,
+                                        const int32_t *m_offsets, int groups, int M, int N, int activation, int dtype,
+                                        void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * Router.  logits [T, E] -> for each token its top_k experts:
+ *   score = softmax(logits) or sigmoid(logits); the experts are taken by highest logit, or
+ *   with bias [E] (fp32, sigmoid only) by highest score + bias, the lowest index first
+ *   among equals; weight = score (divided by the sum of the chosen ones if renormalize),
+ *   times scale.
+ * An expert whose logit is -inf or NaN is masked: never chosen, no part of the softmax.  A
+ * choice that finds no expert left is -1 with weight 0, so a fully masked token is routed
+ * nowhere.
+ *   weights fp32 [T, top_k], experts int32 [T, top_k];
+ *   m_offsets int32 [E + 1]: expert e's rows, as nvfp4_linear and nvfp4_gemm_grouped take;
+ *   rows int32 [T, top_k]: the row of each choice in expert order (by expert, then token),
+ *   -1 for none.
+ * T <= 2^20, E <= 256, top_k <= min(E, 32).  The workspace
+ * (nvfp4_moe_route_workspace_size) is needed for T > 128 only.
+ */
+enum { NVFP4_SCORE_SOFTMAX = 0, NVFP4_SCORE_SIGMOID = 1 };
+NVFP4_API size_t nvfp4_moe_route_workspace_size(int T, int E);
+NVFP4_API int nvfp4_moe_route(const void *logits, int dtype, const float *bias, int T, int E, int top_k, int scoring,
+                              int renormalize, float scale, float *weights, int32_t *experts, int32_t *rows,
+                              int32_t *m_offsets, void *workspace, size_t workspace_bytes, void *stream);
+/* Gradient of the logits [T, E] (their dtype) from that of the weights [T, top_k]; the
+ * choice itself is constant, and so is the bias. */
+NVFP4_API int nvfp4_moe_route_backward(const float *dweights, const void *logits, int dtype, const int32_t *experts,
+                                       int T, int E, int top_k, int scoring, int renormalize, float scale,
+                                       void *dlogits, void *stream);
+/*
+ * Movement of 16-bit rows of K elements (K % 8 == 0) between token order and expert order.
+ *   dispatch: X_rows[rows[t, j]] = X[t]; rows that no choice owns are zero.
+ *   combine:  Y[t] = residual[t] + sum_j weights[t, j] * X_rows[rows[t, j]], in fp32 in the
+ *             order of j; weights NULL: all ones (the gradient of dispatch).
+ *   combine_backward: dX_rows[rows[t, j]] = weights[t, j] * dY[t] (other rows zero) and
+ *             dweights[t, j] = <X_rows[rows[t, j]], dY[t]>, 0 for choices without a row.
+ * X_rows has T * top_k rows.
+ */
+NVFP4_API int nvfp4_moe_dispatch(const void *X, const int32_t *rows, const int32_t *m_offsets, int T, int E,
+                                 int top_k, int K, void *X_rows, void *stream);
+NVFP4_API int nvfp4_moe_combine(const void *X_rows, int dtype, const int32_t *rows, const float *weights,
+                                const void *residual, int T, int top_k, int K, void *Y, void *stream);
+NVFP4_API int nvfp4_moe_combine_backward(const void *dY, const void *X_rows, int dtype, const int32_t *rows,
+                                         const float *weights, const int32_t *m_offsets, int T, int E, int top_k,
+                                         int K, void *dX_rows, float *dweights, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

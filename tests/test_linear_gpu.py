@@ -1,0 +1,228 @@
+"""The 16-bit linear layers on the GPU against 64-bit forms, within bounds derived from the
+number formats (ref16.py): tile edges, ragged and empty groups, strides, activations, and
+gradients against the formula and against differences."""
+import math
+
+import pytest
+import torch
+
+import ref16 as R
+
+pytestmark = pytest.mark.gpu
+
+
+def make(shape, dtype, seed, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * scale).to(dtype).cuda()
+
+
+def offsets(cuts):
+    return torch.tensor(cuts, dtype=torch.int32, device="cuda")
+
+
+def check_forward(nv, M, N, K, act="none", bias=False, residual=False, dtype=torch.bfloat16, cuts=None, z=False):
+    G = 1 if cuts is None else len(cuts) - 1
+    x, w = make((M, K), dtype, 1), make((G * N, K), dtype, 2, K ** -0.5)
+    b = make((N,) if cuts is None else (G, N), dtype, 3, 0.5) if bias else None
+    No = N // 2 if act == "swiglu" else N
+    r = make((M, No), dtype, 4) if residual else None
+    if cuts is None:
+        got = nv.linear(x, w, bias=b, activation=act, residual=r, return_preact=z)
+    else:
+        got = nv.linear_grouped(x, w, offsets(cuts), bias=b, activation=act, return_preact=z)
+    nv.device_status()
+    y, ey, zz, ez = R.forward64(x, w, cuts or [0, M], b, act, r)
+    if z:
+        R.assert_close(got[1], zz, ez, "z")
+        got = got[0]
+    R.assert_close(got, y, ey, "y")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M,N,K", [
+    (1, 8, 8), (1, 256, 64), (2, 264, 72), (15, 512, 128), (16, 248, 200), (17, 1024, 1032), (31, 128, 64),
+    (33, 320, 456), (64, 4096, 512), (65, 264, 2048), (127, 256, 264), (128, 2048, 1024), (129, 520, 128),
+    (200, 1000, 640), (256, 256, 4096), (257, 768, 64), (300, 2056, 96), (513, 264, 8), (1025, 1288, 520),
+])
+def test_shapes(nv, cuda_dev, M, N, K, dtype):
+    check_forward(nv, M, N, K, dtype=dtype)
+
+
+@pytest.mark.parametrize("act", R.ACTS)
+@pytest.mark.parametrize("M,N,K", [(1, 512, 256), (5, 288, 136), (48, 1056, 512), (130, 544, 264), (700, 1312, 192)])
+def test_epilogue(nv, cuda_dev, act, M, N, K):
+    for dtype in (torch.bfloat16, torch.float16):
+        check_forward(nv, M, N, K, act, bias=True, residual=True, dtype=dtype, z=True)
+        check_forward(nv, M, N, K, act, bias=True, dtype=dtype)
+        check_forward(nv, M, N, K, act, residual=True, dtype=dtype)
+
+
+GROUPS = [
+    [0, 5], [0, 0, 3, 3, 40], [0, 1, 2, 3, 4, 5], [0, 17, 17, 50, 300], [0, 256, 512, 700], [0, 300, 301, 301, 557, 900],
+    [0] * 20 + [9], [0, 33, 66, 99, 132, 165, 198], list(range(0, 65 * 8, 8)),
+]
+
+
+@pytest.mark.parametrize("cuts", GROUPS, ids=lambda c: f"G{len(c) - 1}M{c[-1]}")
+def test_groups(nv, cuda_dev, cuts):
+    check_forward(nv, cuts[-1], 264, 136, cuts=cuts)
+    check_forward(nv, cuts[-1], 544, 200, "swiglu", bias=True, cuts=cuts, z=True, dtype=torch.float16)
+    check_forward(nv, cuts[-1], 256, 512, "gelu_tanh", bias=True, cuts=cuts)
+
+
+def test_rows_outside_groups_are_zero(nv, cuda_dev):
+    """Offsets that leave rows out at both ends, and ends past the last row (clamped)."""
+    x, w = make((300, 128), torch.bfloat16, 1), make((2 * 64, 128), torch.bfloat16, 2)
+    y, z = nv.linear_grouped(x, w, offsets([7, 100, 250]), activation="silu", return_preact=True)
+    ref, e, zr, ez = R.forward64(x, w, [7, 100, 250], None, "silu", None)
+    R.assert_close(y, ref, e)
+    R.assert_close(z, zr, ez)
+    assert not y[:7].any() and not y[250:].any() and not z[:7].any() and not z[250:].any()
+    y = nv.linear_grouped(x, w, offsets([-5, 100, 5000]))
+    R.assert_close(y, *R.forward64(x, w, [0, 100, 300], None, "none", None)[:2])
+    y = nv.linear_grouped(x, w, offsets([0, 0, 0]))
+    assert not y.any()
+
+
+def test_empty(nv, cuda_dev):
+    w = make((64, 32), torch.bfloat16, 2)
+    x = w.new_empty((0, 32))
+    assert nv.linear(x, w).shape == (0, 64)
+    dx, dw, db = nv.linear_backward(x.new_empty((0, 64)), x, w, bias_grad=True)
+    assert dx.shape == (0, 32) and not dw.any() and not db.any()
+
+
+@pytest.mark.parametrize("M", [1, 20, 300])
+def test_strided_rows(nv, cuda_dev, M):
+    """x as a slice of wider rows, whose other columns hold NaN."""
+    wide = torch.full((M, 512), math.nan, dtype=torch.bfloat16, device="cuda")
+    wide[:, 64:64 + 136] = make((M, 136), torch.bfloat16, 1)
+    x, w = wide[:, 64:64 + 136], make((264, 136), torch.bfloat16, 2)
+    R.assert_close(nv.linear(x, w), *R.forward64(x, w, [0, M], None, "none", None)[:2])
+    dy = make((M, 264), torch.bfloat16, 3)
+    _, dw, _ = nv.linear_backward(dy, x, w)
+    (_, _), (ref, e), _ = R.backward64(dy, x, w, [0, M], None, "none")
+    R.assert_close(dw, ref, e)
+
+
+def test_other_groups_values_stay_out(nv, cuda_dev):
+    """Infinities and NaN in another group's rows and weights reach only that group."""
+    cuts = [0, 21, 40, 73]
+    x, w, dy = make((73, 72), torch.bfloat16, 1), make((3 * 72, 72), torch.bfloat16, 2), make((73, 72), torch.bfloat16, 3)
+    clean = [t.clone() for t in (x, w, dy)]
+    for t, rows in ((x, slice(21, 40)), (w, slice(72, 144)), (dy, slice(21, 40))):
+        t[rows] = math.nan
+        t[rows, ::3] = math.inf
+    o = offsets(cuts)
+    for bad, good in ((nv.linear_grouped(x, w, o), nv.linear_grouped(clean[0], clean[1], o)),
+                      (nv.linear_grouped_backward(dy, x, w, o)[0],
+                       nv.linear_grouped_backward(clean[2], clean[0], clean[1], o)[0])):
+        assert torch.equal(bad[:21], good[:21]) and torch.equal(bad[40:], good[40:])
+        assert not torch.isfinite(bad[21:40]).any()
+    bad = nv.linear_grouped_backward(dy, x, w, o, bias_grad=True)
+    good = nv.linear_grouped_backward(clean[2], clean[0], clean[1], o, bias_grad=True)
+    for i, n in ((1, 72), (2, 1)):
+        assert torch.equal(bad[i][:n], good[i][:n]) and torch.equal(bad[i][2 * n:], good[i][2 * n:])
+
+
+@pytest.mark.parametrize("act", R.ACTS)
+@pytest.mark.parametrize("M,N,K", [(1, 32, 8), (7, 96, 72), (64, 256, 256), (65, 288, 520), (130, 544, 64),
+                                   (333, 1024, 264), (1000, 160, 136)])
+def test_backward(nv, cuda_dev, act, M, N, K):
+    for dtype in (torch.bfloat16, torch.float16):
+        No = N // 2 if act == "swiglu" else N
+        x, w, dy = make((M, K), dtype, 1), make((N, K), dtype, 2, K ** -0.5), make((M, No), dtype, 3)
+        z = make((M, N), dtype, 4)
+        got = nv.linear_backward(dy, x, w, preact=z if act != "none" else None, activation=act, bias_grad=True)
+        nv.device_status()
+        ref = R.backward64(dy, x, w, [0, M], z, act)
+        for a, (r, e), n in zip(got, ref, ("dx", "dw", "db")):
+            R.assert_close(a, r.reshape(a.shape), e.reshape(a.shape), n)
+
+
+@pytest.mark.parametrize("cuts", GROUPS, ids=lambda c: f"G{len(c) - 1}M{c[-1]}")
+def test_backward_groups(nv, cuda_dev, cuts):
+    for act, N, K, dtype in (("none", 72, 264, torch.bfloat16), ("swiglu", 288, 136, torch.bfloat16),
+                             ("relu", 264, 72, torch.float16)):
+        M, G, No = cuts[-1], len(cuts) - 1, N // 2 if act == "swiglu" else N
+        x, w, dy = make((M, K), dtype, 1), make((G * N, K), dtype, 2, K ** -0.5), make((M, No), dtype, 3)
+        z = make((M, N), dtype, 4)
+        got = nv.linear_grouped_backward(dy, x, w, offsets(cuts), preact=z, activation=act, bias_grad=True)
+        nv.device_status()
+        for a, (r, e), n in zip(got, R.backward64(dy, x, w, cuts, z, act), ("dx", "dw", "db")):
+            R.assert_close(a, r, e, n)
+
+
+@pytest.mark.parametrize("act", R.ACTS)
+def test_gradient_against_differences(nv, cuda_dev, act):
+    """<dL/dp, d> against (L(p + h d) - L(p - h d)) / 2h of the 64-bit forward pass, for
+    L = <y, dy>.  The operator's gradients are off by a few roundings u of 16-bit values (a
+    relative error of the inner product below 4u of the norms' product); the difference
+    quotient is off by O(h^2)."""
+    M, N, K, dtype = 24, 64, 40, torch.float16
+    x, w, b = make((M, K), dtype, 1), make((N, K), dtype, 2, 0.3), make((N,), dtype, 3)
+    dy = make((M, N // 2 if act == "swiglu" else N), dtype, 4)
+    y, z = nv.linear(x, w, bias=b, activation=act, return_preact=True)
+    grads = nv.linear_backward(dy, x, w, preact=z, activation=act, bias_grad=True)
+    for i, p in enumerate((x, w, b)):
+        d = make(p.shape, torch.float16, 10 + i).double()
+        h = 1e-4
+
+        def loss(s):
+            q = [t.double() for t in (x, w, b)]
+            q[i] = q[i] + s * d
+            return (R.act64(q[0] @ q[1].t() + q[2], act) * dy.double()).sum()
+
+        diff = ((loss(h) - loss(-h)) / (2 * h)).item()
+        got = (grads[i].double() * d).sum().item()
+        norm = (grads[i].double().norm() * d.norm()).item()
+        if act == "relu":  # entries whose sign flips within h d do not matter at this h
+            assert abs(got - diff) <= 8 * R.U[dtype] * norm
+        else:
+            assert abs(got - diff) <= 4 * R.U[dtype] * norm + 1e-6 * norm
+
+
+def test_same_bits_every_time(nv, cuda_dev):
+    cuts = [0, 100, 101, 400]
+    x, w, dy = make((400, 328), torch.bfloat16, 1), make((3 * 320, 328), torch.bfloat16, 2), make((400, 320), torch.bfloat16, 3)
+    z, o = make((400, 320), torch.bfloat16, 4), offsets(cuts)
+
+    def once():
+        return [nv.linear_grouped(x, w, o, activation="silu"), nv.linear(x[:3], w[:320]), nv.linear(x, w[:320]),
+                *nv.linear_grouped_backward(dy, x, w, o, preact=z, activation="silu", bias_grad=True)]
+
+    first = once()
+    for _ in range(5):
+        for a, b in zip(first, once()):
+            assert torch.equal(a, b)
+
+
+def test_side_stream_and_graph(nv, cuda_dev):
+    """The calls run on the current stream, and a captured graph follows inputs and offsets
+    that change in place."""
+    x, w = make((96, 128), torch.bfloat16, 1), make((4 * 128, 128), torch.bfloat16, 2)
+    o = offsets([0, 10, 20, 60, 96])
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        nv.linear_grouped(x, w, o)
+    s.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        y = nv.linear_grouped(x, w, o)
+    for cuts in ([0, 10, 20, 60, 96], [0, 0, 50, 50, 90]):
+        o.copy_(offsets(cuts))
+        x.copy_(make((96, 128), torch.bfloat16, cuts[2]))
+        g.replay()
+        torch.cuda.synchronize()
+        R.assert_close(y, *R.forward64(x, w, cuts, None, "none", None)[:2])
+
+
+def test_large_offsets(nv, cuda_dev):
+    """An output of more than 2^31 elements: the last rows are where they belong."""
+    M, N, K = 140_000, 16_384, 64
+    x, w = make((M, K), torch.bfloat16, 1), make((N, K), torch.bfloat16, 2)
+    y = nv.linear(x, w)
+    nv.device_status()
+    for a in (0, 131_072 - 8, M - 16):
+        R.assert_close(y[a:a + 16], *R.forward64(x[a:a + 16], w, [0, 16], None, "none", None)[:2])

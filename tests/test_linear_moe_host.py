@@ -1,0 +1,87 @@
+"""CPU: what the 16-bit linear and mixture-of-experts entry points refuse, before any
+device is touched."""
+import ctypes as C
+
+import pytest
+import torch
+
+P = C.c_void_p(1 << 20)    # never dereferenced: the checks run first
+ODD = C.c_void_p((1 << 20) + 8)
+INVALID, SHAPE, ALIGN, WORKSPACE = -1, -2, -3, -7
+
+
+def linear(nv, X=P, ldx=64, W=P, bias=None, residual=None, Y=P, Z=None, offs=None, G=1, M=4, N=64, K=64, act=0, dt=0):
+    return nv.lib().nvfp4_linear(X, ldx, W, bias, residual, Y, Z, offs, G, M, N, K, act, dt, None)
+
+
+@pytest.mark.parametrize("args,status", [
+    (dict(X=None), INVALID), (dict(W=None), INVALID), (dict(Y=None), INVALID), (dict(act=5), INVALID),
+    (dict(act=-1), INVALID), (dict(dt=2), INVALID), (dict(G=0), INVALID), (dict(G=2), INVALID),
+    (dict(M=-1), SHAPE), (dict(N=0), SHAPE), (dict(N=12), SHAPE), (dict(K=12, ldx=16), SHAPE), (dict(K=0), SHAPE),
+    (dict(ldx=56), SHAPE), (dict(ldx=68), SHAPE), (dict(N=72, act=4), SHAPE), (dict(G=257, offs=P), SHAPE),
+    (dict(X=ODD), ALIGN), (dict(W=ODD), ALIGN), (dict(Y=ODD), ALIGN), (dict(Z=ODD), ALIGN),
+    (dict(residual=ODD), ALIGN), (dict(bias=C.c_void_p((1 << 20) + 1)), ALIGN),
+    (dict(offs=C.c_void_p((1 << 20) + 2), G=2), ALIGN),
+])
+def test_linear_refusals(nv, args, status):
+    assert linear(nv, **args) == status
+
+
+def test_gradient_refusals(nv):
+    L = nv.lib()
+    assert L.nvfp4_linear_dgrad(None, P, P, None, 1, 4, 64, 64, 0, None) == INVALID
+    assert L.nvfp4_linear_dgrad(P, P, P, None, 1, 4, 60, 64, 0, None) == SHAPE
+    assert L.nvfp4_linear_dgrad(P, P, ODD, None, 1, 4, 64, 64, 0, None) == ALIGN
+    assert L.nvfp4_linear_wgrad(P, P, 64, None, None, 1, 4, 64, 64, 0, None) == INVALID
+    assert L.nvfp4_linear_wgrad(P, P, 32, P, None, 1, 4, 64, 64, 0, None) == SHAPE
+    assert L.nvfp4_linear_wgrad(P, ODD, 64, P, None, 1, 4, 64, 64, 0, None) == ALIGN
+    need = L.nvfp4_activation_backward_workspace_size(1, 100, 64)
+    assert need > 0 and L.nvfp4_activation_backward_workspace_size(0, 100, 64) == 0
+    assert L.nvfp4_activation_backward(P, P, P, P, None, 1, 100, 64, 1, 0, None, 0, None) == WORKSPACE
+    assert L.nvfp4_activation_backward(P, P, P, P, None, 1, 100, 64, 1, 0, P, need - 1, None) == WORKSPACE
+    assert L.nvfp4_activation_backward(P, None, P, None, None, 1, 100, 64, 1, 0, None, 0, None) == INVALID
+    assert L.nvfp4_activation_backward(P, P, P, None, None, 1, 100, 48, 4, 0, None, 0, None) == SHAPE
+    assert L.nvfp4_activation_backward(P, ODD, P, None, None, 1, 100, 64, 1, 0, None, 0, None) == ALIGN
+    assert L.nvfp4_activation_backward(P, None, None, None, None, 1, 100, 64, 0, 0, None, 0, None) == 0  # nothing to do
+
+
+def route(nv, logits=P, dt=0, bias=None, T=4, E=8, k=2, scoring=0, w=P, e=P, r=P, o=P, ws=None, n=0):
+    return nv.lib().nvfp4_moe_route(logits, dt, bias, T, E, k, scoring, 1, 1.0, w, e, r, o, ws, n, None)
+
+
+@pytest.mark.parametrize("args,status", [
+    (dict(logits=None), INVALID), (dict(w=None), INVALID), (dict(e=None), INVALID), (dict(r=None), INVALID),
+    (dict(o=None), INVALID), (dict(dt=3), INVALID), (dict(scoring=2), INVALID), (dict(bias=P), INVALID),
+    (dict(T=-1), SHAPE), (dict(T=(1 << 20) + 1), SHAPE), (dict(E=0), SHAPE), (dict(E=257), SHAPE), (dict(k=0), SHAPE),
+    (dict(k=9), SHAPE), (dict(E=64, k=33), SHAPE), (dict(logits=C.c_void_p((1 << 20) + 1)), ALIGN),
+    (dict(logits=C.c_void_p((1 << 20) + 2), dt=2), ALIGN), (dict(T=129), WORKSPACE),
+    (dict(T=129, ws=P, n=63), WORKSPACE),
+])
+def test_route_refusals(nv, args, status):
+    assert route(nv, **args) == status
+
+
+def test_move_refusals(nv):
+    L = nv.lib()
+    assert L.nvfp4_moe_route_workspace_size(129, 8) == 64 and L.nvfp4_moe_route_workspace_size(5, 0) == 0
+    assert L.nvfp4_moe_dispatch(None, P, P, 4, 8, 2, 64, P, None) == INVALID
+    assert L.nvfp4_moe_dispatch(P, P, P, 4, 8, 2, 60, P, None) == SHAPE
+    assert L.nvfp4_moe_dispatch(P, P, P, 4, 8, 33, 64, P, None) == SHAPE
+    assert L.nvfp4_moe_dispatch(ODD, P, P, 4, 8, 2, 64, P, None) == ALIGN
+    assert L.nvfp4_moe_combine(P, 2, P, P, None, 4, 2, 64, P, None) == INVALID
+    assert L.nvfp4_moe_combine(P, 0, P, P, ODD, 4, 2, 64, P, None) == ALIGN
+    assert L.nvfp4_moe_combine_backward(P, P, 0, P, None, P, 4, 8, 2, 64, P, P, None) == INVALID
+    assert L.nvfp4_moe_combine_backward(P, P, 0, P, P, P, -1, 8, 2, 64, P, P, None) == SHAPE
+    assert L.nvfp4_moe_route_backward(P, P, 0, None, 4, 8, 2, 0, 1, 1.0, P, None) == INVALID
+
+
+def test_python_refuses_host_tensors(nv):
+    x, w = torch.zeros(4, 64, dtype=torch.bfloat16), torch.zeros(64, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError):
+        nv.linear(x, w)
+    with pytest.raises(ValueError):
+        nv.moe_route(torch.zeros(4, 8), 2)
+    r = nv.Routing(torch.zeros(4, 2), *(torch.zeros(4, 2, dtype=torch.int32) for _ in range(2)),
+                   torch.zeros(9, dtype=torch.int32))
+    with pytest.raises(ValueError):
+        nv.moe_dispatch(x, r)
