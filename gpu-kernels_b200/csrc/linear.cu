@@ -189,12 +189,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const uint32_t bar_full = base + kOffBar;            // [stages], leader's used: both CTAs' data
     const uint32_t bar_empty = bar_full + 8 * kStages;   // [stages]
     const uint32_t bar_tail = bar_empty + 8 * kStages;   // [stages] wgrad: a group's last slot has landed
-    const uint32_t bar_acc_full = bar_tail + 8 * kStages;
+    const uint32_t bar_ready = bar_tail + 8 * kStages;   // [stages] wgrad: that slot is cleared in both CTAs
+    const uint32_t bar_acc_full = bar_ready + 8 * kStages;
     const uint32_t bar_acc_empty = bar_acc_full + 16;
     const uint32_t bar_drain = bar_acc_empty + 16;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(base_ptr + kOffBar + (3 * kStages + 5) * 8);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(base_ptr + kOffBar + (4 * kStages + 5) * 8);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
-    static_assert((3 * kStages + 5) * 8 + 8 <= kBarBytes, "barrier region");
+    static_assert((4 * kStages + 5) * 8 + 8 <= kBarBytes, "barrier region");
     int *g_r0 = reinterpret_cast<int *>(base_ptr + kOffTables);
     int *g_r1 = g_r0 + kMaxGroups + 1;
     int *g_t0 = g_r1 + kMaxGroups + 1;
@@ -206,9 +207,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const int n_c = FORM == kWgrad ? (p.out_cols + p.bt - 1) / p.bt : 0;
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; s++) {
-            mbar_init(bar_full + 8 * s, 2);  // one arrival from each CTA's producer
+            mbar_init(bar_full + 8 * s, 1);
             mbar_init(bar_empty + 8 * s, 1);
             mbar_init(bar_tail + 8 * s, 1);
+            mbar_init(bar_ready + 8 * s, 2);
         }
         for (int b = 0; b < 2; b++) {
             mbar_init(bar_acc_full + 8 * b, 1);
@@ -272,6 +274,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (elect_one()) {
             uint32_t stage = 0, phase = 0, issued_mask = 0, issued_parity = 0;
             uint32_t tail_mask = 0, tail_parity = 0;  // tail barriers used; parity of their next phase
+            const uint32_t lead_full = map_to_cta(bar_full, 0), own_tail = map_to_cta(bar_tail, rank);
             bool ok = true;
             for (int t = pair; ok && t < n_tiles; t += num_pairs) {
                 const Tile ti = tile_at(t);
@@ -286,14 +289,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                         break;
                     }
                     const bool tail = kb == nkb - 1 && dirty_tail(ti);
-                    const uint32_t bar = tail ? map_to_cta(bar_tail + 8 * stage, rank)
-                                              : map_to_cta(bar_full + 8 * stage, 0);
-                    mbar_arrive_expect_tx_cluster(bar, tx_bytes);
+                    // both CTAs' copies complete on the leader's barrier; a slot to be cleared
+                    // lands on each CTA's own tail barrier instead
+                    const uint32_t bar = tail ? own_tail + 8 * stage : lead_full + 8 * stage;
                     if (tail) {
+                        if (rank == 0) mbar_arrive(bar_full + 8 * stage);
+                        mbar_arrive_expect_tx(bar_tail + 8 * stage, tx_bytes);
                         tail_mask |= 1u << stage;
                         tail_parity ^= 1u << stage;
                         issued_mask &= ~(1u << stage);
                     } else {
+                        if (rank == 0) mbar_arrive_expect_tx(bar_full + 8 * stage, 2 * tx_bytes);
                         issued_mask |= 1u << stage;
                         issued_parity = (issued_parity & ~(1u << stage)) | (phase << stage);
                     }
@@ -335,7 +341,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             const uint32_t empty0 = map_to_cta(bar_empty, 0), empty1 = map_to_cta(bar_empty, 1);
             const uint32_t accf0 = map_to_cta(bar_acc_full, 0), accf1 = map_to_cta(bar_acc_full, 1);
             const uint64_t a_desc = operand_desc<kAmn>(sA), b_desc = operand_desc<kBmn>(sB);
-            uint32_t stage = 0, phase = 0;
+            uint32_t stage = 0, phase = 0, ready_parity = 0;
             int local = 0;
             bool ok = true, any = false;
             for (int t = pair; ok && t < n_tiles; t += num_pairs, local++) {
@@ -344,7 +350,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 const uint32_t idesc = idesc_f16(kBf16, kAmn, kBmn, 256, (uint32_t)width_of(ti));
                 const uint32_t buf = local & 1, use = local >> 1;
                 const uint32_t d_tmem = tmem_base + buf * kAccCols;
-                if (!spin_parity_cluster(bar_acc_empty + 8 * buf, (use & 1) ^ 1, tmo, abort_flag)) {
+                if (!spin_parity(bar_acc_empty + 8 * buf, (use & 1) ^ 1, tmo, abort_flag)) {
                     report_timeout(abort_flag, p.ctl.status);
                     ok = false;
                     break;
@@ -352,7 +358,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 tc_fence_after();
                 const int red = FORM == kWgrad ? ti.rows : p.red;
                 for (int kb = 0; kb < nkb; kb++) {
-                    if (!spin_parity_cluster(bar_full + 8 * stage, phase, tmo, abort_flag)) {
+                    bool landed = spin_parity(bar_full + 8 * stage, phase, tmo, abort_flag);
+                    if (landed && kb == nkb - 1 && dirty_tail(ti)) {
+                        landed = wait_parity_cluster(bar_ready + 8 * stage, (ready_parity >> stage) & 1, tmo, abort_flag);
+                        ready_parity ^= 1u << stage;
+                    }
+                    if (!landed) {
                         report_timeout(abort_flag, p.ctl.status);
                         ok = false;
                         break;
@@ -417,7 +428,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(map_to_cta(bar_full + 8 * stage, 0));
+                if (lane == 0) mbar_arrive_cluster(map_to_cta(bar_ready + 8 * stage, 0));
             }
         }
     } else {

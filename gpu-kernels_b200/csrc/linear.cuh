@@ -102,38 +102,6 @@ __device__ __forceinline__ void tma_load_3d_hint(uint32_t dst, const CUtensorMap
         : "memory");
 }
 
-// Arrive on a barrier of either CTA of the cluster and add `bytes` to what it expects.
-__device__ __forceinline__ void mbar_arrive_expect_tx_cluster(uint32_t cluster_addr, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.release.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(cluster_addr),
-                 "r"(bytes)
-                 : "memory");
-}
-
-// Polling wait with cluster-scope acquire (bounded as wait_parity).
-__device__ __forceinline__ bool spin_parity_cluster(uint32_t bar, uint32_t parity, uint64_t timeout_ns,
-                                                    volatile int *abort) {
-    auto test = [&]() -> bool {
-        uint32_t ok;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(ok)
-            : "r"(bar), "r"(parity)
-            : "memory");
-        return ok != 0;
-    };
-    if (test()) return true;
-    const uint64_t t0 = global_timer_ns();
-    for (uint32_t i = 1;; i++) {
-        if (test()) return true;
-        if ((i & 63) == 0) {
-            if (*abort) return false;
-            if (global_timer_ns() - t0 > timeout_ns) return false;
-        }
-    }
-}
-
 // 16 lanes x 32 fp32 columns as matrix fragments: with l the lane, r[4i], r[4i+1] hold row
 // l/4 and columns 8i + 2(l%4), +1; r[4i+2], r[4i+3] the same columns of row l/4 + 8.
 __device__ __forceinline__ void tmem_ld_16x256b_x4(uint32_t taddr, uint32_t (&r)[16]) {
