@@ -40,6 +40,7 @@ PRODUCT_UNITS = [("runtime", os.path.join(CSRC, "runtime.cu"), []),
                  ("gemm_pair", os.path.join(CSRC, "gemm_pair.cu"), []),
                  ("gemm_decode", os.path.join(CSRC, "gemm_decode.cu"), []),
                  ("linear", os.path.join(CSRC, "linear.cu"), []),
+                 ("linear_decode", os.path.join(CSRC, "linear_decode.cu"), []),
                  ("linear_grad", os.path.join(CSRC, "linear_grad.cu"), []),
                  ("moe", os.path.join(CSRC, "moe.cu"), []),
                  ("host_pipeline", os.path.join(CSRC, "host_pipeline.cu"), []),

@@ -3,9 +3,10 @@
 //
 // A cluster of two CTAs computes 256 features x up to 256 tokens with
 // tcgen05.mma.cta_group::2 (kind::f16, fp32 accumulators).  Each CTA stages its 128
-// features and its half of the tokens by TMA into a 6-slot ring of 64 reduction elements
-// (32 KB a slot); two accumulators of 256 columns fill the tensor memory, so the epilogue
-// of one tile runs under the MMAs of the next.
+// features and its half of the tokens by TMA into a ring of slots of 64 reduction elements:
+// 6 of 32 KB for 256 tokens, up to 10 for the smaller token tiles, which need more slots in
+// flight to cover the same latency with less work in each.  Two accumulators of 256 columns
+// fill the tensor memory, so the epilogue of one tile runs under the MMAs of the next.
 //
 // Warps: 0 TMA producer, 1 MMA issue (leader CTA) and TMEM owner, 2-9 epilogue, 10 (wgrad)
 // clears the rows past a group's end in its last slot.
@@ -18,19 +19,18 @@
 namespace nvfp4 {
 namespace linear {
 
-constexpr int kStages = 6;
+constexpr int kMaxStages = 12;
+constexpr int kRingBytes = 6 * 2 * kTileBytes;  // p.stages slots of A (16 KB) and B (bt * 64 bytes)
 constexpr int kEpiWarps = 8;
 constexpr int kTailWarp = 2 + kEpiWarps;
 constexpr int kThreads = 32 * (kTailWarp + 1);
 constexpr int kMaxTokens = 256;  // of a tile
 constexpr int kAccCols = 256;
 
-constexpr int kOffA = 0;
-constexpr int kOffB = kOffA + kStages * kTileBytes;
-constexpr int kOffStage = kOffB + kStages * kTileBytes;  // per epilogue warp 2 KB: 32 tokens x 32 features
+constexpr int kOffStage = kRingBytes;  // per epilogue warp 2 KB: 32 tokens x 32 features
 constexpr int kStageWarp = 32 * 64;
 constexpr int kOffBar = kOffStage + kEpiWarps * kStageWarp;
-constexpr int kBarBytes = 256;
+constexpr int kBarBytes = 512;
 constexpr int kOffTables = kOffBar + kBarBytes;
 constexpr int kSmem = kOffTables + 3 * (kMaxGroups + 1) * 4 + 1024;
 static_assert(kSmem <= 232448, "shared memory budget");
@@ -185,17 +185,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t *base_ptr = smem_raw + (base - smem_u32(smem_raw));
-    const uint32_t sA = base + kOffA, sB = base + kOffB;
+    const int n_stages = p.stages;
+    const uint32_t slot = kTileBytes + (uint32_t)p.bt * 64u;  // a slot: A, then B
+    const uint32_t sA = base, sB = base + kTileBytes;
     const uint32_t bar_full = base + kOffBar;            // [stages], leader's used: both CTAs' data
-    const uint32_t bar_empty = bar_full + 8 * kStages;   // [stages]
-    const uint32_t bar_tail = bar_empty + 8 * kStages;   // [stages] wgrad: a group's last slot has landed
-    const uint32_t bar_ready = bar_tail + 8 * kStages;   // [stages] wgrad: that slot is cleared in both CTAs
-    const uint32_t bar_acc_full = bar_ready + 8 * kStages;
+    const uint32_t bar_empty = bar_full + 8 * kMaxStages;   // [stages]
+    const uint32_t bar_tail = bar_empty + 8 * kMaxStages;   // [stages] wgrad: a group's last slot has landed
+    const uint32_t bar_ready = bar_tail + 8 * kMaxStages;   // [stages] wgrad: that slot is cleared in both CTAs
+    const uint32_t bar_acc_full = bar_ready + 8 * kMaxStages;
     const uint32_t bar_acc_empty = bar_acc_full + 16;
     const uint32_t bar_drain = bar_acc_empty + 16;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(base_ptr + kOffBar + (4 * kStages + 5) * 8);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(base_ptr + kOffBar + (4 * kMaxStages + 5) * 8);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
-    static_assert((4 * kStages + 5) * 8 + 8 <= kBarBytes, "barrier region");
+    static_assert((4 * kMaxStages + 5) * 8 + 8 <= kBarBytes, "barrier region");
     int *g_r0 = reinterpret_cast<int *>(base_ptr + kOffTables);
     int *g_r1 = g_r0 + kMaxGroups + 1;
     int *g_t0 = g_r1 + kMaxGroups + 1;
@@ -206,7 +208,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const int n_f = (p.features + 255) / 256;
     const int n_c = FORM == kWgrad ? (p.out_cols + p.bt - 1) / p.bt : 0;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kStages; s++) {
+        for (int s = 0; s < n_stages; s++) {
             mbar_init(bar_full + 8 * s, 1);
             mbar_init(bar_empty + 8 * s, 1);
             mbar_init(bar_tail + 8 * s, 1);
@@ -303,7 +305,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                         issued_mask |= 1u << stage;
                         issued_parity = (issued_parity & ~(1u << stage)) | (phase << stage);
                     }
-                    const uint32_t dA = sA + stage * kTileBytes, dB = sB + stage * kTileBytes;
+                    const uint32_t dA = sA + stage * slot, dB = sB + stage * slot;
                     const int k0 = kb * kBlockK;
                     if constexpr (FORM == kForward) {
                         tma_load_3d_pair(dA, &tmap_a, bar, k0, f0, ti.group);
@@ -318,7 +320,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                         for (int c = 0; c < p.bt / 2; c += 64)
                             tma_load_2d_pair(dB + c * 128, &tmap_b, bar, b0 + c, ti.row0 + k0);
                     }
-                    if (++stage == kStages) {
+                    if (++stage == (uint32_t)n_stages) {
                         stage = 0;
                         phase ^= 1;
                     }
@@ -327,7 +329,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             grid_launch_dependents();
             if (!ok) {  // let the copies in flight land before the memory goes
                 volatile int never = 0;
-                for (int s = 0; s < kStages; s++) {
+                for (int s = 0; s < n_stages; s++) {
                     if (rank == 0 && (issued_mask & (1u << s)))
                         wait_parity(bar_full + 8 * s, (issued_parity >> s) & 1, p.ctl.drain_timeout_ns, &never);
                     if (tail_mask & (1u << s))
@@ -369,8 +371,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                         break;
                     }
                     tc_fence_after();
-                    const uint64_t a = a_desc + (uint64_t)(stage * (kTileBytes >> 4));
-                    const uint64_t b = b_desc + (uint64_t)(stage * (kTileBytes >> 4));
+                    const uint64_t a = a_desc + (uint64_t)(stage * (slot >> 4));
+                    const uint64_t b = b_desc + (uint64_t)(stage * (slot >> 4));
                     any = true;
                     if ((kb + 1) * kBlockK <= red) {
 #pragma unroll
@@ -385,7 +387,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     }
                     mma_commit_pair(empty0 + 8 * stage);
                     mma_commit_pair(empty1 + 8 * stage);
-                    if (++stage == kStages) {
+                    if (++stage == (uint32_t)n_stages) {
                         stage = 0;
                         phase ^= 1;
                     }
@@ -411,7 +413,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 const Tile ti = tile_at(t);
                 slots += (uint32_t)blocks_of(ti);
                 if (!dirty_tail(ti)) continue;
-                const uint32_t stage = (slots - 1) % kStages;
+                const uint32_t stage = (slots - 1) % (uint32_t)n_stages;
                 if (!wait_parity(bar_tail + 8 * stage, (parity >> stage) & 1, tmo, abort_flag)) {
                     if (lane == 0) report_timeout(abort_flag, p.ctl.status);
                     ok = false;
@@ -421,7 +423,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 const int valid = (ti.rows - 1) % kBlockK + 1, end = (valid + 15) & ~15;
                 const int per = (end - valid) * 8;  // 16-byte pieces of one 64-column chunk
                 for (int i = lane; i < per; i += 32) {
-                    const uint32_t at = (uint32_t)(valid * 128 + i * 16) + stage * kTileBytes;
+                    const uint32_t at = (uint32_t)(valid * 128 + i * 16) + stage * slot;
                     st_shared_v4(sA + at, 0u, 0u, 0u, 0u);
                     st_shared_v4(sA + 8192 + at, 0u, 0u, 0u, 0u);
                     for (int c = 0; c < p.bt / 2; c += 64) st_shared_v4(sB + c * 128 + at, 0u, 0u, 0u, 0u);
@@ -531,30 +533,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 }
 
 // ------------------------------------------------------------------------- host side
-template <typename T>
-static constexpr CUtensorMapDataType tma_type() {
-    return std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-}
-
-// [rows, cols] with a row pitch, as boxes of 64 columns (one swizzle row) by box_rows.
-template <typename T>
-static int map_rows(CUtensorMap *m, const void *base, int64_t rows, int cols, int64_t pitch, int box_rows) {
-    const uint64_t dims[2] = {(uint64_t)cols, (uint64_t)rows}, strides[1] = {(uint64_t)pitch * 2};
-    const uint32_t box[2] = {64, (uint32_t)box_rows};
-    return encode_tiled(m, tma_type<T>(), 2, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
-}
-
-// The weight [groups, N, K].
-template <typename T>
-static int map_weight(CUtensorMap *m, const void *base, int groups, int N, int K, int box_rows) {
-    const uint64_t dims[3] = {(uint64_t)K, (uint64_t)N, (uint64_t)groups};
-    const uint64_t strides[2] = {(uint64_t)K * 2, (uint64_t)N * (uint64_t)K * 2};
-    const uint32_t box[3] = {64, (uint32_t)box_rows, 1};
-    return encode_tiled(m, tma_type<T>(), 3, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
-}
-
 template <typename T, int FORM>
-static int launch_pair(const CUtensorMap &a, const CUtensorMap &b, const Params &p, int64_t tiles, const DeviceInfo &di,
+static int launch_pair(const CUtensorMap &a, const CUtensorMap &b, Params p, int64_t tiles, const DeviceInfo &di,
                        cudaStream_t stream) {
     auto kern = linear_pair_kernel<T, FORM>;
     static int configured[64] = {};
@@ -564,6 +544,7 @@ static int launch_pair(const CUtensorMap &a, const CUtensorMap &b, const Params 
         configured[di.device] = 1;
     }
     if (tiles > INT_MAX) return NVFP4_ERR_SHAPE;
+    p.stages = std::min(kMaxStages, kRingBytes / (kTileBytes + p.bt * 64));
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -579,20 +560,53 @@ static int launch_pair(const CUtensorMap &a, const CUtensorMap &b, const Params 
     return cuda_status(cudaGetLastError());
 }
 
-// Tokens of a tile.
+// Tokens of a tile.  A slot of 64 reduction elements costs a pair about 150 ns for its 256
+// features plus 1.07 ns a token (measured from 32 to 256 tokens, N = K = 4096), so few wide
+// tiles win, unless their number fills the last wave of pairs badly.
+//   dense: the M tokens in n equal tiles, n chosen by waves x cost;
+//   groups (their rows are known on the device only): up to twice the mean rows, so that
+//   most groups are one tile or 256-token tiles; a tile's MMAs follow its own rows.
 static int token_tile(int64_t m, int groups, int n_f, int pairs) {
-    (void)groups;
-    (void)n_f;
-    (void)pairs;
-    int bt = 32;
-    while (bt < kMaxTokens && bt < m) bt *= 2;
-    return bt;
+    if (groups > 1) {
+        int bt = 32;
+        while (bt < kMaxTokens && (int64_t)bt * groups < 2 * m) bt *= 2;
+        return bt;
+    }
+    int best = kMaxTokens;
+    double least = 1e300;
+    const int64_t n0 = (m + kMaxTokens - 1) / kMaxTokens;
+    for (int64_t n = n0; n <= 4 * n0; n++) {
+        const int bt = (int)(((m + n - 1) / n + 31) / 32 * 32);
+        const int64_t tiles = (m + bt - 1) / bt * n_f, waves = (tiles + pairs - 1) / pairs;
+        const double cost = (double)waves * (150.0 + 1.07 * bt);
+        if (cost < least) {
+            least = cost;
+            best = bt;
+        }
+    }
+    return best;
+}
+
+// Whether the split-reduction kernel takes a forward call (at most kDecodeTokens rows).  It
+// wins where 256-feature tiles are too few to stream the weights on every SM; with enough
+// of them the persistent kernel does, without a reduction between CTAs.  Measured (us, this
+// kernel / persistent): N=4096 K=4096 M=1 10.7/16.0, M=64 16.3/16.5, M=128 23.7/17.7;
+// N=4096 K=14336 M=64 28.5/44.4, M=128 36.9/48.0; N=14336 K=4096 M=1 21.8/23.4, M=64
+// 25.1/24.4; N=28672 K=8192 M=1 74.0/76.4, M=64 83.3/81.5; 8 experts N=28672 K=4096, 32 rows
+// 295/280.
+static bool use_decode(int m, int groups, int n_f, int K) {
+    if (m > kDecodeTokens) return false;
+    const int64_t tiles = (int64_t)n_f * std::min(groups, m);
+    if (m <= 32) return tiles <= 128;
+    if (m <= 64) return tiles <= 37;
+    return tiles <= 18 && K >= 8192;
 }
 
 template <typename T>
 static int forward_t(const void *X, int64_t ldx, const void *W, Params p, int K, const DeviceInfo &di,
                      cudaStream_t s) {
     const int n_f = (p.features + 255) / 256;
+    if (use_decode(p.m_total, p.groups, n_f, K)) return decode_forward<T>(X, ldx, W, p, K, di, s);
     p.bt = token_tile(p.m_total, p.groups, n_f, di.sm_count / 2);
     p.strip = 8;
     p.red = K;

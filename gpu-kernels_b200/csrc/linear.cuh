@@ -7,6 +7,7 @@
 // orientation streams the weights for a single token.
 #pragma once
 #include <cmath>
+#include <type_traits>
 
 #include "common.cuh"
 #include "epilogue.cuh"
@@ -41,7 +42,7 @@ struct Params {
     int strip;             // feature tiles that sweep the tokens together (L2 reuse)
     int act;
     int splits;            // decode: CTAs that share a tile's reduction
-    int stages;            // decode: ring slots
+    int stages;            // ring slots
     int ncap;              // decode: token rows of a ring slot
     KernelCtl ctl;
 };
@@ -93,12 +94,12 @@ __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap
         "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(z), "r"(bar_cluster)
         : "memory");
 }
-__device__ __forceinline__ void tma_load_3d_hint(uint32_t dst, const CUtensorMap *tmap, uint32_t bar, int32_t x,
-                                                 int32_t y, int32_t z, uint64_t policy) {
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *tmap, uint32_t bar, int32_t x, int32_t y,
+                                            int32_t z) {
     asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
-        " [%0], [%1, {%2, %3, %4}], [%5], %6;" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(z), "r"(bar), "l"(policy)
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(z), "r"(bar)
         : "memory");
 }
 
@@ -198,6 +199,34 @@ __device__ __forceinline__ void build_tables(const int *m_offsets, int G, int m_
     }
     if (lane == 0) t0[0] = 0;
 }
+
+// ------------------------------------------------------------------------- host side
+template <typename T>
+constexpr CUtensorMapDataType tma_type() {
+    return std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+}
+
+// [rows, cols] with a row pitch, as boxes of 64 columns (one swizzle row) by box_rows.
+template <typename T>
+inline int map_rows(CUtensorMap *m, const void *base, int64_t rows, int cols, int64_t pitch, int box_rows) {
+    const uint64_t dims[2] = {(uint64_t)cols, (uint64_t)rows}, strides[1] = {(uint64_t)pitch * 2};
+    const uint32_t box[2] = {64, (uint32_t)box_rows};
+    return encode_tiled(m, tma_type<T>(), 2, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+// The weight [groups, N, K].
+template <typename T>
+inline int map_weight(CUtensorMap *m, const void *base, int groups, int N, int K, int box_rows) {
+    const uint64_t dims[3] = {(uint64_t)K, (uint64_t)N, (uint64_t)groups};
+    const uint64_t strides[2] = {(uint64_t)K * 2, (uint64_t)N * (uint64_t)K * 2};
+    const uint32_t box[3] = {64, (uint32_t)box_rows, 1};
+    return encode_tiled(m, tma_type<T>(), 3, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+// linear_decode.cu: the forward product for at most kDecodeTokens token rows in all.
+constexpr int kDecodeTokens = 128;
+template <typename T>
+int decode_forward(const void *X, int64_t ldx, const void *W, Params p, int K, const DeviceInfo &di, cudaStream_t s);
 
 }  // namespace linear
 }  // namespace nvfp4

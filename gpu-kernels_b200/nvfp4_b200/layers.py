@@ -16,17 +16,22 @@ from ._lib import ACTIVATIONS, check, lib
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_device = torch._C._cuda_getDevice
+_entries = {}  # entry points by name, bound on their first call
 
 
 def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
-def call(name: str, device: torch.device, *args) -> None:
-    """One entry point on `device`'s current stream (the last argument of each of them)."""
-    index = device.index
-    fn = getattr(lib(), name)
-    if index == torch.cuda.current_device():
+def call(name: str, index: int, *args) -> None:
+    """One entry point on the current stream of CUDA device `index` (the stream is the last
+    argument of each of them).  A decode step is a few microseconds of GPU time a call, so
+    the path from here to the launch is kept short."""
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(lib(), name)
+    if index == _device():
         status = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
@@ -35,45 +40,44 @@ def call(name: str, device: torch.device, *args) -> None:
         check(status, name)
 
 
-def _need(ok: bool, what: str) -> None:
-    if not ok:
-        raise ValueError(what)
-
-
 def _matrix(t: torch.Tensor, name: str, shape, like: torch.Tensor) -> torch.Tensor:
     """A contiguous CUDA tensor of this shape, of `like`'s type and device."""
-    if t.dtype != like.dtype or t.device != like.device or t.shape != shape or not t.is_contiguous():
+    if t.dtype != like.dtype or t.get_device() != like.get_device() or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {like.dtype} tensor {tuple(shape)} on {like.device}")
     return t
 
 
 def _rows(x: torch.Tensor, name: str) -> Tuple[int, int, int]:
     """(rows, columns, row pitch) of a 2-D 16-bit CUDA tensor whose rows are contiguous."""
-    if not x.is_cuda or x.dim() != 2 or x.dtype not in (torch.bfloat16, torch.float16):
+    if not x.is_cuda or x.ndim != 2 or _DTYPES.get(x.dtype, 2) == 2:
         raise ValueError(f"{name} must be a 2-D bf16 or fp16 CUDA tensor")
     M, K = x.shape
-    pitch = x.stride(0) if M > 1 else max(K, x.stride(0))
-    if (K > 1 and x.stride(1) != 1) or pitch < K:
-        raise ValueError(f"{name} must have contiguous rows")
-    if K % 8 or pitch % 8:
+    if x.is_contiguous():
+        pitch = K
+    else:
+        pitch, unit = x.stride()
+        if M <= 1:
+            pitch = max(K, pitch)
+        if (K > 1 and unit != 1) or pitch < K:
+            raise ValueError(f"{name} must have contiguous rows")
+    if K % 8 or pitch % 8 or not K:
         raise ValueError(f"{name} must have a multiple of 8 columns, rows 16 bytes aligned")
     return M, K, pitch
 
 
 def _weight(w: torch.Tensor, groups: int, K: int, x: torch.Tensor) -> int:
     """Rows N of one group's weight."""
-    if w.dim() != 2 or w.shape[1] != K or w.shape[0] % groups:
+    if w.ndim != 2 or w.shape[1] != K or w.shape[0] % groups:
         raise ValueError(f"w must be [{'groups * ' if groups > 1 else ''}N, {K}]")
-    _matrix(w, "w", w.shape, x)
-    N = w.shape[0] // groups
+    N = _matrix(w, "w", w.shape, x).shape[0] // groups
     if N % 8 or not N:
         raise ValueError("N must be a multiple of 8")
     return N
 
 
 def _offsets(m_offsets: torch.Tensor, x: torch.Tensor) -> int:
-    if m_offsets.dtype != torch.int32 or m_offsets.dim() != 1 or m_offsets.numel() < 2 or \
-            m_offsets.device != x.device or not m_offsets.is_contiguous():
+    if m_offsets.dtype != torch.int32 or m_offsets.ndim != 1 or m_offsets.numel() < 2 or \
+            m_offsets.get_device() != x.get_device() or not m_offsets.is_contiguous():
         raise ValueError("m_offsets must be a contiguous 1-D int32 tensor of groups + 1 entries on the device")
     if m_offsets.numel() > 257:
         raise ValueError("at most 256 groups")
@@ -97,12 +101,12 @@ def _forward(x, w, m_offsets, bias, activation, residual, out, return_preact):
     N = _weight(w, G, K, x)
     act, No = _activation(activation, N)
     if bias is not None:
-        _matrix(bias, "bias", (N,) if bias.dim() == 1 and G == 1 else (G, N), x)
+        _matrix(bias, "bias", (N,) if bias.ndim == 1 and G == 1 else (G, N), x)
     if residual is not None:
         _matrix(residual, "residual", (M, No), x)
     y = x.new_empty((M, No)) if out is None else _matrix(out, "out", (M, No), x)
     z = x.new_empty((M, N)) if return_preact else None
-    call("nvfp4_linear", x.device, x.data_ptr(), pitch, w.data_ptr(), _ptr(bias), _ptr(residual), y.data_ptr(),
+    call("nvfp4_linear", x.get_device(), x.data_ptr(), pitch, w.data_ptr(), _ptr(bias), _ptr(residual), y.data_ptr(),
          _ptr(z), _ptr(m_offsets), G, M, N, K, act, _DTYPES[x.dtype])
     return (y, z) if return_preact else y
 
@@ -136,16 +140,17 @@ def _backward(dy, x, w, m_offsets, preact, activation, bias_grad):
     act, No = _activation(activation, N)
     _matrix(dy, "dy", (M, No), x)
     if act:
-        _need(preact is not None, "an activation's gradient needs preact")
+        if preact is None:
+            raise ValueError("an activation's gradient needs preact")
         _matrix(preact, "preact", (M, N), x)
-    dtype, dev, offs = _DTYPES[x.dtype], x.device, _ptr(m_offsets)
+    dtype, dev, offs = _DTYPES[x.dtype], x.get_device(), _ptr(m_offsets)
     dz = x.new_empty((M, N)) if act else dy
     db = ws = None
     ws_bytes = 0
     if bias_grad:
         db = x.new_empty((N,) if m_offsets is None else (G, N))
         ws_bytes = lib().nvfp4_activation_backward_workspace_size(G, M, N)
-        ws = torch.empty(ws_bytes // 4, dtype=torch.float32, device=dev)
+        ws = x.new_empty(ws_bytes // 4, dtype=torch.float32)
     if act or bias_grad:
         call("nvfp4_activation_backward", dev, dy.data_ptr(), _ptr(preact) if act else None,
              dz.data_ptr() if act else None, _ptr(db), offs, G, M, N, act, dtype, _ptr(ws), ws_bytes)
