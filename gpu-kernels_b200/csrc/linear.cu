@@ -482,23 +482,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 const int f = feat0 + lane;
                 T *out = static_cast<T *>(p.y) + ((int64_t)ti.group * p.features + f) * p.out_cols + ti.col * p.bt;
                 const int cols = min(p.bt, p.out_cols - ti.col * p.bt);
+                // whole 32-byte sectors where the rows allow it
+                const bool wide = p.out_cols % 16 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 31u) == 0;
                 for (int c = half * 32; c < cols; c += 64) {
                     uint32_t r[32];
                     tmem_ld_32x32b_x32(acc + c, r);
                     tmem_ld_wait();
                     if (f >= p.features) continue;
+                    uint32_t v[16];
 #pragma unroll
-                    for (int q = 0; q < 4; q++) {
-                        if (c + q * 8 >= cols) continue;
-                        uint4 v = make_uint4(0u, 0u, 0u, 0u);  // a group without rows: its gradient is zero
-                        if (ti.rows > 0) {
-                            const uint32_t *s = r + q * 8;
-                            auto pk = [&](int i) {
-                                return Type16<T>::pack(__uint_as_float(s[i]), __uint_as_float(s[i + 1]));
-                            };
-                            v = make_uint4(pk(0), pk(2), pk(4), pk(6));
-                        }
-                        *reinterpret_cast<uint4 *>(out + c + q * 8) = v;
+                    for (int i = 0; i < 16; i++)  // a group without rows: its gradient is zero
+                        v[i] = ti.rows > 0 ? Type16<T>::pack(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])) : 0u;
+                    if (wide) {
+#pragma unroll
+                        for (int q = 0; q < 2; q++)
+                            if (c + q * 16 < cols)
+                                st_global_v8(out + c + q * 16, *reinterpret_cast<uint32_t(*)[8]>(&v[q * 8]));
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < 4; q++)
+                            if (c + q * 8 < cols)
+                                *reinterpret_cast<uint4 *>(out + c + q * 8) =
+                                    make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
                     }
                 }
             }

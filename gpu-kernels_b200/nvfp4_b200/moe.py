@@ -56,7 +56,7 @@ def moe_route(logits: torch.Tensor, top_k: int, scoring: str = "softmax", bias: 
     experts, rows = logits.new_empty((2, T, top_k), dtype=torch.int32).unbind(0)
     m_offsets = logits.new_empty(E + 1, dtype=torch.int32)
     ws, ws_bytes = None, 0
-    if T > 128:
+    if T > 64:
         ws_bytes = lib().nvfp4_moe_route_workspace_size(T, E)
         ws = logits.new_empty(ws_bytes // 4, dtype=torch.int32)
     call("nvfp4_moe_route", logits.get_device(), logits.data_ptr(), _DTYPES[logits.dtype], _ptr(bias), T, E, top_k, score,

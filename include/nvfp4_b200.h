@@ -386,7 +386,7 @@ NVFP4_API int nvfp4_activation_backward(const void *dY, const void *Z, void *dZ,
  *   rows int32 [T, top_k]: the row of each choice in expert order (by expert, then token),
  *   -1 for none.
  * T <= 2^20, E <= 256, top_k <= min(E, 32).  The workspace
- * (nvfp4_moe_route_workspace_size) is needed for T > 128 only.
+ * (nvfp4_moe_route_workspace_size) is needed for T > 64 only.
  */
 enum { NVFP4_SCORE_SOFTMAX = 0, NVFP4_SCORE_SIGMOID = 1 };
 NVFP4_API size_t nvfp4_moe_route_workspace_size(int T, int E);

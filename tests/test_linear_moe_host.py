@@ -63,7 +63,7 @@ def test_route_refusals(nv, args, status):
 
 def test_move_refusals(nv):
     L = nv.lib()
-    assert L.nvfp4_moe_route_workspace_size(129, 8) == 64 and L.nvfp4_moe_route_workspace_size(5, 0) == 0
+    assert L.nvfp4_moe_route_workspace_size(129, 8) >= 64 and L.nvfp4_moe_route_workspace_size(5, 0) == 0
     assert L.nvfp4_moe_dispatch(None, P, P, 4, 8, 2, 64, P, None) == INVALID
     assert L.nvfp4_moe_dispatch(P, P, P, 4, 8, 2, 60, P, None) == SHAPE
     assert L.nvfp4_moe_dispatch(P, P, P, 4, 8, 33, 64, P, None) == SHAPE
