@@ -1,5 +1,5 @@
-"""Build libnvfp4_b200.so (the product), libnvfp4_diag.so (its diagnostic twin) and
-the runner executable in-tree for sm_100a.
+"""Build libnvfp4_b200.so (the product), libnvfp4_diag.so (its diagnostic twin), the
+runner executable and the torch binding of the 16-bit operators in-tree for sm_100a.
 
     python gpu-kernels_b200/build.py [--force] [-v]
 
@@ -27,6 +27,8 @@ OBJ = os.path.join(HERE, "_build")
 OUT = os.path.join(HERE, "nvfp4_b200", "libnvfp4_b200.so")
 DIAG_OUT = os.path.join(HERE, "nvfp4_diag", "libnvfp4_diag.so")
 RUNNER = os.path.join(HERE, "nvfp4_b200", "nvfp4_runner")
+BIND = os.path.join(HERE, "nvfp4_b200", "_torch_bind.so")
+BIND_SRC = os.path.join(CSRC, "torch_bind.cpp")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 CFLAGS = ARCH + ["-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
@@ -60,7 +62,8 @@ def _headers():
 
 
 def _inputs():
-    return _headers() + [src for _, src, _ in PRODUCT_UNITS + DIAG_UNITS] + [os.path.join(CSRC, "runner_main.cu")]
+    return _headers() + [src for _, src, _ in PRODUCT_UNITS + DIAG_UNITS] + [os.path.join(CSRC, "runner_main.cu"),
+                                                                             BIND_SRC]
 
 
 def _obj(name):
@@ -87,10 +90,29 @@ def _link(out, objs):
     os.replace(out + ".tmp", out)
 
 
+def _build_bind(force):
+    """The CPython extension of the torch-facing operators (host code only, g++)."""
+    newest = max(os.path.getmtime(f) for f in (BIND_SRC, os.path.join(INCLUDE, "nvfp4_b200.h"), os.path.abspath(__file__)))
+    if not force and os.path.exists(BIND) and os.path.getmtime(BIND) >= newest:
+        return
+    import sysconfig
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+    libs = library_paths()
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++20", "-fPIC", "-shared", "-fvisibility=hidden", "-w",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *[f"-I{d}" for d in include_paths() + [sysconfig.get_paths()["include"],
+                                                  os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include")]],
+           BIND_SRC, "-o", BIND + ".tmp", *[f"-L{d}" for d in libs], *[f"-Wl,-rpath,{d}" for d in libs],
+           "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-ltorch", "-lc10_cuda", "-lc10"]
+    subprocess.check_call(cmd)
+    os.replace(BIND + ".tmp", BIND)
+
+
 def build(force: bool = False, verbose: bool = False, jobs: int = 0) -> str:
-    """Build both libraries and the runner executable (which links the product library
-    from its own directory); returns the product library's path."""
-    outs = (OUT, DIAG_OUT, RUNNER)
+    """Build both libraries, the runner executable (which links the product library from its
+    own directory) and the torch binding; returns the product library's path."""
+    outs = (OUT, DIAG_OUT, RUNNER, BIND)
     if not force and all(os.path.exists(p) for p in outs):
         if min(os.path.getmtime(p) for p in outs) >= max(os.path.getmtime(f) for f in _inputs()):
             return OUT
@@ -100,7 +122,9 @@ def build(force: bool = False, verbose: bool = False, jobs: int = 0) -> str:
     # longest units first: the decode instantiations and the CTA-pair kernel dominate
     order = sorted(units, key=lambda u: (not u[0].startswith(("decode_inst", "gemm_pair")), u[0]))
     with ThreadPoolExecutor(max_workers=jobs or max(1, os.cpu_count() or 1)) as ex:
+        bind = ex.submit(_build_bind, force)
         list(ex.map(lambda u: _compile(u, force, hm, verbose), order))
+        bind.result()
     product = [_obj(n) for n, _, _ in PRODUCT_UNITS]
     _link(OUT, product)
     _link(DIAG_OUT, [o for o in product if not o.endswith("/gemm_pair.o")] + [_obj(n) for n, _, _ in DIAG_UNITS])

@@ -25,7 +25,6 @@ class Epilogue(C.Structure):
 
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu_tanh": 3, "swiglu": 4}
 
-DTYPES = {"bf16": 0, "f16": 1, "f32": 2}
 SCORES = {"softmax": 0, "sigmoid": 1}
 
 SIGNATURES = {
