@@ -6,13 +6,14 @@
 // features and its half of the tokens by TMA into a ring of slots of 64 reduction elements:
 // 6 of 32 KB for 256 tokens, up to 10 for the smaller token tiles, which need more slots in
 // flight to cover the same latency with less work in each.  Two accumulators of 256 columns
-// fill the tensor memory, so the epilogue of one tile runs under the MMAs of the next.
+// fill the tensor memory, so the epilogue of one tile runs under the MMAs of the next; or,
+// for "wide" tiles, one tile of up to 512 tokens uses both: each A tile is then read once for
+// twice the tokens, which pays where there is only one round of tiles to run anyway.
 //
 // Warps: 0 TMA producer, 1 MMA issue (leader CTA) and TMEM owner, 2-9 epilogue, 10 (wgrad)
 // clears the rows past a group's end in its last slot.
 #include <algorithm>
 #include <climits>
-#include <cstdlib>
 
 #include "linear.cuh"
 
@@ -27,6 +28,7 @@ constexpr int kThreads = 32 * (kTailWarp + 1);
 constexpr int kMaxTokens = 256;  // of a tile
 constexpr int kAccCols = 256;
 
+constexpr int kBox = 32 * 64;  // wgrad: 32 rows x 32 columns; two a warp, one of them in what the ring leaves
 constexpr int kOffStage = kRingBytes;  // per epilogue warp 2 KB: 32 tokens x 32 features
 constexpr int kStageWarp = 32 * 64;
 constexpr int kOffBar = kOffStage + kEpiWarps * kStageWarp;
@@ -177,16 +179,30 @@ __device__ __forceinline__ void store_piece(const Params &p, uint32_t (&ra)[16],
 }
 
 template <typename T, int FORM>
+__device__ __forceinline__ void store_act(const Params &p, uint32_t (&ra)[16], uint32_t (&rb)[16], uint32_t stage,
+                                          const float (&bias)[4], int row0, int n_rows, int feat0, int lane) {
+    switch (FORM == kForward ? p.act : (int)kActNone) {
+        case kActRelu: store_piece<T, kActRelu>(p, ra, rb, stage, bias, row0, n_rows, feat0, lane); break;
+        case kActSilu: store_piece<T, kActSilu>(p, ra, rb, stage, bias, row0, n_rows, feat0, lane); break;
+        case kActGeluTanh: store_piece<T, kActGeluTanh>(p, ra, rb, stage, bias, row0, n_rows, feat0, lane); break;
+        case kActSwiglu: store_piece<T, kActSwiglu>(p, ra, rb, stage, bias, row0, n_rows, feat0, lane); break;
+        default: store_piece<T, kActNone>(p, ra, rb, stage, bias, row0, n_rows, feat0, lane);
+    }
+}
+
+template <typename T, int FORM>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
-                       const Params p) {
+                       const __grid_constant__ CUtensorMap tmap_d, const Params p) {
     constexpr bool kAmn = FORM != kForward, kBmn = FORM == kWgrad;
     constexpr bool kBf16 = sizeof(T) == 2 && !std::is_same<T, __half>::value;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t *base_ptr = smem_raw + (base - smem_u32(smem_raw));
     const int n_stages = p.stages;
-    const uint32_t slot = kTileBytes + (uint32_t)p.bt * 64u;  // a slot: A, then B
+    const int subs_max = FORM == kWgrad ? 1 : 1 + p.wide, tile_tokens = p.bt * subs_max;
+    const uint32_t sub_bytes = (uint32_t)p.bt * 64u;  // this CTA's half of bt tokens
+    const uint32_t slot = kTileBytes + sub_bytes * subs_max;  // a slot: A, then B
     const uint32_t sA = base, sB = base + kTileBytes;
     const uint32_t bar_full = base + kOffBar;            // [stages], leader's used: both CTAs' data
     const uint32_t bar_empty = bar_full + 8 * kMaxStages;   // [stages]
@@ -230,7 +246,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
     grid_dependency_wait();  // nothing of global memory is read or written before this
     if (warp == 2)
-        build_tables(p.m_offsets, p.groups, p.m_total, FORM == kWgrad ? 0 : p.bt, FORM == kWgrad ? n_f * n_c : n_f,
+        build_tables(p.m_offsets, p.groups, p.m_total, FORM == kWgrad ? 0 : tile_tokens, FORM == kWgrad ? n_f * n_c : n_f,
                      lane, g_r0, g_r1, g_t0);
     tc_fence_before();
     cluster_sync();
@@ -250,23 +266,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
         ti.group = lo;
         const int r0 = g_r0[lo], n = g_r1[lo] - r0;
-        const int others = FORM == kWgrad ? n_c : (n + p.bt - 1) / p.bt;
+        const int others = FORM == kWgrad ? n_c : (n + tile_tokens - 1) / tile_tokens;
         const int local = t - g_t0[lo], per_strip = p.strip * others;
         const int s = local / per_strip, f0 = s * p.strip, fs = min(p.strip, n_f - f0), rem = local - s * per_strip;
-        ti.f = f0 + rem % fs;
-        const int o = rem / fs;
-        ti.col = o;
-        ti.row0 = FORM == kWgrad ? r0 : r0 + o * p.bt;
-        ti.rows = FORM == kWgrad ? n : min(p.bt, n - o * p.bt);
+        if (FORM == kWgrad) {  // the columns fastest: 2-3 % faster than the features at 4096 x 14336 x 4096
+            ti.col = rem % others;
+            ti.f = f0 + rem / others;
+            ti.row0 = r0;
+            ti.rows = n;
+        } else {
+            const int o = rem / fs;
+            ti.col = 0;
+            ti.f = f0 + rem % fs;
+            ti.row0 = r0 + o * tile_tokens;
+            ti.rows = min(tile_tokens, n - o * tile_tokens);
+        }
         return ti;
     };
     auto blocks_of = [&](const Tile &ti) {
         return ((FORM == kWgrad ? ti.rows : p.red) + kBlockK - 1) / kBlockK;
     };
-    // MMA columns of a tile: its tokens, rounded up to the instruction's step of 16 (each
-    // CTA holds half of them); the rounding's rows are loaded but never stored.
-    auto width_of = [&](const Tile &ti) { return FORM == kWgrad ? p.bt : (ti.rows + 15) & ~15; };
-    const uint32_t tx_bytes = kTileBytes + (p.bt / 2) * 128;
+    // Parts of a tile (two for a wide one with more than bt tokens), the tokens of each, and
+    // its MMA columns: the tokens rounded up to the instruction's step of 16 (each CTA holds
+    // half of them); the rounding's rows are loaded but never stored.
+    auto subs_of = [&](const Tile &ti) { return FORM != kWgrad && ti.rows > p.bt ? 2 : 1; };
+    auto sub_rows = [&](const Tile &ti, int s) { return s ? ti.rows - p.bt : min(ti.rows, p.bt); };
+    auto width_of = [&](const Tile &ti, int s) { return FORM == kWgrad ? p.bt : (sub_rows(ti, s) + 15) & ~15; };
     // wgrad: reduction rows past the group's end belong to the next group; the last slot's
     // are cleared unless the MMA's 16-row steps end exactly with the group
     auto dirty_tail = [&](const Tile &ti) { return FORM == kWgrad && (ti.rows & 15) != 0; };
@@ -283,7 +308,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 const int nkb = blocks_of(ti);
                 const int f0 = ti.f * 256 + (int)rank * 128;
                 const int b0 = FORM == kWgrad ? ti.col * p.bt + (int)rank * (p.bt / 2)
-                                              : ti.row0 + (int)rank * (width_of(ti) / 2);
+                                              : ti.row0 + (int)rank * (width_of(ti, 0) / 2);
+                const int subs = subs_of(ti);
+                const int b1 = subs == 2 ? ti.row0 + p.bt + (int)rank * (width_of(ti, 1) / 2) : 0;
+                const uint32_t tx_bytes = kTileBytes + sub_bytes * subs;
                 for (int kb = 0; kb < nkb; kb++) {
                     if (!wait_parity(bar_empty + 8 * stage, phase ^ 1, tmo, abort_flag)) {
                         report_timeout(abort_flag, p.ctl.status);
@@ -310,10 +338,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     if constexpr (FORM == kForward) {
                         tma_load_3d_pair(dA, &tmap_a, bar, k0, f0, ti.group);
                         tma_load_2d_pair(dB, &tmap_b, bar, k0, b0);
+                        if (subs == 2) tma_load_2d_pair(dB + sub_bytes, &tmap_b, bar, k0, b1);
                     } else if constexpr (FORM == kDgrad) {
                         tma_load_3d_pair(dA, &tmap_a, bar, f0, k0, ti.group);
                         tma_load_3d_pair(dA + 8192, &tmap_a, bar, f0 + 64, k0, ti.group);
                         tma_load_2d_pair(dB, &tmap_b, bar, k0, b0);
+                        if (subs == 2) tma_load_2d_pair(dB + sub_bytes, &tmap_b, bar, k0, b1);
                     } else {
                         tma_load_2d_pair(dA, &tmap_a, bar, f0, ti.row0 + k0);
                         tma_load_2d_pair(dA + 8192, &tmap_a, bar, f0 + 64, ti.row0 + k0);
@@ -344,20 +374,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             const uint32_t accf0 = map_to_cta(bar_acc_full, 0), accf1 = map_to_cta(bar_acc_full, 1);
             const uint64_t a_desc = operand_desc<kAmn>(sA), b_desc = operand_desc<kBmn>(sB);
             uint32_t stage = 0, phase = 0, ready_parity = 0;
-            int local = 0;
+            int local = 0;  // accumulators handed over so far: buffer local & 1, its use local / 2
             bool ok = true, any = false;
-            for (int t = pair; ok && t < n_tiles; t += num_pairs, local++) {
+            for (int t = pair; ok && t < n_tiles; t += num_pairs) {
                 const Tile ti = tile_at(t);
-                const int nkb = blocks_of(ti);
-                const uint32_t idesc = idesc_f16(kBf16, kAmn, kBmn, 256, (uint32_t)width_of(ti));
-                const uint32_t buf = local & 1, use = local >> 1;
-                const uint32_t d_tmem = tmem_base + buf * kAccCols;
-                if (!spin_parity(bar_acc_empty + 8 * buf, (use & 1) ^ 1, tmo, abort_flag)) {
-                    report_timeout(abort_flag, p.ctl.status);
-                    ok = false;
-                    break;
-                }
+                const int nkb = blocks_of(ti), subs = subs_of(ti);
+                // a wide launch uses both accumulators in every tile
+                for (int s = 0; s < subs_max && ok; s++)
+                    if (!spin_parity(bar_acc_empty + 8 * ((local + s) & 1), (((local + s) >> 1) & 1) ^ 1, tmo,
+                                     abort_flag)) {
+                        report_timeout(abort_flag, p.ctl.status);
+                        ok = false;
+                    }
+                if (!ok) break;
                 tc_fence_after();
+                const uint32_t d0 = tmem_base + (local & 1) * kAccCols, d1 = tmem_base + kAccCols;
+                const uint32_t idesc0 = idesc_f16(kBf16, kAmn, kBmn, 256, (uint32_t)width_of(ti, 0));
+                const uint32_t idesc1 = subs == 2 ? idesc_f16(kBf16, kAmn, kBmn, 256, (uint32_t)width_of(ti, 1)) : 0u;
                 const int red = FORM == kWgrad ? ti.rows : p.red;
                 for (int kb = 0; kb < nkb; kb++) {
                     bool landed = spin_parity(bar_full + 8 * stage, phase, tmo, abort_flag);
@@ -377,12 +410,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     if ((kb + 1) * kBlockK <= red) {
 #pragma unroll
                         for (int j = 0; j < 4; j++)
-                            mma_f16_pair(d_tmem, a + j * kStep16<kAmn>, b + j * kStep16<kBmn>, idesc,
+                            mma_f16_pair(d0, a + j * kStep16<kAmn>, b + j * kStep16<kBmn>, idesc0,
                                          (kb | j) != 0 ? 1u : 0u);
                     } else {  // what is left, in steps of 16 (zeros past the end)
                         const int steps = (red - kb * kBlockK + 15) / 16;
                         for (int j = 0; j < steps; j++)
-                            mma_f16_pair(d_tmem, a + j * kStep16<kAmn>, b + j * kStep16<kBmn>, idesc,
+                            mma_f16_pair(d0, a + j * kStep16<kAmn>, b + j * kStep16<kBmn>, idesc0,
+                                         (kb | j) != 0 ? 1u : 0u);
+                    }
+                    if (subs == 2) {
+                        const uint64_t b2 = b + (sub_bytes >> 4);
+                        const int steps = min(4, (red - kb * kBlockK + 15) / 16);
+                        for (int j = 0; j < steps; j++)
+                            mma_f16_pair(d1, a + j * kStep16<kAmn>, b2 + j * kStep16<kBmn>, idesc1,
                                          (kb | j) != 0 ? 1u : 0u);
                     }
                     mma_commit_pair(empty0 + 8 * stage);
@@ -393,8 +433,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     }
                 }
                 if (!ok) break;
-                mma_commit_pair(accf0 + 8 * buf);
-                mma_commit_pair(accf1 + 8 * buf);
+                for (int s = 0; s < subs_max; s++, local++) {
+                    mma_commit_pair(accf0 + 8 * (local & 1));
+                    mma_commit_pair(accf1 + 8 * (local & 1));
+                }
             }
             if (!ok && any) {
                 volatile int never = 0;
@@ -437,12 +479,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         // ------------------------------------------------------------ epilogue (warps 2..9, both CTAs)
         const int quarter = warp & 3, half = (warp - 2) >> 2;
         const uint32_t lead_acc_empty = map_to_cta(bar_acc_empty, 0);
-        const uint32_t stage = base + kOffStage + (warp - 2) * kStageWarp;
+        const uint32_t stage = base + kOffStage - (FORM == kWgrad ? kTileBytes : 0) +
+                               (warp - 2) * (FORM == kWgrad ? 2 * kBox : kStageWarp);
         const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
         int local = 0;
-        for (int t = pair; t < n_tiles; t += num_pairs, local++) {
+        uint32_t boxes = 0;
+        bool ok = true;
+        for (int t = pair; ok && t < n_tiles; t += num_pairs) {
             const Tile ti = tile_at(t);
-            const uint32_t buf = local & 1, use = local >> 1;
             const int feat0 = ti.f * 256 + (int)rank * 128 + quarter * 32;
             float bias[4] = {0.f, 0.f, 0.f, 0.f};
             if (FORM == kForward && p.bias) {
@@ -453,63 +497,58 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                         bias[q] = Type16<T>::load(static_cast<const T *>(p.bias) + (int64_t)ti.group * p.features + f);
                 }
             }
-            if (!wait_parity(bar_acc_full + 8 * buf, use & 1, tmo, abort_flag)) {
-                if (lane == 0) report_timeout(abort_flag, p.ctl.status);
-                break;
-            }
-            tc_fence_after();
-            const uint32_t acc = tmem_base + lane_base + buf * kAccCols;
-            if constexpr (FORM != kWgrad) {
-                for (int c = half * 32; c < ti.rows; c += 64) {
-                    uint32_t ra[16], rb[16];
-                    tmem_ld_16x256b_x4(acc + c, ra);
-                    tmem_ld_16x256b_x4(acc + (16u << 16) + c, rb);
-                    tmem_ld_wait();
-                    const int n = ti.rows - c, row = ti.row0 + c;
-                    if (feat0 >= p.features) continue;
-                    switch (FORM == kForward ? p.act : (int)kActNone) {
-                        case kActRelu: store_piece<T, kActRelu>(p, ra, rb, stage, bias, row, n, feat0, lane); break;
-                        case kActSilu: store_piece<T, kActSilu>(p, ra, rb, stage, bias, row, n, feat0, lane); break;
-                        case kActGeluTanh:
-                            store_piece<T, kActGeluTanh>(p, ra, rb, stage, bias, row, n, feat0, lane);
-                            break;
-                        case kActSwiglu: store_piece<T, kActSwiglu>(p, ra, rb, stage, bias, row, n, feat0, lane); break;
-                        default: store_piece<T, kActNone>(p, ra, rb, stage, bias, row, n, feat0, lane);
-                    }
+            for (int sub = 0; sub < subs_max; sub++, local++) {
+                const uint32_t buf = local & 1, use = local >> 1;
+                if (!wait_parity(bar_acc_full + 8 * buf, use & 1, tmo, abort_flag)) {
+                    if (lane == 0) report_timeout(abort_flag, p.ctl.status);
+                    ok = false;
+                    break;
                 }
-            } else {
-                // a lane is a row of dW: 32 columns of it, 64 contiguous bytes, at a time
-                const int f = feat0 + lane;
-                T *out = static_cast<T *>(p.y) + ((int64_t)ti.group * p.features + f) * p.out_cols + ti.col * p.bt;
-                const int cols = min(p.bt, p.out_cols - ti.col * p.bt);
-                // whole 32-byte sectors where the rows allow it
-                const bool wide = p.out_cols % 16 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 31u) == 0;
-                for (int c = half * 32; c < cols; c += 64) {
-                    uint32_t r[32];
-                    tmem_ld_32x32b_x32(acc + c, r);
-                    tmem_ld_wait();
-                    if (f >= p.features) continue;
-                    uint32_t v[16];
+                tc_fence_after();
+                const uint32_t acc = tmem_base + lane_base + buf * kAccCols;
+                if constexpr (FORM != kWgrad) {
+                    const int rows = sub < subs_of(ti) ? sub_rows(ti, sub) : 0;
+                    for (int c = half * 32; c < rows; c += 64) {
+                        uint32_t ra[16], rb[16];
+                        tmem_ld_16x256b_x4(acc + c, ra);
+                        tmem_ld_16x256b_x4(acc + (16u << 16) + c, rb);
+                        tmem_ld_wait();
+                        if (feat0 >= p.features) continue;
+                        store_act<T, FORM>(p, ra, rb, stage, bias, ti.row0 + sub * p.bt + c, rows - c, feat0, lane);
+                    }
+                } else {
+                    // a lane is a row of dW: 32 rows x 32 columns at a time through shared memory,
+                    // in the 64-byte swizzle, and out as one box that the tensor map clips to the
+                    // group's rows and columns
+                    const int cols = min(p.bt, p.out_cols - ti.col * p.bt);
+                    for (int c = half * 32; c < cols; c += 64) {
+                        uint32_t r[32];
+                        tmem_ld_32x32b_x32(acc + c, r);
+                        tmem_ld_wait();
+                        if (feat0 >= p.features) continue;
+                        uint32_t v[16];
 #pragma unroll
-                    for (int i = 0; i < 16; i++)  // a group without rows: its gradient is zero
-                        v[i] = ti.rows > 0 ? Type16<T>::pack(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])) : 0u;
-                    if (wide) {
-#pragma unroll
-                        for (int q = 0; q < 2; q++)
-                            if (c + q * 16 < cols)
-                                st_global_v8(out + c + q * 16, *reinterpret_cast<uint32_t(*)[8]>(&v[q * 8]));
-                    } else {
+                        for (int i = 0; i < 16; i++)  // a group without rows: its gradient is zero
+                            v[i] = ti.rows > 0 ? Type16<T>::pack(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])) : 0u;
+                        const uint32_t box = stage + (boxes++ & 1) * kBox;
+                        if (lane == 0) bulk_wait_group_read<1>();  // the box's last store has read it
+                        __syncwarp();
 #pragma unroll
                         for (int q = 0; q < 4; q++)
-                            if (c + q * 8 < cols)
-                                *reinterpret_cast<uint4 *>(out + c + q * 8) =
-                                    make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+                            st_shared_v4(box + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4), v[4 * q], v[4 * q + 1],
+                                         v[4 * q + 2], v[4 * q + 3]);
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) {
+                            tma_store_3d(&tmap_d, box, ti.col * p.bt + c, feat0, ti.group);
+                            bulk_commit_group();
+                        }
                     }
                 }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster_cta_release(lead_acc_empty + 8 * buf);
             }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster_cta_release(lead_acc_empty + 8 * buf);
         }
         if constexpr (FORM != kWgrad)
             if (p.m_offsets) {  // rows outside every group (tokens that were not routed) are zero
@@ -524,6 +563,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     if (p.z) clear(p.z, p.features);
                 }
             }
+        if (FORM == kWgrad && lane == 0) bulk_wait_group<0>();  // stores done before the memory goes
         __syncwarp();
     }
 
@@ -539,8 +579,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
 // ------------------------------------------------------------------------- host side
 template <typename T, int FORM>
-static int launch_pair(const CUtensorMap &a, const CUtensorMap &b, Params p, int64_t tiles, const DeviceInfo &di,
-                       cudaStream_t stream) {
+static int launch_pair(const CUtensorMap &a, const CUtensorMap &b, const CUtensorMap &d, Params p, int64_t tiles,
+                       const DeviceInfo &di, cudaStream_t stream) {
     auto kern = linear_pair_kernel<T, FORM>;
     static int configured[64] = {};
     if (!configured[di.device]) {
@@ -549,7 +589,8 @@ static int launch_pair(const CUtensorMap &a, const CUtensorMap &b, Params p, int
         configured[di.device] = 1;
     }
     if (tiles > INT_MAX) return NVFP4_ERR_SHAPE;
-    p.stages = std::min(kMaxStages, kRingBytes / (kTileBytes + p.bt * 64));
+    const int ring = kRingBytes - (FORM == kWgrad ? kTileBytes : 0);
+    p.stages = std::min(kMaxStages, ring / (kTileBytes + p.bt * 64 * (1 + p.wide)));
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -560,35 +601,45 @@ static int launch_pair(const CUtensorMap &a, const CUtensorMap &b, Params p, int
     cfg.stream = stream;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (cudaLaunchKernelEx(&cfg, kern, a, b, p) != cudaSuccess) return NVFP4_ERR_CUDA;
+    if (cudaLaunchKernelEx(&cfg, kern, a, b, d, p) != cudaSuccess) return NVFP4_ERR_CUDA;
     count_launch();
     return cuda_status(cudaGetLastError());
 }
 
 // Tokens of a tile.  A slot of 64 reduction elements costs a pair about 150 ns for its 256
 // features plus 1.07 ns a token (measured from 32 to 256 tokens, N = K = 4096), so few wide
-// tiles win, unless their number fills the last wave of pairs badly.
-//   dense: the M tokens in n equal tiles, n chosen by waves x cost;
+// tiles win, unless their number fills the last round of pairs badly.
+//   dense: the M tokens in n equal tiles, n chosen by rounds x cost; or in wide tiles (two
+//     parts that share the A tile, up to 512 tokens), whose epilogue, about 20 ns a token,
+//     no other tile's MMAs hide.  As tiles of 192 / wide tiles of 2 x 192 tokens, us: M=333
+//     N=14344 K=4104 56.6/47.4, M=333 N=14336 K=4096 45.5/41.6; but M=1024 N=K=4096 as
+//     tiles of 256 / of 2 x 256 32.6/48.9 (fewer tiles than pairs);
 //   groups (their rows are known on the device only): up to twice the mean rows, so that
-//   most groups are one tile or 256-token tiles; a tile's MMAs follow its own rows.
-static int token_tile(int64_t m, int groups, int n_f, int pairs) {
+//     most groups are one tile or 256-token tiles; a tile's MMAs follow its own rows.  Wide
+//     tiles were slower or the same (64 experts of 4096 x 2048, 512 rows each, 537/590 us).
+struct TokenTile {
+    int bt, wide;
+};
+static TokenTile token_tile(int64_t m, int groups, int n_f, int pairs, int red) {
+    TokenTile best = {kMaxTokens, 0};
     if (groups > 1) {
-        int bt = 32;
-        while (bt < kMaxTokens && (int64_t)bt * groups < 2 * m) bt *= 2;
-        return bt;
+        best.bt = 32;
+        while (best.bt < kMaxTokens && (int64_t)best.bt * groups < 2 * m) best.bt *= 2;
+        return best;
     }
-    int best = kMaxTokens;
     double least = 1e300;
+    const int nkb = (red + kBlockK - 1) / kBlockK;
     const int64_t n0 = (m + kMaxTokens - 1) / kMaxTokens;
-    for (int64_t n = n0; n <= 4 * n0; n++) {
-        const int bt = (int)(((m + n - 1) / n + 31) / 32 * 32);
-        const int64_t tiles = (m + bt - 1) / bt * n_f, waves = (tiles + pairs - 1) / pairs;
-        const double cost = (double)waves * (150.0 + 1.07 * bt);
-        if (cost < least) {
-            least = cost;
-            best = bt;
+    for (int64_t n = n0; n <= 4 * n0; n++)
+        for (int wide = 0; wide <= (n > 1 ? 1 : 0); wide++) {
+            const int bt = (int)(((m + n - 1) / n + 31) / 32 * 32), tokens = bt * (1 + wide);
+            const int64_t tiles = (m + tokens - 1) / tokens * n_f, rounds = (tiles + pairs - 1) / pairs;
+            const double cost = (double)rounds * nkb * (150.0 + 1.07 * tokens) + (wide ? rounds : 1) * 20.0 * tokens;
+            if (cost < least) {
+                least = cost;
+                best = {bt, wide};
+            }
         }
-    }
     return best;
 }
 
@@ -612,7 +663,9 @@ static int forward_t(const void *X, int64_t ldx, const void *W, Params p, int K,
                      cudaStream_t s) {
     const int n_f = (p.features + 255) / 256;
     if (use_decode(p.m_total, p.groups, n_f, K)) return decode_forward<T>(X, ldx, W, p, K, di, s);
-    p.bt = token_tile(p.m_total, p.groups, n_f, di.sm_count / 2);
+    const TokenTile tt = token_tile(p.m_total, p.groups, n_f, di.sm_count / 2, K);
+    p.bt = tt.bt;
+    p.wide = tt.wide;
     p.strip = 8;
     p.red = K;
     CUtensorMap a, b;
@@ -620,13 +673,15 @@ static int forward_t(const void *X, int64_t ldx, const void *W, Params p, int K,
     if (!st) st = map_rows<T>(&b, X, p.m_total, K, ldx, p.bt / 2);
     if (st) return st;
     const int64_t token_tiles = (p.m_total + p.bt - 1) / p.bt + (p.m_offsets ? p.groups : 0);
-    return launch_pair<T, kForward>(a, b, p, token_tiles * n_f, di, s);
+    return launch_pair<T, kForward>(a, b, b, p, token_tiles * n_f, di, s);
 }
 
 template <typename T>
 static int dgrad_t(const void *dZ, const void *W, Params p, int N, const DeviceInfo &di, cudaStream_t s) {
     const int n_f = (p.features + 255) / 256;
-    p.bt = token_tile(p.m_total, p.groups, n_f, di.sm_count / 2);
+    const TokenTile tt = token_tile(p.m_total, p.groups, n_f, di.sm_count / 2, N);
+    p.bt = tt.bt;
+    p.wide = tt.wide;
     p.strip = 8;
     p.red = N;
     CUtensorMap a, b;
@@ -634,7 +689,7 @@ static int dgrad_t(const void *dZ, const void *W, Params p, int N, const DeviceI
     if (!st) st = map_rows<T>(&b, dZ, p.m_total, N, N, p.bt / 2);
     if (st) return st;
     const int64_t token_tiles = (p.m_total + p.bt - 1) / p.bt + (p.m_offsets ? p.groups : 0);
-    return launch_pair<T, kDgrad>(a, b, p, token_tiles * n_f, di, s);
+    return launch_pair<T, kDgrad>(a, b, b, p, token_tiles * n_f, di, s);
 }
 
 template <typename T>
@@ -642,12 +697,13 @@ static int wgrad_t(const void *dZ, const void *X, int64_t ldx, Params p, const D
     const int n_f = (p.features + 255) / 256;
     p.bt = 256;
     p.strip = 8;
-    CUtensorMap a, b;
+    CUtensorMap a, b, d;
     int st = map_rows<T>(&a, dZ, std::max(p.m_total, 1), p.features, p.features, 64);
     if (!st) st = map_rows<T>(&b, X, std::max(p.m_total, 1), p.out_cols, ldx, 64);
+    if (!st) st = map_gradient<T>(&d, p.y, p.groups, p.features, p.out_cols);
     if (st) return st;
     const int64_t tiles = (int64_t)p.groups * n_f * ((p.out_cols + p.bt - 1) / p.bt);
-    return launch_pair<T, kWgrad>(a, b, p, tiles, di, s);
+    return launch_pair<T, kWgrad>(a, b, d, p, tiles, di, s);
 }
 
 // Sizes and pointers that the entry points have in common.

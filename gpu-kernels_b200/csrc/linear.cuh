@@ -39,11 +39,13 @@ struct Params {
     int red;               // reduction length: K (forward), N (dgrad); wgrad: the group's rows
     int out_cols;          // row length of y
     int bt;                // tokens of a tile (wgrad: output columns of a tile)
+    int wide;              // 1: a tile is two of them beside each other, sharing the A tile
     int strip;             // feature tiles that sweep the tokens together (L2 reuse)
     int act;
     int splits;            // decode: CTAs that share a tile's reduction
     int stages;            // ring slots
     int ncap;              // decode: token rows of a ring slot
+    int prefetch;          // decode: weight tiles a CTA hints into L2 before the previous kernel ends
     KernelCtl ctl;
 };
 
@@ -101,6 +103,19 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *tma
         " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
         "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(z), "r"(bar)
         : "memory");
+}
+
+__device__ __forceinline__ void tma_prefetch_3d(const CUtensorMap *tmap, int32_t x, int32_t y, int32_t z) {
+    asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(
+                     reinterpret_cast<uint64_t>(tmap)),
+                 "r"(x), "r"(y), "r"(z)
+                 : "memory");
+}
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap *tmap, uint32_t src, int32_t x, int32_t y, int32_t z) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(
+                     reinterpret_cast<uint64_t>(tmap)),
+                 "r"(x), "r"(y), "r"(z), "r"(src)
+                 : "memory");
 }
 
 // 16 lanes x 32 fp32 columns as matrix fragments: with l the lane, r[4i], r[4i+1] hold row
@@ -221,6 +236,15 @@ inline int map_weight(CUtensorMap *m, const void *base, int groups, int N, int K
     const uint64_t strides[2] = {(uint64_t)K * 2, (uint64_t)N * (uint64_t)K * 2};
     const uint32_t box[3] = {64, (uint32_t)box_rows, 1};
     return encode_tiled(m, tma_type<T>(), 3, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+// The weight's gradient [groups, N, K], written in boxes of 32 rows x 32 columns.
+template <typename T>
+inline int map_gradient(CUtensorMap *m, const void *base, int groups, int N, int K) {
+    const uint64_t dims[3] = {(uint64_t)K, (uint64_t)N, (uint64_t)groups};
+    const uint64_t strides[2] = {(uint64_t)K * 2, (uint64_t)N * (uint64_t)K * 2};
+    const uint32_t box[3] = {32, 32, 1};
+    return encode_tiled(m, tma_type<T>(), 3, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 // linear_decode.cu: the forward product for at most kDecodeTokens token rows in all.

@@ -8,8 +8,10 @@
 // CTAs add disjoint pieces of it in the order of the parts (the same bits every time) and
 // run the epilogue on them.  No workspace, no atomics, no second launch.
 //
-// The ring is sized so that two or three CTAs share an SM: the prologue and the reduction of
-// one run under the loads of another.
+// The ring is sized so that two CTAs share an SM: the prologue and the reduction of one run
+// under the loads of another.  Measured, M = 1: N=K=4096 7.6 us (4.4 TB/s), N=14336 K=4096
+// 21.7 us (5.4), N=28672 K=8192 73.8 us (6.4 of a copy's 6.55): bound by the weights' bytes,
+// and for the smaller ones by what a launch, the first loads and the cluster's sum take.
 //
 // Warps: 0 TMA producer, 1 MMA issue and TMEM owner, 2-5 read the accumulator out; all six
 // reduce.
@@ -25,6 +27,7 @@ constexpr int kDecThreads = 192;
 constexpr int kDecMaxStages = 8;
 constexpr int kDecMaxSplits = 8;
 constexpr int kDecBarBytes = 256;
+constexpr int kDecSmem = 112 * 1024;  // two CTAs an SM
 
 __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
     float4 v;
@@ -118,6 +121,16 @@ __global__ void __launch_bounds__(kDecThreads)
         tmem_alloc(smem_u32(tmem_slot), tmem_cols);
         tmem_relinquish();
     }
+    // The next kernel in the stream may start its own set-up as soon as there is room.
+    grid_launch_dependents();
+    // Before the wait only hints: the first weight tiles of a dense layer start their way
+    // into L2 while the previous kernel finishes (a hint reads no value, so it does not
+    // matter that the previous kernel may still write them).
+    const int n_f = (p.features + 127) / 128;
+    const int nkb = (p.red + kBlockK - 1) / kBlockK;
+    const int kb0 = (int)((int64_t)nkb * split / splits), kb1 = (int)((int64_t)nkb * (split + 1) / splits);
+    if (!p.m_offsets && warp == 0 && lane < min(p.prefetch, kb1 - kb0))
+        tma_prefetch_3d(&tmap_a, (kb0 + lane) * kBlockK, tile * 128, 0);
     grid_dependency_wait();  // nothing of global memory is read or written before this
     tc_fence_before();
     __syncthreads();
@@ -126,7 +139,6 @@ __global__ void __launch_bounds__(kDecThreads)
     const uint64_t tmo = p.ctl.wait_timeout_ns;
 
     // Tiles are numbered over the groups that have rows: the others' weights are not read.
-    const int n_f = (p.features + 127) / 128;
     int g = p.m_offsets ? -1 : 0, f = tile;
     if (p.m_offsets) {
         int nth = tile / n_f;
@@ -147,8 +159,6 @@ __global__ void __launch_bounds__(kDecThreads)
     int r0 = 0, r1 = 0;
     if (g >= 0) group_rows(p.m_offsets, g, p.m_total, r0, r1);
     const int rows = r1 - r0, n16 = (rows + 15) & ~15;
-    const int nkb = (p.red + kBlockK - 1) / kBlockK;
-    const int kb0 = (int)((int64_t)nkb * split / splits), kb1 = (int)((int64_t)nkb * (split + 1) / splits);
 
     if (rows > 0) {  // the same for every CTA of the cluster
         if (warp == 0) {
@@ -228,10 +238,12 @@ __global__ void __launch_bounds__(kDecThreads)
         if (splits > 1) cluster_sync();
         else __syncthreads();
 
+        // each CTA of the cluster finishes its share of the tokens, whole rows of the tile
+        const int share = (rows + splits - 1) / splits, t0 = min(rows, split * share), t1 = min(rows, t0 + share);
         const uint32_t part_addr = base;
         const int feat0 = f * 128;
         if (p.act == kActSwiglu) {
-            for (int i = split * kDecThreads + threadIdx.x; i < rows * 8; i += splits * kDecThreads) {
+            for (int i = t0 * 8 + (int)threadIdx.x; i < t1 * 8; i += kDecThreads) {
                 const int t = i >> 3, c = i & 7;  // 8 of the tile's 64 outputs
                 const int gf = (c >> 1) * 32 + (c & 1) * 8;
                 if (feat0 + gf >= p.features) continue;
@@ -251,7 +263,7 @@ __global__ void __launch_bounds__(kDecThreads)
                 put8<T>(p.y, at, gate);
             }
         } else {
-            for (int i = split * kDecThreads + threadIdx.x; i < rows * 16; i += splits * kDecThreads) {
+            for (int i = t0 * 16 + (int)threadIdx.x; i < t1 * 16; i += kDecThreads) {
                 const int t = i >> 4, c = (i & 15) * 8;
                 if (feat0 + c >= p.features) continue;
                 float v[8];
@@ -286,7 +298,6 @@ __global__ void __launch_bounds__(kDecThreads)
                     reinterpret_cast<uint4 *>(static_cast<T *>(p.z) + row * p.features)[c] = zero;
         }
     }
-    grid_launch_dependents();
     __syncthreads();
     if (warp == 1) {
         tc_fence_after();
@@ -307,10 +318,10 @@ int decode_forward(const void *X, int64_t ldx, const void *W, Params p, int K, c
     while (p.splits < kDecMaxSplits && tiles * p.splits * 2 <= 2 * di.sm_count && nkb >= p.splits * 8) p.splits *= 2;
     const int64_t grid = tiles * p.splits;
     if (grid > INT_MAX) return NVFP4_ERR_SHAPE;
-    // two CTAs an SM when they are all resident at once, three when they come in waves
+    // use_decode() keeps the grid within two CTAs an SM, so all of them are resident at once
     const int slot = kTileBytes + p.ncap * 128;
-    const int budget = grid <= 2 * di.sm_count ? 112 * 1024 : 74 * 1024;
-    p.stages = std::max(2, std::min(kDecMaxStages, (budget - 1024 - kDecBarBytes) / slot));
+    p.prefetch = 4;
+    p.stages = std::max(2, std::min(kDecMaxStages, (kDecSmem - 1024 - kDecBarBytes) / slot));
     const int smem = p.stages * slot + kDecBarBytes + 1024;
     CUtensorMap a, b;
     int st = map_weight<T>(&a, W, p.groups, p.features, K, 128);
@@ -319,7 +330,7 @@ int decode_forward(const void *X, int64_t ldx, const void *W, Params p, int K, c
     auto kern = linear_decode_kernel<T>;
     static int configured[64] = {};
     if (!configured[di.device]) {
-        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 116 * 1024) != cudaSuccess)
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kDecSmem) != cudaSuccess)
             return NVFP4_ERR_CUDA;
         configured[di.device] = 1;
     }
