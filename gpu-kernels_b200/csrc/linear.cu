@@ -240,6 +240,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         prefetch_tmap(&tmap_a);
         prefetch_tmap(&tmap_b);
     }
+    __syncwarp();
     if (warp == 1) {
         tmem_alloc_pair(smem_u32(tmem_slot), 512);
         tmem_relinquish_pair();
@@ -249,7 +250,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         build_tables(p.m_offsets, p.groups, p.m_total, FORM == kWgrad ? 0 : tile_tokens, FORM == kWgrad ? n_f * n_c : n_f,
                      lane, g_r0, g_r1, g_t0);
     tc_fence_before();
-    cluster_sync();
+    warp_cluster_sync();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     const uint64_t tmo = p.ctl.wait_timeout_ns;
@@ -287,11 +288,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         return ((FORM == kWgrad ? ti.rows : p.red) + kBlockK - 1) / kBlockK;
     };
     // Parts of a tile (two for a wide one with more than bt tokens), the tokens of each, and
-    // its MMA columns: the tokens rounded up to the instruction's step of 16 (each CTA holds
-    // half of them); the rounding's rows are loaded but never stored.
+    // its MMA columns: the tokens rounded up to 32, the step of N for a CTA pair (multiples of
+    // 16 are for one CTA alone).  Each CTA holds half of them; the rounding's rows are loaded
+    // but never stored.
     auto subs_of = [&](const Tile &ti) { return FORM != kWgrad && ti.rows > p.bt ? 2 : 1; };
     auto sub_rows = [&](const Tile &ti, int s) { return s ? ti.rows - p.bt : min(ti.rows, p.bt); };
-    auto width_of = [&](const Tile &ti, int s) { return FORM == kWgrad ? p.bt : (sub_rows(ti, s) + 15) & ~15; };
+    auto width_of = [&](const Tile &ti, int s) { return FORM == kWgrad ? p.bt : (sub_rows(ti, s) + 31) & ~31; };
     // wgrad: reduction rows past the group's end belong to the next group; the last slot's
     // are cleared unless the MMA's 16-row steps end exactly with the group
     auto dirty_tail = [&](const Tile &ti) { return FORM == kWgrad && (ti.rows & 15) != 0; };
@@ -357,6 +359,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 }
             }
             grid_launch_dependents();
+            // The MMAs release slots with arrivals that the tensor core sends, to the other CTA
+            // too, whenever they complete; no thread's barrier orders them.  Take in the last
+            // ones: one that came after this CTA's end would arrive on a barrier of the next
+            // CTA here.
+            for (int s = 0; ok && s < n_stages; s++) {
+                if (!wait_parity(bar_empty + 8 * stage, phase ^ 1, tmo, abort_flag)) {
+                    report_timeout(abort_flag, p.ctl.status);
+                    ok = false;
+                }
+                if (++stage == (uint32_t)n_stages) {
+                    stage = 0;
+                    phase ^= 1;
+                }
+            }
             if (!ok) {  // let the copies in flight land before the memory goes
                 volatile int never = 0;
                 for (int s = 0; s < n_stages; s++) {
@@ -438,6 +454,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     mma_commit_pair(accf1 + 8 * (local & 1));
                 }
             }
+            // likewise the epilogues' last arrivals, the other CTA's among them
+            for (int s = 0; ok && s < 2; s++)
+                if (!spin_parity(bar_acc_empty + 8 * ((local + s) & 1), (((local + s) >> 1) & 1) ^ 1, tmo, abort_flag)) {
+                    report_timeout(abort_flag, p.ctl.status);
+                    ok = false;
+                }
             if (!ok && any) {
                 volatile int never = 0;
                 mma_commit_pair(map_to_cta(bar_drain, 0));
@@ -456,7 +478,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 slots += (uint32_t)blocks_of(ti);
                 if (!dirty_tail(ti)) continue;
                 const uint32_t stage = (slots - 1) % (uint32_t)n_stages;
-                if (!wait_parity(bar_tail + 8 * stage, (parity >> stage) & 1, tmo, abort_flag)) {
+                if (!warp_wait_parity(bar_tail + 8 * stage, (parity >> stage) & 1, tmo, abort_flag, lane)) {
                     if (lane == 0) report_timeout(abort_flag, p.ctl.status);
                     ok = false;
                     break;
@@ -473,6 +495,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive_cluster(map_to_cta(bar_ready + 8 * stage, 0));
+                __syncwarp();
             }
         }
     } else {
@@ -499,7 +522,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             }
             for (int sub = 0; sub < subs_max; sub++, local++) {
                 const uint32_t buf = local & 1, use = local >> 1;
-                if (!wait_parity(bar_acc_full + 8 * buf, use & 1, tmo, abort_flag)) {
+                if (!warp_wait_parity(bar_acc_full + 8 * buf, use & 1, tmo, abort_flag, lane)) {
                     if (lane == 0) report_timeout(abort_flag, p.ctl.status);
                     ok = false;
                     break;
@@ -543,11 +566,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                             tma_store_3d(&tmap_d, box, ti.col * p.bt + c, feat0, ti.group);
                             bulk_commit_group();
                         }
+                        __syncwarp();
                     }
                 }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive_cluster_cta_release(lead_acc_empty + 8 * buf);
+                __syncwarp();
             }
         }
         if constexpr (FORM != kWgrad)
@@ -569,7 +594,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
     __syncwarp();
     tc_fence_before();
-    cluster_sync();  // no CTA leaves while its peer may still signal it
+    warp_cluster_sync();  // no CTA leaves while its peer may still signal it
     if (warp == 1) {
         __syncwarp();
         tc_fence_after();

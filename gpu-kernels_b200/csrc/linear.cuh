@@ -3,8 +3,8 @@
 //
 // All of them compute with the FEATURES of the output on the MMA's M side (the weight is
 // operand A) and the TOKENS on its N side: N is a run-time field of the instruction, so a
-// tile of a ragged group costs what its own rows cost, from 16 to 256, and the same
-// orientation streams the weights for a single token.
+// tile of a ragged group costs what its own rows cost (in steps of 32 on a CTA pair, of 16 on
+// one CTA, up to 256), and the same orientation streams the weights for a single token.
 #pragma once
 #include <cmath>
 #include <type_traits>
@@ -116,6 +116,24 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap *tmap, uint32_t s
                      reinterpret_cast<uint64_t>(tmap)),
                  "r"(x), "r"(y), "r"(z), "r"(src)
                  : "memory");
+}
+
+// Bounded wait by a whole warp, whose lanes are together when it returns: lane 0 polls, the
+// shuffle brings the others.  What follows (tcgen05.ld, stmatrix, barrier.cluster: .aligned)
+// needs all of them at once; lanes that polled each for itself would see the phase complete
+// at different polls, and the compiler may leave them apart until the branch for a wait that
+// gave up joins again, after the role's loop.
+__device__ __forceinline__ bool warp_wait_parity(uint32_t bar, uint32_t parity, uint64_t timeout_ns,
+                                                 volatile int *abort, int lane) {
+    int ok = 1;
+    if (lane == 0) ok = wait_parity(bar, parity, timeout_ns, abort);
+    return __shfl_sync(0xffffffffu, ok, 0) != 0;
+}
+
+// barrier.cluster is .aligned too: bring the warp's lanes together before it.
+__device__ __forceinline__ void warp_cluster_sync() {
+    __syncwarp();
+    cluster_sync();
 }
 
 // 16 lanes x 32 fp32 columns as matrix fragments: with l the lane, r[4i], r[4i+1] hold row

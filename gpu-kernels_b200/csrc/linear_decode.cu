@@ -117,6 +117,7 @@ __global__ void __launch_bounds__(kDecThreads)
         prefetch_tmap(&tmap_a);
         prefetch_tmap(&tmap_b);
     }
+    __syncwarp();
     if (warp == 1) {
         tmem_alloc(smem_u32(tmem_slot), tmem_cols);
         tmem_relinquish();
@@ -184,6 +185,17 @@ __global__ void __launch_bounds__(kDecThreads)
                         phase ^= 1;
                     }
                 }
+                // the MMAs' last arrivals have to come before the CTA ends
+                for (int s = 0; ok && s < p.stages; s++) {
+                    if (!wait_parity(bar_empty + 8 * stage, phase ^ 1, tmo, abort_flag)) {
+                        report_timeout(abort_flag, p.ctl.status);
+                        ok = false;
+                    }
+                    if (++stage == (uint32_t)p.stages) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                }
                 if (!ok) {
                     volatile int never = 0;
                     for (int s = 0; s < p.stages; s++)
@@ -220,7 +232,7 @@ __global__ void __launch_bounds__(kDecThreads)
             __syncwarp();
         } else {
             // every MMA has read its slot, so the ring's memory takes the partial tile
-            if (!wait_parity(bar_acc, 0, tmo, abort_flag)) {
+            if (!warp_wait_parity(bar_acc, 0, tmo, abort_flag, lane)) {
                 if (lane == 0) report_timeout(abort_flag, p.ctl.status);
             }
             tc_fence_after();
@@ -235,7 +247,7 @@ __global__ void __launch_bounds__(kDecThreads)
             }
             tc_fence_before();
         }
-        if (splits > 1) cluster_sync();
+        if (splits > 1) warp_cluster_sync();
         else __syncthreads();
 
         // each CTA of the cluster finishes its share of the tokens, whole rows of the tile
@@ -281,7 +293,7 @@ __global__ void __launch_bounds__(kDecThreads)
                 put8<T>(p.y, at, v);
             }
         }
-        if (splits > 1) cluster_sync();  // the others may still read this CTA's part
+        if (splits > 1) warp_cluster_sync();  // the others may still read this CTA's part
     }
     if (p.m_offsets) {  // rows outside every group are zero
         int lo, hi, unused;

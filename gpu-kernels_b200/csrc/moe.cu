@@ -236,6 +236,7 @@ __global__ void __launch_bounds__(kRouteThreads, 3) moe_route_kernel(const Route
         if (lane == 0) total[e] = c;
     }
     if (p.chunks > 1) {
+        __syncwarp();  // barrier.cluster is .aligned
         cluster_sync();
         const int rank = blockIdx.x % kClusterChunks, cluster = blockIdx.x / kClusterChunks;
         const int per = (p.E + kClusterChunks - 1) / kClusterChunks;  // this CTA's experts
@@ -251,6 +252,7 @@ __global__ void __launch_bounds__(kRouteThreads, 3) moe_route_kernel(const Route
             }
             p.counts[(int64_t)cluster * p.E + e] = sum;
         }
+        __syncwarp();
         cluster_sync();  // the others may still read this CTA's counts
         return;
     }

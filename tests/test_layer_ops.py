@@ -1,0 +1,60 @@
+"""The torch.library operators of the 16-bit layers and the mixture of experts: schemas and
+fake (shape) implementations on the CPU; on a GPU, autograd through a whole layer gives what
+the direct calls give."""
+import pytest
+import torch
+
+
+def test_fake_shapes_without_a_gpu(nv):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    ops = torch.ops.nvfp4_b200
+    with FakeTensorMode():
+        x, w = torch.empty(30, 64, dtype=torch.bfloat16), torch.empty(4 * 96, 64, dtype=torch.bfloat16)
+        offs = torch.empty(5, dtype=torch.int32)
+        assert ops.linear(x, w).shape == (30, 384)
+        assert ops.linear(x, w, offs, None, "swiglu").shape == (30, 48)
+        y, z = ops.linear_preact(x, w, offs, None, "swiglu")
+        assert y.shape == (30, 48) and z.shape == (30, 96) and y.dtype == torch.bfloat16
+        r = ops.moe_route(torch.empty(15, 4), 2)
+        assert [t.shape for t in r] == [(15, 2), (15, 2), (15, 2), (5,)] and r[0].dtype == torch.float32
+        xs = ops.moe_dispatch(torch.empty(15, 64, dtype=torch.bfloat16), *r)
+        assert xs.shape == (30, 64)
+        assert ops.moe_combine(xs, *r).shape == (15, 64)
+
+
+@pytest.mark.gpu
+def test_autograd_through_a_layer(nv, cuda_dev):
+    ops = torch.ops.nvfp4_b200
+    T, E, k, K, F, dt = 70, 8, 2, 64, 96, torch.bfloat16
+    g = torch.Generator().manual_seed(3)
+
+    def rnd(*s, scale=1.0):
+        return (torch.randn(*s, generator=g) * scale).to(dt).cuda().requires_grad_()
+
+    x, wr = rnd(T, K), rnd(E, K, scale=0.1)
+    w1, b1, w2 = rnd(E * 2 * F, K, scale=0.1), rnd(E, 2 * F, scale=0.1), rnd(E * K, F, scale=0.1)
+    logits, _ = ops.linear_preact(x, wr)
+    r = ops.moe_route(logits, k)
+    xs = ops.moe_dispatch(x, *r)
+    h, z = ops.linear_preact(xs, w1, r[3], b1, "swiglu")
+    ys, _ = ops.linear_preact(h, w2, r[3])
+    y = ops.moe_combine(ys, *r, x)
+    dy = torch.randn(T, K, generator=g).to(dt).cuda()
+    grads = torch.autograd.grad(y, [x, wr, w1, b1, w2], dy)
+
+    with torch.no_grad():
+        route = nv.Routing(*(t.detach() for t in r))
+        dys, dwt = nv.moe_combine_backward(dy, ys.detach(), route)
+        dh, dw2, _ = nv.linear_grouped_backward(dys, h.detach(), w2, route.m_offsets)
+        dxs, dw1, db1 = nv.linear_grouped_backward(dh, xs.detach(), w1, route.m_offsets, preact=z, activation="swiglu",
+                                                   bias_grad=True)
+        dl = nv.moe_route_backward(dwt, logits.detach(), route)
+        dxr, dwr, _ = nv.linear_backward(dl, x, wr)
+        dx = dy.float() + nv.moe_dispatch_backward(dxs, route).float() + dxr.float()
+    nv.device_status()
+    for got, want in zip(grads[1:], (dwr, dw1, db1, dw2)):
+        assert torch.equal(got, want)
+    # three bf16 terms summed in bf16, in autograd's order: two roundings of at most 2^-8
+    # of a partial sum, which is at most the sum of the terms' magnitudes
+    size = dy.float().abs() + nv.moe_dispatch_backward(dxs, route).float().abs() + dxr.float().abs()
+    assert ((grads[0].float() - dx).abs() <= 2.0 ** -7 * size).all()
