@@ -45,7 +45,6 @@ struct Params {
     int splits;            // decode: CTAs that share a tile's reduction
     int stages;            // ring slots
     int ncap;              // decode: token rows of a ring slot
-    int prefetch;          // decode: weight tiles a CTA hints into L2 before the previous kernel ends
     KernelCtl ctl;
 };
 
@@ -105,12 +104,6 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *tma
         : "memory");
 }
 
-__device__ __forceinline__ void tma_prefetch_3d(const CUtensorMap *tmap, int32_t x, int32_t y, int32_t z) {
-    asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(
-                     reinterpret_cast<uint64_t>(tmap)),
-                 "r"(x), "r"(y), "r"(z)
-                 : "memory");
-}
 __device__ __forceinline__ void tma_store_3d(const CUtensorMap *tmap, uint32_t src, int32_t x, int32_t y, int32_t z) {
     asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(
                      reinterpret_cast<uint64_t>(tmap)),

@@ -122,17 +122,9 @@ __global__ void __launch_bounds__(kDecThreads)
         tmem_alloc(smem_u32(tmem_slot), tmem_cols);
         tmem_relinquish();
     }
-    // The next kernel in the stream may start its own set-up as soon as there is room.
-    grid_launch_dependents();
-    // Before the wait only hints: the first weight tiles of a dense layer start their way
-    // into L2 while the previous kernel finishes (a hint reads no value, so it does not
-    // matter that the previous kernel may still write them).
     const int n_f = (p.features + 127) / 128;
     const int nkb = (p.red + kBlockK - 1) / kBlockK;
     const int kb0 = (int)((int64_t)nkb * split / splits), kb1 = (int)((int64_t)nkb * (split + 1) / splits);
-    if (!p.m_offsets && warp == 0 && lane < min(p.prefetch, kb1 - kb0))
-        tma_prefetch_3d(&tmap_a, (kb0 + lane) * kBlockK, tile * 128, 0);
-    grid_dependency_wait();  // nothing of global memory is read or written before this
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -332,7 +324,6 @@ int decode_forward(const void *X, int64_t ldx, const void *W, Params p, int K, c
     if (grid > INT_MAX) return NVFP4_ERR_SHAPE;
     // use_decode() keeps the grid within two CTAs an SM, so all of them are resident at once
     const int slot = kTileBytes + p.ncap * 128;
-    p.prefetch = 4;
     p.stages = std::max(2, std::min(kDecMaxStages, (kDecSmem - 1024 - kDecBarBytes) / slot));
     const int smem = p.stages * slot + kDecBarBytes + 1024;
     CUtensorMap a, b;
@@ -347,19 +338,17 @@ int decode_forward(const void *X, int64_t ldx, const void *W, Params p, int K, c
         configured[di.device] = 1;
     }
     cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = p.splits;
-    attr[1].val.clusterDim.y = 1;
-    attr[1].val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = p.splits;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
     cfg.gridDim = dim3((unsigned)grid);
     cfg.blockDim = dim3(kDecThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cfg.attrs = attr;
-    cfg.numAttrs = 2;
+    cfg.numAttrs = 1;
     if (cudaLaunchKernelEx(&cfg, kern, a, b, p) != cudaSuccess) return NVFP4_ERR_CUDA;
     count_launch();
     return cuda_status(cudaGetLastError());

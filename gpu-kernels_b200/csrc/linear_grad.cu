@@ -35,8 +35,6 @@ template <typename T>
 __global__ void __launch_bounds__(kGradThreads) activation_backward_kernel(const GradParams p) {
     __shared__ ChunkTables tab;
     __shared__ float sums[kGradRowLanes][kGradLanes][17];  // 17: no bank conflicts between units
-    grid_dependency_wait();
-    grid_launch_dependents();
     if (threadIdx.x < 32) build_tables(p.m_offsets, p.groups, p.m_total, kGradRows, 1, threadIdx.x, tab.r0, tab.r1, tab.c0);
     __syncthreads();
     const int chunk = blockIdx.y;
@@ -115,8 +113,6 @@ template <typename T>
 __global__ void __launch_bounds__(256) bias_sum_kernel(const float *partial, T *db, const int *m_offsets, int groups,
                                                        int m_total, int N) {
     __shared__ int before;  // first chunk of this group
-    grid_dependency_wait();
-    grid_launch_dependents();
     const int g = blockIdx.y;
     if (threadIdx.x < 32) {
         int c = 0;
@@ -145,16 +141,7 @@ static int64_t grad_chunks(int groups, int M) { return ((int64_t)M + kGradRows -
 
 template <typename Kernel, typename... Args>
 static int launch(Kernel kern, dim3 grid, int threads, cudaStream_t stream, Args... args) {
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
-    cfg.stream = stream;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    if (cudaLaunchKernelEx(&cfg, kern, args...) != cudaSuccess) return NVFP4_ERR_CUDA;
+    kern<<<grid, threads, 0, stream>>>(args...);
     count_launch();
     return cuda_status(cudaGetLastError());
 }

@@ -213,8 +213,6 @@ __global__ void __launch_bounds__(kRouteThreads, 3) moe_route_kernel(const Route
     const int t0 = blockIdx.x * p.chunk, n = max(0, min(p.chunk, p.T - t0));
     for (int i = threadIdx.x; i < p.E * words; i += kRouteThreads) bits[i] = 0u;
     __syncthreads();
-    grid_dependency_wait();
-    grid_launch_dependents();
     float bias[NI];
 #pragma unroll
     for (int i = 0; i < NI; i++) bias[i] = p.bias && lane + 32 * i < p.E ? p.bias[lane + 32 * i] : 0.0f;
@@ -272,8 +270,6 @@ __global__ void __launch_bounds__(kRouteThreads) moe_rows_kernel(const RoutePara
     const int words = p.chunk / 32;
     const int t0 = blockIdx.x * p.chunk, n = min(p.chunk, p.T - t0);
     for (int i = threadIdx.x; i < p.E * words; i += kRouteThreads) bits[i] = 0u;
-    grid_dependency_wait();
-    grid_launch_dependents();
     __syncthreads();
     for (int i = threadIdx.x; i < n * p.k; i += kRouteThreads) {
         const int e = p.experts[(int64_t)t0 * p.k + i], t = i / p.k;
@@ -327,8 +323,6 @@ __global__ void __launch_bounds__(256) moe_route_backward_kernel(const T *logits
                                                                  int k, int use_sigmoid, int renormalize, float scale) {
     const int lane = threadIdx.x & 31;
     const int t = blockIdx.x * 8 + (threadIdx.x >> 5);
-    grid_dependency_wait();
-    grid_launch_dependents();
     if (t >= n_tokens) return;
     const T *l = logits + (int64_t)t * E;
     float v[NI], g[NI];
@@ -451,8 +445,6 @@ __device__ __forceinline__ void zero_spare_rows(const MoveParams &p) {
 }
 
 __global__ void __launch_bounds__(kMoveThreads) moe_dispatch_kernel(const MoveParams p) {
-    grid_dependency_wait();
-    grid_launch_dependents();
     const int slab = blockIdx.x % p.s.slabs, block = blockIdx.x / p.s.slabs;
     const int in_cta = threadIdx.x / p.s.lanes;
     const int64_t t = (int64_t)block * p.s.tokens + in_cta;
@@ -470,8 +462,6 @@ __global__ void __launch_bounds__(kMoveThreads) moe_dispatch_kernel(const MovePa
 
 template <typename T>
 __global__ void __launch_bounds__(kMoveThreads) moe_combine_kernel(const MoveParams p) {
-    grid_dependency_wait();
-    grid_launch_dependents();
     const int slab = blockIdx.x % p.s.slabs, block = blockIdx.x / p.s.slabs;
     const int in_cta = threadIdx.x / p.s.lanes;
     const int64_t t = (int64_t)block * p.s.tokens + in_cta;
@@ -519,8 +509,6 @@ __global__ void __launch_bounds__(kMoveThreads) moe_combine_kernel(const MovePar
 template <typename T>
 __global__ void __launch_bounds__(kMoveThreads) moe_combine_backward_kernel(const MoveParams p) {
     __shared__ float part[kMoveThreads / 32][4];
-    grid_dependency_wait();
-    grid_launch_dependents();
     const int in_cta = threadIdx.x / p.s.lanes, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t t = (int64_t)blockIdx.x * p.s.tokens + in_cta;
     const bool on = in_cta < p.s.tokens && t < p.T;
@@ -575,31 +563,31 @@ __global__ void __launch_bounds__(kMoveThreads) moe_combine_backward_kernel(cons
 // ---------------------------------------------------------------------------------------
 // launches
 // ---------------------------------------------------------------------------------------
-template <typename... Args, typename Kernel>
+template <typename Kernel, typename... Args>
+static int launch(Kernel kern, int grid, int threads, size_t smem, cudaStream_t stream, Args... args) {
+    kern<<<grid, threads, smem, stream>>>(args...);
+    count_launch();
+    return cuda_status(cudaGetLastError());
+}
+
+template <typename Kernel, typename... Args>
 static int launch_cluster(Kernel kern, int cluster, int grid, int threads, size_t smem, cudaStream_t stream,
                           Args... args) {
     cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = cluster;
-    attr[1].val.clusterDim.y = 1;
-    attr[1].val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cfg.attrs = attr;
-    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    cfg.numAttrs = 1;
     if (cudaLaunchKernelEx(&cfg, kern, args...) != cudaSuccess) return NVFP4_ERR_CUDA;
     count_launch();
     return cuda_status(cudaGetLastError());
-}
-
-template <typename... Args, typename Kernel>
-static int launch(Kernel kern, int grid, int threads, size_t smem, cudaStream_t stream, Args... args) {
-    return launch_cluster<Args...>(kern, 1, grid, threads, smem, stream, args...);
 }
 
 template <typename T, int NI, bool SIGMOID>
@@ -609,14 +597,14 @@ static int route_t(const RouteParams &p, cudaStream_t s) {
     if (smem > 32768 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                              (int)smem) != cudaSuccess)
         return NVFP4_ERR_CUDA;
-    if (p.chunks == 1) return launch<RouteParams>(kern, 1, kRouteThreads, smem, s, p);
+    if (p.chunks == 1) return launch(kern, 1, kRouteThreads, smem, s, p);
     const int grid = (p.chunks + kClusterChunks - 1) / kClusterChunks * kClusterChunks;
-    int st = launch_cluster<RouteParams>(kern, kClusterChunks, grid, kRouteThreads, smem, s, p);
+    int st = launch_cluster(kern, kClusterChunks, grid, kRouteThreads, smem, s, p);
     if (st) return st;
     if (smem > 32768 && cudaFuncSetAttribute(moe_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                              (int)smem) != cudaSuccess)
         return NVFP4_ERR_CUDA;
-    return launch<RouteParams>(moe_rows_kernel, p.chunks, kRouteThreads, smem, s, p);
+    return launch(moe_rows_kernel, p.chunks, kRouteThreads, smem, s, p);
 }
 
 template <typename T, bool SIGMOID>
@@ -635,8 +623,7 @@ static int route(const RouteParams &p, cudaStream_t s) {
 template <typename T, int NI>
 static int route_backward_t(const void *logits, const float *dw, const int *experts, void *dl, int n, int E, int k,
                             int sg, int rn, float scale, cudaStream_t s) {
-    return launch<const T *, const float *, const int *, T *, int, int, int, int, int, float>(
-        moe_route_backward_kernel<T, NI>, (n + 7) / 8, 256, 0, s, static_cast<const T *>(logits), dw, experts,
+    return launch(moe_route_backward_kernel<T, NI>, (n + 7) / 8, 256, 0, s, static_cast<const T *>(logits), dw, experts,
         static_cast<T *>(dl), n, E, k, sg, rn, scale);
 }
 
@@ -762,7 +749,7 @@ int nvfp4_moe_dispatch(const void *X, const int32_t *rows, const int32_t *m_offs
     p.k = top_k;
     p.E = E;
     p.s = moe::move_shape(K);
-    return moe::launch<moe::MoveParams>(moe::moe_dispatch_kernel, (T + p.s.tokens - 1) / p.s.tokens * p.s.slabs,
+    return moe::launch(moe::moe_dispatch_kernel, (T + p.s.tokens - 1) / p.s.tokens * p.s.slabs,
                                         moe::kMoveThreads, 0, static_cast<cudaStream_t>(stream), p);
 }
 
@@ -789,8 +776,8 @@ int nvfp4_moe_combine(const void *X_rows, int dtype, const int32_t *rows, const 
     const int grid = (T + p.s.tokens - 1) / p.s.tokens * p.s.slabs;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     return dtype == NVFP4_BF16
-               ? moe::launch<moe::MoveParams>(moe::moe_combine_kernel<__nv_bfloat16>, grid, moe::kMoveThreads, 0, s, p)
-               : moe::launch<moe::MoveParams>(moe::moe_combine_kernel<__half>, grid, moe::kMoveThreads, 0, s, p);
+               ? moe::launch(moe::moe_combine_kernel<__nv_bfloat16>, grid, moe::kMoveThreads, 0, s, p)
+               : moe::launch(moe::moe_combine_kernel<__half>, grid, moe::kMoveThreads, 0, s, p);
 }
 
 int nvfp4_moe_combine_backward(const void *dY, const void *X_rows, int dtype, const int32_t *rows,
@@ -821,9 +808,9 @@ int nvfp4_moe_combine_backward(const void *dY, const void *X_rows, int dtype, co
     p.s = moe::move_shape(K);
     const int grid = (T + p.s.tokens - 1) / p.s.tokens;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return dtype == NVFP4_BF16 ? moe::launch<moe::MoveParams>(moe::moe_combine_backward_kernel<__nv_bfloat16>, grid,
+    return dtype == NVFP4_BF16 ? moe::launch(moe::moe_combine_backward_kernel<__nv_bfloat16>, grid,
                                                               moe::kMoveThreads, 0, s, p)
-                               : moe::launch<moe::MoveParams>(moe::moe_combine_backward_kernel<__half>, grid,
+                               : moe::launch(moe::moe_combine_backward_kernel<__half>, grid,
                                                               moe::kMoveThreads, 0, s, p);
 }
 
