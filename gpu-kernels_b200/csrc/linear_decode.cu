@@ -9,9 +9,11 @@
 // run the epilogue on them.  No workspace, no atomics, no second launch.
 //
 // The ring is sized so that two CTAs share an SM: the prologue and the reduction of one run
-// under the loads of another.  Measured, M = 1: N=K=4096 7.6 us (4.4 TB/s), N=14336 K=4096
-// 21.7 us (5.4), N=28672 K=8192 73.8 us (6.4 of a copy's 6.55): bound by the weights' bytes,
-// and for the smaller ones by what a launch, the first loads and the cluster's sum take.
+// under the loads of another, and as a programmatic dependent the next call's set-up runs
+// under this one's end (one token, N=K=4096, 12.4 -> 9.4 us a call).  Measured, M = 1:
+// N=K=4096 9.1 us on the GPU, N=14336 K=4096 21.7 us (5.4 TB/s), N=28672 K=8192 73.8 us
+// (6.4 of a copy's 6.55): bound by the weights' bytes, and for the smaller ones by what a
+// launch, the first loads and the cluster's sum take.
 //
 // Warps: 0 TMA producer, 1 MMA issue and TMEM owner, 2-5 read the accumulator out; all six
 // reduce.
@@ -125,6 +127,9 @@ __global__ void __launch_bounds__(kDecThreads)
     const int n_f = (p.features + 127) / 128;
     const int nkb = (p.red + kBlockK - 1) / kBlockK;
     const int kb0 = (int)((int64_t)nkb * split / splits), kb1 = (int)((int64_t)nkb * (split + 1) / splits);
+    // Launched as a programmatic dependent: the set-up above runs while the previous kernel
+    // finishes, nothing of global memory is read or written before it has.
+    grid_dependency_wait();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -177,6 +182,7 @@ __global__ void __launch_bounds__(kDecThreads)
                         phase ^= 1;
                     }
                 }
+                grid_launch_dependents();  // all loads issued: the next kernel may set itself up
                 // the MMAs' last arrivals have to come before the CTA ends
                 for (int s = 0; ok && s < p.stages; s++) {
                     if (!wait_parity(bar_empty + 8 * stage, phase ^ 1, tmo, abort_flag)) {
@@ -338,17 +344,19 @@ int decode_forward(const void *X, int64_t ldx, const void *W, Params p, int K, c
         configured[di.device] = 1;
     }
     cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = p.splits;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.gridDim = dim3((unsigned)grid);
     cfg.blockDim = dim3(kDecThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     if (cudaLaunchKernelEx(&cfg, kern, a, b, p) != cudaSuccess) return NVFP4_ERR_CUDA;
     count_launch();
     return cuda_status(cudaGetLastError());

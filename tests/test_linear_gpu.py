@@ -226,3 +226,24 @@ def test_large_offsets(nv, cuda_dev):
     nv.device_status()
     for a in (0, 131_072 - 8, M - 16):
         R.assert_close(y[a:a + 16], *R.forward64(x[a:a + 16], w, [0, 16], None, "none", None)[:2])
+
+
+def test_refusals(nv, cuda_dev):
+    """Arguments of the wrong shape, type or device raise ValueError; a pointer that is not
+    16-byte aligned is the library's to refuse."""
+    x, w = make((8, 64), torch.bfloat16, 1), make((128, 64), torch.bfloat16, 2)
+    o = offsets([0, 4, 8])
+    for bad in (lambda: nv.linear(x.float(), w), lambda: nv.linear(x, w.half()), lambda: nv.linear(x, w.cpu()),
+                lambda: nv.linear(x[:, :60], w[:, :60].contiguous()), lambda: nv.linear(x, w[:, ::2]),
+                lambda: nv.linear(x, w, bias=w[0]), lambda: nv.linear(x, w, residual=x),
+                lambda: nv.linear(x, w, activation="tanh"), lambda: nv.linear(x, w[:120], activation="swiglu"),
+                lambda: nv.linear(x, w, out=x), lambda: nv.linear(x.t(), w), lambda: nv.linear_grouped(x, w, None),
+                lambda: nv.linear_grouped(x, w, o.long()), lambda: nv.linear_grouped(x, w, o[:1]),
+                lambda: nv.linear_grouped(x, w[:127], o), lambda: nv.linear_backward(x, x, w),
+                lambda: nv.linear_backward(make((8, 128), torch.bfloat16, 3), x, w, activation="relu")):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(nv.NVFP4Error):
+        nv.linear(torch.zeros(8 * 72 + 4, dtype=torch.bfloat16, device="cuda")[4:4 + 8 * 72].view(8, 72)[:, :64], w)
+    with pytest.raises(TypeError):
+        nv.linear(x)

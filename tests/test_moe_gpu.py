@@ -245,3 +245,24 @@ def test_nvfp4_experts_take_the_routing(nv, cuda_dev):
     y16 = nv.moe_combine(nv.linear_grouped(xs, w, r.m_offsets), r)
     nv.device_status()
     assert ((y4.double() - y16.double()).norm() / y16.double().norm()).item() < 0.25
+
+
+def test_refusals(nv, cuda_dev):
+    l = logits_of(8, 16, torch.float32, 1)
+    x = torch.zeros(8, 64, dtype=torch.bfloat16, device="cuda")
+    r = nv.moe_route(l, 2)
+    for bad in (lambda: nv.moe_route(l.double(), 2), lambda: nv.moe_route(l[:, ::2], 2), lambda: nv.moe_route(l[0], 2),
+                lambda: nv.moe_route(l, 2, scoring="tanh"), lambda: nv.moe_route(l, 2, bias=l[0]),
+                lambda: nv.moe_route(l, 2, scoring="sigmoid", bias=l[0].bfloat16()),
+                lambda: nv.moe_dispatch(x[:4], r), lambda: nv.moe_dispatch(x[:, :60].contiguous(), r),
+                lambda: nv.moe_dispatch(x.float(), r), lambda: nv.moe_combine(x, r),
+                lambda: nv.moe_dispatch(x, (r.weights, r.experts)),
+                lambda: nv.moe_combine_backward(x[:4], torch.zeros(16, 64, dtype=torch.bfloat16, device="cuda"), r),
+                lambda: nv.moe_route_backward(r.weights[:4], l, r)):
+        with pytest.raises(ValueError):
+            bad()
+    for k in (0, 17):
+        with pytest.raises(nv.NVFP4Error):
+            nv.moe_route(l, k)
+    with pytest.raises(nv.NVFP4Error):
+        nv.moe_route(torch.zeros(4, 300, device="cuda"), 2)
