@@ -672,7 +672,8 @@ static TokenTile token_tile(int64_t m, int groups, int n_f, int pairs, int red) 
     return best;
 }
 
-// Whether the split-reduction kernel takes a forward call (at most kDecodeTokens rows).  It
+// Whether the split-reduction kernel takes a forward product or an input gradient (at most
+// kDecodeTokens rows).  It
 // wins where 256-feature tiles are too few to stream the weights on every SM; with enough
 // of them the persistent kernel does, without a reduction between CTAs.  Measured (us, this
 // kernel / persistent): N=4096 K=4096 M=1 10.7/16.0, M=64 16.3/16.5, M=128 23.7/17.7;
@@ -691,7 +692,7 @@ template <typename T>
 static int forward_t(const void *X, int64_t ldx, const void *W, Params p, int K, const DeviceInfo &di,
                      cudaStream_t s) {
     const int n_f = (p.features + 255) / 256;
-    if (use_decode(p.m_total, p.groups, n_f, K)) return decode_forward<T>(X, ldx, W, p, K, di, s);
+    if (use_decode(p.m_total, p.groups, n_f, K)) return decode_product<T, kForward>(X, ldx, W, p, K, di, s);
     const TokenTile tt = token_tile(p.m_total, p.groups, n_f, di.sm_count / 2, K);
     p.bt = tt.bt;
     p.wide = tt.wide;
@@ -708,6 +709,7 @@ static int forward_t(const void *X, int64_t ldx, const void *W, Params p, int K,
 template <typename T>
 static int dgrad_t(const void *dZ, const void *W, Params p, int N, const DeviceInfo &di, cudaStream_t s) {
     const int n_f = (p.features + 255) / 256;
+    if (use_decode(p.m_total, p.groups, n_f, N)) return decode_product<T, kDgrad>(dZ, N, W, p, N, di, s);
     const TokenTile tt = token_tile(p.m_total, p.groups, n_f, di.sm_count / 2, N);
     p.bt = tt.bt;
     p.wide = tt.wide;
@@ -724,7 +726,10 @@ static int dgrad_t(const void *dZ, const void *W, Params p, int N, const DeviceI
 template <typename T>
 static int wgrad_t(const void *dZ, const void *X, int64_t ldx, Params p, const DeviceInfo &di, cudaStream_t s) {
     const int n_f = (p.features + 255) / 256;
-    p.bt = 256;
+    // 256 x 256 tiles, or 256 x 128 where the others would leave half the pairs idle: a tile's
+    // time is its tokens' (8192 tokens, N = K = 1024: 52 us in 16 tiles, 39 in 32; but 4096
+    // tokens, N = K = 2048: 36 in 64, 42 in 128)
+    p.bt = (int64_t)p.groups * n_f * ((p.out_cols + 255) / 256) * 2 <= di.sm_count / 2 ? 128 : 256;
     p.strip = 8;
     CUtensorMap a, b, d;
     int st = map_rows<T>(&a, dZ, std::max(p.m_total, 1), p.features, p.features, 64);

@@ -258,10 +258,11 @@ inline int map_gradient(CUtensorMap *m, const void *base, int groups, int N, int
     return encode_tiled(m, tma_type<T>(), 3, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
-// linear_decode.cu: the forward product for at most kDecodeTokens token rows in all.
+// linear_decode.cu: the forward product (B = X, red = K) or the input gradient (B = dZ, red =
+// N) for at most kDecodeTokens token rows in all.
 constexpr int kDecodeTokens = 128;
-template <typename T>
-int decode_forward(const void *X, int64_t ldx, const void *W, Params p, int K, const DeviceInfo &di, cudaStream_t s);
+template <typename T, int FORM>
+int decode_product(const void *B, int64_t ldb, const void *W, Params p, int red, const DeviceInfo &di, cudaStream_t s);
 
 }  // namespace linear
 }  // namespace nvfp4

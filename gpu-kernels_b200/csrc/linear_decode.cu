@@ -1,5 +1,5 @@
-// linear_decode.cu — the 16-bit linear layer for few tokens (a decode step): bound by
-// streaming the weights once.
+// linear_decode.cu — the 16-bit linear layer, or its input gradient, for few tokens (a decode
+// step): bound by streaming the weights once.
 //
 // One CTA multiplies 128 weight rows (the MMA's M) by the tokens (its N, a multiple of 16)
 // over a part of the reduction; a cluster of up to 8 CTAs splits the reduction of a tile, so
@@ -88,11 +88,11 @@ __device__ __forceinline__ void put8(void *dst, int64_t at, const float (&v)[8])
     *reinterpret_cast<uint4 *>(static_cast<T *>(dst) + at) = pack8<T>(v);
 }
 
-template <typename T>
+template <typename T, int FORM>
 __global__ void __launch_bounds__(kDecThreads)
     linear_decode_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                          const Params p) {
-    constexpr bool kBf16 = !std::is_same<T, __half>::value;
+    constexpr bool kBf16 = !std::is_same<T, __half>::value, kAmn = FORM == kDgrad;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t *base_ptr = smem_raw + (base - smem_u32(smem_raw));
@@ -174,7 +174,12 @@ __global__ void __launch_bounds__(kDecThreads)
                     mbar_arrive_expect_tx(bar, bytes);
                     issued |= 1u << stage;
                     parity = (parity & ~(1u << stage)) | (phase << stage);
-                    tma_load_3d(dA, &tmap_a, bar, kb * kBlockK, f * 128, g);
+                    if constexpr (kAmn) {
+                        tma_load_3d(dA, &tmap_a, bar, f * 128, kb * kBlockK, g);
+                        tma_load_3d(dA + 8192, &tmap_a, bar, f * 128 + 64, kb * kBlockK, g);
+                    } else {
+                        tma_load_3d(dA, &tmap_a, bar, kb * kBlockK, f * 128, g);
+                    }
                     for (int c = 0; c < n16; c += 16)
                         tma_load_2d(dA + kTileBytes + c * 128, &tmap_b, bar, kb * kBlockK, r0 + c);
                     if (++stage == (uint32_t)p.stages) {
@@ -204,8 +209,8 @@ __global__ void __launch_bounds__(kDecThreads)
             __syncwarp();
         } else if (warp == 1) {
             if (elect_one()) {
-                const uint32_t idesc = idesc_f16(kBf16, false, false, 128, (uint32_t)n16);
-                const uint64_t a_desc = operand_desc<false>(base), b_desc = operand_desc<false>(base + kTileBytes);
+                const uint32_t idesc = idesc_f16(kBf16, kAmn, false, 128, (uint32_t)n16);
+                const uint64_t a_desc = operand_desc<kAmn>(base), b_desc = operand_desc<false>(base + kTileBytes);
                 uint32_t stage = 0, phase = 0;
                 for (int kb = kb0; kb < kb1; kb++) {
                     if (!spin_parity(bar_full + 8 * stage, phase, tmo, abort_flag)) {
@@ -217,7 +222,7 @@ __global__ void __launch_bounds__(kDecThreads)
                     const uint64_t b = b_desc + (uint64_t)(stage * (slot >> 4));
                     const int steps = min(4, (p.red - kb * kBlockK + 15) / 16);
                     for (int j = 0; j < steps; j++)
-                        mma_f16(tmem_base, a + j * kStep16<false>, b + j * kStep16<false>, idesc,
+                        mma_f16(tmem_base, a + j * kStep16<kAmn>, b + j * kStep16<false>, idesc,
                                 kb != kb0 || j != 0 ? 1u : 0u);
                     mma_commit(bar_empty + 8 * stage);
                     if (++stage == (uint32_t)p.stages) {
@@ -315,13 +320,13 @@ __global__ void __launch_bounds__(kDecThreads)
     }
 }
 
-template <typename T>
-int decode_forward(const void *X, int64_t ldx, const void *W, Params p, int K, const DeviceInfo &di, cudaStream_t s) {
+template <typename T, int FORM>
+int decode_product(const void *X, int64_t ldx, const void *W, Params p, int red, const DeviceInfo &di, cudaStream_t s) {
     if (p.m_total > kDecodeTokens) return NVFP4_ERR_SHAPE;
     const int n_f = (p.features + 127) / 128;
     const int64_t tiles = (int64_t)n_f * std::min(p.groups, p.m_total);
-    const int nkb = (K + kBlockK - 1) / kBlockK;
-    p.red = K;
+    const int nkb = (red + kBlockK - 1) / kBlockK;
+    p.red = red;
     p.ncap = (p.m_total + 15) & ~15;
     // split while every CTA still fits on the GPU at once (two an SM) and has 4 slots to load
     p.splits = 1;
@@ -333,10 +338,11 @@ int decode_forward(const void *X, int64_t ldx, const void *W, Params p, int K, c
     p.stages = std::max(2, std::min(kDecMaxStages, (kDecSmem - 1024 - kDecBarBytes) / slot));
     const int smem = p.stages * slot + kDecBarBytes + 1024;
     CUtensorMap a, b;
-    int st = map_weight<T>(&a, W, p.groups, p.features, K, 128);
-    if (!st) st = map_rows<T>(&b, X, p.m_total, K, ldx, 16);
+    int st = FORM == kDgrad ? map_weight<T>(&a, W, p.groups, red, p.features, 64)
+                            : map_weight<T>(&a, W, p.groups, p.features, red, 128);
+    if (!st) st = map_rows<T>(&b, X, p.m_total, red, ldx, 16);
     if (st) return st;
-    auto kern = linear_decode_kernel<T>;
+    auto kern = linear_decode_kernel<T, FORM>;
     static int configured[64] = {};
     if (!configured[di.device]) {
         if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kDecSmem) != cudaSuccess)
@@ -362,10 +368,13 @@ int decode_forward(const void *X, int64_t ldx, const void *W, Params p, int K, c
     return cuda_status(cudaGetLastError());
 }
 
-template int decode_forward<__nv_bfloat16>(const void *, int64_t, const void *, Params, int, const DeviceInfo &,
-                                           cudaStream_t);
-template int decode_forward<__half>(const void *, int64_t, const void *, Params, int, const DeviceInfo &,
-                                    cudaStream_t);
+#define INSTANCE(T, FORM) \
+    template int decode_product<T, FORM>(const void *, int64_t, const void *, Params, int, const DeviceInfo &, cudaStream_t)
+INSTANCE(__nv_bfloat16, kForward);
+INSTANCE(__half, kForward);
+INSTANCE(__nv_bfloat16, kDgrad);
+INSTANCE(__half, kDgrad);
+#undef INSTANCE
 
 }  // namespace linear
 }  // namespace nvfp4

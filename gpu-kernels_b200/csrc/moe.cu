@@ -3,10 +3,10 @@
 // movement of token rows to expert order and back, and the gradients of all of them.
 //
 // Measured: router of 16 tokens, 64 experts, one launch, 4.1 us; 16381 tokens, 256 experts, 8
-// choices with a bias 31 us in two launches (28 us for the choice, bound by instruction issue: some
-// 900 a token, a third of them the 256 exact sigmoids that the ranking needs; its bytes would
-// take 3 us).  Dispatch, combine and its gradient of 8191 tokens x 8 x 2048: 47, 48 and 94 us =
-// 6.4, 6.3 and 6.1 TB/s of a copy's 6.55.
+// choices with a bias 28 us in two launches, most of it the choice, bound by instruction issue
+// (its bytes would take 3 us); ranking every expert exactly, with a sort in each lane, 31 us.
+// Dispatch, combine and its gradient of 8191 tokens x 8 x 2048: 47, 48 and 94 us = 6.4, 6.3
+// and 6.1 TB/s of a copy's 6.55.
 //
 // Every result is computed in a fixed order, so it has the same bits on every call: rows
 // are numbered by counting bits, never by the order in which atomics arrive.
