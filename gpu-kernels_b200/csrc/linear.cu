@@ -10,9 +10,10 @@
 // for "wide" tiles, one tile of up to 512 tokens uses both: each A tile is then read once for
 // twice the tokens, which pays where there is only one round of tiles to run anyway.
 //
-// Launched in plain stream order, as the gradient's other kernels are: as programmatic
-// dependents of each other they gained nothing (415 us a step of 64 experts either way) and
-// stopped for good once in about 10^5 steps, none of their bounded waits running.
+// Launched in plain stream order, as all kernels of the gradient are, the split-reduction
+// kernel's input gradient among them: as programmatic dependents of each other they gained
+// nothing (415 us a step of 64 experts either way) and stopped for good once in about 10^5
+// steps, none of their bounded waits running.  The cause was not found.
 //
 // Large products run at the rate of the library's own 16-bit product, both held by the
 // power cap (N = M = K = 8192, back to back: 780-805 us = 1.37-1.41 PFLOP/s against 745-758;
@@ -613,7 +614,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
 // ------------------------------------------------------------------------- host side
 template <typename T, int FORM>
-static int launch_pair(const CUtensorMap &a, const CUtensorMap &b, const CUtensorMap &d, Params p, int64_t tiles,
+static int launch_pair(const CUtensorMap &a, const CUtensorMap &b, const CUtensorMap &d, Params p, const Plan &plan,
                        const DeviceInfo &di, cudaStream_t stream) {
     auto kern = linear_pair_kernel<T, FORM>;
     static int configured[64] = {};
@@ -622,11 +623,11 @@ static int launch_pair(const CUtensorMap &a, const CUtensorMap &b, const CUtenso
             return NVFP4_ERR_CUDA;
         configured[di.device] = 1;
     }
-    if (tiles > INT_MAX) return NVFP4_ERR_SHAPE;
-    const int ring = kRingBytes - (FORM == kWgrad ? kTileBytes : 0);
-    p.stages = std::min(kMaxStages, ring / (kTileBytes + p.bt * 64 * (1 + p.wide)));
+    if (plan.tiles > INT_MAX) return NVFP4_ERR_SHAPE;
+    p.stages = plan.stages;
+    p.strip = 8;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(2 * (unsigned)std::min<int64_t>(tiles, di.sm_count / 2));
+    cfg.gridDim = dim3(2 * (unsigned)std::min<int64_t>(plan.tiles, di.sm_count / 2));
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = kSmem;
     cfg.stream = stream;
@@ -688,56 +689,69 @@ static bool use_decode(int m, int groups, int n_f, int K) {
     return tiles <= 18 && K >= 8192;
 }
 
+Plan make_plan(int form, int groups, bool ragged, int m_total, int features, int red, int sm_count) {
+    Plan plan = {};
+    const int n_f = (features + 255) / 256, pairs = sm_count / 2;
+    if (form == kWgrad) {
+        // 256 x 256 tiles, or 256 x 128 where the others would leave half the pairs idle: a
+        // tile's time is its tokens' (8192 tokens, N = K = 1024: 52 us in 16 tiles, 39 in 32;
+        // but 4096 tokens, N = K = 2048: 36 in 64, 42 in 128)
+        plan.bt = (int64_t)groups * n_f * ((red + 255) / 256) * 2 <= pairs ? 128 : 256;
+        plan.tiles = (int64_t)groups * n_f * ((red + plan.bt - 1) / plan.bt);
+    } else {
+        if (use_decode(m_total, groups, n_f, red)) {
+            plan_decode(form, groups, m_total, features, red, sm_count, &plan);
+            return plan;
+        }
+        const TokenTile tt = token_tile(m_total, groups, n_f, pairs, red);
+        plan.bt = tt.bt;
+        plan.wide = tt.wide;
+        plan.tiles = ((m_total + plan.bt - 1) / plan.bt + (ragged ? groups : 0)) * (int64_t)n_f;
+    }
+    const int ring = kRingBytes - (form == kWgrad ? kTileBytes : 0);
+    plan.stages = std::min(kMaxStages, ring / (kTileBytes + plan.bt * 64 * (1 + plan.wide)));
+    return plan;
+}
+
 template <typename T>
 static int forward_t(const void *X, int64_t ldx, const void *W, Params p, int K, const DeviceInfo &di,
                      cudaStream_t s) {
-    const int n_f = (p.features + 255) / 256;
-    if (use_decode(p.m_total, p.groups, n_f, K)) return decode_product<T, kForward>(X, ldx, W, p, K, di, s);
-    const TokenTile tt = token_tile(p.m_total, p.groups, n_f, di.sm_count / 2, K);
-    p.bt = tt.bt;
-    p.wide = tt.wide;
-    p.strip = 8;
+    const Plan plan = make_plan(kForward, p.groups, p.m_offsets, p.m_total, p.features, K, di.sm_count);
+    if (plan.decode) return decode_product<T, kForward>(X, ldx, W, p, plan, K, di, s);
+    p.bt = plan.bt;
+    p.wide = plan.wide;
     p.red = K;
     CUtensorMap a, b;
     int st = map_weight<T>(&a, W, p.groups, p.features, K, 128);
     if (!st) st = map_rows<T>(&b, X, p.m_total, K, ldx, p.bt / 2);
     if (st) return st;
-    const int64_t token_tiles = (p.m_total + p.bt - 1) / p.bt + (p.m_offsets ? p.groups : 0);
-    return launch_pair<T, kForward>(a, b, b, p, token_tiles * n_f, di, s);
+    return launch_pair<T, kForward>(a, b, b, p, plan, di, s);
 }
 
 template <typename T>
 static int dgrad_t(const void *dZ, const void *W, Params p, int N, const DeviceInfo &di, cudaStream_t s) {
-    const int n_f = (p.features + 255) / 256;
-    if (use_decode(p.m_total, p.groups, n_f, N)) return decode_product<T, kDgrad>(dZ, N, W, p, N, di, s);
-    const TokenTile tt = token_tile(p.m_total, p.groups, n_f, di.sm_count / 2, N);
-    p.bt = tt.bt;
-    p.wide = tt.wide;
-    p.strip = 8;
+    const Plan plan = make_plan(kDgrad, p.groups, p.m_offsets, p.m_total, p.features, N, di.sm_count);
+    if (plan.decode) return decode_product<T, kDgrad>(dZ, N, W, p, plan, N, di, s);
+    p.bt = plan.bt;
+    p.wide = plan.wide;
     p.red = N;
     CUtensorMap a, b;
     int st = map_weight<T>(&a, W, p.groups, N, p.features, 64);
     if (!st) st = map_rows<T>(&b, dZ, p.m_total, N, N, p.bt / 2);
     if (st) return st;
-    const int64_t token_tiles = (p.m_total + p.bt - 1) / p.bt + (p.m_offsets ? p.groups : 0);
-    return launch_pair<T, kDgrad>(a, b, b, p, token_tiles * n_f, di, s);
+    return launch_pair<T, kDgrad>(a, b, b, p, plan, di, s);
 }
 
 template <typename T>
 static int wgrad_t(const void *dZ, const void *X, int64_t ldx, Params p, const DeviceInfo &di, cudaStream_t s) {
-    const int n_f = (p.features + 255) / 256;
-    // 256 x 256 tiles, or 256 x 128 where the others would leave half the pairs idle: a tile's
-    // time is its tokens' (8192 tokens, N = K = 1024: 52 us in 16 tiles, 39 in 32; but 4096
-    // tokens, N = K = 2048: 36 in 64, 42 in 128)
-    p.bt = (int64_t)p.groups * n_f * ((p.out_cols + 255) / 256) * 2 <= di.sm_count / 2 ? 128 : 256;
-    p.strip = 8;
+    const Plan plan = make_plan(kWgrad, p.groups, p.m_offsets, p.m_total, p.features, p.out_cols, di.sm_count);
+    p.bt = plan.bt;
     CUtensorMap a, b, d;
     int st = map_rows<T>(&a, dZ, std::max(p.m_total, 1), p.features, p.features, 64);
     if (!st) st = map_rows<T>(&b, X, std::max(p.m_total, 1), p.out_cols, ldx, 64);
     if (!st) st = map_gradient<T>(&d, p.y, p.groups, p.features, p.out_cols);
     if (st) return st;
-    const int64_t tiles = (int64_t)p.groups * n_f * ((p.out_cols + p.bt - 1) / p.bt);
-    return launch_pair<T, kWgrad>(a, b, d, p, tiles, di, s);
+    return launch_pair<T, kWgrad>(a, b, d, p, plan, di, s);
 }
 
 // Sizes and pointers that the entry points have in common.

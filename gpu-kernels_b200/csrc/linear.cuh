@@ -258,11 +258,26 @@ inline int map_gradient(CUtensorMap *m, const void *base, int groups, int N, int
     return encode_tiled(m, tma_type<T>(), 3, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
+// How a product is launched, from its sizes and the GPU's SM count alone.
+struct Plan {
+    int decode;        // 1: the split-reduction kernel, 0: the persistent CTA-pair kernel
+    int bt, wide;      // pair: tokens of a tile part (wgrad: columns of a tile), two parts a tile
+    int splits;        // decode: CTAs that share a tile's reduction
+    int stages;        // ring slots
+    int programmatic;  // launched as a programmatic dependent of the previous kernel
+    int64_t tiles;     // pair: tiles, an upper bound for row groups; decode: CTAs
+};
+// linear.cu.  features: the output's (N, for the input gradient K); red: the reduction (K, for
+// the input gradient N; the weight gradient's columns K).
+Plan make_plan(int form, int groups, bool ragged, int m_total, int features, int red, int sm_count);
+
 // linear_decode.cu: the forward product (B = X, red = K) or the input gradient (B = dZ, red =
 // N) for at most kDecodeTokens token rows in all.
 constexpr int kDecodeTokens = 128;
+void plan_decode(int form, int groups, int m_total, int features, int red, int sm_count, Plan *plan);
 template <typename T, int FORM>
-int decode_product(const void *B, int64_t ldb, const void *W, Params p, int red, const DeviceInfo &di, cudaStream_t s);
+int decode_product(const void *B, int64_t ldb, const void *W, Params p, const Plan &plan, int red, const DeviceInfo &di,
+                   cudaStream_t s);
 
 }  // namespace linear
 }  // namespace nvfp4

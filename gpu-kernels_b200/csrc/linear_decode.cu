@@ -127,8 +127,8 @@ __global__ void __launch_bounds__(kDecThreads)
     const int n_f = (p.features + 127) / 128;
     const int nkb = (p.red + kBlockK - 1) / kBlockK;
     const int kb0 = (int)((int64_t)nkb * split / splits), kb1 = (int)((int64_t)nkb * (split + 1) / splits);
-    // Launched as a programmatic dependent: the set-up above runs while the previous kernel
-    // finishes, nothing of global memory is read or written before it has.
+    // As a programmatic dependent (plan_decode) the set-up above runs while the previous kernel
+    // finishes; nothing of global memory is read or written before it has.
     grid_dependency_wait();
     tc_fence_before();
     __syncthreads();
@@ -320,23 +320,34 @@ __global__ void __launch_bounds__(kDecThreads)
     }
 }
 
-template <typename T, int FORM>
-int decode_product(const void *X, int64_t ldx, const void *W, Params p, int red, const DeviceInfo &di, cudaStream_t s) {
-    if (p.m_total > kDecodeTokens) return NVFP4_ERR_SHAPE;
-    const int n_f = (p.features + 127) / 128;
-    const int64_t tiles = (int64_t)n_f * std::min(p.groups, p.m_total);
+void plan_decode(int form, int groups, int m_total, int features, int red, int sm_count, Plan *plan) {
+    const int n_f = (features + 127) / 128;
+    const int64_t tiles = (int64_t)n_f * std::min(groups, m_total);
     const int nkb = (red + kBlockK - 1) / kBlockK;
+    plan->decode = 1;
+    // split while every CTA still fits on the GPU at once (two an SM) and has 4 slots to load
+    plan->splits = 1;
+    while (plan->splits < kDecMaxSplits && tiles * plan->splits * 2 <= 2 * sm_count && nkb >= plan->splits * 8)
+        plan->splits *= 2;
+    // use_decode() keeps the grid within two CTAs an SM, so all of them are resident at once
+    plan->tiles = tiles * plan->splits;
+    const int slot = kTileBytes + ((m_total + 15) & ~15) * 128;
+    plan->stages = std::max(2, std::min(kDecMaxStages, (kDecSmem - 1024 - kDecBarBytes) / slot));
+    // The forward form only.  A programmatic dependent inside the gradient's launches is what
+    // once stopped a stream (linear.cu), so the input gradient waits its turn.
+    plan->programmatic = form == kForward;
+}
+
+template <typename T, int FORM>
+int decode_product(const void *X, int64_t ldx, const void *W, Params p, const Plan &plan, int red, const DeviceInfo &di,
+                   cudaStream_t s) {
+    if (p.m_total > kDecodeTokens) return NVFP4_ERR_SHAPE;
+    if (plan.tiles > INT_MAX) return NVFP4_ERR_SHAPE;
     p.red = red;
     p.ncap = (p.m_total + 15) & ~15;
-    // split while every CTA still fits on the GPU at once (two an SM) and has 4 slots to load
-    p.splits = 1;
-    while (p.splits < kDecMaxSplits && tiles * p.splits * 2 <= 2 * di.sm_count && nkb >= p.splits * 8) p.splits *= 2;
-    const int64_t grid = tiles * p.splits;
-    if (grid > INT_MAX) return NVFP4_ERR_SHAPE;
-    // use_decode() keeps the grid within two CTAs an SM, so all of them are resident at once
-    const int slot = kTileBytes + p.ncap * 128;
-    p.stages = std::max(2, std::min(kDecMaxStages, (kDecSmem - 1024 - kDecBarBytes) / slot));
-    const int smem = p.stages * slot + kDecBarBytes + 1024;
+    p.splits = plan.splits;
+    p.stages = plan.stages;
+    const int smem = p.stages * (kTileBytes + p.ncap * 128) + kDecBarBytes + 1024;
     CUtensorMap a, b;
     int st = FORM == kDgrad ? map_weight<T>(&a, W, p.groups, red, p.features, 64)
                             : map_weight<T>(&a, W, p.groups, p.features, red, 128);
@@ -357,19 +368,20 @@ int decode_product(const void *X, int64_t ldx, const void *W, Params p, int red,
     attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3((unsigned)grid);
+    cfg.gridDim = dim3((unsigned)plan.tiles);
     cfg.blockDim = dim3(kDecThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cfg.attrs = attr;
-    cfg.numAttrs = 2;
+    cfg.numAttrs = plan.programmatic ? 2 : 1;
     if (cudaLaunchKernelEx(&cfg, kern, a, b, p) != cudaSuccess) return NVFP4_ERR_CUDA;
     count_launch();
     return cuda_status(cudaGetLastError());
 }
 
 #define INSTANCE(T, FORM) \
-    template int decode_product<T, FORM>(const void *, int64_t, const void *, Params, int, const DeviceInfo &, cudaStream_t)
+    template int decode_product<T, FORM>(const void *, int64_t, const void *, Params, const Plan &, int, \
+                                         const DeviceInfo &, cudaStream_t)
 INSTANCE(__nv_bfloat16, kForward);
 INSTANCE(__half, kForward);
 INSTANCE(__nv_bfloat16, kDgrad);

@@ -8,6 +8,7 @@
 #include "common.cuh"
 #include "epilogue.cuh"
 #include "gemm_decode.cuh"
+#include "linear.cuh"
 #include "quant_common.cuh"
 
 int epilogue_from(const nvfp4_epilogue *epi, int N, nvfp4::Epi *out);  // capi.cu
@@ -55,6 +56,16 @@ __global__ void __launch_bounds__(256) scale_codes_kernel(const uint16_t *__rest
 using namespace nvfp4;
 
 extern "C" {
+
+int nvfp4_linear_plan(int form, int groups, int ragged, int M, int N, int K, int sm_count, int *plan) {
+    if (form < linear::kForward || form > linear::kWgrad || groups < 1 || M < 1 || N < 8 || K < 8 || sm_count < 2 || !plan)
+        return NVFP4_ERR_INVALID;
+    const bool dgrad = form == linear::kDgrad;
+    const linear::Plan p = linear::make_plan(form, groups, ragged != 0, M, dgrad ? K : N, dgrad ? N : K, sm_count);
+    const int v[6] = {p.decode, p.bt, p.wide, p.splits, p.stages, p.programmatic};
+    std::copy(v, v + 6, plan);
+    return NVFP4_OK;
+}
 
 int nvfp4_gemm_decode_trace(const uint8_t *A, const uint8_t *SFA, const uint8_t *B, const uint8_t *SFB, float alpha,
                             uint16_t *D, int M, int N, int K, void *workspace, size_t workspace_bytes, uint64_t *trace,

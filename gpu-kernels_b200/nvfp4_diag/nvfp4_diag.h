@@ -57,6 +57,15 @@ NVFP4_API int nvfp4_probe_mma_rate(int mode, int iters, double *tflops, double *
  * specification for every bf16 amax. */
 NVFP4_API int nvfp4_scale_codes(const uint16_t *amax_bf16, int64_t n, const float *global_scale, uint8_t *codes,
                                 void *stream);
+/*
+ * nvfp4_linear_plan: how the 16-bit product of these sizes is launched on a GPU of
+ * sm_count SMs, by the code that the launches themselves use (host only).  form 0 forward,
+ * 1 input gradient, 2 weight gradient; ragged: m_offsets is given.  plan receives [0] 1
+ * the split-reduction kernel, 0 the CTA-pair kernel; [1] tokens of a tile part (form 2:
+ * columns of a tile), [2] 1 if tiles have two parts; [3] CTAs that share a tile's
+ * reduction; [4] ring slots; [5] 1 if launched as a programmatic dependent.
+ */
+NVFP4_API int nvfp4_linear_plan(int form, int groups, int ragged, int M, int N, int K, int sm_count, int *plan);
 
 #ifdef __cplusplus
 }

@@ -85,3 +85,19 @@ def test_python_refuses_host_tensors(nv):
                    torch.zeros(9, dtype=torch.int32))
     with pytest.raises(ValueError):
         nv.moe_dispatch(x, r)
+
+
+def test_gradients_are_launched_in_stream_order():
+    """No kernel of the gradient is a programmatic dependent, the few-token input gradient
+    included; the forward product of few tokens is one."""
+    import nvfp4_diag
+    seen = set()
+    for M in (1, 16, 64, 128, 129, 1000):
+        for N, K in ((8, 8), (4096, 4096), (8192, 512), (512, 8192), (14336, 4096)):
+            for groups in (0, 1, 8):
+                for form in ("dgrad", "wgrad"):
+                    p = nvfp4_diag.linear_plan(form, M, N, K, groups)
+                    assert not p["programmatic"], (form, M, N, K, groups)
+                    seen.add((form, p["decode"]))
+    assert ("dgrad", 1) in seen and ("dgrad", 0) in seen
+    assert nvfp4_diag.linear_plan("forward", 1, 4096, 4096)["programmatic"]
