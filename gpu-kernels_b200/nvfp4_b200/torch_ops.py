@@ -102,7 +102,7 @@ def linear_preact(x: torch.Tensor, w: torch.Tensor, m_offsets: Optional[torch.Te
                   bias: Optional[torch.Tensor] = None, activation: str = "none",
                   residual: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """linear with its gradient: (y, z), z the pre-activation kept for the backward pass (an
-    empty tensor without an activation; not differentiable)."""
+    empty tensor without an activation).  z carries no gradient: a loss on it alone raises."""
     if activation == "none":
         return native.linear(x, w, m_offsets, bias, 0, residual, None, False), x.new_empty(0)
     return native.linear(x, w, m_offsets, bias, _activation(activation), residual, None, True)
@@ -134,6 +134,7 @@ def _linear_backward_fake(dy, x, w, m_offsets, z, activation, bias_grad):
 def _linear_context(ctx, inputs, output):
     x, w, m_offsets, bias, activation, residual = inputs
     ctx.save_for_backward(x, w, m_offsets, output[1])
+    ctx.mark_non_differentiable(output[1])
     ctx.activation, ctx.has_bias, ctx.has_residual = activation, bias is not None, residual is not None
     ctx.set_materialize_grads(False)
 

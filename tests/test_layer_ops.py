@@ -22,6 +22,23 @@ def test_fake_shapes_without_a_gpu(nv):
         assert ops.moe_combine(xs, *r).shape == (15, 64)
 
 
+def test_preactivation_carries_no_gradient(nv):
+    """linear_preact's z is not differentiable: a loss on it refuses instead of losing the
+    term in silence."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    ops = torch.ops.nvfp4_b200
+    with FakeTensorMode():
+        x = torch.empty(30, 64, dtype=torch.bfloat16, requires_grad=True)
+        w = torch.empty(96, 64, dtype=torch.bfloat16, requires_grad=True)
+        for act in ("silu", "swiglu", "none"):
+            y, z = ops.linear_preact(x, w, None, None, act)
+            assert y.requires_grad and not z.requires_grad
+            with pytest.raises(RuntimeError, match="does not require grad"):
+                z.float().square().sum().backward()
+            gx, gw = torch.autograd.grad(y.sum(), [x, w])
+            assert gx.shape == x.shape and gw.shape == w.shape
+
+
 @pytest.mark.gpu
 def test_autograd_through_a_layer(nv, cuda_dev):
     ops = torch.ops.nvfp4_b200
