@@ -135,7 +135,8 @@ def _linear_context(ctx, inputs, output):
     x, w, m_offsets, bias, activation, residual = inputs
     ctx.save_for_backward(x, w, m_offsets, output[1])
     ctx.mark_non_differentiable(output[1])
-    ctx.activation, ctx.has_bias, ctx.has_residual = activation, bias is not None, residual is not None
+    ctx.activation, ctx.has_residual = activation, residual is not None
+    ctx.bias_shape = None if bias is None else bias.shape  # dense: [N] or [1, N]
     ctx.set_materialize_grads(False)
 
 
@@ -144,8 +145,9 @@ def _linear_grad(ctx, dy, _dz):
         return None, None, None, None, None, None
     x, w, m_offsets, z = ctx.saved_tensors
     dy = dy.contiguous()
-    dx, dw, db = torch.ops.nvfp4_b200.linear_backward(dy, x, w, m_offsets, z, ctx.activation, ctx.has_bias)
-    return dx, dw, None, db if ctx.has_bias else None, None, dy if ctx.has_residual else None
+    has_bias = ctx.bias_shape is not None
+    dx, dw, db = torch.ops.nvfp4_b200.linear_backward(dy, x, w, m_offsets, z, ctx.activation, has_bias)
+    return dx, dw, None, db.view(ctx.bias_shape) if has_bias else None, None, dy if ctx.has_residual else None
 
 
 linear_preact.register_autograd(_linear_grad, setup_context=_linear_context)

@@ -39,6 +39,19 @@ def test_preactivation_carries_no_gradient(nv):
             assert gx.shape == x.shape and gw.shape == w.shape
 
 
+def test_bias_gradient_has_the_bias_shape(nv):
+    """A dense layer takes its bias as [N] or [1, N] (one row of a grouped layer's)."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    ops = torch.ops.nvfp4_b200
+    with FakeTensorMode():
+        x, w = torch.empty(30, 64, dtype=torch.bfloat16), torch.empty(96, 64, dtype=torch.bfloat16)
+        for offs, shape in ((None, (96,)), (None, (1, 96)), (torch.empty(2, dtype=torch.int32), (1, 96)),
+                            (torch.empty(4, dtype=torch.int32), (3, 32))):
+            b = torch.empty(shape, dtype=torch.bfloat16, requires_grad=True)
+            y, _ = ops.linear_preact(x, w, offs, b, "silu")
+            assert torch.autograd.grad(y.sum(), b)[0].shape == shape
+
+
 @pytest.mark.gpu
 def test_autograd_through_a_layer(nv, cuda_dev):
     ops = torch.ops.nvfp4_b200
