@@ -199,12 +199,12 @@ PyObject *linear(PyObject *const *a) {
     return tuple_of<2>({wrap(std::move(y)), wrap(std::move(z))});
 }
 
-// linear_backward(dy, x, w, m_offsets, preact, activation, bias_grad)
+// linear_backward(dy, x, w, m_offsets, preact, activation, bias_grad, input_grad, weight_grad)
 PyObject *linear_backward(PyObject *const *a) {
     const at::Tensor &dy = tensor(a[0], "dy"), &x = tensor(a[1], "x"), &w = tensor(a[2], "w");
     const at::Tensor *offs = maybe(a[3], "m_offsets"), *z = maybe(a[4], "preact");
     const int act = (int)integer(a[5]);
-    const bool bias_grad = truth(a[6]);
+    const bool bias_grad = truth(a[6]), input_grad = truth(a[7]), weight_grad = truth(a[8]);
     const Rows r = rows_of(x, "x");
     const int G = groups_of(offs, x), N = weight_rows(w, G, r, x), No = out_columns(act, N);
     const auto type = x.scalar_type();
@@ -214,9 +214,10 @@ PyObject *linear_backward(PyObject *const *a) {
         expect(*z, "preact", {r.M, N}, type, x);
     }
     const int32_t *o = static_cast<const int32_t *>(ptr(offs));
-    at::Tensor dz = act ? empty({r.M, N}, type, x) : dy, db, ws;
+    at::Tensor dz = dy, db, ws;
     const Stream s(x);
-    if (act || bias_grad) {
+    if (bias_grad || (act && (input_grad || weight_grad))) {
+        if (act) dz = empty({r.M, N}, type, x);
         size_t bytes = 0;
         if (bias_grad) {
             db = offs ? empty({G, N}, type, x) : empty({N}, type, x);
@@ -228,12 +229,19 @@ PyObject *linear_backward(PyObject *const *a) {
                              bias_grad ? ws.data_ptr() : nullptr, bytes, s.handle),
               "nvfp4_activation_backward");
     }
-    at::Tensor dx = empty({r.M, r.K}, type, x), dw = empty(w.sizes(), type, x);
-    check(L.dgrad(dz.data_ptr(), w.data_ptr(), dx.data_ptr(), o, G, r.M, N, r.K, r.dtype, s.handle),
-          "nvfp4_linear_dgrad");
-    check(L.wgrad(dz.data_ptr(), x.data_ptr(), r.pitch, dw.data_ptr(), o, G, r.M, N, r.K, r.dtype, s.handle),
-          "nvfp4_linear_wgrad");
-    return tuple_of<3>({wrap(std::move(dx)), wrap(std::move(dw)), bias_grad ? wrap(std::move(db)) : none()});
+    at::Tensor dx, dw;
+    if (input_grad) {
+        dx = empty({r.M, r.K}, type, x);
+        check(L.dgrad(dz.data_ptr(), w.data_ptr(), dx.data_ptr(), o, G, r.M, N, r.K, r.dtype, s.handle),
+              "nvfp4_linear_dgrad");
+    }
+    if (weight_grad) {
+        dw = empty(w.sizes(), type, x);
+        check(L.wgrad(dz.data_ptr(), x.data_ptr(), r.pitch, dw.data_ptr(), o, G, r.M, N, r.K, r.dtype, s.handle),
+              "nvfp4_linear_wgrad");
+    }
+    return tuple_of<3>({input_grad ? wrap(std::move(dx)) : none(), weight_grad ? wrap(std::move(dw)) : none(),
+                        bias_grad ? wrap(std::move(db)) : none()});
 }
 
 struct Logits {
@@ -405,7 +413,7 @@ PyObject *entry(PyObject *, PyObject *const *args, Py_ssize_t n) {
 }
 
 #define METHOD(name, n) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(&entry<name, n>)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {METHOD(bind, 12),           METHOD(linear, 8),          METHOD(linear_backward, 7),
+PyMethodDef methods[] = {METHOD(bind, 12),           METHOD(linear, 8),          METHOD(linear_backward, 9),
                          METHOD(moe_route, 6),       METHOD(moe_route_backward, 6), METHOD(moe_dispatch, 2),
                          METHOD(moe_combine, 4),     METHOD(moe_combine_backward, 3), {nullptr, nullptr, 0, nullptr}};
 

@@ -49,17 +49,20 @@ def linear_grouped(x: torch.Tensor, w: torch.Tensor, m_offsets: torch.Tensor, bi
 
 
 def linear_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, preact: Optional[torch.Tensor] = None,
-                    activation: str = "none", bias_grad: bool = False):
-    """Gradients (dx [M, K], dw [N, K], db [N] or None) of linear() for dy [M, Nout]; the
-    residual's gradient is dy itself.  preact: linear's z, needed with an activation."""
-    return native.linear_backward(dy, x, w, None, preact, _activation(activation), bias_grad)
+                    activation: str = "none", bias_grad: bool = False, input_grad: bool = True,
+                    weight_grad: bool = True):
+    """Gradients (dx [M, K], dw [N, K], db [N]) of linear() for dy [M, Nout], None for those
+    that are not wanted; the residual's gradient is dy itself.  preact: linear's z, needed
+    with an activation."""
+    return native.linear_backward(dy, x, w, None, preact, _activation(activation), bias_grad, input_grad, weight_grad)
 
 
 def linear_grouped_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, m_offsets: torch.Tensor,
                             preact: Optional[torch.Tensor] = None, activation: str = "none",
-                            bias_grad: bool = False):
-    """Gradients (dx, dw [groups * N, K], db [groups, N] or None) of linear_grouped(); zero
-    for a group without rows and for rows outside every group."""
+                            bias_grad: bool = False, input_grad: bool = True, weight_grad: bool = True):
+    """Gradients (dx, dw [groups * N, K], db [groups, N], None for those that are not wanted)
+    of linear_grouped(); zero for a group without rows and for rows outside every group."""
     if m_offsets is None:
         raise ValueError("m_offsets must be a tensor")
-    return native.linear_backward(dy, x, w, m_offsets, preact, _activation(activation), bias_grad)
+    return native.linear_backward(dy, x, w, m_offsets, preact, _activation(activation), bias_grad, input_grad,
+                                  weight_grad)

@@ -116,26 +116,26 @@ def _linear_preact_fake(x, w, m_offsets=None, bias=None, activation="none", resi
 
 @torch.library.custom_op("nvfp4_b200::linear_backward", mutates_args=(), device_types="cuda")
 def linear_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, m_offsets: Optional[torch.Tensor],
-                    z: torch.Tensor, activation: str,
-                    bias_grad: bool) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """(dx, dw, db); db is empty unless bias_grad."""
-    dx, dw, db = native.linear_backward(dy, x, w, m_offsets, None if activation == "none" else z,
-                                        _activation(activation), bias_grad)
-    return dx, dw, x.new_empty(0) if db is None else db
+                    z: torch.Tensor, activation: str, bias_grad: bool, input_grad: bool = True,
+                    weight_grad: bool = True) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dx, dw, db); empty where they are not wanted."""
+    out = native.linear_backward(dy, x, w, m_offsets, None if activation == "none" else z, _activation(activation),
+                                 bias_grad, input_grad, weight_grad)
+    return tuple(x.new_empty(0) if t is None else t for t in out)
 
 
 @linear_backward.register_fake
-def _linear_backward_fake(dy, x, w, m_offsets, z, activation, bias_grad):
+def _linear_backward_fake(dy, x, w, m_offsets, z, activation, bias_grad, input_grad=True, weight_grad=True):
     groups, N, _ = _out_columns(w, m_offsets, activation)
     db = (0,) if not bias_grad else (N,) if m_offsets is None else (groups, N)
-    return torch.empty_like(x), torch.empty_like(w), x.new_empty(db)
+    return x.new_empty(x.shape if input_grad else 0), w.new_empty(w.shape if weight_grad else 0), x.new_empty(db)
 
 
 def _linear_context(ctx, inputs, output):
     x, w, m_offsets, bias, activation, residual = inputs
     ctx.save_for_backward(x, w, m_offsets, output[1])
     ctx.mark_non_differentiable(output[1])
-    ctx.activation, ctx.has_residual = activation, residual is not None
+    ctx.activation = activation
     ctx.bias_shape = None if bias is None else bias.shape  # dense: [N] or [1, N]
     ctx.set_materialize_grads(False)
 
@@ -145,9 +145,12 @@ def _linear_grad(ctx, dy, _dz):
         return None, None, None, None, None, None
     x, w, m_offsets, z = ctx.saved_tensors
     dy = dy.contiguous()
-    has_bias = ctx.bias_shape is not None
-    dx, dw, db = torch.ops.nvfp4_b200.linear_backward(dy, x, w, m_offsets, z, ctx.activation, has_bias)
-    return dx, dw, None, db.view(ctx.bias_shape) if has_bias else None, None, dy if ctx.has_residual else None
+    for_x, for_w, _, for_bias, _, for_residual = (*ctx.needs_input_grad, *[False] * 6)[:6]  # trailing defaults are left out
+    dx = dw = db = None
+    if for_x or for_w or for_bias:
+        dx, dw, db = torch.ops.nvfp4_b200.linear_backward(dy, x, w, m_offsets, z, ctx.activation, for_bias, for_x, for_w)
+    return (dx if for_x else None, dw if for_w else None, None, db.view(ctx.bias_shape) if for_bias else None, None,
+            dy if for_residual else None)
 
 
 linear_preact.register_autograd(_linear_grad, setup_context=_linear_context)

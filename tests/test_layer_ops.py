@@ -52,6 +52,30 @@ def test_bias_gradient_has_the_bias_shape(nv):
             assert torch.autograd.grad(y.sum(), b)[0].shape == shape
 
 
+def test_frozen_inputs_cost_no_gradient(nv):
+    """The backward pass asks for the gradients that are wanted, no others."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.utils._python_dispatch import TorchDispatchMode
+    ops, seen = torch.ops.nvfp4_b200, []
+
+    class Log(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            out = func(*args, **(kwargs or {}))
+            if func is ops.linear_backward.default:
+                seen.append([tuple(t.shape) for t in out])
+            return out
+
+    for wanted in ((1, 1, 1), (1, 0, 0), (0, 1, 0), (0, 0, 1), (0, 1, 1)):
+        with FakeTensorMode(), Log():
+            x, w, b = (torch.empty(s, dtype=torch.bfloat16, requires_grad=bool(r))
+                       for s, r in zip(((30, 64), (96, 64), (96,)), wanted))
+            ops.linear_preact(x, w, None, b, "silu")[0].sum().backward()
+            for t, r in zip((x, w, b), wanted):
+                assert (t.grad is not None) == bool(r)
+                assert not r or t.grad.shape == t.shape
+        assert seen.pop() == [s if r else (0,) for s, r in zip(((30, 64), (96, 64), (96,)), wanted)]
+
+
 @pytest.mark.gpu
 def test_autograd_through_a_layer(nv, cuda_dev):
     ops = torch.ops.nvfp4_b200

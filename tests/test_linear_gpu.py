@@ -153,6 +153,30 @@ def test_backward_groups(nv, cuda_dev, cuts):
             R.assert_close(a, r, e, n)
 
 
+@pytest.mark.parametrize("M,cuts", [(5, None), (300, None), (300, [0, 100, 100, 290])])
+def test_wanted_gradients_only(nv, cuda_dev, M, cuts):
+    """Leaving out a gradient leaves the others' bits, and launches what is left."""
+    G, N, K = 1 if cuts is None else len(cuts) - 1, 96, 136
+    x, w, dy = make((M, K), torch.bfloat16, 1), make((G * N, K), torch.bfloat16, 2), make((M, N), torch.bfloat16, 3)
+    z = make((M, N), torch.bfloat16, 4)
+
+    def run(**wanted):
+        n = nv.launch_count()
+        if cuts is None:
+            out = nv.linear_backward(dy, x, w, preact=z, activation="silu", **wanted)
+        else:
+            out = nv.linear_grouped_backward(dy, x, w, offsets(cuts), preact=z, activation="silu", **wanted)
+        return out, nv.launch_count() - n
+
+    (dx, dw, db), n = run(bias_grad=True)
+    assert n == 4
+    for want in ((1, 0, 1), (0, 1, 1), (0, 0, 1), (1, 0, 0), (0, 1, 0)):
+        got, n = run(input_grad=bool(want[0]), weight_grad=bool(want[1]), bias_grad=bool(want[2]))
+        assert n == 1 + sum(want)
+        for a, b, on in zip(got, (dx, dw, db), want):
+            assert (a is None) if not on else torch.equal(a, b)
+
+
 @pytest.mark.parametrize("act", R.ACTS)
 def test_gradient_against_differences(nv, cuda_dev, act):
     """<dL/dp, d> against (L(p + h d) - L(p - h d)) / 2h of the 64-bit forward pass, for
