@@ -152,6 +152,19 @@ at::Tensor empty(at::IntArrayRef shape, at::ScalarType type, const at::Tensor &l
     return at::detail::empty_cuda(shape, type, like.device(), std::nullopt);
 }
 
+// `out` may not share memory with an input of the call: tiles are stored while others are
+// still being read.
+void apart(const at::Tensor &out, const at::Tensor *in, const char *name) {
+    if (!in || !out.numel() || !in->numel()) return;
+    const auto end = [](const at::Tensor &t) {
+        int64_t last = 0;
+        for (int64_t d = 0; d < t.dim(); d++) last += (t.size(d) - 1) * t.stride(d);
+        return static_cast<const char *>(t.data_ptr()) + (last + 1) * t.element_size();
+    };
+    if (static_cast<const char *>(out.data_ptr()) < end(*in) && static_cast<const char *>(in->data_ptr()) < end(out))
+        refuse(std::string("out must not share memory with ") + name);
+}
+
 // The current stream of the tensors' device, made current for the call.
 struct Stream {
     explicit Stream(const at::Tensor &t)
@@ -186,8 +199,18 @@ PyObject *linear(PyObject *const *a) {
         else expect(*bias, "bias", {G, N}, type, x);
     }
     if (res) expect(*res, "residual", {r.M, No}, type, x);
-    at::Tensor y = a[6] == Py_None ? empty({r.M, No}, type, x) : expect(tensor(a[6], "out"), "out", {r.M, No}, type, x);
-    at::Tensor z;
+    at::Tensor y, z;
+    if (a[6] == Py_None) {
+        y = empty({r.M, No}, type, x);
+    } else {
+        y = expect(tensor(a[6], "out"), "out", {r.M, No}, type, x);
+        apart(y, &x, "x");
+        apart(y, &w, "w");
+        apart(y, bias, "bias");
+        apart(y, offs, "m_offsets");
+        // the residual itself is fine: each element is read where it is then written
+        if (res && res->data_ptr() != y.data_ptr()) apart(y, res, "residual");
+    }
     const bool preact = truth(a[7]);
     if (preact) z = empty({r.M, N}, type, x);
     const Stream s(x);

@@ -32,7 +32,8 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
     x [M, K] bf16 or fp16 (rows may be a slice of wider ones, 16-byte aligned), w [N, K],
     bias [N], residual [M, N]; activation "none", "relu", "silu", "gelu_tanh" or "swiglu"
     (rows of w and bias interleaved in blocks of 16 gate, 16 up: swiglu_interleave; N/2
-    output columns).  return_preact: also z = x @ w.T + bias [M, N], which linear_backward
+    output columns).  out: where y goes; it may be the residual, and shares memory with no
+    other input.  return_preact: also z = x @ w.T + bias [M, N], which linear_backward
     takes when there is an activation."""
     return native.linear(x, w, None, bias, _activation(activation), residual, out, return_preact)
 

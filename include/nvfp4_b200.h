@@ -348,7 +348,8 @@ enum { NVFP4_BF16 = 0, NVFP4_F16 = 1, NVFP4_F32 = 2 };
  *   [groups, N] or NULL; activation NVFP4_ACT_* (SwiGLU as for nvfp4_gemm_epilogue: gate
  *   and up rows of W interleaved in blocks of 16, N % 32 == 0, N/2 output columns; silu
  *   and gelu from exp, not the tanh approximation); residual [M, Nout] or NULL;
- *   Y [M, Nout]; Z [M, N] receives z (rounded) for the backward pass, or NULL.
+ *   Y [M, Nout]; Z [M, N] receives z (rounded) for the backward pass, or NULL.  Y may be
+ *   the residual; otherwise neither Y nor Z shares memory with an input.
  * With m_offsets, rows of Y (and Z) outside every group are set to zero.
  */
 NVFP4_API int nvfp4_linear(const void *X, int64_t ldx, const void *W, const void *bias, const void *residual, void *Y,

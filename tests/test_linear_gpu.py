@@ -252,6 +252,30 @@ def test_large_offsets(nv, cuda_dev):
         R.assert_close(y[a:a + 16], *R.forward64(x[a:a + 16], w, [0, 16], None, "none", None)[:2])
 
 
+def test_out(nv, cuda_dev):
+    """out is written in place; it may be the residual, and shares memory with no other input."""
+    M, K = 300, 136
+    wide = make((M, 2 * K), torch.bfloat16, 1)
+    x, w, r = wide[:, :K], make((K, K), torch.bfloat16, 2), make((M, K), torch.bfloat16, 3)
+    want = nv.linear(x, w, residual=r, activation="silu")
+    out = torch.empty_like(r)
+    assert nv.linear(x, w, residual=r, activation="silu", out=out) is not None and torch.equal(out, want)
+    nv.linear(x, w, residual=r, activation="silu", out=r)
+    assert torch.equal(r, want)
+    xc, b = x.contiguous(), make((M * K + K,), torch.bfloat16, 4)
+    big = make((M + 1, K), torch.bfloat16, 5)
+    o = torch.zeros(M * K, dtype=torch.int32, device="cuda")
+    for call, name in ((lambda: nv.linear(xc, w, out=xc), "x"), (lambda: nv.linear(big[1:], w, out=big[:M]), "x"),
+                       (lambda: nv.linear(x, w, out=wide.view(-1)[M * K:].view(M, K)), "x"),
+                       (lambda: nv.linear(x[:K], w, out=w), "w"),
+                       (lambda: nv.linear(x, w, bias=b[8:8 + K], out=b[:M * K].view(M, K)), "bias"),
+                       (lambda: nv.linear(x, w, residual=big[1:], out=big[:M]), "residual"),
+                       (lambda: nv.linear_grouped(x, w, o[:2], out=o.view(torch.bfloat16)[:M * K].view(M, K)),
+                        "m_offsets")):
+        with pytest.raises(ValueError, match="share memory with " + name):
+            call()
+
+
 def test_refusals(nv, cuda_dev):
     """Arguments of the wrong shape, type or device raise ValueError; a pointer that is not
     16-byte aligned is the library's to refuse."""
