@@ -165,6 +165,17 @@ void apart(const at::Tensor &out, const at::Tensor *in, const char *name) {
         refuse(std::string("out must not share memory with ") + name);
 }
 
+// Runs f (allocations and calls of the C ABI) without the GIL: a launch waits where the
+// stream's queue is full, and what it waits for may be a host callback that needs the GIL.
+template <typename F>
+int unlocked(F f) {
+    struct Unlock {
+        PyThreadState *state = PyEval_SaveThread();
+        ~Unlock() { PyEval_RestoreThread(state); }
+    } unlock;
+    return f();
+}
+
 // The current stream of the tensors' device, made current for the call.
 struct Stream {
     explicit Stream(const at::Tensor &t)
@@ -200,9 +211,7 @@ PyObject *linear(PyObject *const *a) {
     }
     if (res) expect(*res, "residual", {r.M, No}, type, x);
     at::Tensor y, z;
-    if (a[6] == Py_None) {
-        y = empty({r.M, No}, type, x);
-    } else {
+    if (a[6] != Py_None) {
         y = expect(tensor(a[6], "out"), "out", {r.M, No}, type, x);
         apart(y, &x, "x");
         apart(y, &w, "w");
@@ -212,11 +221,14 @@ PyObject *linear(PyObject *const *a) {
         if (res && res->data_ptr() != y.data_ptr()) apart(y, res, "residual");
     }
     const bool preact = truth(a[7]);
-    if (preact) z = empty({r.M, N}, type, x);
-    const Stream s(x);
-    check(L.linear(x.data_ptr(), r.pitch, w.data_ptr(), ptr(bias), ptr(res), y.data_ptr(),
-                   preact ? z.data_ptr() : nullptr, static_cast<const int32_t *>(ptr(offs)), G, r.M, N, r.K, act,
-                   r.dtype, s.handle),
+    check(unlocked([&] {
+              if (!y.defined()) y = empty({r.M, No}, type, x);
+              if (preact) z = empty({r.M, N}, type, x);
+              const Stream s(x);
+              return L.linear(x.data_ptr(), r.pitch, w.data_ptr(), ptr(bias), ptr(res), y.data_ptr(),
+                              preact ? z.data_ptr() : nullptr, static_cast<const int32_t *>(ptr(offs)), G, r.M, N, r.K,
+                              act, r.dtype, s.handle);
+          }),
           "nvfp4_linear");
     if (!preact) return wrap(std::move(y));
     return tuple_of<2>({wrap(std::move(y)), wrap(std::move(z))});
@@ -237,32 +249,38 @@ PyObject *linear_backward(PyObject *const *a) {
         expect(*z, "preact", {r.M, N}, type, x);
     }
     const int32_t *o = static_cast<const int32_t *>(ptr(offs));
-    at::Tensor dz = dy, db, ws;
-    const Stream s(x);
-    if (bias_grad || (act && (input_grad || weight_grad))) {
-        if (act) dz = empty({r.M, N}, type, x);
-        size_t bytes = 0;
-        if (bias_grad) {
-            db = offs ? empty({G, N}, type, x) : empty({N}, type, x);
-            bytes = L.act_backward_ws(G, r.M, N);
-            ws = empty({(int64_t)(bytes / 4)}, at::kFloat, x);
+    at::Tensor dx, dw, db;
+    const char *where = "nvfp4_activation_backward";
+    const int status = unlocked([&] {
+        at::Tensor dz = dy, ws;
+        const Stream s(x);
+        int st = NVFP4_OK;
+        if (bias_grad || (act && (input_grad || weight_grad))) {
+            if (act) dz = empty({r.M, N}, type, x);
+            size_t bytes = 0;
+            if (bias_grad) {
+                db = offs ? empty({G, N}, type, x) : empty({N}, type, x);
+                bytes = L.act_backward_ws(G, r.M, N);
+                ws = empty({(int64_t)(bytes / 4)}, at::kFloat, x);
+            }
+            st = L.act_backward(dy.data_ptr(), act ? z->data_ptr() : nullptr, act ? dz.data_ptr() : nullptr,
+                                bias_grad ? db.data_ptr() : nullptr, o, G, r.M, N, act, r.dtype,
+                                bias_grad ? ws.data_ptr() : nullptr, bytes, s.handle);
         }
-        check(L.act_backward(dy.data_ptr(), act ? z->data_ptr() : nullptr, act ? dz.data_ptr() : nullptr,
-                             bias_grad ? db.data_ptr() : nullptr, o, G, r.M, N, act, r.dtype,
-                             bias_grad ? ws.data_ptr() : nullptr, bytes, s.handle),
-              "nvfp4_activation_backward");
-    }
-    at::Tensor dx, dw;
-    if (input_grad) {
-        dx = empty({r.M, r.K}, type, x);
-        check(L.dgrad(dz.data_ptr(), w.data_ptr(), dx.data_ptr(), o, G, r.M, N, r.K, r.dtype, s.handle),
-              "nvfp4_linear_dgrad");
-    }
-    if (weight_grad) {
-        dw = empty(w.sizes(), type, x);
-        check(L.wgrad(dz.data_ptr(), x.data_ptr(), r.pitch, dw.data_ptr(), o, G, r.M, N, r.K, r.dtype, s.handle),
-              "nvfp4_linear_wgrad");
-    }
+        if (!st && input_grad) {
+            where = "nvfp4_linear_dgrad";
+            dx = empty({r.M, r.K}, type, x);
+            st = L.dgrad(dz.data_ptr(), w.data_ptr(), dx.data_ptr(), o, G, r.M, N, r.K, r.dtype, s.handle);
+        }
+        if (!st && weight_grad) {
+            where = "nvfp4_linear_wgrad";
+            dw = empty(w.sizes(), type, x);
+            st = L.wgrad(dz.data_ptr(), x.data_ptr(), r.pitch, dw.data_ptr(), o, G, r.M, N, r.K, r.dtype,
+                         s.handle);
+        }
+        return st;
+    });
+    check(status, where);
     return tuple_of<3>({input_grad ? wrap(std::move(dx)) : none(), weight_grad ? wrap(std::move(dw)) : none(),
                         bias_grad ? wrap(std::move(db)) : none()});
 }
@@ -293,17 +311,24 @@ PyObject *moe_route(PyObject *const *a) {
         if (scoring != NVFP4_SCORE_SIGMOID) refuse("a selection bias needs sigmoid scoring");
         expect(*bias, "bias", {r.E}, at::kFloat, l);
     }
-    at::Tensor weights = empty({r.T, k}, at::kFloat, l), experts = empty({r.T, k}, at::kInt, l);
-    at::Tensor rows = empty({r.T, k}, at::kInt, l), offs = empty({r.E + 1}, at::kInt, l), ws;
-    size_t bytes = 0;
-    if (r.T > 64) {  // fewer tokens need none
-        bytes = L.route_ws(r.T, r.E);
-        ws = empty({(int64_t)(bytes / 4)}, at::kInt, l);
-    }
-    const Stream s(l);
-    check(L.route(l.data_ptr(), r.dtype, static_cast<const float *>(ptr(bias)), r.T, r.E, k, scoring, renormalize,
-                  scale, weights.data_ptr<float>(), experts.data_ptr<int>(), rows.data_ptr<int>(),
-                  offs.data_ptr<int>(), bytes ? ws.data_ptr() : nullptr, bytes, s.handle),
+    at::Tensor weights, experts, rows, offs;
+    check(unlocked([&] {
+              weights = empty({r.T, k}, at::kFloat, l);
+              experts = empty({r.T, k}, at::kInt, l);
+              rows = empty({r.T, k}, at::kInt, l);
+              offs = empty({r.E + 1}, at::kInt, l);
+              at::Tensor ws;
+              size_t bytes = 0;
+              if (r.T > 64) {  // fewer tokens need none
+                  bytes = L.route_ws(r.T, r.E);
+                  ws = empty({(int64_t)(bytes / 4)}, at::kInt, l);
+              }
+              const Stream s(l);
+              return L.route(l.data_ptr(), r.dtype, static_cast<const float *>(ptr(bias)), r.T, r.E, k, scoring,
+                             renormalize, scale, weights.data_ptr<float>(), experts.data_ptr<int>(),
+                             rows.data_ptr<int>(), offs.data_ptr<int>(), bytes ? ws.data_ptr() : nullptr, bytes,
+                             s.handle);
+          }),
           "nvfp4_moe_route");
     return tuple_of<4>({wrap(std::move(weights)), wrap(std::move(experts)), wrap(std::move(rows)),
                         wrap(std::move(offs))});
@@ -320,10 +345,13 @@ PyObject *moe_route_backward(PyObject *const *a) {
     const int k = small(e.size(1), "top_k");
     expect(e, "experts", {r.T, k}, at::kInt, l);
     expect(dw, "dweights", {r.T, k}, at::kFloat, l);
-    at::Tensor dl = empty({r.T, r.E}, l.scalar_type(), l);
-    const Stream s(l);
-    check(L.route_backward(dw.data_ptr<float>(), l.data_ptr(), r.dtype, e.data_ptr<int>(), r.T, r.E, k, scoring,
-                           renormalize, scale, dl.data_ptr(), s.handle),
+    at::Tensor dl;
+    check(unlocked([&] {
+              dl = empty({r.T, r.E}, l.scalar_type(), l);
+              const Stream s(l);
+              return L.route_backward(dw.data_ptr<float>(), l.data_ptr(), r.dtype, e.data_ptr<int>(), r.T, r.E, k,
+                                      scoring, renormalize, scale, dl.data_ptr(), s.handle);
+          }),
           "nvfp4_moe_route_backward");
     return wrap(std::move(dl));
 }
@@ -371,9 +399,13 @@ PyObject *moe_dispatch(PyObject *const *a) {
     const at::Tensor &x = matrix16(a[0], "x");
     const Routed r = routed(a[1], x);
     const int K = columns(x, "x", r.T);
-    at::Tensor out = empty({(int64_t)r.T * r.k, K}, x.scalar_type(), x);
-    const Stream s(x);
-    check(L.dispatch(x.data_ptr(), r.rows, r.offs, r.T, r.E, r.k, K, out.data_ptr(), s.handle), "nvfp4_moe_dispatch");
+    at::Tensor out;
+    check(unlocked([&] {
+              out = empty({(int64_t)r.T * r.k, K}, x.scalar_type(), x);
+              const Stream s(x);
+              return L.dispatch(x.data_ptr(), r.rows, r.offs, r.T, r.E, r.k, K, out.data_ptr(), s.handle);
+          }),
+          "nvfp4_moe_dispatch");
     return wrap(std::move(out));
 }
 
@@ -385,9 +417,12 @@ PyObject *moe_combine(PyObject *const *a) {
     const at::Tensor *res = maybe(a[2], "residual");
     if (res) expect(*res, "residual", {r.T, K}, x.scalar_type(), x);
     const float *weights = truth(a[3]) ? r.weights : nullptr;
-    at::Tensor y = empty({r.T, K}, x.scalar_type(), x);
-    const Stream s(x);
-    check(L.combine(x.data_ptr(), dtype16(x), r.rows, weights, ptr(res), r.T, r.k, K, y.data_ptr(), s.handle),
+    at::Tensor y;
+    check(unlocked([&] {
+              y = empty({r.T, K}, x.scalar_type(), x);
+              const Stream s(x);
+              return L.combine(x.data_ptr(), dtype16(x), r.rows, weights, ptr(res), r.T, r.k, K, y.data_ptr(), s.handle);
+          }),
           "nvfp4_moe_combine");
     return wrap(std::move(y));
 }
@@ -398,10 +433,14 @@ PyObject *moe_combine_backward(PyObject *const *a) {
     const Routed r = routed(a[2], x);
     const int K = columns(x, "x_rows", (int64_t)r.T * r.k);
     expect(dy, "dy", {r.T, K}, x.scalar_type(), x);
-    at::Tensor dx = empty({(int64_t)r.T * r.k, K}, x.scalar_type(), x), dw = empty({r.T, r.k}, at::kFloat, x);
-    const Stream s(x);
-    check(L.combine_backward(dy.data_ptr(), x.data_ptr(), dtype16(x), r.rows, r.weights, r.offs, r.T, r.E, r.k, K,
-                             dx.data_ptr(), dw.data_ptr<float>(), s.handle),
+    at::Tensor dx, dw;
+    check(unlocked([&] {
+              dx = empty({(int64_t)r.T * r.k, K}, x.scalar_type(), x);
+              dw = empty({r.T, r.k}, at::kFloat, x);
+              const Stream s(x);
+              return L.combine_backward(dy.data_ptr(), x.data_ptr(), dtype16(x), r.rows, r.weights, r.offs, r.T, r.E,
+                                        r.k, K, dx.data_ptr(), dw.data_ptr<float>(), s.handle);
+          }),
           "nvfp4_moe_combine_backward");
     return tuple_of<2>({wrap(std::move(dx)), wrap(std::move(dw))});
 }

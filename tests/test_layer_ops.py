@@ -1,6 +1,10 @@
 """The torch.library operators of the 16-bit layers and the mixture of experts: schemas and
 fake (shape) implementations on the CPU; on a GPU, autograd through a whole layer gives what
 the direct calls give."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -112,3 +116,33 @@ def test_autograd_through_a_layer(nv, cuda_dev):
     # of a partial sum, which is at most the sum of the terms' magnitudes
     size = dy.float().abs() + nv.moe_dispatch_backward(dxs, route).float().abs() + dxr.float().abs()
     assert ((grads[0].float() - dx).abs() <= 2.0 ** -7 * size).all()
+
+
+GIL = """
+import ctypes, sys, torch
+sys.path.insert(0, "gpu-kernels_b200")
+import nvfp4_b200 as nv
+from nvfp4_b200 import _bind
+from nvfp4_b200._lib import check
+# every entry point answers whether its caller holds the GIL: 0 (no) is the good status
+held = ctypes.cast(ctypes.pythonapi.PyGILState_Check, ctypes.c_void_p).value
+_bind._load().bind(check, *[held] * len(_bind._ENTRIES))
+b, f = torch.bfloat16, torch.float32
+x, w, l = torch.zeros(80, 64, dtype=b, device="cuda"), torch.zeros(64, 64, dtype=b, device="cuda"), \
+    torch.zeros(80, 8, device="cuda")
+i = torch.zeros(80, 1, dtype=torch.int32, device="cuda")
+r = nv.Routing(torch.zeros(80, 1, device="cuda"), i, i, torch.zeros(9, dtype=torch.int32, device="cuda"))
+for call in (lambda: nv.linear(x, w), lambda: nv.linear_backward(x, x, w, preact=x, activation="relu"),
+             lambda: nv.moe_route(l, 2), lambda: nv.moe_route_backward(r.weights, l, r), lambda: nv.moe_dispatch(x, r),
+             lambda: nv.moe_combine(x, r), lambda: nv.moe_combine_backward(x, x, r)):
+    call()
+print("done")
+"""
+
+
+@pytest.mark.gpu
+def test_calls_release_the_gil(cuda_dev):
+    """The library is called without the GIL, as through ctypes."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    out = subprocess.run([sys.executable, "-c", GIL], cwd=root, capture_output=True, text=True, timeout=300)
+    assert out.stdout.strip() == "done", out.stderr[-2000:]
