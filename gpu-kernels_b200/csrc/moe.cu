@@ -11,6 +11,7 @@
 // Every result is computed in a fixed order, so it has the same bits on every call: rows
 // are numbered by counting bits, never by the order in which atomics arrive.
 #include <algorithm>
+#include <atomic>
 #include <climits>
 
 #include "common.cuh"
@@ -658,20 +659,34 @@ static int launch_cluster(Kernel kern, int cluster, int grid, int threads, size_
     return cuda_status(cudaGetLastError());
 }
 
+// The bits of the largest chunk.  The limit is set once per kernel and device, to this size:
+// it is shared by all threads, so a call that set its own could lower it under another's
+// launch.
+constexpr int kMaxBitBytes = kMaxExperts * (kMaxTokens / kMaxChunks / 32) * 4;
+template <typename Kernel>
+static int allow_bits(Kernel kern, std::atomic<bool> *configured) {
+    DeviceInfo di;
+    int st = device_info(&di);
+    if (st) return st;
+    if (configured[di.device]) return NVFP4_OK;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxBitBytes) != cudaSuccess)
+        return NVFP4_ERR_CUDA;
+    configured[di.device] = true;
+    return NVFP4_OK;
+}
+
 template <typename T, int NI, bool SIGMOID>
 static int route_t(const RouteParams &p, cudaStream_t s) {
     auto kern = moe_route_kernel<T, NI, SIGMOID>;
     const size_t smem = (size_t)p.E * (p.chunk / 32) * 4;
-    if (smem > 32768 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             (int)smem) != cudaSuccess)
-        return NVFP4_ERR_CUDA;
+    static std::atomic<bool> configured[64] = {}, configured_rows[64] = {};
+    int st = smem > 32768 ? allow_bits(kern, configured) : NVFP4_OK;
+    if (!st && smem > 32768) st = allow_bits(moe_rows_kernel, configured_rows);
+    if (st) return st;
     if (p.chunks == 1) return launch(kern, 1, kRouteThreads, smem, s, p);
     const int grid = (p.chunks + kClusterChunks - 1) / kClusterChunks * kClusterChunks;
-    int st = launch_cluster(kern, kClusterChunks, grid, kRouteThreads, smem, s, p);
+    st = launch_cluster(kern, kClusterChunks, grid, kRouteThreads, smem, s, p);
     if (st) return st;
-    if (smem > 32768 && cudaFuncSetAttribute(moe_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             (int)smem) != cudaSuccess)
-        return NVFP4_ERR_CUDA;
     return launch(moe_rows_kernel, p.chunks, kRouteThreads, smem, s, p);
 }
 

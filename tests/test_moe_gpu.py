@@ -266,3 +266,38 @@ def test_refusals(nv, cuda_dev):
             nv.moe_route(l, k)
     with pytest.raises(nv.NVFP4Error):
         nv.moe_route(torch.zeros(4, 300, device="cuda"), 2)
+
+
+def test_route_from_two_threads(nv, cuda_dev):
+    """Two threads route numbers of tokens that need different amounts of shared memory (more
+    than 262144 tokens of 256 experts), at the same time: neither call fails, and every row
+    is numbered as by the other calls of the same logits."""
+    import threading
+    E, k, errors = 256, 2, []
+    logits = [torch.randn(T, E, device="cuda", generator=torch.Generator("cuda").manual_seed(T)).bfloat16()
+              for T in (1 << 20, 300_000)]
+    first = [nv.moe_route(l, k) for l in logits]
+    for l, r in zip(logits, first):
+        flat = r.experts.flatten().long()
+        order = torch.sort(flat, stable=True).indices
+        assert torch.equal(r.rows.flatten()[order], torch.arange(len(flat), device="cuda", dtype=torch.int32))
+        assert torch.equal(torch.diff(r.m_offsets), torch.bincount(flat, minlength=E).int())
+        assert torch.equal(r.experts[:, 0].long(), l.float().max(1).indices)
+    torch.cuda.synchronize()
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(300):
+                    r = nv.moe_route(logits[i], k)
+                torch.cuda.current_stream().synchronize()
+                assert all(torch.equal(a, b) for a, b in zip(r, first[i]))
+        except Exception as e:  # noqa: BLE001
+            errors.append(repr(e))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1, 0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
