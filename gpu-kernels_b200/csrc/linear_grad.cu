@@ -110,8 +110,10 @@ __global__ void __launch_bounds__(kGradThreads) activation_backward_kernel(const
     }
 }
 
+// chunks: of the workspace.  Offsets that decrease, which the host cannot see, may count
+// more; none is read past it.
 template <typename T>
-__global__ void __launch_bounds__(256) bias_sum_kernel(const float *partial, T *db, const int *m_offsets, int groups,
+__global__ void __launch_bounds__(256) bias_sum_kernel(const float *partial, T *db, const int *m_offsets, int chunks,
                                                        int m_total, int N) {
     __shared__ int before;  // first chunk of this group
     const int g = blockIdx.y;
@@ -128,7 +130,7 @@ __global__ void __launch_bounds__(256) bias_sum_kernel(const float *partial, T *
     __syncthreads();
     int a, z;
     group_rows(m_offsets, g, m_total, a, z);
-    const int n = (z - a + kGradRows - 1) / kGradRows;
+    const int n = max(0, min((z - a + kGradRows - 1) / kGradRows, chunks - before));
     const int c = blockIdx.x * 256 + threadIdx.x;
     if (c >= N) return;
     const float *src = partial + (int64_t)before * N + c;
@@ -154,7 +156,7 @@ static int activation_backward(const GradParams &p, T *db, cudaStream_t s) {
     int st = launch(activation_backward_kernel<T>, grid, kGradThreads, s, p);
     if (st || !db) return st;
     return launch(bias_sum_kernel<T>, dim3((p.N + 255) / 256, p.groups), 256, s, (const float *)p.partial, db,
-                  p.m_offsets, p.groups, p.m_total, p.N);
+                  p.m_offsets, (int)grad_chunks(p.groups, p.m_total), p.m_total, p.N);
 }
 
 }  // namespace linear

@@ -242,6 +242,22 @@ def test_side_stream_and_graph(nv, cuda_dev):
         R.assert_close(y, *R.forward64(x, w, cuts, None, "none", None)[:2])
 
 
+def test_decreasing_offsets_stay_in_the_workspace(nv, cuda_dev):
+    """Offsets that decrease are a mistake that only the device sees: they count more 64-row
+    chunks than the workspace holds, and none past its end is read."""
+    G, M, N = 64, 640, 64
+    o = offsets([0, M] * (G // 2) + [0])
+    size = nv.lib().nvfp4_activation_backward_workspace_size(G, M, N)
+    ws = torch.full((4 * G * M // 64 * N,), math.nan, device="cuda")  # room for every chunk, NaN past `size`
+    dy = torch.ones(M, N, dtype=torch.bfloat16, device="cuda")
+    db = torch.empty(G, N, dtype=torch.bfloat16, device="cuda")
+    assert size // 4 < G // 2 * M // 64 * N < ws.numel()
+    assert nv.lib().nvfp4_activation_backward(dy.data_ptr(), None, None, db.data_ptr(), o.data_ptr(), G, M, N, 0, 0,
+                                              ws.data_ptr(), size, torch.cuda.current_stream().cuda_stream) == 0
+    nv.device_status()
+    assert (db[0] == M).all() and not db[1].any() and torch.isfinite(db).all()
+
+
 def test_large_offsets(nv, cuda_dev):
     """An output of more than 2^31 elements: the last rows are where they belong."""
     M, N, K = 140_000, 16_384, 64
