@@ -38,7 +38,8 @@ __global__ void __launch_bounds__(kGradThreads) activation_backward_kernel(const
     __shared__ float sums[kGradRowLanes][kGradLanes][17];  // 17: no bank conflicts between units
     if (threadIdx.x < 32) build_tables(p.m_offsets, p.groups, p.m_total, kGradRows, 1, threadIdx.x, tab.r0, tab.r1, tab.c0);
     __syncthreads();
-    const int chunk = blockIdx.y;
+    const int col_blocks = ((p.act == kActSwiglu ? p.N / 2 : p.N) / 8 + kGradLanes - 1) / kGradLanes;
+    const int chunk = blockIdx.x / col_blocks, col_block = blockIdx.x - chunk * col_blocks;
     if (chunk >= tab.c0[p.groups]) return;
     int g = 0, hi = p.groups - 1;
     while (g < hi) {
@@ -48,7 +49,7 @@ __global__ void __launch_bounds__(kGradThreads) activation_backward_kernel(const
     const int row0 = tab.r0[g] + (chunk - tab.c0[g]) * kGradRows, row1 = min(row0 + kGradRows, tab.r1[g]);
     const bool glu = p.act == kActSwiglu;
     const int No = glu ? p.N / 2 : p.N;
-    const int unit = blockIdx.x * kGradLanes + (threadIdx.x & 31), rl = threadIdx.x >> 5;
+    const int unit = col_block * kGradLanes + (threadIdx.x & 31), rl = threadIdx.x >> 5;
     const int col = unit * 8;  // column of dY
     // columns of Z: the same, or the gate's (and 16 further the up's) for SwiGLU
     const int zc = glu ? (col >> 4) * 32 + (col & 15) : col;
@@ -100,7 +101,7 @@ __global__ void __launch_bounds__(kGradThreads) activation_backward_kernel(const
     // one thread a column of the CTA's units: the eight row lanes in order
     const int per_unit = glu ? 16 : 8;
     for (int i = threadIdx.x; i < kGradLanes * per_unit; i += kGradThreads) {
-        const int u = i / per_unit, e = i % per_unit, c = (blockIdx.x * kGradLanes + u) * 8;
+        const int u = i / per_unit, e = i % per_unit, c = (col_block * kGradLanes + u) * 8;
         if (c >= No) continue;
         float s = 0.0f;
 #pragma unroll
@@ -142,6 +143,12 @@ __global__ void __launch_bounds__(256) bias_sum_kernel(const float *partial, T *
 
 static int64_t grad_chunks(int groups, int M) { return ((int64_t)M + kGradRows - 1) / kGradRows + (groups > 1 ? groups : 0); }
 
+// CTAs: chunks x blocks of columns, the columns fastest.
+static int64_t grad_blocks(int groups, int M, int N, int act) {
+    const int No = act == kActSwiglu ? N / 2 : N;
+    return grad_chunks(groups, M) * ((No / 8 + kGradLanes - 1) / kGradLanes);
+}
+
 template <typename Kernel, typename... Args>
 static int launch(Kernel kern, dim3 grid, int threads, cudaStream_t stream, Args... args) {
     kern<<<grid, threads, 0, stream>>>(args...);
@@ -151,8 +158,7 @@ static int launch(Kernel kern, dim3 grid, int threads, cudaStream_t stream, Args
 
 template <typename T>
 static int activation_backward(const GradParams &p, T *db, cudaStream_t s) {
-    const int No = p.act == kActSwiglu ? p.N / 2 : p.N;
-    const dim3 grid((No / 8 + kGradLanes - 1) / kGradLanes, (unsigned)grad_chunks(p.groups, p.m_total));
+    const dim3 grid((unsigned)grad_blocks(p.groups, p.m_total, p.N, p.act));
     int st = launch(activation_backward_kernel<T>, grid, kGradThreads, s, p);
     if (st || !db) return st;
     return launch(bias_sum_kernel<T>, dim3((p.N + 255) / 256, p.groups), 256, s, (const float *)p.partial, db,
@@ -179,7 +185,7 @@ int nvfp4_activation_backward(const void *dY, const void *Z, void *dZ, void *dbi
     if (groups < 1 || (groups > 1 && !m_offsets)) return NVFP4_ERR_INVALID;
     if (groups > linear::kMaxGroups || M < 0 || N < 8 || N % 8 || (activation == NVFP4_ACT_SWIGLU && N % 32))
         return NVFP4_ERR_SHAPE;
-    if (linear::grad_chunks(groups, M) > 65535) return NVFP4_ERR_SHAPE;
+    if (linear::grad_blocks(groups, M, N, activation) > INT_MAX) return NVFP4_ERR_SHAPE;
     const bool act = activation != NVFP4_ACT_NONE;
     if (M && (!dY || (act && (!Z || !dZ)))) return NVFP4_ERR_INVALID;
     if (!act && !dbias) return NVFP4_OK;  // dZ is dY

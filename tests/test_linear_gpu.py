@@ -258,6 +258,18 @@ def test_decreasing_offsets_stay_in_the_workspace(nv, cuda_dev):
     assert (db[0] == M).all() and not db[1].any() and torch.isfinite(db).all()
 
 
+def test_gradient_of_many_rows(nv, cuda_dev):
+    """More 64-row chunks than a grid's second dimension has blocks."""
+    M, N, K = 64 * 65535 + 70, 8, 8
+    g = torch.Generator("cuda").manual_seed(1)
+    x, dy, z = (torch.randn(M, s, device="cuda", generator=g).bfloat16() for s in (K, N, N))
+    w = make((N, K), torch.bfloat16, 2)
+    dx, dw, db = nv.linear_backward(dy, x, w, preact=z, activation="relu", bias_grad=True)
+    nv.device_status()
+    for got, (r, e), n in zip((dx, dw, db), R.backward64(dy, x, w, [0, M], z, "relu"), ("dx", "dw", "db")):
+        R.assert_close(got, r.reshape(got.shape), e.reshape(got.shape), n)
+
+
 def test_large_offsets(nv, cuda_dev):
     """An output of more than 2^31 elements: the last rows are where they belong."""
     M, N, K = 140_000, 16_384, 64
