@@ -759,6 +759,7 @@ static int check_sizes(int groups, const int *m_offsets, int M, int N, int K, in
     if (dtype != NVFP4_BF16 && dtype != NVFP4_F16) return NVFP4_ERR_INVALID;
     if (groups < 1 || (groups > 1 && !m_offsets)) return NVFP4_ERR_INVALID;
     if (groups > kMaxGroups || M < 0 || N < 8 || N % 8 || K < 8 || K % 8) return NVFP4_ERR_SHAPE;
+    if (M > kMaxExtent || N > kMaxExtent || K > kMaxExtent) return NVFP4_ERR_SHAPE;
     if ((int64_t)N * K > ((int64_t)1 << 40) / 2) return NVFP4_ERR_SHAPE;  // a tensor map's strides are below 2^40
     if (reinterpret_cast<uintptr_t>(m_offsets) & 3u) return NVFP4_ERR_ALIGN;
     return NVFP4_OK;

@@ -18,6 +18,7 @@ namespace nvfp4 {
 namespace linear {
 
 constexpr int kMaxGroups = 256;
+constexpr int kMaxExtent = INT32_MAX - 1023;       // of rows and columns: rounding up to a tile stays in 32 bits
 constexpr int kBlockK = 64;                        // reduction elements of a ring slot: one 128-byte swizzle row
 constexpr int kTileBytes = 128 * kBlockK * 2;      // one CTA's A tile: 128 features
 

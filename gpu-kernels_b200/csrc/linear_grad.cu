@@ -185,6 +185,7 @@ int nvfp4_activation_backward(const void *dY, const void *Z, void *dZ, void *dbi
     if (groups < 1 || (groups > 1 && !m_offsets)) return NVFP4_ERR_INVALID;
     if (groups > linear::kMaxGroups || M < 0 || N < 8 || N % 8 || (activation == NVFP4_ACT_SWIGLU && N % 32))
         return NVFP4_ERR_SHAPE;
+    if (M > linear::kMaxExtent || N > linear::kMaxExtent) return NVFP4_ERR_SHAPE;
     if (linear::grad_blocks(groups, M, N, activation) > INT_MAX) return NVFP4_ERR_SHAPE;
     const bool act = activation != NVFP4_ACT_NONE;
     if (M && (!dY || (act && (!Z || !dZ)))) return NVFP4_ERR_INVALID;

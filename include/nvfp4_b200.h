@@ -338,7 +338,7 @@ NVFP4_API uint64_t nvfp4_launch_count(void);
  * Row groups: m_offsets (groups + 1 int32 on the device, non-decreasing, clamped to
  * [0, M]) makes group g the rows [m_offsets[g], m_offsets[g+1]); group g uses weight rows
  * [g*N, (g+1)*N) of W [groups * N, K] and bias row g.  m_offsets NULL with groups = 1: one
- * dense layer over all M rows.  groups <= 256; M >= 0; N, K multiples of 8.
+ * dense layer over all M rows.  groups <= 256; 0 <= M <= 2^31 - 1024; N, K multiples of 8.
  */
 enum { NVFP4_BF16 = 0, NVFP4_F16 = 1, NVFP4_F32 = 2 };
 

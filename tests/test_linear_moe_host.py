@@ -45,6 +45,16 @@ def test_gradient_refusals(nv):
     assert L.nvfp4_activation_backward(P, None, None, None, None, 1, 100, 64, 0, 0, None, 0, None) == 0  # nothing to do
 
 
+def test_extents_that_round_past_32_bits(nv):
+    """The last 1023 sizes below 2^31 would round up past 32 bits inside the kernels."""
+    big, L = (1 << 31) - 1, nv.lib()
+    assert linear(nv, M=big) == SHAPE and linear(nv, N=big - 7, K=8) == SHAPE
+    assert linear(nv, N=8, K=big - 7, ldx=big - 7) == SHAPE
+    assert L.nvfp4_linear_dgrad(P, P, P, None, 1, big, 8, 8, 0, None) == SHAPE
+    assert L.nvfp4_linear_wgrad(P, P, 8, P, None, 1, big, 8, 8, 0, None) == SHAPE
+    assert L.nvfp4_activation_backward(P, P, P, None, None, 1, big, 8, 1, 0, None, 0, None) == SHAPE
+
+
 def route(nv, logits=P, dt=0, bias=None, T=4, E=8, k=2, scoring=0, w=P, e=P, r=P, o=P, ws=None, n=0):
     return nv.lib().nvfp4_moe_route(logits, dt, bias, T, E, k, scoring, 1, 1.0, w, e, r, o, ws, n, None)
 
