@@ -639,7 +639,8 @@ static int launch_pair(const CUtensorMap &a, const CUtensorMap &b, const CUtenso
 // Tokens of a tile.  A slot of 64 reduction elements costs a pair about 150 ns for its 256
 // features plus 1.07 ns a token (measured from 32 to 256 tokens, N = K = 4096), so few wide
 // tiles win, unless their number fills the last round of pairs badly.
-//   dense: the M tokens in n equal tiles, n chosen by rounds x cost; or in wide tiles (two
+//   dense: the M tokens in n equal tiles, n chosen by rounds x cost (by the eight sizes that a
+//     tile can have, so the choice takes as long for a million tokens as for a thousand); or in wide tiles (two
 //     parts that share the A tile, up to 512 tokens), whose epilogue, about 20 ns a token,
 //     no other tile's MMAs hide.  As tiles of 192 / wide tiles of 2 x 192 tokens, us: M=333
 //     N=14344 K=4104 56.6/47.4, M=333 N=14336 K=4096 45.5/41.6; but M=1024 N=K=4096 as
@@ -660,9 +661,11 @@ static TokenTile token_tile(int64_t m, int groups, int n_f, int pairs, int red) 
     double least = 1e300;
     const int nkb = (red + kBlockK - 1) / kBlockK;
     const int64_t n0 = (m + kMaxTokens - 1) / kMaxTokens;
-    for (int64_t n = n0; n <= 4 * n0; n++)
+    for (int bt = kMaxTokens; bt >= 32; bt -= 32) {  // down to a quarter of the fewest tiles' tokens
+        const int64_t n = (m + bt - 1) / bt;
+        if (n > 4 * n0) break;
         for (int wide = 0; wide <= (n > 1 ? 1 : 0); wide++) {
-            const int bt = (int)(((m + n - 1) / n + 31) / 32 * 32), tokens = bt * (1 + wide);
+            const int tokens = bt * (1 + wide);
             const int64_t tiles = (m + tokens - 1) / tokens * n_f, rounds = (tiles + pairs - 1) / pairs;
             const double cost = (double)rounds * nkb * (150.0 + 1.07 * tokens) + (wide ? rounds : 1) * 20.0 * tokens;
             if (cost < least) {
@@ -670,6 +673,7 @@ static TokenTile token_tile(int64_t m, int groups, int n_f, int pairs, int red) 
                 best = {bt, wide};
             }
         }
+    }
     return best;
 }
 

@@ -55,6 +55,18 @@ def test_extents_that_round_past_32_bits(nv):
     assert L.nvfp4_activation_backward(P, P, P, None, None, 1, big, 8, 1, 0, None, 0, None) == SHAPE
 
 
+def test_plan_of_many_tokens_is_quick(nv):
+    """The host's choice of tiles takes as long for 2^31 tokens as for a few."""
+    import time
+
+    import nvfp4_diag
+    nvfp4_diag.lib()
+    t = time.perf_counter()
+    for _ in range(100):
+        p = nvfp4_diag.linear_plan("forward", (1 << 31) - 1024, 8, 4096)
+    assert p["bt"] == 256 and time.perf_counter() - t < 0.1
+
+
 def route(nv, logits=P, dt=0, bias=None, T=4, E=8, k=2, scoring=0, w=P, e=P, r=P, o=P, ws=None, n=0):
     return nv.lib().nvfp4_moe_route(logits, dt, bias, T, E, k, scoring, 1, 1.0, w, e, r, o, ws, n, None)
 
