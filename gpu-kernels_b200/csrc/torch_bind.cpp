@@ -116,7 +116,7 @@ Rows rows_of(const at::Tensor &x, const char *name) {
         refuse(std::string(name) + " must be a 2-D bf16 or fp16 CUDA tensor");
     r.M = small(x.size(0), "the number of rows");
     r.K = small(x.size(1), "the number of columns");
-    r.pitch = r.M > 1 ? x.stride(0) : std::max<int64_t>(r.K, x.stride(0));
+    r.pitch = r.M > 1 ? x.stride(0) : r.K;  // a single row's stride says nothing
     if ((r.K > 1 && x.stride(1) != 1) || r.pitch < r.K) refuse(std::string(name) + " must have contiguous rows");
     if (r.K % 8 || r.pitch % 8 || !r.K)
         refuse(std::string(name) + " must have a multiple of 8 columns, rows 16 bytes aligned");

@@ -105,6 +105,17 @@ def test_strided_rows(nv, cuda_dev, M):
     R.assert_close(dw, ref, e)
 
 
+def test_one_row_of_any_stride(nv, cuda_dev):
+    """The stride of a single row does not matter, whatever it is."""
+    w, dy = make((264, 136), torch.bfloat16, 2), make((1, 264), torch.bfloat16, 3)
+    for cols in (137, 4099):
+        x = make((2, cols), torch.bfloat16, 1)[:1, :136]
+        assert x.stride(0) == cols
+        R.assert_close(nv.linear(x, w), *R.forward64(x, w, [0, 1], None, "none", None)[:2])
+        for got, (r, e) in zip(nv.linear_backward(dy, x, w)[:2], R.backward64(dy, x, w, [0, 1], None, "none")):
+            R.assert_close(got, r, e)
+
+
 def test_other_groups_values_stay_out(nv, cuda_dev):
     """Infinities and NaN in another group's rows and weights reach only that group."""
     cuts = [0, 21, 40, 73]
