@@ -173,16 +173,18 @@ __device__ __forceinline__ float act(float y) {
     return y;
 }
 
-// Derivative of act at z (not SwiGLU, which has two arguments).
+// Derivative of act at z (not SwiGLU, which has two arguments).  Where sigma has rounded to 0
+// or 1 the derivative is that: the other term's factor sigma (1 - sigma) is 0, and z or its
+// square, which passes fp32 from 5e19 on, would make it NaN.
 __device__ __forceinline__ float act_grad(int a, float z) {
     if (a == kActRelu) return z > 0.0f ? 1.0f : 0.0f;
     if (a == kActSilu) {
-        const float s = sigma(z);
-        return fmaf(z * s, 1.0f - s, s);
+        const float s = sigma(z), d = s * (1.0f - s);
+        return d == 0.0f ? s : fmaf(z, d, s);
     }
     if (a == kActGeluTanh) {
-        const float s = sigma(2.0f * kGelu0 * fmaf(kGelu1 * z * z, z, z));
-        return fmaf(z * s * (1.0f - s), 2.0f * kGelu0 * fmaf(3.0f * kGelu1 * z, z, 1.0f), s);
+        const float s = sigma(2.0f * kGelu0 * fmaf(kGelu1 * z * z, z, z)), d = s * (1.0f - s);
+        return d == 0.0f ? s : fmaf(z * d, 2.0f * kGelu0 * fmaf(3.0f * kGelu1 * z, z, 1.0f), s);
     }
     return 1.0f;
 }

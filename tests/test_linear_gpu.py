@@ -151,6 +151,21 @@ def test_backward(nv, cuda_dev, act, M, N, K):
             R.assert_close(a, r.reshape(a.shape), e.reshape(a.shape), n)
 
 
+@pytest.mark.parametrize("act", ["relu", "silu", "gelu_tanh"])
+def test_backward_of_large_preactivations(nv, cuda_dev, act):
+    """Pre-activations up to the largest bf16 value, whose square passes fp32, and infinities:
+    the slope is 0 or 1 there."""
+    v = torch.tensor([-math.inf, -3.38e38, -1e30, -6e19, -1e10, -300.0, -90.0, 90.0, 300.0, 1e10, 6e19, 1e30, 3.38e38,
+                      math.inf, 0.0, 1.0], device="cuda").bfloat16()
+    N = v.numel()
+    x, w = make((4, 8), torch.bfloat16, 1), make((N, 8), torch.bfloat16, 2)
+    dy, z = make((4, N), torch.bfloat16, 3), v.expand(4, N).contiguous()
+    got = nv.linear_backward(dy, x, w, preact=z, activation=act, bias_grad=True)
+    # infinities: the limits, which are the slopes at the largest values
+    for a, (r, e), n in zip(got, R.backward64(dy, x, w, [0, 4], z.clamp(-3.38e38, 3.38e38), act), ("dx", "dw", "db")):
+        R.assert_close(a, r.reshape(a.shape), e.reshape(a.shape), n)
+
+
 @pytest.mark.parametrize("cuts", GROUPS, ids=lambda c: f"G{len(c) - 1}M{c[-1]}")
 def test_backward_groups(nv, cuda_dev, cuts):
     for act, N, K, dtype in (("none", 72, 264, torch.bfloat16), ("swiglu", 288, 136, torch.bfloat16),
