@@ -8,7 +8,7 @@
 // accumulators of 256 columns
 // fill the tensor memory, so the epilogue of one tile runs under the MMAs of the next; or,
 // for "wide" tiles, one tile of up to 512 tokens uses both: each A tile is then read once for
-// twice the tokens, which pays where there is only one round of tiles to run anyway.
+// twice the tokens, which pays where there is only one round of tiles to run (token_tile).
 //
 // Launched in plain stream order, as all kernels of the gradient are, the split-reduction
 // kernel's input gradient among them: as programmatic dependents of each other they gained
@@ -16,9 +16,9 @@
 // steps, none of their bounded waits running.  The cause was not found.
 //
 // Large products run at the rate of the library's own 16-bit product, both held by the
-// power cap (N = M = K = 8192, back to back: 780-805 us = 1.37-1.41 PFLOP/s against 745-758;
-// input gradient of 4096 x 14336 x 4096 370-400 us against 394, weight gradient 353-370
-// against 365).  Small tiles are held by L2: a CTA takes about 98 GB/s whatever the number
+// power cap (calls of both in turn, us: 8192^3 with residual 797 against 812 without, 1.38
+// PFLOP/s; 8192 x 28672 x 8192 2903 against 2967; of 4096 x 14336 x 4096 the input gradient
+// 380 against 370, the weight gradient 353 against 366).  Small tiles are held by L2: a CTA takes about 98 GB/s whatever the number
 // of slots.  The barriers of a slot have CTA scope: announcing each CTA's own bytes on the
 // leader's barrier with cluster-scope arrivals, and acquiring at cluster scope, took 1416 us.
 //
@@ -640,11 +640,13 @@ static int launch_pair(const CUtensorMap &a, const CUtensorMap &b, const CUtenso
 // features plus 1.07 ns a token (measured from 32 to 256 tokens, N = K = 4096), so few wide
 // tiles win, unless their number fills the last round of pairs badly.
 //   dense: the M tokens in n equal tiles, n chosen by rounds x cost (by the eight sizes that a
-//     tile can have, so the choice takes as long for a million tokens as for a thousand); or in wide tiles (two
-//     parts that share the A tile, up to 512 tokens), whose epilogue, about 20 ns a token,
-//     no other tile's MMAs hide.  As tiles of 192 / wide tiles of 2 x 192 tokens, us: M=333
-//     N=14344 K=4104 56.6/47.4, M=333 N=14336 K=4096 45.5/41.6; but M=1024 N=K=4096 as
-//     tiles of 256 / of 2 x 256 32.6/48.9 (fewer tiles than pairs);
+//     tile can have, so the choice takes as long for a million tokens as for a thousand);
+//     or, where that leaves one round, in wide tiles: two parts that share the A tile, up to
+//     512 tokens, whose epilogue, about 20 ns a token, no other tile's MMAs hide.  One round,
+//     us without / with wide tiles: M=333 N=14344 K=4104 70.4/54.6, M=450 78.1/65.3; M=385
+//     N=14344 K=2056 37.1/32.1.  More rounds expose an epilogue each: 8192^3 with residual
+//     797/910, 8192 x 28672 x 8192 2903/3464, 3000 x 8192 x 8192 319/396, 4096 x 6144 x 6144
+//     267/304 (calls of both in turn).
 //   groups (their rows are known on the device only): up to twice the mean rows, so that
 //     most groups are one tile or 256-token tiles; a tile's MMAs follow its own rows.  Wide
 //     tiles were slower or the same (64 experts of 4096 x 2048, 512 rows each, 537/590 us).
@@ -667,7 +669,8 @@ static TokenTile token_tile(int64_t m, int groups, int n_f, int pairs, int red) 
         for (int wide = 0; wide <= (n > 1 ? 1 : 0); wide++) {
             const int tokens = bt * (1 + wide);
             const int64_t tiles = (m + tokens - 1) / tokens * n_f, rounds = (tiles + pairs - 1) / pairs;
-            const double cost = (double)rounds * nkb * (150.0 + 1.07 * tokens) + (wide ? rounds : 1) * 20.0 * tokens;
+            if (wide && rounds > 1) continue;  // its epilogues would run under no MMAs
+            const double cost = (double)rounds * nkb * (150.0 + 1.07 * tokens) + 20.0 * tokens;
             if (cost < least) {
                 least = cost;
                 best = {bt, wide};

@@ -45,6 +45,21 @@ def test_gradient_refusals(nv):
     assert L.nvfp4_activation_backward(P, None, None, None, None, 1, 100, 64, 0, 0, None, 0, None) == 0  # nothing to do
 
 
+def test_wide_tiles_run_in_one_round(nv):
+    """A tile of two parts hides no epilogue under another tile: only where one round of the
+    pairs takes all tiles, forward and input gradient."""
+    import nvfp4_diag
+    wide = 0
+    for N, K in ((8192, 8192), (28672, 8192), (14344, 4104), (14336, 4096), (6144, 6144), (4096, 14336), (1024, 4096)):
+        for M in (257, 300, 333, 450, 512, 1000, 1500, 3000, 4096, 8192, 16384):
+            for form, features in (("forward", N), ("dgrad", K)):
+                p = nvfp4_diag.linear_plan(form, M, N, K)
+                if p["wide"]:
+                    wide += 1
+                    assert -(-M // (2 * p["bt"])) * -(-features // 256) <= 148 // 2, (form, M, N, K)
+    assert wide and nvfp4_diag.linear_plan("forward", 333, 14344, 4104)["wide"]
+
+
 def test_extents_that_round_past_32_bits(nv):
     """The last 1023 sizes below 2^31 would round up past 32 bits inside the kernels."""
     big, L = (1 << 31) - 1, nv.lib()
