@@ -70,6 +70,77 @@ def test_groups(nv, cuda_dev, cuts):
     check_forward(nv, cuts[-1], 256, 512, "gelu_tanh", bias=True, cuts=cuts)
 
 
+def plan(form, M, N, K, groups=0):
+    import nvfp4_diag
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    return nvfp4_diag.linear_plan(form, M, N, K, groups, sms)
+
+
+@pytest.mark.parametrize("act", R.ACTS)
+def test_wide_tiles(nv, cuda_dev, act):
+    """Tiles of two parts: ends in the first part, in the second, and full ones."""
+    for M, N, K, dtype, residual in ((257, 14368, 2056, torch.bfloat16, True), (333, 14368, 2056, torch.float16, False),
+                                     (385, 14368, 2056, torch.float16, True), (450, 14368, 4104, torch.bfloat16, True),
+                                     (512, 14368, 4104, torch.bfloat16, False)):
+        p = plan("forward", M, N, K)
+        assert p["wide"] and p["bt"] < M <= 2 * p["bt"]
+        check_forward(nv, M, N, K, act, bias=True, residual=residual, dtype=dtype, z=True)
+
+
+@pytest.mark.parametrize("M,dtype", [(257, torch.bfloat16), (333, torch.float16), (450, torch.bfloat16)])
+def test_wide_tiles_input_gradient(nv, cuda_dev, M, dtype):
+    N, K = 4104, 14344
+    assert plan("dgrad", M, N, K)["wide"]
+    x, w, dy = make((M, K), dtype, 1), make((N, K), dtype, 2, K ** -0.5), make((M, N), dtype, 3)
+    z = make((M, N), dtype, 4)
+    dx, _, db = nv.linear_backward(dy, x, w, preact=z, activation="silu", bias_grad=True, weight_grad=False)
+    nv.device_status()
+    ref = R.backward64(dy, x, w, [0, M], z, "silu")
+    R.assert_close(dx, *ref[0], "dx")
+    R.assert_close(db, *(t.flatten() for t in ref[2]), "db")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M,N,K", [(1, 512, 8200), (16, 264, 16384), (64, 512, 8200), (100, 520, 8200), (128, 512, 8200)])
+def test_few_tokens_long_reduction(nv, cuda_dev, M, N, K, dtype):
+    """The split-reduction kernel where its ring goes round and eight CTAs share a tile, forward
+    and (with N and K exchanged) input gradient, up to its most tokens."""
+    for form, n, k in (("forward", N, K), ("dgrad", K, N)):
+        p = plan(form, M, n, k)
+        assert p["decode"] and p["splits"] == 8 and -(-K // 64) // 8 > p["stages"]
+    check_forward(nv, M, N, K, "silu", bias=True, residual=True, dtype=dtype, z=True)
+    if N % 32 == 0:
+        check_forward(nv, M, N, K, "swiglu", bias=True, residual=True, dtype=dtype, z=True)
+    x, w, dy = make((M, N), dtype, 1), make((K, N), dtype, 2, K ** -0.5), make((M, K), dtype, 3)
+    dx, dw, _ = nv.linear_backward(dy, x, w)
+    nv.device_status()
+    for got, (r, e), n in zip((dx, dw), R.backward64(dy, x, w, [0, M], None, "none"), ("dx", "dw")):
+        R.assert_close(got, r, e, n)
+
+
+def test_few_tokens_long_reduction_by_groups(nv, cuda_dev):
+    cuts = [0, 3, 3, 20, 21, 40]
+    M, N, K = cuts[-1], 264, 8200
+    for form, n, k in (("forward", N, K), ("dgrad", K, N)):
+        p = plan(form, M, n, k, len(cuts) - 1)
+        assert p["decode"] and p["splits"] == 8 and -(-K // 64) // 8 > p["stages"]
+    check_forward(nv, M, N, K, "relu", bias=True, cuts=cuts, z=True)
+    G = len(cuts) - 1
+    x, w, dy = make((M, N), torch.bfloat16, 1), make((G * K, N), torch.bfloat16, 2, K ** -0.5), make((M, K), torch.bfloat16, 3)
+    dx = nv.linear_grouped_backward(dy, x, w, offsets(cuts), weight_grad=False)[0]
+    nv.device_status()
+    R.assert_close(dx, *R.backward64(dy, x, w, cuts, None, "none")[0], "dx")
+
+
+@pytest.mark.parametrize("bt,M,N,K", [(64, 130, 264, 72), (96, 450, 9480, 72), (128, 200, 6152, 520),
+                                      (160, 130, 14368, 520), (192, 333, 6152, 1032), (224, 200, 14368, 1032),
+                                      (256, 500, 14368, 520)])
+def test_every_tile_width(nv, cuda_dev, bt, M, N, K):
+    p = plan("forward", M, N, K)
+    assert not p["decode"] and p["bt"] == bt and not p["wide"]
+    check_forward(nv, M, N, K, bias=True)
+
+
 def test_rows_outside_groups_are_zero(nv, cuda_dev):
     """Offsets that leave rows out at both ends, and ends past the last row (clamped)."""
     x, w = make((300, 128), torch.bfloat16, 1), make((2 * 64, 128), torch.bfloat16, 2)

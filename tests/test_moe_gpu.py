@@ -73,6 +73,29 @@ def test_route_masks(nv, cuda_dev):
     assert torch.isfinite(r.weights).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("E,k", [(33, 4), (64, 8), (100, 6), (128, 8), (200, 8), (256, 1), (256, 8), (256, 32)])
+def test_biased_choice(nv, cuda_dev, E, k, dtype):
+    """Sigmoid scores with a bias at two, four and eight experts a lane: exact ties (more
+    experts at the top than candidates are kept), scores one rounding apart, and masks."""
+    T = 40
+    g = torch.Generator().manual_seed(E + k)
+    l = torch.randn(T, E, generator=g) * 2
+    l[:8] = l[:8].round()                                # tied scores
+    l[8:12] = 0.5                                        # all tied
+    l[12:16] = 1.0 + torch.randint(0, 4, (4, E), generator=g) * 2.0 ** -22  # a few fp32 roundings apart
+    l[16:20] = 30.0 + torch.rand(4, E, generator=g)      # scores that round to 1
+    l[20:24] = -60.0 - torch.rand(4, E, generator=g)     # scores far below the bias's rounding
+    l[24:28][:, ::2] = -math.inf
+    l[28] = -math.inf
+    l[29, 1:] = -math.inf
+    l = l.to(dtype).cuda()
+    bias = torch.randn(E, generator=g) * 0.05
+    for b in (torch.zeros(E), bias, bias.bfloat16().float(), torch.full((E,), 0.25), bias * 1e4):
+        for renorm in (True, False):
+            check_route(nv, l, k, "sigmoid", b.cuda(), renorm)
+
+
 @pytest.mark.parametrize("T,E,k", [(0, 8, 2), (5000, 256, 8), (40_000, 16, 3)])
 def test_route_many_tokens(nv, cuda_dev, T, E, k):
     """Every row is used once, in order of expert and token (several chunks of tokens)."""
