@@ -681,19 +681,24 @@ static TokenTile token_tile(int64_t m, int groups, int n_f, int pairs, int red) 
 }
 
 // Whether the split-reduction kernel takes a forward product or an input gradient (at most
-// kDecodeTokens rows).  It
-// wins where 256-feature tiles are too few to stream the weights on every SM; with enough
-// of them the persistent kernel does, without a reduction between CTAs.  Measured (us, this
-// kernel / persistent): N=4096 K=4096 M=1 10.7/16.0, M=64 16.3/16.5, M=128 23.7/17.7;
-// N=4096 K=14336 M=64 28.5/44.4, M=128 36.9/48.0; N=14336 K=4096 M=1 21.8/23.4, M=64
-// 25.1/24.4; N=28672 K=8192 M=1 74.0/76.4, M=64 83.3/81.5; 8 experts N=28672 K=4096, 32 rows
-// 295/280.
-static bool use_decode(int m, int groups, int n_f, int K) {
+// kDecodeTokens rows).  It wins where 256-feature tiles are too few to stream the weights on
+// every SM, or the reduction is long; with more tokens its tiles re-read them more often, and
+// the persistent kernel, without a reduction between CTAs, does.  The input gradient gives way
+// earlier: it is launched in plain order (plan_decode).  Measured with weights that are not
+// in L2, us, this kernel / persistent (features x reduction):
+//   forward         1 token 4096 x 4096 9.9/20.7, 14336 x 4096 22.8/27.0, 28672 x 8192 73.0/80.8;
+//                   64 tokens 4096 x 4096 15.8/20.7, 14336 x 4096 24.8/28.8, 28672 x 8192
+//                   79.9/84.1; 128 tokens 1024 x 4096 12.3/20.8, 4096 x 4096 21.2/20.8, 8192 x
+//                   4096 23.4/22.3, 4096 x 16384 37.3/61.7, 8192 x 2048 17.6/14.6
+//   input gradient  1 token 4096 x 4096 12.5/20.7; 64 tokens 4096 x 4096 18.6/20.7, 14336 x 4096
+//                   26.9/24.8; 128 tokens 4096 x 4096 24.8/20.7, 4096 x 16384 39.7/61.7
+//   groups          8 of 2048 x 2048, 64 rows 10.7/14.7; 64 of them 87.0/84.8
+static bool use_decode(int form, int m, int groups, int n_f, int red) {
     if (m > kDecodeTokens) return false;
     const int64_t tiles = (int64_t)n_f * std::min(groups, m);
     if (m <= 32) return tiles <= 128;
-    if (m <= 64) return tiles <= 37;
-    return tiles <= 18 && K >= 8192;
+    if (m <= 64) return tiles <= (form == kForward ? 128 : 37);
+    return tiles <= 32 && red >= (form == kForward ? 4096 : 8192);
 }
 
 Plan make_plan(int form, int groups, bool ragged, int m_total, int features, int red, int sm_count) {
@@ -706,7 +711,7 @@ Plan make_plan(int form, int groups, bool ragged, int m_total, int features, int
         plan.bt = (int64_t)groups * n_f * ((red + 255) / 256) * 2 <= pairs ? 128 : 256;
         plan.tiles = (int64_t)groups * n_f * ((red + plan.bt - 1) / plan.bt);
     } else {
-        if (use_decode(m_total, groups, n_f, red)) {
+        if (use_decode(form, m_total, groups, n_f, red)) {
             plan_decode(form, groups, m_total, features, red, sm_count, &plan);
             return plan;
         }

@@ -60,6 +60,26 @@ def test_wide_tiles_run_in_one_round(nv):
     assert wide and nvfp4_diag.linear_plan("forward", 333, 14344, 4104)["wide"]
 
 
+def test_kernel_of_few_tokens(nv):
+    """The choice where both kernels were measured: the faster one's, within 6 %.  Features,
+    reduction, tokens, and the times (us) of the split-reduction and the persistent kernel."""
+    import nvfp4_diag
+    for form, features, red, M, split, persistent in (
+            ("forward", 4096, 4096, 1, 9.9, 20.7), ("forward", 14336, 4096, 1, 22.8, 27.0),
+            ("forward", 4096, 4096, 64, 15.8, 20.7), ("forward", 14336, 4096, 64, 24.8, 28.8),
+            ("forward", 20480, 4096, 64, 34.1, 45.5), ("forward", 28672, 8192, 64, 79.9, 84.1),
+            ("forward", 1024, 4096, 96, 10.6, 20.8), ("forward", 1024, 4096, 128, 12.3, 20.8),
+            ("forward", 4096, 4096, 128, 21.2, 20.8), ("forward", 8192, 4096, 128, 23.4, 22.3),
+            ("forward", 4096, 16384, 128, 37.3, 61.7), ("forward", 6144, 8192, 128, 30.1, 35.1),
+            ("forward", 8192, 2048, 128, 17.6, 14.6), ("dgrad", 4096, 4096, 1, 12.5, 20.7),
+            ("dgrad", 4096, 4096, 64, 18.6, 20.7), ("dgrad", 14336, 4096, 64, 26.9, 24.8),
+            ("dgrad", 4096, 4096, 128, 24.8, 20.7), ("dgrad", 4096, 16384, 128, 39.7, 61.7),
+            ("dgrad", 6144, 16384, 128, 48.2, 61.9)):
+        n, k = (features, red) if form == "forward" else (red, features)
+        chosen = split if nvfp4_diag.linear_plan(form, M, n, k)["decode"] else persistent
+        assert chosen <= 1.06 * min(split, persistent), (form, features, red, M)
+
+
 def test_extents_that_round_past_32_bits(nv):
     """The last 1023 sizes below 2^31 would round up past 32 bits inside the kernels."""
     big, L = (1 << 31) - 1, nv.lib()
