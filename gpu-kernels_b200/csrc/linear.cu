@@ -5,22 +5,23 @@
 // tcgen05.mma.cta_group::2 (kind::f16, fp32 accumulators).  Each CTA stages its 128
 // features and its half of the tokens by TMA into a ring of slots of 64 reduction elements:
 // 6 of 32 KB for 256 tokens, up to 10 for smaller token tiles in the same memory.  Two
-// accumulators of 256 columns
-// fill the tensor memory, so the epilogue of one tile runs under the MMAs of the next; or,
-// for "wide" tiles, one tile of up to 512 tokens uses both: each A tile is then read once for
-// twice the tokens, which pays where there is only one round of tiles to run (token_tile).
+// accumulators of 256 columns fill the tensor memory, so the epilogue of one tile runs under
+// the MMAs of the next; or, for "wide" tiles, one tile of up to 512 tokens uses both: each A
+// tile is then read once for twice the tokens, which pays where there is one round of tiles to
+// run, or a long reduction (token_tile).
 //
 // Launched in plain stream order, as all kernels of the gradient are, the split-reduction
 // kernel's input gradient among them: as programmatic dependents of each other they gained
 // nothing (415 us a step of 64 experts either way) and stopped for good once in about 10^5
 // steps, none of their bounded waits running.  The cause was not found.
 //
-// Large products run at the rate of the library's own 16-bit product, both held by the
-// power cap (calls of both in turn, us: 8192^3 with residual 797 against 812 without, 1.38
-// PFLOP/s; 8192 x 28672 x 8192 2903 against 2967; of 4096 x 14336 x 4096 the input gradient
-// 380 against 370, the weight gradient 353 against 366).  Small tiles are held by L2: a CTA takes about 98 GB/s whatever the number
-// of slots.  The barriers of a slot have CTA scope: announcing each CTA's own bytes on the
-// leader's barrier with cluster-scope arrivals, and acquiring at cluster scope, took 1416 us.
+// Large products are held by the power cap.  Calls in turn with the library's 16-bit product,
+// with pauses / kept busy for seconds, us: 8192^3 with residual 797/849 (1.38/1.30 PFLOP/s)
+// against 812/782 without; 8192 x 28672 x 8192 2903/2949 against 2967/2748; of 4096 x 14336 x
+// 4096 the input gradient 380/377 against 370/366, the weight gradient 353 against 366.  Small
+// tiles are held by L2: a CTA takes about 98 GB/s whatever the number of slots.  The barriers
+// of a slot have CTA scope: announcing each CTA's own bytes on the leader's barrier with
+// cluster-scope arrivals, and acquiring at cluster scope, took 1416 us for 8192^3.
 //
 // Warps: 0 TMA producer, 1 MMA issue (leader CTA) and TMEM owner, 2-9 epilogue, 10 (wgrad)
 // clears the rows past a group's end in its last slot.
@@ -641,15 +642,21 @@ static int launch_pair(const CUtensorMap &a, const CUtensorMap &b, const CUtenso
 // tiles win, unless their number fills the last round of pairs badly.
 //   dense: the M tokens in n equal tiles, n chosen by rounds x cost (by the eight sizes that a
 //     tile can have, so the choice takes as long for a million tokens as for a thousand);
-//     or, where that leaves one round, in wide tiles: two parts that share the A tile, up to
-//     512 tokens, whose epilogue, about 20 ns a token, no other tile's MMAs hide.  One round,
-//     us without / with wide tiles: M=333 N=14344 K=4104 70.4/54.6, M=450 78.1/65.3; M=385
-//     N=14344 K=2056 37.1/32.1.  More rounds expose an epilogue each: 8192^3 with residual
-//     797/910, 8192 x 28672 x 8192 2903/3464, 3000 x 8192 x 8192 319/396, 4096 x 6144 x 6144
-//     267/304 (calls of both in turn).
+//     or in wide tiles: two parts that share the A tile, up to 512 tokens, whose epilogue,
+//     about 20 ns a token, no other tile's MMAs hide.  They pay for one round, us without /
+//     with: M=333 N=14344 K=4104 70.4/54.6, M=450 78.1/65.3; M=385 N=14344 K=2056 37.1/32.1.
+//     More rounds expose an epilogue each, in calls with pauses: 8192^3 with residual 797/910,
+//     8192 x 28672 x 8192 2903/3464, 3000 x 8192 x 8192 319/396, 4096 x 6144 x 6144 267/304;
+//     kept busy for seconds, under the power cap, 849/870, 2949/2922, 332/328, 252/252.  With
+//     reductions of 200 slots and more the epilogue is 5 % of a tile and the A tiles' second
+//     reading costs as much: the input gradient of 4096 x 14336 x 4096 390/396 with pauses and
+//     392/375 without, 2048 x 8192 x 14336 380/385 and 402/373.  There they are taken if they
+//     fill the rounds as well as the narrow ones (8192 x 4096 x 14336, 7 rounds of 256 tokens
+//     against 4 of 512: 701/814 and 734/743).
 //   groups (their rows are known on the device only): up to twice the mean rows, so that
 //     most groups are one tile or 256-token tiles; a tile's MMAs follow its own rows.  Wide
 //     tiles were slower or the same (64 experts of 4096 x 2048, 512 rows each, 537/590 us).
+constexpr int kWideSlots = 200;
 struct TokenTile {
     int bt, wide;
 };
@@ -661,22 +668,25 @@ static TokenTile token_tile(int64_t m, int groups, int n_f, int pairs, int red) 
         return best;
     }
     double least = 1e300;
+    int64_t narrow = 0;  // rounds x tokens of the best tiles of one part
     const int nkb = (red + kBlockK - 1) / kBlockK;
     const int64_t n0 = (m + kMaxTokens - 1) / kMaxTokens;
-    for (int bt = kMaxTokens; bt >= 32; bt -= 32) {  // down to a quarter of the fewest tiles' tokens
-        const int64_t n = (m + bt - 1) / bt;
-        if (n > 4 * n0) break;
-        for (int wide = 0; wide <= (n > 1 ? 1 : 0); wide++) {
+    for (int wide = 0; wide <= 1; wide++)
+        for (int bt = kMaxTokens; bt >= 32; bt -= 32) {  // down to a quarter of the fewest tiles' tokens
+            const int64_t n = (m + bt - 1) / bt;
+            if (n > 4 * n0) break;
+            if (wide && n == 1) continue;
             const int tokens = bt * (1 + wide);
             const int64_t tiles = (m + tokens - 1) / tokens * n_f, rounds = (tiles + pairs - 1) / pairs;
-            if (wide && rounds > 1) continue;  // its epilogues would run under no MMAs
-            const double cost = (double)rounds * nkb * (150.0 + 1.07 * tokens) + 20.0 * tokens;
+            if (wide && rounds > 1 && (nkb < kWideSlots || rounds * tokens > narrow)) continue;
+            const double cost =
+                (double)rounds * nkb * (150.0 + 1.07 * tokens) + (wide ? rounds : 1) * 20.0 * tokens;
             if (cost < least) {
                 least = cost;
                 best = {bt, wide};
+                if (!wide) narrow = rounds * tokens;
             }
         }
-    }
     return best;
 }
 

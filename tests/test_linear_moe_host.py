@@ -45,19 +45,25 @@ def test_gradient_refusals(nv):
     assert L.nvfp4_activation_backward(P, None, None, None, None, 1, 100, 64, 0, 0, None, 0, None) == 0  # nothing to do
 
 
-def test_wide_tiles_run_in_one_round(nv):
+def test_wide_tiles_hide_their_epilogue(nv):
     """A tile of two parts hides no epilogue under another tile: only where one round of the
-    pairs takes all tiles, forward and input gradient."""
+    pairs takes all tiles, or a long reduction outweighs it and no round is lost."""
     import nvfp4_diag
-    wide = 0
+    seen = set()
     for N, K in ((8192, 8192), (28672, 8192), (14344, 4104), (14336, 4096), (6144, 6144), (4096, 14336), (1024, 4096)):
         for M in (257, 300, 333, 450, 512, 1000, 1500, 3000, 4096, 8192, 16384):
-            for form, features in (("forward", N), ("dgrad", K)):
+            for form, features, red in (("forward", N, K), ("dgrad", K, N)):
                 p = nvfp4_diag.linear_plan(form, M, N, K)
                 if p["wide"]:
-                    wide += 1
-                    assert -(-M // (2 * p["bt"])) * -(-features // 256) <= 148 // 2, (form, M, N, K)
-    assert wide and nvfp4_diag.linear_plan("forward", 333, 14344, 4104)["wide"]
+                    n_f, tiles = -(-features // 256), -(-M // p["bt"])
+                    rounds = -(-(-(-tiles // 2) * n_f) // 74)
+                    assert rounds == 1 or red > 199 * 64, (form, M, N, K)
+                    seen.add(rounds == 1)
+    assert seen == {True, False}
+    assert nvfp4_diag.linear_plan("forward", 333, 14344, 4104)["wide"]
+    assert nvfp4_diag.linear_plan("dgrad", 4096, 14336, 4096)["wide"]
+    assert not nvfp4_diag.linear_plan("forward", 8192, 8192, 8192)["wide"]
+    assert not nvfp4_diag.linear_plan("dgrad", 8192, 14336, 4096)["wide"]
 
 
 def test_kernel_of_few_tokens(nv):
