@@ -9,11 +9,12 @@
 // run the epilogue on them.  No workspace, no atomics, no second launch.
 //
 // The ring is sized so that two CTAs share an SM: the prologue and the reduction of one run
-// under the loads of another, and as a programmatic dependent the next call's set-up runs
-// under this one's end (one token, N=K=4096, 12.4 -> 9.4 us a call).  Measured, M = 1:
-// N=K=4096 9.1 us on the GPU, N=14336 K=4096 21.7 us (5.4 TB/s), N=28672 K=8192 73.8 us
-// (6.4 of a copy's 6.55): bound by the weights' bytes, and for the smaller ones by what a
-// launch, the first loads and the cluster's sum take.
+// under the loads of another, and as a programmatic dependent the next forward call's set-up
+// runs under this one's end (one token, N=K=4096, 12.4 -> 9.4 us a call).  Measured, M = 1, on
+// the GPU: N=K=4096 7.4 us with the weight left in L2 by the call before, 9.6 us from memory
+// (3.5 TB/s); N=14336 K=4096 22.3 us (5.3), N=28672 K=8192 74 us (6.3 of a copy's 6.55): bound
+// by the weights' bytes, and for the smaller ones by what a launch, the first loads and the
+// cluster's sum take.
 //
 // Warps: 0 TMA producer, 1 MMA issue and TMEM owner, 2-5 read the accumulator out; all six
 // reduce.

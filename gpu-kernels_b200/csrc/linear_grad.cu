@@ -1,10 +1,18 @@
 // linear_grad.cu — gradient of the linear layers' epilogue: dZ = dY * act'(Z), and the bias
 // gradient (column sums of dZ by row group), in one pass over dY and Z.
 //
+// dZ is rounded to the 16-bit type here, and the two products that follow take it so: their
+// tensor instructions read 16-bit operands, and a dZ of 32 bits as two parts would double both
+// products' instructions and the bytes of dZ.  It costs one more rounding than a 32-bit dZ
+// would: the norm of dX's and dW's error grows from 0.0017 to 0.0023 of theirs in bf16.  In
+// fp16 a dZ past 65504 becomes an infinity (for SwiGLU the factor is not bounded), as any fp16
+// gradient does, for the loss scale to catch.  The bias gradient sums the unrounded dZ.
+//
 // Bound by memory: dY and Z are read once and dZ written once, 16 bytes a thread.  The
 // column sums are kept in fp32: each CTA sums 64 rows of one group, and a second kernel adds
 // the CTAs' sums in row order, so the result has the same bits on every call.  16387 rows of
-// 2048 columns with SwiGLU and 64 groups: 31 us (5.4 TB/s), and 7 us for the groups' sums.
+// 2048 columns with SwiGLU and 64 groups: 33 us (5.1 TB/s), and 6.5 us for the groups' sums; 4096 x 14336
+// with gelu 75 us (4.7 TB/s) and 11 us.
 #include <algorithm>
 #include <climits>
 

@@ -6,6 +6,9 @@ type or device, NVFP4Error for a bad status.
 
     z = x @ w.T + bias;  y = act(z) + residual          (fp32, rounded once)
 
+These functions record no autograd graph: their results do not require grad, whatever their
+inputs do.  torch.ops.nvfp4_b200.linear_preact is the differentiable form.
+
 Row groups (mixture of experts) are given by m_offsets, as for gemm_grouped: group g is rows
 m_offsets[g] .. m_offsets[g+1] and uses weight rows g*N .. (g+1)*N.
 """
@@ -54,7 +57,8 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, preact: 
                     weight_grad: bool = True):
     """Gradients (dx [M, K], dw [N, K], db [N]) of linear() for dy [M, Nout], None for those
     that are not wanted; the residual's gradient is dy itself.  preact: linear's z, needed
-    with an activation."""
+    with an activation.  dz = dy * act'(z) is rounded to the 16-bit type before the products
+    (in fp16 an infinity past 65504); db sums it unrounded."""
     return native.linear_backward(dy, x, w, None, preact, _activation(activation), bias_grad, input_grad, weight_grad)
 
 

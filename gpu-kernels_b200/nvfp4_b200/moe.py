@@ -7,6 +7,8 @@ of token rows to expert order and back, and their gradients.
     y = moe_combine(ys, r, residual=x)                 # weighted sum back in token order
 
 Asynchronous on torch's current stream; nothing of the routing passes through the host.
+These functions record no autograd graph; the operators of the same names in
+torch.ops.nvfp4_b200 do.
 """
 from typing import NamedTuple, Optional
 

@@ -331,8 +331,9 @@ NVFP4_API uint64_t nvfp4_launch_count(void);
  * 16-bit layers (no counterpart in the reference): the linear layers that stay in bf16 or
  * fp16 beside the NVFP4 ones, their experts, and the router around both.  dtype is one of
  * NVFP4_BF16, NVFP4_F16 (and NVFP4_F32 for the router's logits).  All sums, statistics and
- * activations are fp32; every result is rounded once, to its 16-bit type.  Results are the
- * same bits on every call.  Nothing is allocated; workspaces come from the caller and need
+ * activations are fp32; every result is rounded once, to its 16-bit type.  (A backward pass
+ * with an activation is two results after each other: dZ, rounded, and its products.)
+ * Results are the same bits on every call.  Nothing is allocated; workspaces come from the caller and need
  * no initial value.  Tensors are contiguous, 16-byte aligned, unless a row pitch is given.
  *
  * Row groups: m_offsets (groups + 1 int32 on the device, non-decreasing, clamped to
@@ -363,7 +364,8 @@ NVFP4_API int nvfp4_linear_dgrad(const void *dZ, const void *W, void *dX, const 
 NVFP4_API int nvfp4_linear_wgrad(const void *dZ, const void *X, int64_t ldx, void *dW, const int32_t *m_offsets,
                                  int groups, int M, int N, int K, int dtype, void *stream);
 /*
- * Gradient of the epilogue: dZ [M, N] = dY [M, Nout] * act'(Z), and, when dbias is given,
+ * Gradient of the epilogue: dZ [M, N] = dY [M, Nout] * act'(Z), rounded to dtype (in fp16
+ * past 65504 an infinity) for nvfp4_linear_dgrad and _wgrad, and, when dbias is given,
  * dbias [groups, N] = the column sums of the unrounded dZ by group.  With NVFP4_ACT_NONE dZ
  * is dY: only dbias is computed, Z and dZ may be NULL.  Rows of dZ outside every group are
  * not written.  The workspace is needed for dbias only.

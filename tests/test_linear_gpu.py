@@ -100,6 +100,20 @@ def test_wide_tiles_input_gradient(nv, cuda_dev, M, dtype):
     R.assert_close(db, *(t.flatten() for t in ref[2]), "db")
 
 
+def test_wide_tiles_in_rounds(nv, cuda_dev):
+    """Wide tiles one after the other on a pair (a long reduction), forward and input gradient."""
+    for form, M, N, K in (("forward", 700, 14344, 12808), ("dgrad", 1550, 12808, 6152)):
+        p = plan(form, M, N, K)
+        assert p["wide"] and -(-M // (2 * p["bt"])) * -(-(N if form == "forward" else K) // 256) > 74
+    check_forward(nv, 700, 14344, 12808, "silu", bias=True, residual=True, dtype=torch.float16, z=True)
+    M, N, K = 1550, 12808, 6152
+    x, w, dy = make((M, K), torch.bfloat16, 1), make((N, K), torch.bfloat16, 2, N ** -0.5), make((M, N), torch.bfloat16, 3)
+    dx = nv.linear_backward(dy, x, w, weight_grad=False)[0]
+    nv.device_status()
+    ref = dy.double() @ w.double()
+    R.assert_close(dx, ref, R.acc(N) * (dy.double().abs() @ w.double().abs()), "dx")
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("M,N,K", [(1, 512, 8200), (16, 264, 16384), (64, 512, 8200), (100, 520, 8200), (128, 512, 8200)])
 def test_few_tokens_long_reduction(nv, cuda_dev, M, N, K, dtype):
@@ -220,6 +234,35 @@ def test_backward(nv, cuda_dev, act, M, N, K):
         ref = R.backward64(dy, x, w, [0, M], z, act)
         for a, (r, e), n in zip(got, ref, ("dx", "dw", "db")):
             R.assert_close(a, r.reshape(a.shape), e.reshape(a.shape), n)
+
+
+@pytest.mark.parametrize("act", ["relu", "silu", "gelu_tanh", "swiglu"])
+def test_gradient_of_the_epilogue_is_rounded_once(nv, cuda_dev, act):
+    """The products of the backward pass take dZ = dY act'(Z) in the 16-bit type, rounded as the
+    activation's gradient leaves it; the bias gradient sums it unrounded.  In fp16 a dZ past
+    65504 is an infinity, and no dX that it enters is finite."""
+    M, N, K = 70, 96, 72
+    for dtype in (torch.bfloat16, torch.float16):
+        No = N // 2 if act == "swiglu" else N
+        x, w, dy = make((M, K), dtype, 1), make((N, K), dtype, 2), make((M, No), dtype, 3)
+        z = make((M, N), dtype, 4)
+        dz = torch.empty(M, N, dtype=dtype, device="cuda")
+        s = torch.cuda.current_stream().cuda_stream
+
+        def rounded(dy):
+            assert nv.lib().nvfp4_activation_backward(dy.data_ptr(), z.data_ptr(), dz.data_ptr(), None, None, 1, M, N,
+                                                      nv._lib.ACTIVATIONS[act], int(dtype == torch.float16), None, 0,
+                                                      s) == 0
+            return dz
+
+        got = nv.linear_backward(dy, x, w, preact=z, activation=act)
+        want = nv.linear_backward(rounded(dy), x, w)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    for row, v in ((3, 4.0), (5, 1.5), (7, 2.4)):
+        z[row], dy[row] = v, 60000.0
+    past = R.dact64(dy.double(), z.double(), act).abs() >= 65520  # halfway to the next step of fp16
+    assert torch.equal(rounded(dy).isinf(), past) and past.any() == (act != "relu")
+    assert not nv.linear_backward(dy, x, w, preact=z, activation=act)[0][past.any(1)].isfinite().any()
 
 
 @pytest.mark.parametrize("act", ["relu", "silu", "gelu_tanh"])
