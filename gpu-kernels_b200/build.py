@@ -45,6 +45,8 @@ PRODUCT_UNITS = [("runtime", os.path.join(CSRC, "runtime.cu"), []),
                  ("linear_decode", os.path.join(CSRC, "linear_decode.cu"), []),
                  ("linear_grad", os.path.join(CSRC, "linear_grad.cu"), []),
                  ("moe", os.path.join(CSRC, "moe.cu"), []),
+                 ("embedding", os.path.join(CSRC, "embedding.cu"), []),
+                 ("logprobs", os.path.join(CSRC, "logprobs.cu"), []),
                  ("host_pipeline", os.path.join(CSRC, "host_pipeline.cu"), []),
                  ("capi", os.path.join(CSRC, "capi.cu"), [])]
 PRODUCT_UNITS += [(f"decode_inst_{m}", os.path.join(CSRC, "decode_inst.cu"), [f"-DNVFP4_DECODE_MPAD={m}"])

@@ -1,0 +1,628 @@
+// logprobs.cu — log probabilities of given tokens from rows of logits, with the entropy and
+// the most probable alternatives, and the gradient of the logits.
+//
+// One pass over a row.  With c = log2(e) / temperature and m the maximum so far, a thread keeps
+//   S0 = sum 2^(c (x - m)),  S1 = sum (x - m) 2^(c (x - m))
+// and rescales both when its maximum moves, once for a batch of vectors at most.  Parts are
+// joined the same way; then log p = (x - m) / temperature - ln S0 and the entropy is
+// ln S0 - S1 / S0 / temperature: nothing is subtracted that is large beside the result.
+//
+// Alternatives: a row's k-th highest value cannot be below the k-th highest of 32 disjoint
+// parts' maxima, which the pass has at hand; only threads whose own maximum reaches that
+// bound can hold a candidate, so a few percent of the row are read again (from L2), and the
+// candidates are ranked by counting.  The rare row with more candidates than are kept (long
+// runs of equal logits) takes rounds of "highest value, lowest tokens first".
+//
+// A row is one CTA's, or is cut between the CTAs of a cluster when there are few rows; the
+// parts meet in distributed shared memory.  Every sum has a fixed order.
+#include <algorithm>
+#include <climits>
+#include <cmath>
+#include <type_traits>
+
+#include "common.cuh"
+#include "ptx.cuh"
+#include "types16.cuh"
+
+namespace nvfp4 {
+namespace logprobs {
+
+constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
+constexpr int kMaxTop = 32;
+constexpr int kCandidates = 512;   // one a thread when they are ranked
+constexpr int kMaxCluster = 8;
+constexpr float kCoolest = 1e-30f, kHottest = 1e30f;  // temperatures: c and kFar / c stay normal numbers
+constexpr int kBatch = 4;          // vectors of a thread in flight
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kFar = -200.0f;    // 2^-200 is zero in fp32: where the exponents of masked logits are put
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <typename T>
+constexpr int kVec = 16 / (int)sizeof(T);
+
+template <typename T>
+__device__ __forceinline__ float to_float(T v) {
+    return Type16<T>::load(&v);
+}
+template <>
+__device__ __forceinline__ float to_float<float>(float v) {
+    return v;
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack(const uint4 &v, float (&f)[kVec<T>]) {
+    if constexpr (sizeof(T) == 4) {
+        f[0] = __uint_as_float(v.x);
+        f[1] = __uint_as_float(v.y);
+        f[2] = __uint_as_float(v.z);
+        f[3] = __uint_as_float(v.w);
+    } else {
+        unpack8<T>(v, f);
+    }
+}
+
+// A row as 16-byte vectors at 16-byte addresses; the first and the last may reach past it.
+template <typename T>
+struct Row {
+    const T *x;   // first element
+    int shift;    // elements of the first vector before it
+    int n;        // elements
+    __device__ __forceinline__ Row(const T *p, int len)
+        : x(p), shift((int)((reinterpret_cast<uintptr_t>(p) & 15u) / sizeof(T))), n(len) {}
+    __device__ __forceinline__ int vectors() const { return (int)(((int64_t)n + shift + kVec<T> - 1) / kVec<T>); }
+    __device__ __forceinline__ int first(int v) const { return v * kVec<T> - shift; }  // may be negative
+    // -inf past the row's ends; its elements alone are read
+    __device__ __forceinline__ void load(int v, float (&f)[kVec<T>]) const {
+        const int e = first(v);
+        if (e >= 0 && e + kVec<T> <= n) {
+            unpack<T>(__ldg(reinterpret_cast<const uint4 *>(x + e)), f);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kVec<T>; i++) f[i] = e + i >= 0 && e + i < n ? to_float<T>(x[e + i]) : -INFINITY;
+        }
+    }
+};
+
+struct Params {
+    const void *logits, *targets;
+    int64_t ld;
+    int target8;       // targets are 64-bit
+    int T, V, k;
+    float temperature, c, far;  // c = log2(e) / temperature, far = kFar / c
+    float *logprobs, *entropy, *top_logprobs, *lse;
+    int *top_tokens;
+};
+
+__device__ __forceinline__ int64_t target_of(const void *targets, int wide, int64_t t) {
+    return wide ? static_cast<const int64_t *>(targets)[t] : static_cast<const int *>(targets)[t];
+}
+
+// A number whose signed order is the floats' order, both zeros alike.
+__device__ __forceinline__ int order_key(float v) {
+    const int u = __float_as_int(v + 0.0f);
+    return u ^ ((u >> 31) & 0x7fffffff);
+}
+__device__ __forceinline__ float key_value(int key) { return __int_as_float(key ^ ((key >> 31) & 0x7fffffff)); }
+// Unsigned order of (value, lowest token first).
+__device__ __forceinline__ uint64_t pair_key(float v, int token) {
+    return ((uint64_t)((uint32_t)order_key(v) ^ 0x80000000u) << 32) | (uint32_t)~token;
+}
+__device__ __forceinline__ float pair_value(uint64_t k) { return key_value((int)((uint32_t)(k >> 32) ^ 0x80000000u)); }
+__device__ __forceinline__ int pair_token(uint64_t k) { return (int)~(uint32_t)k; }
+
+struct Stats {
+    float m, s0, s1;  // maximum (of the logits themselves), and the sums relative to it
+};
+// fmaxf takes the bound where the difference is NaN: of two infinities, or of a masked NaN.
+__device__ __forceinline__ Stats join(const Stats &a, const Stats &b, const Params &p) {
+    Stats r;
+    r.m = fmaxf(a.m, b.m);
+    const float da = fmaxf(a.m - r.m, p.far), db = fmaxf(b.m - r.m, p.far);
+    const float fa = ex2(da * p.c), fb = ex2(db * p.c);
+    r.s0 = a.s0 * fa + b.s0 * fb;
+    r.s1 = fmaf(a.s0, da, a.s1) * fa + fmaf(b.s0, db, b.s1) * fb;
+    return r;
+}
+__device__ __forceinline__ Stats shuffle(const Stats &a, int o) {
+    return {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s0, o),
+            __shfl_xor_sync(0xffffffffu, a.s1, o)};
+}
+
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t n;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(n));
+    return n;
+}
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint64_t ld_cluster_u64(uint32_t addr) {
+    uint64_t v;
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
+    return v;
+}
+
+struct Shared {
+    uint64_t cand[kCandidates];
+    uint64_t top[kMaxTop];        // this CTA's alternatives, highest first
+    Stats part[kWarps];
+    float best[kThreads];         // the threads' maxima
+    int winners[kThreads];
+    int count[kWarps + 1];
+    float bound;
+    int n_winners, n_cand, n_top;
+};
+
+// Ranks n <= kThreads distinct keys by counting; the first k to out.
+__device__ __forceinline__ void rank_keys(const uint64_t *keys, int n, int k, uint64_t *out) {
+    if ((int)threadIdx.x < n) {
+        const uint64_t mine = keys[threadIdx.x];
+        int rank = 0;
+        for (int j = 0; j < n; j++) rank += keys[j] > mine;
+        if (rank < k) out[rank] = mine;
+    }
+}
+
+// The alternatives of vectors [v0, v1) where equal values are too many to keep: the highest
+// value that is left, then its tokens from the lowest, until there are k.
+template <typename T>
+__device__ __noinline__ void select_rounds(const Row<T> &row, int v0, int v1, int k, Shared &s) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int have = 0, last = INT_MAX;  // order_key of +inf is below INT_MAX
+    while (have < k) {
+        int best = INT_MIN;
+        for (int v = v0 + (int)threadIdx.x; v < v1; v += kThreads) {
+            float f[kVec<T>];
+            row.load(v, f);
+#pragma unroll
+            for (int i = 0; i < kVec<T>; i++) {
+                const int key = f[i] > -INFINITY ? order_key(f[i]) : INT_MIN;
+                if (key < last) best = max(best, key);
+            }
+        }
+        best = __reduce_max_sync(0xffffffffu, best);
+        __syncthreads();
+        if (lane == 0) s.count[warp] = best;
+        __syncthreads();
+        for (int w = 0; w < kWarps; w++) best = max(best, s.count[w]);
+        if (best == INT_MIN) break;
+        for (int base = v0; base < v1 && have < k; base += kThreads) {
+            const int v = base + (int)threadIdx.x;
+            float f[kVec<T>];
+            int n = 0;
+            if (v < v1) {
+                row.load(v, f);
+#pragma unroll
+                for (int i = 0; i < kVec<T>; i++) n += f[i] > -INFINITY && order_key(f[i]) == best;
+            }
+            int before = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, before, o);
+                if (lane >= o) before += u;
+            }
+            __syncthreads();  // the counts of the round before have been read
+            if (lane == 31) s.count[warp] = before;
+            __syncthreads();
+            int at = have + before - n, total = 0;
+            for (int w = 0; w < kWarps; w++) {
+                if (w < warp) at += s.count[w];
+                total += s.count[w];
+            }
+            if (n)
+#pragma unroll
+                for (int i = 0; i < kVec<T>; i++)
+                    if (f[i] > -INFINITY && order_key(f[i]) == best) {
+                        if (at < k) s.top[at] = pair_key(f[i], row.first(v) + i);
+                        at++;
+                    }
+            have = min(k, have + total);
+        }
+        last = best;
+    }
+    if (threadIdx.x == 0) s.n_top = have;
+}
+
+template <typename T, bool ENTROPY, bool TOP>
+__global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const Params p) {
+    __shared__ Shared s;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int parts = (int)cluster_size(), part = (int)cluster_ctarank();
+    for (int64_t t = blockIdx.x / parts; t < p.T; t += gridDim.x / parts) {
+        const Row<T> row(static_cast<const T *>(p.logits) + t * p.ld, p.V);
+        const int nv = row.vectors();
+        const int v0 = (int)((int64_t)nv * part / parts), v1 = (int)((int64_t)nv * (part + 1) / parts);
+        float target = -INFINITY;
+        bool ignored = true;
+        if (part == 0 && threadIdx.x == 0) {
+            const int64_t at = target_of(p.targets, p.target8, t);
+            ignored = at < 0 || at >= p.V;
+            if (!ignored) target = to_float<T>(row.x[at]);
+        }
+        // ---- the pass
+        Stats a = {-INFINITY, 0.0f, 0.0f};
+        for (int64_t v = v0 + (int)threadIdx.x; v < v1; v += kBatch * kThreads) {
+            float f[kBatch][kVec<T>];
+#pragma unroll
+            for (int b = 0; b < kBatch; b++) {
+                if (v + b * kThreads < v1) {
+                    row.load((int)(v + b * kThreads), f[b]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kVec<T>; i++) f[b][i] = -INFINITY;
+                }
+            }
+            float m = f[0][0];
+#pragma unroll
+            for (int b = 0; b < kBatch; b++)
+#pragma unroll
+                for (int i = 0; i < kVec<T>; i++) m = fmaxf(m, f[b][i]);
+            if (m > a.m) {
+                const float d = fmaxf(a.m - m, p.far), scale = ex2(d * p.c);
+                if (ENTROPY) a.s1 = fmaf(a.s0, d, a.s1) * scale;
+                a.s0 *= scale;
+                a.m = m;
+            }
+#pragma unroll
+            for (int b = 0; b < kBatch; b++)
+#pragma unroll
+                for (int i = 0; i < kVec<T>; i++) {
+                    const float d = fmaxf(f[b][i] - a.m, p.far), e = ex2(d * p.c);
+                    a.s0 += e;
+                    if (ENTROPY) a.s1 = fmaf(d, e, a.s1);
+                }
+        }
+        // ---- statistics of the CTA
+        if (TOP) s.best[threadIdx.x] = a.m;
+        Stats w = a;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) w = join(w, shuffle(w, o), p);
+        if (lane == 0) s.part[warp] = w;
+        if (threadIdx.x == 0) s.n_winners = s.n_cand = s.n_top = 0;
+        __syncthreads();
+        if (TOP) {
+            // ---- candidates: the lanes' columns of maxima, sorted; the k-th is the bound
+            if (warp == 0) {
+                float b = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < kWarps; i++) b = fmaxf(b, s.best[i * 32 + lane]);
+#pragma unroll
+                for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+                    for (int o = size >> 1; o; o >>= 1) {
+                        const float other = __shfl_xor_sync(0xffffffffu, b, o);
+                        const bool high = ((lane & o) == 0) == ((lane & size) == 0);  // descending overall
+                        b = high ? fmaxf(b, other) : fminf(b, other);
+                    }
+                b = __shfl_sync(0xffffffffu, b, p.k - 1);
+                if (lane == 0) s.bound = b;
+            }
+            __syncthreads();
+            const float bound = s.bound;
+            if (a.m > -INFINITY && a.m >= bound) s.winners[atomicAdd(&s.n_winners, 1)] = (int)threadIdx.x;
+            __syncthreads();
+            const int per = (v1 - v0 + kThreads - 1) / kThreads;  // vectors of a thread, at most
+            const int all = s.n_winners * per;
+            for (int i = threadIdx.x; i < all; i += kThreads) {
+                const int v = v0 + s.winners[i / per] + i % per * kThreads;
+                if (v >= v1) continue;
+                float f[kVec<T>];
+                row.load(v, f);
+#pragma unroll
+                for (int e = 0; e < kVec<T>; e++)
+                    if (f[e] > -INFINITY && f[e] >= bound) {
+                        const int at = atomicAdd(&s.n_cand, 1);
+                        if (at < kCandidates) s.cand[at] = pair_key(f[e], row.first(v) + e);
+                    }
+            }
+            __syncthreads();
+            const int n = s.n_cand;
+            if (n <= kCandidates) {
+                rank_keys(s.cand, n, p.k, s.top);
+                if (threadIdx.x == 0) s.n_top = min(n, p.k);
+            } else {
+                select_rounds<T>(row, v0, v1, p.k, s);
+            }
+        }
+        // ---- join the CTAs' parts, finish the row
+        if (parts > 1) {
+            __syncwarp();
+            cluster_sync();
+        } else if (TOP) {
+            __syncthreads();
+        }
+        if (part == 0) {
+            Stats all = {-INFINITY, 0.0f, 0.0f};
+            if (warp == 0) {
+                for (int i = lane; i < parts * kWarps; i += 32) {
+                    const uint32_t at = map_to_cta(smem_u32(&s.part[i % kWarps]), i / kWarps);
+                    all = join(all, {ld_cluster_f32(at), ld_cluster_f32(at + 4), ld_cluster_f32(at + 8)}, p);
+                }
+#pragma unroll
+                for (int o = 16; o; o >>= 1) all = join(all, shuffle(all, o), p);
+                // lane 0's for all: a join's two sides round differently
+                all.m = __shfl_sync(0xffffffffu, all.m, 0);
+                all.s0 = __shfl_sync(0xffffffffu, all.s0, 0);
+                all.s1 = __shfl_sync(0xffffffffu, all.s1, 0);
+            }
+            const float l = logf(all.s0);
+            if (threadIdx.x == 0) {
+                const bool empty = all.m == -INFINITY;
+                const bool none = !(target > -INFINITY);
+                p.lse[t] = empty ? -INFINITY : all.m / p.temperature + l;
+                p.logprobs[t] = ignored ? 0.0f : empty || none ? -INFINITY : (target - all.m) / p.temperature - l;
+                if (ENTROPY) p.entropy[t] = empty ? 0.0f : l - all.s1 / all.s0 / p.temperature;
+            }
+            if (TOP) {
+                int n = s.n_top;
+                if (parts > 1) {
+                    // candidates have been ranked: their place takes the parts' alternatives
+                    if ((int)threadIdx.x < parts * kMaxTop) {
+                        const int q = threadIdx.x / kMaxTop, j = threadIdx.x % kMaxTop;
+                        const int have = (int)__float_as_int(ld_cluster_f32(map_to_cta(smem_u32(&s.n_top), q)));
+                        s.cand[threadIdx.x] = j < have ? ld_cluster_u64(map_to_cta(smem_u32(&s.top[j]), q))
+                                                       : (uint64_t)(kMaxCluster * kMaxTop - threadIdx.x - 1);  // below all
+                    }
+                    n = 0;
+                    for (int q = 0; q < parts; q++)
+                        n += (int)__float_as_int(ld_cluster_f32(map_to_cta(smem_u32(&s.n_top), q)));
+                    n = min(n, p.k);
+                    __syncthreads();
+                    // ranked into the other half, since s.top may still be read as a part
+                    uint64_t *merged = s.cand + kMaxCluster * kMaxTop;
+                    rank_keys(s.cand, parts * kMaxTop, p.k, merged);
+                    __syncthreads();
+                    if ((int)threadIdx.x < n) s.top[threadIdx.x] = merged[threadIdx.x];
+                    __syncthreads();
+                }
+                if (warp == 0 && lane < p.k) {
+                    const int64_t at = t * p.k + lane;
+                    const float v = lane < n ? pair_value(s.top[lane]) : -INFINITY;
+                    p.top_tokens[at] = lane < n ? pair_token(s.top[lane]) : -1;
+                    p.top_logprobs[at] = lane < n ? (v - all.m) / p.temperature - l : -INFINITY;
+                }
+            }
+        }
+        if (parts > 1) {
+            __syncwarp();
+            cluster_sync();  // the first CTA has read the others' parts
+        } else {
+            __syncthreads();
+        }
+    }
+}
+
+// ------------------------------------------------------------------------- gradient
+struct GradParams {
+    const float *dlogprobs, *dentropy, *lse, *entropy;
+    const void *logits, *targets;
+    void *dlogits;
+    int64_t ld, ldd;
+    int target8;
+    int V, W;
+    int chunks;  // CTAs of a row
+    float inv_temperature;
+};
+
+constexpr int kGradThreads = 256;
+constexpr int kGradBatch = 4;
+
+// Elementwise, with the row's scalars in registers: bound by reading and writing the logits.
+// SAME: the gradient's rows have the logits' alignment, so whole vectors go out.
+template <typename T, bool SAME>
+__global__ void __launch_bounds__(kGradThreads) logprobs_grad_kernel(const GradParams p) {
+    const int64_t t = blockIdx.x / p.chunks;
+    const int chunk = (int)(blockIdx.x - t * p.chunks);
+    const T *x = static_cast<const T *>(p.logits) + t * p.ld;
+    T *d = static_cast<T *>(p.dlogits) + t * p.ldd;
+    const int64_t target = target_of(p.targets, p.target8, t);
+    const float g = target >= 0 && target < p.V ? p.dlogprobs[t] * p.inv_temperature : 0.0f;
+    const float h = p.dentropy ? p.dentropy[t] * p.inv_temperature : 0.0f;
+    const float H = p.dentropy ? p.entropy[t] : 0.0f;
+    const float lse = p.lse[t];
+    const float a = fmaf(h, H, g);  // d = -p (g + h H + h log p)
+    auto grad = [&](float v, int64_t e) {
+        if (e >= p.V || !(v > -INFINITY)) return 0.0f;
+        float l = fmaf(v, p.inv_temperature, -lse);
+        l = l > 0.0f ? 0.0f : l;  // of logits past 2^24 nothing but their rounding is left: p stays below 1
+        const float q = ex2(l * kLog2e);
+        const float y = q == 0.0f ? 0.0f : -q * fmaf(h, l, a);
+        return e == target ? y + g : y;
+    };
+    auto put = [](float v) {
+        if constexpr (sizeof(T) == 4) return v;
+        else return Type16<T>::round(v);
+    };
+    if constexpr (SAME) {
+        const Row<T> row(x, p.W);
+        const int nv = row.vectors();
+        const int64_t v0 = (int64_t)chunk * kGradBatch * kGradThreads + threadIdx.x;
+        uint4 raw[kGradBatch];
+#pragma unroll
+        for (int i = 0; i < kGradBatch; i++) {
+            const int64_t v = v0 + i * kGradThreads;
+            const int64_t e = v * kVec<T> - row.shift;
+            if (v < nv && e >= 0 && e + kVec<T> <= p.W) raw[i] = *reinterpret_cast<const uint4 *>(x + e);
+        }
+#pragma unroll
+        for (int i = 0; i < kGradBatch; i++) {
+            const int64_t v = v0 + i * kGradThreads;
+            if (v >= nv) break;
+            const int64_t e = v * kVec<T> - row.shift;
+            if (e >= 0 && e + kVec<T> <= p.W) {
+                float f[kVec<T>];
+                unpack<T>(raw[i], f);
+#pragma unroll
+                for (int j = 0; j < kVec<T>; j++) f[j] = grad(f[j], e + j);
+                uint4 o;
+                if constexpr (sizeof(T) == 4)
+                    o = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
+                                   __float_as_uint(f[3]));
+                else
+                    o = pack8<T>(f);
+                *reinterpret_cast<uint4 *>(d + e) = o;
+            } else {
+                for (int j = 0; j < kVec<T>; j++)
+                    if (e + j >= 0 && e + j < p.W) d[e + j] = put(grad(to_float<T>(x[e + j]), e + j));
+            }
+        }
+    } else {
+        const int64_t e0 = (int64_t)chunk * kGradBatch * kGradThreads * kVec<T> + threadIdx.x;
+#pragma unroll 4
+        for (int i = 0; i < kGradBatch * kVec<T>; i++) {
+            const int64_t e = e0 + i * kGradThreads;
+            if (e < p.W) d[e] = put(grad(to_float<T>(x[e]), e));
+        }
+    }
+}
+
+// ------------------------------------------------------------------------- host side
+// CTAs that share a row: as many as keep every row's on the GPU at once, while each still has
+// a batch of vectors for every thread.
+static int parts_of(int T, int64_t vectors, int sm_count) {
+    int parts = 1;
+    while (parts < kMaxCluster && (int64_t)T * parts <= sm_count && vectors >= (int64_t)parts * 2 * kThreads)
+        parts *= 2;
+    return parts;
+}
+
+template <typename T, bool ENTROPY, bool TOP>
+static int launch(const Params &p, const DeviceInfo &di, cudaStream_t s) {
+    const int parts = parts_of(p.T, p.V / kVec<T>, di.sm_count);
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = parts;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)(parts == 1 ? std::min<int64_t>(p.T, 2 * di.sm_count) : p.T * parts));
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = s;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, logprobs_kernel<T, ENTROPY, TOP>, p) != cudaSuccess) return NVFP4_ERR_CUDA;
+    count_launch();
+    return cuda_status(cudaGetLastError());
+}
+
+template <typename T>
+static int forward(const Params &p, const DeviceInfo &di, cudaStream_t s) {
+    if (p.entropy) return p.k ? launch<T, true, true>(p, di, s) : launch<T, true, false>(p, di, s);
+    return p.k ? launch<T, false, true>(p, di, s) : launch<T, false, false>(p, di, s);
+}
+
+// CTAs of a row's gradient, at any alignment of the row.
+static int grad_chunks(int W, int size) {
+    const int64_t per = 16 / size, vectors = ((int64_t)W + 2 * per - 2) / per;
+    return (int)((vectors + kGradBatch * kGradThreads - 1) / (kGradBatch * kGradThreads));
+}
+
+template <typename T>
+static int backward(GradParams p, int64_t n_rows, cudaStream_t s) {
+    const uintptr_t from = reinterpret_cast<uintptr_t>(p.logits), to = reinterpret_cast<uintptr_t>(p.dlogits);
+    const bool same = ((from - to) & 15u) == 0 && ((p.ld - p.ldd) * (int64_t)sizeof(T)) % 16 == 0;
+    p.chunks = grad_chunks(p.W, sizeof(T));
+    const unsigned grid = (unsigned)(n_rows * p.chunks);
+    if (same) logprobs_grad_kernel<T, true><<<grid, kGradThreads, 0, s>>>(p);
+    else logprobs_grad_kernel<T, false><<<grid, kGradThreads, 0, s>>>(p);
+    count_launch();
+    return cuda_status(cudaGetLastError());
+}
+
+static bool misaligned(const void *p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) != 0; }
+
+// What both directions check of the logits and targets.
+static int check_rows(const void *logits, int64_t ld, int dtype, const void *targets, int target_bytes, int T, int V,
+                      int W, float temperature) {
+    if (dtype < NVFP4_BF16 || dtype > NVFP4_F32 || (target_bytes != 4 && target_bytes != 8)) return NVFP4_ERR_INVALID;
+    if (!(temperature >= kCoolest) || !(temperature <= kHottest)) return NVFP4_ERR_INVALID;
+    if (T < 0 || V < 1 || V > INT_MAX - 1024 || W < V || W > INT_MAX - 1024 || ld < W) return NVFP4_ERR_SHAPE;
+    if (T && (!logits || !targets)) return NVFP4_ERR_INVALID;
+    if (misaligned(logits, dtype == NVFP4_F32 ? 4 : 2) || misaligned(targets, target_bytes)) return NVFP4_ERR_ALIGN;
+    return NVFP4_OK;
+}
+
+}  // namespace logprobs
+}  // namespace nvfp4
+
+using namespace nvfp4;
+
+extern "C" {
+
+int nvfp4_token_logprobs(const void *logits, int64_t ld, int dtype, const void *targets, int target_bytes, int T,
+                         int V, int top_k, float temperature, float *logprobs, float *entropy, float *top_logprobs,
+                         int32_t *top_tokens, float *lse, void *stream) {
+    int st = logprobs::check_rows(logits, ld, dtype, targets, target_bytes, T, V, V, temperature);
+    if (st) return st;
+    if (top_k < 0 || top_k > logprobs::kMaxTop) return NVFP4_ERR_SHAPE;
+    if (T && (!logprobs || !lse || (top_k && (!top_logprobs || !top_tokens)))) return NVFP4_ERR_INVALID;
+    if (logprobs::misaligned(logprobs, 4) || logprobs::misaligned(entropy, 4) || logprobs::misaligned(lse, 4) ||
+        logprobs::misaligned(top_logprobs, 4) || logprobs::misaligned(top_tokens, 4))
+        return NVFP4_ERR_ALIGN;
+    DeviceInfo di;
+    if ((st = device_info(&di))) return st;
+    if (T == 0) return NVFP4_OK;
+    logprobs::Params p = {};
+    p.logits = logits;
+    p.targets = targets;
+    p.ld = ld;
+    p.target8 = target_bytes == 8;
+    p.T = T;
+    p.V = V;
+    p.k = top_k;
+    p.temperature = temperature;
+    p.c = logprobs::kLog2e / temperature;
+    p.far = logprobs::kFar / p.c;
+    p.logprobs = logprobs;
+    p.entropy = entropy;
+    p.top_logprobs = top_logprobs;
+    p.top_tokens = top_tokens;
+    p.lse = lse;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (dtype == NVFP4_BF16) return logprobs::forward<__nv_bfloat16>(p, di, s);
+    if (dtype == NVFP4_F16) return logprobs::forward<__half>(p, di, s);
+    return logprobs::forward<float>(p, di, s);
+}
+
+int nvfp4_token_logprobs_backward(const float *dlogprobs, const float *dentropy, const void *logits, int64_t ld,
+                                  int dtype, const void *targets, int target_bytes, const float *lse,
+                                  const float *entropy, int T, int V, int W, float temperature, void *dlogits,
+                                  int64_t ldd, void *stream) {
+    int st = logprobs::check_rows(logits, ld, dtype, targets, target_bytes, T, V, W, temperature);
+    if (st) return st;
+    if (ldd < W || (int64_t)T * logprobs::grad_chunks(W, dtype == NVFP4_F32 ? 4 : 2) > INT_MAX) return NVFP4_ERR_SHAPE;
+    if (T && (!dlogprobs || !lse || !dlogits || (dentropy && !entropy))) return NVFP4_ERR_INVALID;
+    if (logprobs::misaligned(dlogprobs, 4) || logprobs::misaligned(dentropy, 4) || logprobs::misaligned(lse, 4) ||
+        logprobs::misaligned(entropy, 4) || logprobs::misaligned(dlogits, dtype == NVFP4_F32 ? 4 : 2))
+        return NVFP4_ERR_ALIGN;
+    DeviceInfo di;
+    if ((st = device_info(&di))) return st;
+    if (T == 0) return NVFP4_OK;
+    logprobs::GradParams p = {};
+    p.dlogprobs = dlogprobs;
+    p.dentropy = dentropy;
+    p.lse = lse;
+    p.entropy = entropy;
+    p.logits = logits;
+    p.targets = targets;
+    p.dlogits = dlogits;
+    p.ld = ld;
+    p.ldd = ldd;
+    p.target8 = target_bytes == 8;
+    p.V = V;
+    p.W = W;
+    p.inv_temperature = 1.0f / temperature;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (dtype == NVFP4_BF16) return logprobs::backward<__nv_bfloat16>(p, T, s);
+    if (dtype == NVFP4_F16) return logprobs::backward<__half>(p, T, s);
+    return logprobs::backward<float>(p, T, s);
+}
+
+}  // extern "C"

@@ -15,6 +15,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cmath>
 #include <string>
 
 #include "../../include/nvfp4_b200.h"
@@ -33,7 +34,13 @@ struct Entries {
     decltype(&nvfp4_moe_dispatch) dispatch;
     decltype(&nvfp4_moe_combine) combine;
     decltype(&nvfp4_moe_combine_backward) combine_backward;
+    decltype(&nvfp4_embedding) embedding;
+    decltype(&nvfp4_embedding_backward_workspace_size) embedding_backward_ws;
+    decltype(&nvfp4_embedding_backward) embedding_backward;
+    decltype(&nvfp4_token_logprobs) logprobs;
+    decltype(&nvfp4_token_logprobs_backward) logprobs_backward;
 } L;
+constexpr int kEntries = sizeof(Entries) / sizeof(void *);
 PyObject *on_status = nullptr;  // called with (status, entry point) where a status is not OK
 
 struct Refused {};  // a Python exception has been set
@@ -445,11 +452,174 @@ PyObject *moe_combine_backward(PyObject *const *a) {
     return tuple_of<2>({wrap(std::move(dx)), wrap(std::move(dw))});
 }
 
+// Token ids, or targets: a contiguous int32 or int64 CUDA tensor.
+int token_bytes(const at::Tensor &t, const char *name) {
+    const auto type = t.scalar_type();
+    if (!t.is_cuda() || (type != at::kInt && type != at::kLong) || !t.is_contiguous())
+        refuse(std::string(name) + " must be a contiguous int32 or int64 CUDA tensor");
+    return type == at::kLong ? 8 : 4;
+}
+
+float scale_of(PyObject *o) {
+    const float v = (float)number(o);
+    if (!std::isfinite(v)) refuse("scale must be a finite number");
+    return v;
+}
+
+// embedding(tokens, table, scale)
+PyObject *embedding(PyObject *const *a) {
+    const at::Tensor &t = tensor(a[0], "tokens"), &table = tensor(a[1], "table");
+    const float scale = scale_of(a[2]);
+    const int bytes = token_bytes(t, "tokens");
+    const Rows r = rows_of(table, "table");
+    if (!r.M) refuse("table must have a row");
+    if (t.device() != table.device()) refuse("tokens must be on the table's device");
+    const int T = small(t.numel(), "the number of tokens");
+    auto shape = t.sizes().vec();
+    shape.push_back(r.K);
+    at::Tensor y;
+    check(unlocked([&] {
+              y = empty(shape, table.scalar_type(), table);
+              const Stream s(table);
+              return L.embedding(t.data_ptr(), bytes, table.data_ptr(), r.pitch, scale, y.data_ptr(), T, r.M, r.K,
+                                 r.dtype, s.handle);
+          }),
+          "nvfp4_embedding");
+    return wrap(std::move(y));
+}
+
+// embedding_backward(dy, tokens, rows, scale)
+PyObject *embedding_backward(PyObject *const *a) {
+    const at::Tensor &dy = tensor(a[0], "dy"), &t = tensor(a[1], "tokens");
+    const int V = small(integer(a[2]), "the number of rows");
+    const float scale = scale_of(a[3]);
+    const int bytes = token_bytes(t, "tokens");
+    if (dy.device() != t.device()) refuse("tokens must be on dy's device");
+    if (dy.dim() != t.dim() + 1 || dy.sizes().slice(0, t.dim()) != t.sizes())
+        refuse("dy must have the tokens' shape and a last dimension of columns");
+    if (dy.dim() != 2 && !dy.is_contiguous()) refuse("dy must be contiguous");
+    if (!V) refuse("the table must have a row");
+    const int T = small(t.numel(), "the number of tokens");
+    Rows r;
+    if (dy.dim() == 2) {
+        r = rows_of(dy, "dy");
+    } else {
+        r.dtype = dtype16(dy);
+        r.K = small(dy.size(-1), "the number of columns");
+        r.pitch = r.K;
+        if (r.dtype < 0) refuse("dy must be a bf16 or fp16 CUDA tensor");
+        if (r.K % 8 || !r.K) refuse("dy must have a multiple of 8 columns");
+    }
+    at::Tensor d;
+    check(unlocked([&] {
+              d = empty({V, r.K}, dy.scalar_type(), dy);
+              const size_t need = L.embedding_backward_ws(T, V, r.K);
+              at::Tensor ws = empty({(int64_t)((need + 3) / 4)}, at::kInt, dy);
+              const Stream s(dy);
+              return L.embedding_backward(dy.data_ptr(), r.pitch, t.data_ptr(), bytes, scale, d.data_ptr(), T, V, r.K,
+                                          r.dtype, ws.data_ptr(), need, s.handle);
+          }),
+          "nvfp4_embedding_backward");
+    return wrap(std::move(d));
+}
+
+struct Vocab {
+    int T, W, V, dtype, target_bytes;
+    int64_t pitch;
+};
+
+// Rows of logits and their targets.
+Vocab vocab_of(const at::Tensor &l, const at::Tensor &targets, PyObject *vocab, double temperature) {
+    Vocab r;
+    r.dtype = l.scalar_type() == at::kFloat ? NVFP4_F32 : dtype16(l);
+    if (!l.is_cuda() || l.dim() != 2 || r.dtype < 0) refuse("logits must be a 2-D bf16, fp16 or fp32 CUDA tensor");
+    r.T = small(l.size(0), "the number of rows");
+    r.W = small(l.size(1), "the number of columns");
+    r.pitch = r.T > 1 ? l.stride(0) : r.W;  // a single row's stride says nothing
+    if (!r.W || (r.W > 1 && l.stride(1) != 1) || r.pitch < r.W) refuse("logits must have contiguous rows");
+    r.V = vocab == Py_None ? r.W : small(integer(vocab), "vocab");
+    if (r.V < 1 || r.V > r.W) refuse("vocab must be between 1 and the logits' columns");
+    r.target_bytes = token_bytes(targets, "targets");
+    if (targets.dim() != 1 || targets.size(0) != r.T || targets.device() != l.device())
+        refuse("targets must have one entry for each row of logits, on their device");
+    if (!(temperature > 0.0) || !std::isfinite(temperature)) refuse("temperature must be a positive number");
+    return r;
+}
+
+// token_logprobs(logits, targets, vocab, top_k, temperature, entropy)
+PyObject *token_logprobs(PyObject *const *a) {
+    const at::Tensor &l = tensor(a[0], "logits"), &targets = tensor(a[1], "targets");
+    const int64_t k = integer(a[3]);
+    const double temperature = number(a[4]);
+    const bool entropy = truth(a[5]);
+    const Vocab r = vocab_of(l, targets, a[2], temperature);
+    if (k < 0 || k > 32) refuse("top_k must be between 0 and 32");
+    at::Tensor logp, ent, top, tokens, lse;
+    check(unlocked([&] {
+              logp = empty({r.T}, at::kFloat, l);
+              lse = empty({r.T}, at::kFloat, l);
+              if (entropy) ent = empty({r.T}, at::kFloat, l);
+              if (k) {
+                  top = empty({r.T, k}, at::kFloat, l);
+                  tokens = empty({r.T, k}, at::kInt, l);
+              }
+              const Stream s(l);
+              return L.logprobs(l.data_ptr(), r.pitch, r.dtype, targets.data_ptr(), r.target_bytes, r.T, r.V, (int)k,
+                                (float)temperature, logp.data_ptr<float>(), entropy ? ent.data_ptr<float>() : nullptr,
+                                k ? top.data_ptr<float>() : nullptr, k ? tokens.data_ptr<int>() : nullptr,
+                                lse.data_ptr<float>(), s.handle);
+          }),
+          "nvfp4_token_logprobs");
+    return tuple_of<5>({wrap(std::move(logp)), entropy ? wrap(std::move(ent)) : none(),
+                        k ? wrap(std::move(top)) : none(), k ? wrap(std::move(tokens)) : none(),
+                        wrap(std::move(lse))});
+}
+
+// token_logprobs_backward(dlogprobs, dentropy, logits, targets, lse, entropy, vocab, temperature, out)
+PyObject *token_logprobs_backward(PyObject *const *a) {
+    const at::Tensor &dl = tensor(a[0], "dlogprobs"), &l = tensor(a[2], "logits"), &targets = tensor(a[3], "targets");
+    const at::Tensor *dent = maybe(a[1], "dentropy"), *ent = maybe(a[5], "entropy");
+    const at::Tensor &lse = tensor(a[4], "lse");
+    const double temperature = number(a[7]);
+    const Vocab r = vocab_of(l, targets, a[6], temperature);
+    expect(dl, "dlogprobs", {r.T}, at::kFloat, l);
+    expect(lse, "lse", {r.T}, at::kFloat, l);
+    if (dent) {
+        if (!ent) refuse("the entropy's gradient needs the entropies");
+        expect(*dent, "dentropy", {r.T}, at::kFloat, l);
+        expect(*ent, "entropy", {r.T}, at::kFloat, l);
+    }
+    at::Tensor d;
+    if (a[8] != Py_None) {
+        d = tensor(a[8], "out");
+        if (d.scalar_type() != l.scalar_type() || d.device() != l.device() || d.sizes() != l.sizes() ||
+            (r.W > 1 && d.stride(1) != 1) || (r.T > 1 && d.stride(0) < r.W))
+            refuse("out must have the logits' shape, type and device, and contiguous rows");
+        // the logits themselves are fine: each element is read where it is then written
+        if (d.data_ptr() != l.data_ptr() || (r.T > 1 && d.stride(0) != l.stride(0))) apart(d, &l, "logits");
+        apart(d, &targets, "targets");
+        apart(d, &dl, "dlogprobs");
+        apart(d, &lse, "lse");
+        apart(d, dent, "dentropy");
+        apart(d, ent, "entropy");
+    }
+    check(unlocked([&] {
+              if (!d.defined()) d = empty({r.T, r.W}, l.scalar_type(), l);
+              const Stream s(l);
+              return L.logprobs_backward(dl.data_ptr<float>(), static_cast<const float *>(ptr(dent)), l.data_ptr(),
+                                         r.pitch, r.dtype, targets.data_ptr(), r.target_bytes, lse.data_ptr<float>(),
+                                         static_cast<const float *>(ptr(ent)), r.T, r.V, r.W, (float)temperature,
+                                         d.data_ptr(), r.T > 1 ? d.stride(0) : r.W, s.handle);
+          }),
+          "nvfp4_token_logprobs_backward");
+    return wrap(std::move(d));
+}
+
 // bind(on_status, addresses of the entry points in the order of Entries)
 PyObject *bind(PyObject *const *a) {
-    static_assert(sizeof(Entries) == 11 * sizeof(void *), "one address each");
-    void *at[11];
-    for (int i = 0; i < 11; i++) at[i] = reinterpret_cast<void *>((uintptr_t)PyLong_AsUnsignedLongLong(a[1 + i]));
+    static_assert(sizeof(Entries) == kEntries * sizeof(void *), "one address each");
+    void *at[kEntries];
+    for (int i = 0; i < kEntries; i++) at[i] = reinterpret_cast<void *>((uintptr_t)PyLong_AsUnsignedLongLong(a[1 + i]));
     if (PyErr_Occurred()) throw Refused();
     memcpy(&L, at, sizeof(L));
     Py_INCREF(a[0]);
@@ -475,9 +645,11 @@ PyObject *entry(PyObject *, PyObject *const *args, Py_ssize_t n) {
 }
 
 #define METHOD(name, n) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(&entry<name, n>)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {METHOD(bind, 12),           METHOD(linear, 8),          METHOD(linear_backward, 9),
+PyMethodDef methods[] = {METHOD(bind, 1 + kEntries), METHOD(linear, 8),          METHOD(linear_backward, 9),
                          METHOD(moe_route, 6),       METHOD(moe_route_backward, 6), METHOD(moe_dispatch, 2),
-                         METHOD(moe_combine, 4),     METHOD(moe_combine_backward, 3), {nullptr, nullptr, 0, nullptr}};
+                         METHOD(moe_combine, 4),     METHOD(moe_combine_backward, 3),
+                         METHOD(embedding, 3),       METHOD(embedding_backward, 4),
+                         METHOD(token_logprobs, 6),  METHOD(token_logprobs_backward, 9), {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_bind", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -14,5 +14,7 @@ from .ops import (create_tensors, device_status, gemm, gemm_epilogue, gemm_group
 from .layers import linear, linear_backward, linear_grouped, linear_grouped_backward  # noqa: F401
 from .moe import (Routing, moe_combine, moe_combine_backward, moe_dispatch, moe_dispatch_backward, moe_route,  # noqa: F401
                   moe_route_backward)
+from .vocab import (TokenLogprobs, embedding, embedding_backward, token_logprobs,  # noqa: F401
+                    token_logprobs_backward)
 from . import runner_io  # noqa: F401,E402
 from . import torch_ops  # noqa: F401,E402  (registers torch.ops.nvfp4_b200.gemm / .quantize)

@@ -275,3 +275,98 @@ def _combine_grad(ctx, dy):
 
 
 moe_combine.register_autograd(_combine_grad, setup_context=_combine_context)
+
+
+# ----------------------------------------------------------------------- vocabulary
+# nvfp4_b200::embedding and ::token_logprobs, differentiable in the table and the logits.
+@torch.library.custom_op("nvfp4_b200::embedding", mutates_args=(), device_types="cuda")
+def embedding(tokens: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+    """scale * table[tokens], zeros for tokens outside the table; differentiable in table."""
+    return native.embedding(tokens, table, scale)
+
+
+@embedding.register_fake
+def _embedding_fake(tokens, table, scale=1.0):
+    return table.new_empty((*tokens.shape, table.shape[1]))
+
+
+@torch.library.custom_op("nvfp4_b200::embedding_backward", mutates_args=(), device_types="cuda")
+def embedding_backward(dy: torch.Tensor, tokens: torch.Tensor, rows: int, scale: float) -> torch.Tensor:
+    return native.embedding_backward(dy, tokens, rows, scale)
+
+
+@embedding_backward.register_fake
+def _embedding_backward_fake(dy, tokens, rows, scale):
+    return dy.new_empty((rows, dy.shape[-1]))
+
+
+def _embedding_context(ctx, inputs, output):
+    tokens, table, ctx.scale = inputs
+    ctx.save_for_backward(tokens)
+    ctx.rows = table.shape[0]
+
+
+def _embedding_grad(ctx, dy):
+    tokens, = ctx.saved_tensors
+    return None, torch.ops.nvfp4_b200.embedding_backward(dy.contiguous(), tokens, ctx.rows, ctx.scale), None
+
+
+embedding.register_autograd(_embedding_grad, setup_context=_embedding_context)
+
+
+@torch.library.custom_op("nvfp4_b200::token_logprobs", mutates_args=(), device_types="cuda")
+def token_logprobs(
+        logits: torch.Tensor, targets: torch.Tensor, vocab: Optional[int] = None, top_k: int = 0,
+        temperature: float = 1.0, entropy: bool = False
+) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(logprobs, entropy, top_logprobs, top_tokens, lse), empty where they are not asked for;
+    the log probabilities and the entropy carry a gradient to the logits."""
+    r = native.token_logprobs(logits, targets, vocab, top_k, temperature, entropy)
+    return tuple(logits.new_empty(0, dtype=torch.int32 if i == 3 else torch.float32) if t is None else t
+                 for i, t in enumerate(r))
+
+
+@token_logprobs.register_fake
+def _token_logprobs_fake(logits, targets, vocab=None, top_k=0, temperature=1.0, entropy=False):
+    T = logits.shape[0]
+
+    def floats(*shape):
+        return logits.new_empty(shape, dtype=torch.float32)
+
+    top = (T, top_k) if top_k else (0,)
+    return floats(T), floats(T if entropy else 0), floats(*top), logits.new_empty(top, dtype=torch.int32), floats(T)
+
+
+@torch.library.custom_op("nvfp4_b200::token_logprobs_backward", mutates_args=(), device_types="cuda")
+def token_logprobs_backward(dlogprobs: torch.Tensor, dentropy: Optional[torch.Tensor], logits: torch.Tensor,
+                            targets: torch.Tensor, lse: torch.Tensor, entropy: torch.Tensor, vocab: Optional[int],
+                            temperature: float) -> torch.Tensor:
+    return native.token_logprobs_backward(dlogprobs, dentropy, logits, targets, lse,
+                                          None if dentropy is None else entropy, vocab, temperature, None)
+
+
+@token_logprobs_backward.register_fake
+def _token_logprobs_backward_fake(dlogprobs, dentropy, logits, targets, lse, entropy, vocab, temperature):
+    return logits.new_empty(logits.shape)
+
+
+def _logprobs_context(ctx, inputs, output):
+    logits, targets, ctx.vocab, _, ctx.temperature, _ = inputs
+    ctx.save_for_backward(logits, targets, output[1], output[4])
+    ctx.mark_non_differentiable(*output[2:])
+    ctx.set_materialize_grads(False)
+
+
+def _logprobs_grad(ctx, dlogprobs, dentropy, *_):
+    if dlogprobs is None and dentropy is None:
+        return None, None, None, None, None, None
+    logits, targets, entropy, lse = ctx.saved_tensors
+    dlogprobs = torch.zeros_like(lse) if dlogprobs is None else dlogprobs.contiguous()
+    if dentropy is not None:
+        dentropy = dentropy.contiguous() if entropy.shape == lse.shape else None
+    d = torch.ops.nvfp4_b200.token_logprobs_backward(dlogprobs, dentropy, logits, targets, lse, entropy, ctx.vocab,
+                                                     ctx.temperature)
+    return d, None, None, None, None, None
+
+
+token_logprobs.register_autograd(_logprobs_grad, setup_context=_logprobs_context)

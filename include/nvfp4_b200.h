@@ -418,6 +418,53 @@ NVFP4_API int nvfp4_moe_combine_backward(const void *dY, const void *X_rows, int
                                          const float *weights, const int32_t *m_offsets, int T, int E, int top_k,
                                          int K, void *dX_rows, float *dweights, void *stream);
 
+/*
+ * Embedding: Y[t] = scale * table[tokens[t]], rounded once (scale 1: the same bits); a token
+ * outside [0, V), such as the -1 of padding, gives a row of zeros.  tokens are int32
+ * (token_bytes 4) or int64 (8); table [V, K] bf16 or fp16 with rows ld apart; Y [T, K].
+ * K and ld multiples of 8.
+ */
+NVFP4_API int nvfp4_embedding(const void *tokens, int token_bytes, const void *table, int64_t ld, float scale, void *Y,
+                              int T, int V, int K, int dtype, void *stream);
+/*
+ * Gradient of the table: dTable[v] = scale * the sum of dY[t] (rows ldy apart) over the
+ * tokens t equal to v, in fp32 and an order that the tokens alone decide, rounded once; rows
+ * that no token names are zero.  Every row of dTable [V, K] is written.
+ */
+NVFP4_API size_t nvfp4_embedding_backward_workspace_size(int T, int V, int K);
+NVFP4_API int nvfp4_embedding_backward(const void *dY, int64_t ldy, const void *tokens, int token_bytes, float scale,
+                                       void *dTable, int T, int V, int K, int dtype, void *workspace,
+                                       size_t workspace_bytes, void *stream);
+
+/*
+ * Log probabilities of rows of logits [T, >= V] (dtype bf16, fp16 or fp32, rows ld elements
+ * apart, any alignment of their type), of the distribution softmax(logits / temperature)
+ * over the first V columns:
+ *   logprobs[t] = log p[targets[t]], 0 for a target outside [0, V) (ignored);
+ *   entropy[t] = -sum p log p, or NULL;
+ *   top_logprobs, top_tokens [T, top_k]: the most probable tokens, the lowest first among
+ *     equals; -1 and -inf where fewer are left (NULL with top_k 0; top_k <= 32);
+ *   lse[t] = log sum exp(logits / temperature), which the gradient takes.
+ * A token whose logit is -inf or NaN is masked: it has probability zero and is no
+ * alternative.  A row with nothing left has log probability and lse -inf and entropy 0; a
+ * logit of +inf makes a row's results NaN.  1e-30 <= temperature <= 1e30.  targets int32 or int64 (target_bytes 4 or 8);
+ * results fp32.
+ */
+NVFP4_API int nvfp4_token_logprobs(const void *logits, int64_t ld, int dtype, const void *targets, int target_bytes,
+                                   int T, int V, int top_k, float temperature, float *logprobs, float *entropy,
+                                   float *top_logprobs, int32_t *top_tokens, float *lse, void *stream);
+/*
+ * Gradient of the logits from those of the log probabilities and, when given, of the
+ * entropies (which then are needed too): with p the probabilities,
+ *   dlogits = (g ([v = target] - p) - h p (log p + entropy)) / temperature
+ * in the logits' type, rows ldd apart; masked columns and columns V to W - 1 are zero.  The
+ * alternatives carry no gradient.  dlogits may be the logits themselves (same rows).
+ */
+NVFP4_API int nvfp4_token_logprobs_backward(const float *dlogprobs, const float *dentropy, const void *logits,
+                                            int64_t ld, int dtype, const void *targets, int target_bytes,
+                                            const float *lse, const float *entropy, int T, int V, int W,
+                                            float temperature, void *dlogits, int64_t ldd, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
