@@ -18,6 +18,7 @@
 #include <climits>
 
 #include "common.cuh"
+#include "moe.cuh"
 #include "ptx.cuh"
 #include "types16.cuh"
 
@@ -54,6 +55,8 @@ struct RouteParams {
     int T, E, k, chunk, chunks;
     int sigmoid, renormalize;
     float scale;
+    int *clear;  // n_clear integers to set to zero
+    int n_clear;
 };
 
 template <typename T>
@@ -284,6 +287,8 @@ __global__ void __launch_bounds__(kRouteThreads, 3) moe_route_kernel(const Route
     const int words = p.chunk / 32;
     const int t0 = blockIdx.x * p.chunk, n = max(0, min(p.chunk, p.T - t0));
     for (int i = threadIdx.x; i < p.E * words; i += kRouteThreads) bits[i] = 0u;
+    if (blockIdx.x == 0)
+        for (int i = threadIdx.x; i < p.n_clear; i += kRouteThreads) p.clear[i] = 0;
     __syncthreads();
     float bias[NI];
 #pragma unroll
@@ -738,18 +743,9 @@ static int move_sizes(int T, int k, int K) {
 
 using namespace nvfp4;
 
-extern "C" {
-
-size_t nvfp4_moe_route_workspace_size(int T, int E) {
-    if (T < 0 || T > moe::kMaxTokens || E < 1 || E > moe::kMaxExperts) return 0;
-    const int c = moe::chunk_tokens(T), chunks = std::max(1, (T + c - 1) / c);
-    const int clusters = (chunks + moe::kClusterChunks - 1) / moe::kClusterChunks;
-    return (size_t)clusters * (moe::kClusterChunks + 1) * E * sizeof(int);
-}
-
-int nvfp4_moe_route(const void *logits, int dtype, const float *bias, int T, int E, int top_k, int scoring,
-                    int renormalize, float scale, float *weights, int32_t *experts, int32_t *rows, int32_t *m_offsets,
-                    void *workspace, size_t workspace_bytes, void *stream) {
+int moe::route_tokens(const void *logits, int dtype, const float *bias, int T, int E, int top_k, int scoring,
+                      int renormalize, float scale, float *weights, int *experts, int *rows, int *m_offsets,
+                      void *workspace, size_t workspace_bytes, int *clear, int n_clear, void *stream) {
     if (dtype < NVFP4_BF16 || dtype > NVFP4_F32 || scoring < NVFP4_SCORE_SOFTMAX || scoring > NVFP4_SCORE_SIGMOID)
         return NVFP4_ERR_INVALID;
     if (T < 0 || T > moe::kMaxTokens || E < 1 || E > moe::kMaxExperts || top_k < 1 || top_k > moe::kMaxTopK ||
@@ -783,10 +779,28 @@ int nvfp4_moe_route(const void *logits, int dtype, const float *bias, int T, int
     p.sigmoid = scoring == NVFP4_SCORE_SIGMOID;
     p.renormalize = renormalize != 0;
     p.scale = scale;
+    p.clear = clear;
+    p.n_clear = n_clear;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (dtype == NVFP4_BF16) return moe::route<__nv_bfloat16>(p, s);
     if (dtype == NVFP4_F16) return moe::route<__half>(p, s);
     return moe::route<float>(p, s);
+}
+
+extern "C" {
+
+size_t nvfp4_moe_route_workspace_size(int T, int E) {
+    if (T < 0 || T > moe::kMaxTokens || E < 1 || E > moe::kMaxExperts) return 0;
+    const int c = moe::chunk_tokens(T), chunks = std::max(1, (T + c - 1) / c);
+    const int clusters = (chunks + moe::kClusterChunks - 1) / moe::kClusterChunks;
+    return (size_t)clusters * (moe::kClusterChunks + 1) * E * sizeof(int);
+}
+
+int nvfp4_moe_route(const void *logits, int dtype, const float *bias, int T, int E, int top_k, int scoring,
+                    int renormalize, float scale, float *weights, int32_t *experts, int32_t *rows, int32_t *m_offsets,
+                    void *workspace, size_t workspace_bytes, void *stream) {
+    return moe::route_tokens(logits, dtype, bias, T, E, top_k, scoring, renormalize, scale, weights, experts, rows,
+                             m_offsets, workspace, workspace_bytes, nullptr, 0, stream);
 }
 
 int nvfp4_moe_route_backward(const float *dweights, const void *logits, int dtype, const int32_t *experts, int T,

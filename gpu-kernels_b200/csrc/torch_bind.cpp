@@ -34,6 +34,8 @@ struct Entries {
     decltype(&nvfp4_moe_dispatch) dispatch;
     decltype(&nvfp4_moe_combine) combine;
     decltype(&nvfp4_moe_combine_backward) combine_backward;
+    decltype(&nvfp4_moe_layer) moe_layer;
+    decltype(&nvfp4_moe_layer_workspace_size) moe_layer_ws;
     decltype(&nvfp4_embedding) embedding;
     decltype(&nvfp4_embedding_backward_workspace_size) embedding_backward_ws;
     decltype(&nvfp4_embedding_backward) embedding_backward;
@@ -452,6 +454,42 @@ PyObject *moe_combine_backward(PyObject *const *a) {
     return tuple_of<2>({wrap(std::move(dx)), wrap(std::move(dw))});
 }
 
+// moe_layer(x, logits, w13, w2, top_k, scoring, bias, renormalize, scale, residual)
+PyObject *moe_layer(PyObject *const *a) {
+    const at::Tensor &x = tensor(a[0], "x"), &l = tensor(a[1], "logits");
+    const at::Tensor &w13 = tensor(a[2], "w13"), &w2 = tensor(a[3], "w2");
+    const int k = small(integer(a[4]), "top_k"), scoring = (int)integer(a[5]);
+    const at::Tensor *bias = maybe(a[6], "bias"), *res = maybe(a[9], "residual");
+    const bool renormalize = truth(a[7]);
+    const float scale = (float)number(a[8]);
+    const Rows r = rows_of(x, "x");
+    const Logits g = logits_of(l);
+    if (l.device() != x.device() || g.T != r.M) refuse("logits must have a row for each of x's, on its device");
+    if (bias) {
+        if (scoring != NVFP4_SCORE_SIGMOID) refuse("a selection bias needs sigmoid scoring");
+        expect(*bias, "bias", {g.E}, at::kFloat, l);
+    }
+    const auto type = x.scalar_type();
+    if (g.E < 1 || w2.dim() != 2 || w2.size(0) != (int64_t)g.E * r.K) refuse("w2 must be [E * " + std::to_string(r.K) + ", F]");
+    const int F = small(w2.size(1), "the hidden size");
+    if (F % 16 || !F) refuse("the hidden size must be a multiple of 16");
+    expect(w2, "w2", {(int64_t)g.E * r.K, F}, type, x);
+    expect(w13, "w13", {(int64_t)g.E * 2 * F, r.K}, type, x);
+    if (res) expect(*res, "residual", {r.M, r.K}, type, x);
+    at::Tensor y;
+    check(unlocked([&] {
+              y = empty({r.M, r.K}, type, x);
+              const size_t need = L.moe_layer_ws(r.M, g.E, k, r.K, F);
+              at::Tensor ws = empty({(int64_t)need}, at::kByte, x);
+              const Stream s(x);
+              return L.moe_layer(x.data_ptr(), r.pitch, l.data_ptr(), g.dtype, static_cast<const float *>(ptr(bias)),
+                                 w13.data_ptr(), w2.data_ptr(), ptr(res), y.data_ptr(), r.M, g.E, k, r.K, F, scoring,
+                                 renormalize, scale, r.dtype, ws.data_ptr(), need, s.handle);
+          }),
+          "nvfp4_moe_layer");
+    return wrap(std::move(y));
+}
+
 // Token ids, or targets: a contiguous int32 or int64 CUDA tensor.
 int token_bytes(const at::Tensor &t, const char *name) {
     const auto type = t.scalar_type();
@@ -648,7 +686,7 @@ PyObject *entry(PyObject *, PyObject *const *args, Py_ssize_t n) {
 PyMethodDef methods[] = {METHOD(bind, 1 + kEntries), METHOD(linear, 8),          METHOD(linear_backward, 9),
                          METHOD(moe_route, 6),       METHOD(moe_route_backward, 6), METHOD(moe_dispatch, 2),
                          METHOD(moe_combine, 4),     METHOD(moe_combine_backward, 3),
-                         METHOD(embedding, 3),       METHOD(embedding_backward, 4),
+                         METHOD(moe_layer, 10),      METHOD(embedding, 3),       METHOD(embedding_backward, 4),
                          METHOD(token_logprobs, 6),  METHOD(token_logprobs_backward, 9), {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_bind", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -12,8 +12,8 @@ from .ops import (create_tensors, device_status, gemm, gemm_epilogue, gemm_group
                   gemm_grouped_epilogue, gemm_host, global_scale, launch_count, matmul_nvfp4, quantize,
                   quantize_dynamic, quantize_grouped, selftest_wait_timeout, set_wait_timeout_ns)
 from .layers import linear, linear_backward, linear_grouped, linear_grouped_backward  # noqa: F401
-from .moe import (Routing, moe_combine, moe_combine_backward, moe_dispatch, moe_dispatch_backward, moe_route,  # noqa: F401
-                  moe_route_backward)
+from .moe import (Routing, moe_combine, moe_combine_backward, moe_dispatch, moe_dispatch_backward, moe_layer,  # noqa: F401
+                  moe_route, moe_route_backward)
 from .vocab import (TokenLogprobs, embedding, embedding_backward, token_logprobs,  # noqa: F401
                     token_logprobs_backward)
 from . import runner_io  # noqa: F401,E402

@@ -15,7 +15,8 @@ PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_torch_bind.so"
 _ENTRIES = ("nvfp4_linear", "nvfp4_linear_dgrad", "nvfp4_linear_wgrad", "nvfp4_activation_backward",
             "nvfp4_activation_backward_workspace_size", "nvfp4_moe_route", "nvfp4_moe_route_workspace_size",
             "nvfp4_moe_route_backward", "nvfp4_moe_dispatch", "nvfp4_moe_combine", "nvfp4_moe_combine_backward",
-            "nvfp4_embedding", "nvfp4_embedding_backward_workspace_size", "nvfp4_embedding_backward",
+            "nvfp4_moe_layer", "nvfp4_moe_layer_workspace_size", "nvfp4_embedding",
+            "nvfp4_embedding_backward_workspace_size", "nvfp4_embedding_backward",
             "nvfp4_token_logprobs", "nvfp4_token_logprobs_backward")
 
 

@@ -73,6 +73,9 @@ SIGNATURES = {
     "nvfp4_moe_combine": (C.c_int, [_vp, C.c_int, _vp, _vp, _vp, C.c_int, C.c_int, C.c_int, _vp, _vp]),
     "nvfp4_moe_combine_backward": (C.c_int, [_vp, _vp, C.c_int, _vp, _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_int,
                                              _vp, _vp, _vp]),
+    "nvfp4_moe_layer_workspace_size": (C.c_size_t, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int]),
+    "nvfp4_moe_layer": (C.c_int, [_vp, C.c_int64, _vp, C.c_int, _vp, _vp, _vp, _vp, _vp, C.c_int, C.c_int, C.c_int,
+                                  C.c_int, C.c_int, C.c_int, C.c_int, C.c_float, C.c_int, _vp, C.c_size_t, _vp]),
     "nvfp4_embedding": (C.c_int, [_vp, C.c_int, _vp, C.c_int64, C.c_float, _vp, C.c_int, C.c_int, C.c_int, C.c_int,
                                   _vp]),
     "nvfp4_embedding_backward_workspace_size": (C.c_size_t, [C.c_int, C.c_int, C.c_int]),

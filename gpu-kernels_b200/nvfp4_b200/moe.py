@@ -15,7 +15,9 @@ from typing import NamedTuple, Optional
 import torch
 
 from ._bind import native
-from ._lib import SCORES
+from ._lib import ACTIVATIONS, SCORES
+
+FEW_TOKENS = 32  # tokens up to which moe_layer is the fused kernel
 
 
 class Routing(NamedTuple):
@@ -71,3 +73,24 @@ def moe_combine_backward(dy: torch.Tensor, x_rows: torch.Tensor, routing: Routin
     """Gradients (dx_rows [T * top_k, K], dweights fp32 [T, top_k]) of moe_combine; the
     residual's gradient is dy itself."""
     return native.moe_combine_backward(dy, x_rows, routing)
+
+
+def moe_layer(x: torch.Tensor, logits: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, top_k: int,
+              scoring: str = "softmax", bias: Optional[torch.Tensor] = None, renormalize: bool = True,
+              scale: float = 1.0, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """A whole mixture-of-experts layer [T, K] from x [T, K] and its router's logits [T, E]:
+
+        y[t] = residual[t] + sum_j weight[t, j] * W2_e silu_mul(W13_e x[t]),  e = expert[t, j]
+
+    with moe_route's choice (the same arguments) and SwiGLU experts: w13 [E * 2F, K], gate and
+    up rows interleaved in blocks of 16 (swiglu_interleave by expert), w2 [E * K, F]; F a
+    multiple of 16.  Up to FEW_TOKENS tokens, a decode step, are two kernels that read the
+    chosen experts' weights once, and the experts' results are summed in fp32.  More go through
+    moe_route, moe_dispatch, linear_grouped and moe_combine, which round each expert's result.
+    For inference: the differentiable form is those four operators."""
+    if isinstance(x, torch.Tensor) and x.dim() == 2 and x.shape[0] > FEW_TOKENS:
+        r = moe_route(logits, top_k, scoring, bias, renormalize, scale)
+        rows = moe_dispatch(x.contiguous(), r)
+        h = native.linear(rows, w13, r.m_offsets, None, ACTIVATIONS["swiglu"], None, None, False)
+        return moe_combine(native.linear(h, w2, r.m_offsets, None, 0, None, None, False), r, residual)
+    return native.moe_layer(x, logits, w13, w2, top_k, _scoring(scoring), bias, renormalize, scale, residual)

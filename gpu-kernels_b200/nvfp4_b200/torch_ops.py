@@ -16,6 +16,7 @@ from ._bind import native
 from .layers import _activation
 from .layout import sf_bytes
 from .moe import _scoring
+from .moe import moe_layer as _moe_layer
 from .ops import gemm as _gemm
 from .ops import gemm_epilogue as _gemm_epilogue
 from .ops import quantize as _quantize
@@ -275,6 +276,20 @@ def _combine_grad(ctx, dy):
 
 
 moe_combine.register_autograd(_combine_grad, setup_context=_combine_context)
+
+
+@torch.library.custom_op("nvfp4_b200::moe_layer", mutates_args=(), device_types="cuda")
+def moe_layer(x: torch.Tensor, logits: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, top_k: int,
+              scoring: str = "softmax", bias: Optional[torch.Tensor] = None, renormalize: bool = True,
+              scale: float = 1.0, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The whole layer from its router's logits; no gradient."""
+    return _moe_layer(x, logits, w13, w2, top_k, scoring, bias, renormalize, scale, residual)
+
+
+@moe_layer.register_fake
+def _moe_layer_fake(x, logits, w13, w2, top_k, scoring="softmax", bias=None, renormalize=True, scale=1.0,
+                    residual=None):
+    return x.new_empty(x.shape)
 
 
 # ----------------------------------------------------------------------- vocabulary

@@ -1,0 +1,227 @@
+"""GPU: the whole mixture-of-experts layer of a few tokens against a plain 64-bit form, and as
+a part of a decode step."""
+import math
+
+import pytest
+import torch
+
+import ref16 as R
+
+pytestmark = pytest.mark.gpu
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def layer(T, E, K, F, dtype, seed, residual=True, logits=torch.float32):
+    g = gen(seed)
+
+    def normal(*shape, scale=1.0):
+        return (torch.randn(*shape, device="cuda", generator=g) * scale).to(dtype)
+
+    return dict(x=normal(T, K), logits=(torch.randn(T, E, device="cuda", generator=g) * 2).to(logits),
+                w13=normal(E * 2 * F, K, scale=K ** -0.5), w2=normal(E * K, F, scale=F ** -0.5),
+                residual=normal(T, K) if residual else None)
+
+
+def layer64(x, logits, w13, w2, k, scoring, bias, renormalize, scale, residual, rounded_rows=False):
+    """(y, bound).  The hidden state is rounded to 16 bits; the weights are a few fp32 operations
+    (within 1e-5); the sum of k products is fp32.  rounded_rows: each expert's result is rounded
+    too, as for more than a few tokens."""
+    (T, K), E, F, u = x.shape, logits.shape[1], w2.shape[1], R.U[x.dtype]
+    weights, experts, _, _ = R.route64(logits, k, scoring, bias, renormalize, scale)
+    y = torch.zeros(T, K, dtype=torch.float64, device="cuda") if residual is None else residual.double()
+    b = 2.0 ** -23 * y.abs()
+    for e in range(E):
+        t, j = (experts == e).nonzero(as_tuple=True)
+        if not len(t):
+            continue
+        w = weights[t, j].cuda()[:, None]
+        X, A, B = x[t.cuda()].double(), w13[e * 2 * F:(e + 1) * 2 * F].double(), w2[e * K:(e + 1) * K].double()
+        z = X @ A.t()
+        ez = R.acc(K) * (X.abs() @ A.abs().t())
+        h, eh = R.act64(z, "swiglu"), R.act_bound(z, ez, "swiglu")
+        eh = eh + u * (h.abs() + eh) + R.TINY[x.dtype]
+        o = h @ B.t()
+        eo = R.acc(F) * ((h.abs() + eh) @ B.abs().t()) + eh @ B.abs().t()
+        if rounded_rows:
+            eo = eo + u * (o.abs() + eo) + R.TINY[x.dtype]
+        y.index_add_(0, t.cuda(), w * o)
+        b.index_add_(0, t.cuda(), w.abs() * (eo + (1e-5 + 2.0 ** -22) * o.abs()))
+    return y, b + 2.0 ** -22 * y.abs()
+
+
+def check(nv, d, k, scoring="softmax", bias=None, renormalize=True, scale=1.0):
+    y = nv.moe_layer(d["x"], d["logits"], d["w13"], d["w2"], k, scoring=scoring, bias=bias, renormalize=renormalize,
+                     scale=scale, residual=d["residual"])
+    torch.cuda.synchronize()
+    nv.device_status()
+    ref, bound = layer64(d["x"], d["logits"], d["w13"], d["w2"], k, scoring, bias, renormalize, scale, d["residual"],
+                         rounded_rows=d["x"].shape[0] > 32)
+    R.assert_close(y, ref, bound)
+    return y
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,E,k,K,F", [
+    (1, 1, 1, 8, 16), (1, 8, 2, 64, 48), (2, 3, 1, 24, 1040), (3, 4, 4, 72, 16), (8, 128, 8, 2048, 768),
+    (9, 5, 1, 2056, 2064), (13, 64, 6, 264, 80), (16, 256, 8, 1024, 64), (17, 2, 2, 1032, 1024),
+    (25, 6, 3, 4104, 32), (32, 40, 32, 40, 32), (32, 1, 1, 2048, 2048), (32, 8, 2, 512, 1408), (31, 2, 2, 2048, 768)])
+def test_moe_layer(nv, cuda_dev, T, E, k, K, F, dtype):
+    """One to four tiles of rows, every size of a group of warps, sizes that fill no chunk, more
+    warps than chunks, experts without a token."""
+    check(nv, layer(T, E, K, F, dtype, T + E, residual=T % 2 == 1, logits=dtype if T % 3 else torch.float32), k)
+
+
+@pytest.mark.parametrize("scoring,bias,renorm,scale", [("softmax", False, False, 1.0), ("sigmoid", False, True, 2.5),
+                                                       ("sigmoid", True, True, 1.0), ("sigmoid", True, False, 0.5)])
+def test_moe_layer_scores(nv, cuda_dev, scoring, bias, renorm, scale):
+    d = layer(11, 40, 256, 160, torch.bfloat16, 3)
+    b = torch.randn(40, device="cuda", generator=gen(1)) * 0.1 if bias else None
+    check(nv, d, 5, scoring, b, renorm, scale)
+
+
+@pytest.mark.parametrize("K,F", [(64, 32), (72, 48), (2048, 1024)])
+def test_moe_layer_masks(nv, cuda_dev, K, F):
+    """Masked experts (-inf, NaN, the lowest value), tokens with fewer experts left than they
+    choose, with none, and a batch of such tokens alone."""
+    d = layer(10, 6, K, F, torch.bfloat16, 5)
+    d["logits"][0] = -math.inf
+    d["logits"][1, 1:] = -math.inf
+    d["logits"][2, ::2] = math.nan
+    d["logits"][3] = torch.finfo(torch.float32).min
+    d["logits"][4, :5] = torch.finfo(torch.float32).min
+    d["logits"][9] = math.nan
+    clean = dict(d, logits=torch.where(d["logits"].isnan(), torch.full_like(d["logits"], -math.inf), d["logits"]))
+    y = check(nv, clean, 3)
+    assert torch.equal(y, nv.moe_layer(d["x"], d["logits"], d["w13"], d["w2"], 3, residual=d["residual"]))
+    assert torch.equal(y[0], d["residual"][0]) and torch.equal(y[9], d["residual"][9])
+    d["logits"][:] = -math.inf
+    assert torch.equal(check(nv, d, 3), d["residual"])
+    assert not check(nv, dict(d, residual=None), 2).any()
+
+
+def test_moe_layer_reads_chosen_experts_only(nv, cuda_dev):
+    """Weights of experts that no token chose, and rows beside the tokens', may hold anything."""
+    E, K, F = 8, 136, 48
+    d = layer(4, E, K, F, torch.float16, 2)
+    d["logits"][:, 4:] = -math.inf
+    want = check(nv, d, 2)
+    for w, rows in (("w13", 2 * F), ("w2", K)):
+        d[w].view(E, rows, -1)[4:] = math.nan
+    wide = torch.full((6, K + 24), math.inf, device="cuda", dtype=torch.float16)
+    wide[1:5, 8:8 + K] = d["x"]
+    d["x"] = wide[1:5, 8:8 + K]
+    got = nv.moe_layer(d["x"], d["logits"], d["w13"], d["w2"], 2, residual=d["residual"])
+    assert torch.equal(got, want)
+
+
+def test_moe_layer_one_expert_for_all(nv, cuda_dev):
+    """Every token to the same expert: the most rows an expert can have."""
+    for T in (8, 9, 16, 24, 25, 32):
+        d = layer(T, 5, 512, 96, torch.bfloat16, T)
+        d["logits"][:, 3] = 50.0
+        check(nv, d, 1)
+        check(nv, d, 2)
+
+
+def test_moe_layer_same_bits_and_agreement(nv, cuda_dev):
+    d = layer(16, 32, 1024, 512, torch.bfloat16, 1)
+    args = d["x"], d["logits"], d["w13"], d["w2"], 4
+    y = nv.moe_layer(*args, residual=d["residual"])
+    for _ in range(20):
+        assert torch.equal(y, nv.moe_layer(*args, residual=d["residual"]))
+    # the rows of a batch are those of each token alone, up to the sums' different order: none,
+    # since a unit's split depends on the weights' sizes alone
+    for t in (0, 7, 15):
+        one = nv.moe_layer(d["x"][t:t + 1], d["logits"][t:t + 1], d["w13"], d["w2"], 4, residual=d["residual"][t:t + 1])
+        assert torch.equal(one[0], y[t])
+
+
+@pytest.mark.parametrize("T", [0, 33, 64, 200])
+def test_moe_layer_more_tokens(nv, cuda_dev, T):
+    d = layer(T, 8, 256, 96, torch.bfloat16, 4)
+    if T == 0:
+        assert nv.moe_layer(d["x"], d["logits"], d["w13"], d["w2"], 2).shape == (0, 256)
+        return
+    check(nv, d, 2)
+    check(nv, dict(d, residual=None), 3, "sigmoid")
+
+
+def test_moe_layer_streams_and_graphs(nv, cuda_dev):
+    """Calls on two streams at once, and two captured graphs whose replays overlap."""
+    a, b = layer(8, 16, 1024, 512, torch.bfloat16, 1), layer(5, 16, 1024, 512, torch.bfloat16, 2)
+
+    def call(d):
+        return nv.moe_layer(d["x"], d["logits"], d["w13"], d["w2"], 4, residual=d["residual"])
+
+    want = [call(a).clone(), call(b).clone()]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        got = []
+        for s, d in zip(streams, (a, b)):
+            with torch.cuda.stream(s):
+                got.append(call(d))
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(want, got))
+    graphs, out = [], []
+    for d in (a, b):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out.append(call(d))
+        graphs.append(g)
+    for _ in range(20):
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(want, out))
+    a["logits"].copy_(b["logits"].flip(0).repeat(2, 1)[:8])  # replays follow inputs changed in place
+    graphs[0].replay()
+    assert torch.equal(out[0], call(a))
+    nv.device_status()
+
+
+def test_moe_layer_refusals(nv, cuda_dev):
+    d = layer(4, 8, 64, 32, torch.bfloat16, 1)
+    x, l, w13, w2 = d["x"], d["logits"], d["w13"], d["w2"]
+    for call in (lambda: nv.moe_layer(x.float(), l, w13, w2, 2), lambda: nv.moe_layer(x.cpu(), l, w13, w2, 2),
+                 lambda: nv.moe_layer(x[:, :60], l, w13, w2, 2), lambda: nv.moe_layer(x, l[:3], w13, w2, 2),
+                 lambda: nv.moe_layer(x, l, w13[:-1], w2, 2), lambda: nv.moe_layer(x, l, w13, w2[:-1], 2),
+                 lambda: nv.moe_layer(x, l, w13.half(), w2, 2), lambda: nv.moe_layer(x, l, w13, w2[:, :24], 2),
+                 lambda: nv.moe_layer(x, l, w13, w2, 2, scoring="none"),
+                 lambda: nv.moe_layer(x, l, w13, w2, 2, bias=torch.zeros(8, device="cuda")),
+                 lambda: nv.moe_layer(x, l, w13, w2, 2, residual=x[:2]),
+                 lambda: nv.moe_layer(x, l.double(), w13, w2, 2)):
+        with pytest.raises(ValueError):
+            call()
+    for k in (0, 9):
+        with pytest.raises(nv.NVFP4Error):
+            nv.moe_layer(x, l, w13, w2, k)
+
+
+def test_decode_step(nv, cuda_dev):
+    """The operators together, as a decode step and its scoring use them: embedding, router,
+    experts, output projection by the same table, log probabilities."""
+    rows, K, F, E = 1000, 256, 128, 16
+    g = gen(7)
+    table = (torch.randn(rows, K, device="cuda", generator=g) * K ** -0.5).bfloat16()
+    router = (torch.randn(E, K, device="cuda", generator=g)).bfloat16()
+    d = layer(6, E, K, F, torch.bfloat16, 8)
+    tokens = torch.tensor([3, 999, -1, 0, 3, 500], device="cuda")
+    x = nv.embedding(tokens, table, K ** 0.5)
+    d["x"] = d["residual"] = x
+    d["logits"] = nv.linear(x, router)
+    y = check(nv, d, 2)
+    assert not y[2].any()  # a padding token: no row, no contribution of any expert
+    logits = nv.linear(y, table)
+    r = nv.token_logprobs(logits, tokens, top_k=3, entropy=True)
+    want = torch.log_softmax(y.double() @ table.double().t(), 1)
+    live = tokens >= 0
+    # the logits are rounded to 16 bits: each by 2^-9 of itself, and so is their log sum exp
+    limit = 2 * (2.0 ** -9 + 2.0 ** -14) * logits.abs().amax(1).double() + 1e-4
+    assert ((r.logprobs.double() - want[torch.arange(6), tokens.clamp_min(0)]).abs() <= limit)[live].all()
+    op = torch.ops.nvfp4_b200.moe_layer(x, d["logits"], d["w13"], d["w2"], 2, "softmax", None, True, 1.0, x)
+    assert torch.equal(op, y)
