@@ -9,19 +9,31 @@
 //
 // The work is a list of units of 16 weight rows: first all of W13 (8 gate rows with their 8 up
 // rows, so SwiGLU stays in a thread), then all of W2, each by active expert; experts without a
-// token are not in it.  Groups of warps take the units in turn, the warps of a group share a
-// unit's reduction and add their parts up in shared memory in order.  Where W2's units begin a
-// group waits for its expert's hidden rows alone (a counter an expert), not for the grid.  The
-// rows' results are left in fp32, and the warp that brings a block of 16 columns its last
-// part forms the weighted sum there, in the order of the choices: the same bits every time.
+// token are not in it.  CTAs take the units in turn.  A W2 unit waits for its expert's hidden
+// rows alone (a counter an expert), not for the grid.  The rows' results are left in fp32, and
+// the warp that brings a block of 16 columns its last part forms the weighted sum there, in
+// the order of the choices: the same bits every time.
 //
-// Weights go through a ring of shared memory that belongs to each thread alone: it copies its
-// own 16-byte pieces asynchronously and reads them back itself, so the stream needs no
-// barrier, and it runs on across units and into W2 while its hidden rows are still being made.
-// A piece is 8 elements of a row; lanes 4g .. 4g + 3 hold row g, which is mma.m16n8k16's A
-// fragment with the reduction's elements permuted, and the tokens are read with the same
-// permutation, so nothing is shuffled.  The products are tiny (8 token columns a tile); the
-// tensor core only has to keep up with memory.
+// Warps: 0-7 multiply, 8 copies weights, 9-10 copy the tokens' (hidden) rows, a tile of 8 each,
+// 11-14 add the parts up and hand them on, a unit each in turn: the stores, the fence and the
+// counter of one unit take 2 us, longer than the weights of a short one.  A stage of the ring is 512 elements of 16 weight
+// rows, one tensor copy, and of the expert's rows, one bulk copy each; the weights run on into
+// W2 while its hidden rows are still being made.  The multiplying warps take the stages in
+// turn, a warp a stage, so that its latencies run under the others' stages.  For each chunk of
+// 32 elements lanes 4g .. 4g + 3 read 64 bytes of row g, which is mma.m16n8k16's A fragment
+// with the chunk's elements permuted, and the tokens are read with the same permutation, so
+// nothing is shuffled.  The products are tiny (8 token columns a tile); the tensor core only
+// has to keep up with memory.  There are as many multiplying warps as stages, so that a warp
+// always has the same stage of the ring: what it waits for is the phase after its last one,
+// and a barrier tells no two phases apart that are further from each other.
+//
+// The weights are seen as [block of 64 elements][row][64] so that a box is eight whole swizzled
+// tiles of 8 rows by 128 bytes for each half of the rows.  Elements past the last whole block
+// are a stage of their own, from a second view that knows the row's end.
+//
+// Measured on the way, E = 8 of 4096 x 14336, one token: pieces of 16 bytes by cp.async 3.6
+// TB/s whatever the depth; a bulk copy for each of the 16 rows 2.8 (82 cycles to issue one);
+// every warp a part of each stage 4.4.
 #include <algorithm>
 #include <climits>
 
@@ -34,14 +46,21 @@
 namespace nvfp4 {
 namespace moe_layer {
 
-constexpr int kThreads = 512;
-constexpr int kWarps = kThreads / 32;
-constexpr int kMaxTokens = 32;             // rows of an expert, so at most four tiles of 8 columns
+constexpr int kWarps = 8;                  // that multiply, at most: one a stage
+constexpr int kMaxTiles = 2;               // of 8 token columns: a warp each copies them
+constexpr int kMaxSets = 4;                // of parts: a warp each adds them up
+constexpr int kWeightWarp = kWarps, kTokenWarp = kWarps + 1, kEpiWarp = kTokenWarp + kMaxTiles;
+constexpr int kThreads = 32 * (kEpiWarp + kMaxSets);
+constexpr int kMaxTokens = 8 * kMaxTiles;  // and so the rows of an expert
 constexpr int kMaxExperts = 256;
 constexpr int kMaxTopK = 32;
-constexpr int kSlots = 6;                  // ring: 16 KB each
-constexpr int kSlotBytes = kThreads * 32;
-constexpr int kMaxTiles = kMaxTokens / 8;
+constexpr int kMaxSize = 1 << 20;          // of K and F
+constexpr int kSegment = 512;              // elements of a row in a stage
+constexpr int kBlocks = kSegment / 64;
+constexpr int kBlockBytes = 16 * 128;      // 64 elements of 16 rows
+constexpr int kPitch = kSegment * 2 + 64;  // bytes between token rows: eight lanes read different banks
+constexpr int kMaxStages = kWarps;
+constexpr int kSmem = 220 * 1024;          // ring and parts; the tables are static
 
 struct Params {
     const void *x, *w13, *w2, *residual;
@@ -50,26 +69,25 @@ struct Params {
     const float *weights;      // [T, k]
     const int *rows;           // [T, k]
     const int *m_offsets;      // [E + 1]
-    int *up_done;              // [E] finished tiles of an expert's hidden rows
-    int *col_done;             // [column blocks] finished tiles
+    int *up_done;              // [E] finished units of an expert's hidden rows
+    int *col_done;             // [column blocks] finished units
     void *h;                   // [T k, hp]
     float *part;               // [T k, K]
     int T, E, k, K, F, hp;
-    int group;                 // warps of a group
+    int stages, stage_bytes;   // of the ring
+    int sets;                  // of parts
     KernelCtl ctl;
 };
 
-__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool live) {
-    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0)
-                 : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-__device__ __forceinline__ void group_barrier(int id, int threads) {
-    asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+// Orders this thread's accesses to global memory with those of bulk copies.
+__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async;" ::: "memory"); }
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *tmap, uint32_t bar, int32_t x, int32_t y,
+                                            int32_t z, int32_t w) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+        : "memory");
 }
 __device__ __forceinline__ int load_acquire(const int *p) {
     int v;
@@ -93,22 +111,39 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 1) moe_layer_kernel(const Params p) {
-    extern __shared__ uint8_t smem[];
+__global__ void __launch_bounds__(kThreads, 1)
+    moe_layer_kernel(const __grid_constant__ CUtensorMap map13, const __grid_constant__ CUtensorMap tail13,
+                     const __grid_constant__ CUtensorMap map2, const __grid_constant__ CUtensorMap tail2, const Params p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = smem_raw + ((0u - smem_u32(smem_raw)) & 1023u);
     __shared__ int act_e[kMaxExperts], act_row[kMaxExperts], act_n[kMaxExperts];
     __shared__ uint16_t row_token[kMaxTokens * kMaxTopK];
-    __shared__ int n_active, n_tiles, ready[kWarps];
+    __shared__ int n_active;
+    __shared__ uint64_t bars[3 * kMaxStages + 2 * kMaxSets];
     __shared__ int abort_word;
     volatile int *abort_flag = &abort_word;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, q = lane & 3;  // fragment row / column, and quarter of 32 elements
-    const int in_group = warp % p.group, group = warp / p.group, groups = kWarps / p.group;
-    const int bar = 1 + group, bar_threads = p.group * 32;
+    const uint32_t bar_weights = smem_u32(bars), bar_tokens = bar_weights + 8 * kMaxStages;
+    const uint32_t bar_empty = bar_tokens + 8 * kMaxStages;
+    const uint32_t bar_part = bar_empty + 8 * kMaxStages, bar_taken = bar_part + 8 * kMaxSets;
 
     // ---- active experts and the rows' tokens
-    if (threadIdx.x == 0) abort_word = 0;
+    if (threadIdx.x == 0) {
+        abort_word = 0;
+        for (int i = 0; i < p.stages; i++) {
+            mbar_init(bar_weights + 8 * i, 1);
+            mbar_init(bar_tokens + 8 * i, kMaxTiles);
+            mbar_init(bar_empty + 8 * i, 1);
+        }
+        for (int i = 0; i < p.sets; i++) {
+            mbar_init(bar_part + 8 * i, p.stages);
+            mbar_init(bar_taken + 8 * i, 1);
+        }
+        fence_barrier_init();
+    }
     if (warp == 0) {
-        int n = 0, tiles = 0;
+        int n = 0;
         for (int e0 = 0; e0 < p.E; e0 += 32) {
             const int e = e0 + lane;
             int r0 = 0, r1 = 0;
@@ -124,12 +159,8 @@ __global__ void __launch_bounds__(kThreads, 1) moe_layer_kernel(const Params p) 
                 act_n[at] = r1 - r0;
             }
             n += __popc(live);
-            tiles += __reduce_add_sync(0xffffffffu, (r1 - r0 + 7) / 8);
         }
-        if (lane == 0) {
-            n_active = n;
-            n_tiles = tiles;
-        }
+        if (lane == 0) n_active = n;
     } else {
         for (int i = threadIdx.x - 32; i < p.T * p.k; i += kThreads - 32) {
             const int r = p.rows[i];
@@ -142,7 +173,33 @@ __global__ void __launch_bounds__(kThreads, 1) moe_layer_kernel(const Params p) 
     T *h = static_cast<T *>(p.h);
     const int units_up = p.F / 8, units_down = (p.K + 15) / 16;
     const int total_up = n_active * units_up, total = total_up + n_active * units_down;
-    const int first = group * (int)gridDim.x + (int)blockIdx.x, stride = groups * (int)gridDim.x;
+    const int first = (int)blockIdx.x, stride = (int)gridDim.x;
+    const uint64_t tmo = p.ctl.wait_timeout_ns;
+    const int tiles_cap = (p.T + 7) / 8;
+    const uint32_t stage_bytes = p.stage_bytes, ring = smem_u32(smem);
+    float4 *sums = reinterpret_cast<float4 *>(smem + p.stages * stage_bytes);  // [set][warp][tile][lane]
+    auto stages_of = [](int red) { return ((red & ~63) + kSegment - 1) / kSegment + ((red & 63) != 0); };
+    // elements of the stage that begins at k0 of a reduction: whole blocks of 64, then the rest
+    auto stage_elements = [](int k0, int red) {
+        const int whole = red & ~63;
+        return k0 < whole ? min(kSegment, whole - k0) : red - k0;
+    };
+
+    struct Unit {
+        bool up;
+        int a, idx, n, row0, red;  // active expert, unit of it, its rows, the reduction
+    };
+    auto unit_at = [&](int u) {
+        Unit r;
+        r.up = u < total_up;
+        const int per = r.up ? units_up : units_down, v = r.up ? u : u - total_up;
+        r.a = v / per;
+        r.idx = v - r.a * per;
+        r.n = act_n[r.a];
+        r.row0 = act_row[r.a];
+        r.red = r.up ? p.K : p.F;
+        return r;
+    };
 
     // y of 16 columns once all their parts are there (or none is to come)
     auto combine = [&](int col0) {
@@ -175,164 +232,229 @@ __global__ void __launch_bounds__(kThreads, 1) moe_layer_kernel(const Params p) 
         }
     };
     if (total == 0) {  // no token has an expert
-        for (int b = (int)blockIdx.x * kWarps + warp; b < units_down; b += (int)gridDim.x * kWarps) combine(b * 16);
+        constexpr int kAll = kThreads / 32;
+        for (int b = (int)blockIdx.x * kAll + warp; b < units_down; b += (int)gridDim.x * kAll) combine(b * 16);
         return;
     }
 
-    // ---- the stream of weights: this thread's pieces of rows g and g + 8 of each unit
-    const uint32_t ring = smem_u32(smem) + threadIdx.x * 16;
-    int iu = first, ic = in_group, i_chunks = 0, i_red = 0, i_slot = 0;
-    const T *pa = nullptr, *pb = nullptr;  // null: past the weight's rows
-    auto open = [&]() {
-        if (iu < total_up) {
-            const int a = iu / units_up, f = iu - a * units_up;
-            i_red = p.K;
-            pa = static_cast<const T *>(p.w13) +
-                 ((int64_t)act_e[a] * 2 * p.F + (f >> 1) * 32 + (f & 1) * 8 + g) * p.K + q * 8;
-            pb = pa + (int64_t)16 * p.K;
-        } else if (iu < total) {
-            const int a = (iu - total_up) / units_down, row = (iu - total_up - a * units_down) * 16 + g;
-            i_red = p.F;
-            const T *w = static_cast<const T *>(p.w2) + ((int64_t)act_e[a] * p.K + row) * p.F + q * 8;
-            pa = row < p.K ? w : nullptr;
-            pb = row + 8 < p.K ? w + (int64_t)8 * p.F : nullptr;
+    if (warp >= kEpiWarp) {
+        // ---- the parts of the units in turn
+        const int set = warp - kEpiWarp;
+        if (set >= p.sets) return;
+        int phase = 0, from_warp = 0, turn = 0;
+        for (int u = first; u < total; u += stride, turn = turn + 1 == p.sets ? 0 : turn + 1) {
+            const Unit un = unit_at(u);
+            const int stages = stages_of(un.red), parts = min(stages, p.stages), from0 = from_warp;
+            from_warp = (from_warp + stages) % p.stages;
+            if (turn != set) continue;
+            if (!linear::warp_wait_parity(bar_part + 8 * set, phase, tmo, abort_flag, lane)) {
+                if (lane == 0) report_timeout(abort_flag, p.ctl.status);
+                break;
+            }
+            phase ^= 1;
+            float4 sum[kMaxTiles];
+#pragma unroll
+            for (int i = 0; i < kMaxTiles; i++) {
+                if (i * 8 >= un.n) break;
+                const float4 *from = sums + (set * kWarps * tiles_cap + i) * 32 + lane;
+                float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int w = 0; w < parts; w++) {  // in the order of the stages
+                    const float4 o = from[((from0 + w) % p.stages) * tiles_cap * 32];
+                    s.x += o.x;
+                    s.y += o.y;
+                    s.z += o.z;
+                    s.w += o.w;
+                }
+                sum[i] = s;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_taken + 8 * set);  // other parts may take their place
+#pragma unroll
+            for (int i = 0; i < kMaxTiles; i++) {
+                if (i * 8 >= un.n) break;
+                const float4 s = sum[i];
+                const int c = i * 8 + 2 * q;  // s.x, s.z: column c, rows g and g + 8; s.y, s.w: column c + 1
+                if (un.up) {
+                    T *to = h + (int64_t)(un.row0 + c) * p.hp + un.idx * 8 + g;
+                    if (c < un.n) to[0] = Type16<T>::round(s.x * linear::sigma(s.x) * s.z);
+                    if (c + 1 < un.n) to[p.hp] = Type16<T>::round(s.y * linear::sigma(s.y) * s.w);
+                } else {
+                    const int row = un.idx * 16 + g;
+                    float *to = p.part + (int64_t)(un.row0 + c) * p.K + row;
+                    if (c < un.n && row < p.K) to[0] = s.x;
+                    if (c < un.n && row + 8 < p.K) to[8] = s.z;
+                    if (c + 1 < un.n && row < p.K) to[p.K] = s.y;
+                    if (c + 1 < un.n && row + 8 < p.K) to[p.K + 8] = s.w;
+                }
+            }
+            __syncwarp();
+            int last = 0;
+            if (lane == 0) {
+                __threadfence();
+                if (un.up) atomicAdd(p.up_done + act_e[un.a], 1);
+                else last = atomicAdd(p.col_done + un.idx, 1) == n_active - 1;
+            }
+            if (__shfl_sync(0xffffffffu, last, 0)) {
+                __threadfence();
+                combine(un.idx * 16);
+            }
+            __syncwarp();
         }
-        i_chunks = (i_red + 31) / 32;
-    };
-    auto issue = [&]() {
-        while (iu < total && ic >= i_chunks) {  // a unit with fewer chunks than the group has warps may have none here
-            iu += stride;
-            ic = in_group;
-            open();
-        }
-        if (iu < total) {
-            const bool in = ic * 32 + q * 8 < i_red;
-            const uint32_t dst = ring + i_slot * kSlotBytes;
-            const bool live_a = in && pa, live_b = in && pb;
-            copy16(dst, live_a ? pa + ic * 32 : static_cast<const T *>(p.w13), live_a);
-            copy16(dst + kThreads * 16, live_b ? pb + ic * 32 : static_cast<const T *>(p.w13), live_b);
-            ic += p.group;
-        }
-        copy_commit();
-        i_slot = i_slot + 1 == kSlots ? 0 : i_slot + 1;
-    };
-    open();
-    for (int s = 0; s < kSlots; s++) issue();
+        return;
+    }
 
-    // ---- the units
-    float4 *sums = reinterpret_cast<float4 *>(smem + kSlots * kSlotBytes);  // [2][warp][tile][lane]
-    const int tiles_cap = (p.T + 7) / 8;
-    int slot = 0, parity = 0, have = -1, turn = 0;
-    for (int u = first; u < total; u += stride, parity ^= 1, turn++) {
-        const bool up = u < total_up;
-        const int per = up ? units_up : units_down, v = up ? u : u - total_up, a = v / per, idx = v - a * per;
-        const int n = act_n[a], row0 = act_row[a], tiles = (n + 7) / 8;
-        const int red = up ? p.K : p.F, chunks = (red + 31) / 32;
-        if (!up && have != a) {
-            // the expert's hidden rows, by all groups of the grid
-            if (in_group == 0 && lane == 0) {
-                const int want = units_up * tiles;
-                int ok = 1;
-                if (load_acquire(p.up_done + act_e[a]) < want) {
+    if (warp >= kWeightWarp) {
+        // ---- copies
+        const bool weights = warp == kWeightWarp;
+        const int tile = warp - kTokenWarp;
+        const uint32_t bar_full = weights ? bar_weights : bar_tokens;
+        int stage = 0, phase = 0, have = -1;
+        uint32_t issued = 0, issued_phase = 0;
+        bool ok = true;
+        for (int u = first; ok && u < total; u += stride) {
+            const Unit un = unit_at(u);
+            const int e = act_e[un.a], rows = weights ? 0 : min(8, un.n - tile * 8);  // a lane a token row
+            const T *from = nullptr;
+            if (!weights && !un.up && have != un.a) {
+                // the expert's hidden rows, by all CTAs of the grid
+                const int want = units_up;
+                int there = 1;
+                if (lane == 0 && load_acquire(p.up_done + e) < want) {
                     const uint64_t t0 = global_timer_ns();
-                    while (load_acquire(p.up_done + act_e[a]) < want) {
-                        if (*abort_flag || global_timer_ns() - t0 > p.ctl.wait_timeout_ns) {
+                    while (load_acquire(p.up_done + e) < want) {
+                        if (*abort_flag || global_timer_ns() - t0 > tmo) {
                             report_timeout(abort_flag, p.ctl.status);
-                            ok = 0;
+                            there = 0;
                             break;
                         }
                     }
                 }
-                ready[group] = ok;
+                ok = __shfl_sync(0xffffffffu, there, 0) != 0;
+                if (!ok) break;
+                have = un.a;
+                fence_proxy_async();
             }
-            group_barrier(bar, bar_threads);
-            const int ok = ready[group];
-            group_barrier(bar, bar_threads);
-            if (!ok) break;
-            have = a;
+            if (lane < rows) {
+                const int r = un.row0 + tile * 8 + lane;
+                from = un.up ? x + row_token[r] * p.ldx : h + (int64_t)r * p.hp;
+            }
+            const int row = un.up ? e * 2 * p.F + (un.idx >> 1) * 32 + (un.idx & 1) * 8 : e * p.K + un.idx * 16;
+            for (int k0 = 0, n; k0 < un.red; k0 += n) {
+                n = stage_elements(k0, un.red);
+                if (!linear::warp_wait_parity(bar_empty + 8 * stage, phase ^ 1, tmo, abort_flag, lane)) {
+                    if (lane == 0) report_timeout(abort_flag, p.ctl.status);
+                    ok = false;
+                    break;
+                }
+                const uint32_t bar = bar_full + 8 * stage, dst = ring + stage * stage_bytes;
+                issued |= 1u << stage;
+                issued_phase = (issued_phase & ~(1u << stage)) | ((uint32_t)phase << stage);
+                if (weights) {
+                    if (lane == 0) {
+                        if (k0 < (un.red & ~63)) {
+                            mbar_arrive_expect_tx(bar, kBlocks * kBlockBytes);  // blocks past the last are filled
+                            if (un.up) tma_load_4d(dst, &map13, bar, 0, row, 0, k0 / 64);
+                            else linear::tma_load_3d(dst, &map2, bar, 0, row, k0 / 64);
+                        } else {
+                            mbar_arrive_expect_tx(bar, kBlockBytes);
+                            if (un.up) linear::tma_load_3d(dst, &tail13, bar, k0, row, 0);
+                            else tma_load_2d(dst, &tail2, bar, k0, row);
+                        }
+                    }
+                } else if (rows > 0) {
+                    if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(rows * n) * 2);
+                    __syncwarp();
+                    if (lane < rows)
+                        bulk_load(dst + kBlocks * kBlockBytes + (tile * 8 + lane) * kPitch, from + k0, (uint32_t)n * 2, bar);
+                } else if (lane == 0) {
+                    mbar_arrive(bar);
+                }
+                __syncwarp();
+                if (++stage == p.stages) {
+                    stage = 0;
+                    phase ^= 1;
+                }
+            }
         }
+        if (!ok && lane == 0) {  // let the copies in flight land before the memory goes
+            volatile int never = 0;
+            for (int i = 0; i < p.stages; i++)
+                if (issued & (1u << i))
+                    wait_parity(bar_full + 8 * i, (issued_phase >> i) & 1, p.ctl.drain_timeout_ns, &never);
+        }
+        __syncwarp();
+        return;
+    }
+
+    // ---- the products: the stages in turn
+    if (warp >= p.stages) return;
+    int phase = 0, turn = 0, set = 0, set_phase = 0;  // turn: the warp of the unit's first stage
+    for (int u = first; u < total; u += stride) {
+        const Unit un = unit_at(u);
+        const int stages = stages_of(un.red), mine = (warp - turn + p.stages) % p.stages;
+        const bool low = un.up || un.idx * 16 + 8 < p.K;  // rows 8 .. 15 exist
         auto accumulate = [&](auto tiles_const) {
             constexpr int NT = decltype(tiles_const)::value;
-            float acc[NT][4];
-            const T *col[NT];
-#pragma unroll
-            for (int i = 0; i < NT; i++) {
-                acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
-                const int c = i * 8 + g;
-                col[i] = c >= n ? nullptr
-                                : (up ? x + row_token[row0 + c] * p.ldx : h + (int64_t)(row0 + c) * p.hp) + q * 8;
-            }
-            for (int c = in_group; c < chunks; c += p.group) {
-                const bool in = c * 32 + q * 8 < red;
-                uint4 b[NT];
-#pragma unroll
-                for (int i = 0; i < NT; i++)
-                    b[i] = in && col[i] ? *reinterpret_cast<const uint4 *>(col[i] + c * 32) : make_uint4(0u, 0u, 0u, 0u);
-                copy_wait<kSlots - 1>();
-                uint4 wa, wb;
-                const uint32_t src = ring + slot * kSlotBytes;
-                ld_shared_v4(src, wa.x, wa.y, wa.z, wa.w);
-                ld_shared_v4(src + kThreads * 16, wb.x, wb.y, wb.z, wb.w);
-#pragma unroll
-                for (int i = 0; i < NT; i++) {
-                    mma<T>(acc[i], wa.x, wb.x, wa.y, wb.y, b[i].x, b[i].y);
-                    mma<T>(acc[i], wa.z, wb.z, wa.w, wb.w, b[i].z, b[i].w);
-                }
-                issue();  // the pieces are in registers: their slot takes the next ones
-                slot = slot + 1 == kSlots ? 0 : slot + 1;
-            }
-            float4 *mine = sums + ((parity * kWarps + warp) * tiles_cap) * 32 + lane;
+            float acc[NT][2][4];
 #pragma unroll
             for (int i = 0; i < NT; i++)
-                if (i < tiles_cap) mine[i * 32] = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
-        };
-        if (tiles == 1) accumulate(std::integral_constant<int, 1>());
-        else if (tiles == 2) accumulate(std::integral_constant<int, 2>());
-        else accumulate(std::integral_constant<int, 4>());
-        group_barrier(bar, bar_threads);
-        // a warp a tile adds the parts up, another one for each unit; the sums' other half takes
-        // the next unit's parts meanwhile
-        for (int i = 0; i < tiles; i++) {
-            if ((turn + i) % p.group != in_group) continue;
-            const float4 *from = sums + ((parity * kWarps + group * p.group) * tiles_cap + i) * 32 + lane;
-            float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int w = 0; w < p.group; w++) {
-                const float4 o = from[w * tiles_cap * 32];
-                s.x += o.x;
-                s.y += o.y;
-                s.z += o.z;
-                s.w += o.w;
+#pragma unroll
+                for (int j = 0; j < 8; j++) acc[i][j >> 2][j & 3] = 0.0f;
+            for (int st = mine; st < stages; st += p.stages) {
+                const int k0 = st * kSegment < (un.red & ~63) ? st * kSegment : un.red & ~63;
+                const int n = stage_elements(k0, un.red);
+                if (!linear::warp_wait_parity(bar_weights + 8 * warp, phase, tmo, abort_flag, lane) ||
+                    !linear::warp_wait_parity(bar_tokens + 8 * warp, phase, tmo, abort_flag, lane))
+                    return false;
+                const uint32_t base = ring + warp * stage_bytes;
+                const uint32_t wat = base + g * 128, tat = base + kBlocks * kBlockBytes + g * kPitch + q * 16;
+                const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll 4
+                for (int c = 0; c * 32 < n; c++) {
+                    const bool in = c * 32 + q * 8 < n;  // past the end the tokens' rows hold anything
+                    const uint32_t at = wat + (c >> 1) * kBlockBytes + ((((c & 1) * 4 + q) ^ g) << 4);
+                    uint4 wa, wb, b[NT];
+                    ld_shared_v4(at, wa.x, wa.y, wa.z, wa.w);
+                    ld_shared_v4(at + 1024, wb.x, wb.y, wb.z, wb.w);
+#pragma unroll
+                    for (int i = 0; i < NT; i++)
+                        ld_shared_v4(tat + i * 8 * kPitch + c * 64, b[i].x, b[i].y, b[i].z, b[i].w);
+                    if (!low) wb = zero;
+#pragma unroll
+                    for (int i = 0; i < NT; i++) {
+                        if (!in || i * 8 + g >= un.n) b[i] = zero;
+                        mma<T>(acc[i][0], wa.x, wb.x, wa.y, wb.y, b[i].x, b[i].y);
+                        mma<T>(acc[i][1], wa.z, wb.z, wa.w, wb.w, b[i].z, b[i].w);
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar_empty + 8 * warp);
+                phase ^= 1;
             }
-            const int c = i * 8 + 2 * q;  // s.x, s.z: column c, rows g and g + 8; s.y, s.w: column c + 1
-            if (up) {
-                T *to = h + (int64_t)(row0 + c) * p.hp + idx * 8 + g;
-                if (c < n) to[0] = Type16<T>::round(s.x * linear::sigma(s.x) * s.z);
-                if (c + 1 < n) to[p.hp] = Type16<T>::round(s.y * linear::sigma(s.y) * s.w);
-                __syncwarp();
-                if (lane == 0) {
-                    __threadfence();
-                    atomicAdd(p.up_done + act_e[a], 1);
-                }
-            } else {
-                const int row = idx * 16 + g;
-                float *to = p.part + (int64_t)(row0 + c) * p.K + row;
-                if (c < n && row < p.K) to[0] = s.x;
-                if (c < n && row + 8 < p.K) to[8] = s.z;
-                if (c + 1 < n && row < p.K) to[p.K] = s.y;
-                if (c + 1 < n && row + 8 < p.K) to[p.K + 8] = s.w;
-                __syncwarp();
-                int last = 0;
-                if (lane == 0) {
-                    __threadfence();
-                    last = atomicAdd(p.col_done + idx, 1) == n_tiles - 1;
-                    __threadfence();
-                }
-                if (__shfl_sync(0xffffffffu, last, 0)) combine(idx * 16);
+            // the set's last parts have been taken
+            if (!linear::warp_wait_parity(bar_taken + 8 * set, set_phase ^ 1, tmo, abort_flag, lane)) return false;
+            if (mine < stages) {
+                float4 *to = sums + (set * kWarps + warp) * tiles_cap * 32 + lane;
+#pragma unroll
+                for (int i = 0; i < NT; i++)
+                    to[i * 32] = make_float4(acc[i][0][0] + acc[i][1][0], acc[i][0][1] + acc[i][1][1],
+                                             acc[i][0][2] + acc[i][1][2], acc[i][0][3] + acc[i][1][3]);
             }
             __syncwarp();
+            if (lane == 0) mbar_arrive(bar_part + 8 * set);
+            __syncwarp();
+            return true;
+        };
+        if (!(un.n > 8 ? accumulate(std::integral_constant<int, 2>()) : accumulate(std::integral_constant<int, 1>()))) {
+            if (lane == 0) report_timeout(abort_flag, p.ctl.status);
+            break;
+        }
+        turn = (turn + stages) % p.stages;
+        if (++set == p.sets) {
+            set = 0;
+            set_phase ^= 1;
         }
     }
-    copy_wait<0>();
 }
 
 // ------------------------------------------------------------------------- host side
@@ -362,22 +484,46 @@ static Layout layout(int T, int E, int k, int K, int F) {
     return l;
 }
 
-// Warps of a group: all of a CTA's where a reduction is long enough for each to have 4 chunks
-// of 32, so that the units are spread over the GPU most evenly.
-static int group_warps(int K, int F) {
-    const int chunks = std::min(K, F) / 32;
-    return chunks >= 64 ? 16 : chunks >= 32 ? 8 : 4;
+// The weight's views: boxes of 8 blocks of 64 elements by 16 rows (W13: 8 gate rows and the 8
+// up rows 16 further on), and of the elements past the last whole block.  Without such a part
+// its view is not used, and the other stands in for it.
+template <typename T>
+static int map_weights(CUtensorMap *map, CUtensorMap *tail, const void *w, int64_t rows, int red, bool pairs) {
+    const uint64_t row = (uint64_t)red * 2, whole = red / 64;
+    const uint64_t n = (uint64_t)rows - (pairs ? 16 : 0);
+    int st = NVFP4_OK;
+    if (pairs) {
+        const uint64_t dims[4] = {64, n, 2, whole}, strides[3] = {row, 16 * row, 128};
+        const uint32_t box[4] = {64, 8, 2, kBlocks};
+        const uint64_t tdims[3] = {(uint64_t)red, n, 2}, tstrides[2] = {row, 16 * row};
+        const uint32_t tbox[3] = {64, 8, 2};
+        if (whole) st = encode_tiled(map, linear::tma_type<T>(), 4, w, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+        if (!st && red % 64)
+            st = encode_tiled(tail, linear::tma_type<T>(), 3, w, tdims, tstrides, tbox, CU_TENSOR_MAP_SWIZZLE_128B);
+    } else {
+        const uint64_t dims[3] = {64, n, whole}, strides[2] = {row, 128};
+        const uint32_t box[3] = {64, 16, kBlocks};
+        const uint64_t tdims[2] = {(uint64_t)red, n}, tstrides[1] = {row};
+        const uint32_t tbox[2] = {64, 16};
+        if (whole) st = encode_tiled(map, linear::tma_type<T>(), 3, w, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+        if (!st && red % 64)
+            st = encode_tiled(tail, linear::tma_type<T>(), 2, w, tdims, tstrides, tbox, CU_TENSOR_MAP_SWIZZLE_128B);
+    }
+    if (!whole) *map = *tail;
+    if (red % 64 == 0) *tail = *map;
+    return st;
 }
 
 template <typename T>
 static int launch(const Params &p, const DeviceInfo &di, cudaStream_t s) {
     auto kern = moe_layer_kernel<T>;
-    const int tiles = (p.T + 7) / 8;
-    const int bytes = kSlots * kSlotBytes + 2 * kWarps * tiles * 512;
+    CUtensorMap map13, tail13, map2, tail2;
+    int st = map_weights<T>(&map13, &tail13, p.w13, (int64_t)p.E * 2 * p.F, p.K, true);
+    if (!st) st = map_weights<T>(&map2, &tail2, p.w2, (int64_t)p.E * p.K, p.F, false);
+    if (st) return st;
     static int configured[64] = {};
     if (!configured[di.device]) {
-        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 kSlots * kSlotBytes + 2 * kWarps * kMaxTiles * 512) != cudaSuccess)
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
             return NVFP4_ERR_CUDA;
         configured[di.device] = 1;
     }
@@ -387,19 +533,19 @@ static int launch(const Params &p, const DeviceInfo &di, cudaStream_t s) {
     attr.val.cooperative = 1;
     cfg.gridDim = dim3((unsigned)di.sm_count);
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = bytes;
+    cfg.dynamicSmemBytes = kSmem;
     cfg.stream = s;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    if (cudaLaunchKernelEx(&cfg, kern, p) != cudaSuccess) return NVFP4_ERR_CUDA;
+    if (cudaLaunchKernelEx(&cfg, kern, map13, tail13, map2, tail2, p) != cudaSuccess) return NVFP4_ERR_CUDA;
     count_launch();
     return cuda_status(cudaGetLastError());
 }
 
 static int check_sizes(int T, int E, int k, int K, int F) {
     if (T < 0 || T > kMaxTokens || E < 1 || E > kMaxExperts || k < 1 || k > kMaxTopK || k > E) return NVFP4_ERR_SHAPE;
-    if (K < 8 || K % 8 || F < 16 || F % 16 || K > (1 << 20) || F > (1 << 20)) return NVFP4_ERR_SHAPE;
-    return NVFP4_OK;
+    if (K < 8 || K % 8 || F < 16 || F % 16 || K > kMaxSize || F > kMaxSize) return NVFP4_ERR_SHAPE;
+    return (int64_t)E * 2 * F > INT_MAX || (int64_t)E * K > INT_MAX ? NVFP4_ERR_SHAPE : NVFP4_OK;
 }
 
 }  // namespace moe_layer
@@ -451,7 +597,11 @@ int nvfp4_moe_layer(const void *X, int64_t ldx, const void *logits, int logits_d
     p.K = K;
     p.F = F;
     p.hp = l.hp;
-    p.group = moe_layer::group_warps(K, F);
+    const int tiles = (T + 7) / 8;
+    p.stage_bytes = (moe_layer::kBlocks * moe_layer::kBlockBytes + 8 * tiles * moe_layer::kPitch + 1023) & ~1023;
+    p.sets = tiles == 1 ? moe_layer::kMaxSets : 3;
+    p.stages = std::min(moe_layer::kMaxStages,
+                        (moe_layer::kSmem - 1024 - p.sets * moe_layer::kWarps * tiles * 512) / p.stage_bytes);
     // the router's checks of its own arguments come before any launch
     st = moe::route_tokens(logits, logits_dtype, bias, T, E, top_k, scoring, renormalize, scale,
                            const_cast<float *>(p.weights), reinterpret_cast<int *>(ws + l.experts),
