@@ -14,11 +14,13 @@
 // the warp that brings a block of 16 columns its last part forms the weighted sum there, in
 // the order of the choices: the same bits every time.
 //
-// Warps: 0-7 multiply, 8 copies weights, 9-10 copy the tokens' (hidden) rows, a tile of 8 each,
-// 11-14 add the parts up and hand them on, a unit each in turn: the stores, the fence and the
-// counter of one unit take 2 us, longer than the weights of a short one.  A stage of the ring is 512 elements of 16 weight
-// rows, one tensor copy, and of the expert's rows, one bulk copy each; the weights run on into
-// W2 while its hidden rows are still being made.  The multiplying warps take the stages in
+// Warps: 0-7 multiply, 8 copies weights, 9-12 add the parts up and hand them on, a unit each in
+// turn: the stores, the fence and the counter of one unit take 2 us, longer than the weights of
+// a short one.  A stage of the ring is 512 elements of 16 weight rows, one tensor copy; the
+// weights run on into W2 while its hidden rows are still being made.  The multiplying warps
+// bring the tokens' (hidden) rows of a stage themselves, by cp.async while its weights are on
+// their way: copies by another warp, or behind the weights in the same queue, came later than
+// the weights (64 experts of 2048 x 2048, 8 tokens: 225 us).  They take the stages in
 // turn, a warp a stage, so that its latencies run under the others' stages.  For each chunk of
 // 32 elements lanes 4g .. 4g + 3 read 64 bytes of row g, which is mma.m16n8k16's A fragment
 // with the chunk's elements permuted, and the tokens are read with the same permutation, so
@@ -47,9 +49,9 @@ namespace nvfp4 {
 namespace moe_layer {
 
 constexpr int kWarps = 8;                  // that multiply, at most: one a stage
-constexpr int kMaxTiles = 2;               // of 8 token columns: a warp each copies them
+constexpr int kMaxTiles = 2;               // of 8 token columns
 constexpr int kMaxSets = 4;                // of parts: a warp each adds them up
-constexpr int kWeightWarp = kWarps, kTokenWarp = kWarps + 1, kEpiWarp = kTokenWarp + kMaxTiles;
+constexpr int kWeightWarp = kWarps, kEpiWarp = kWarps + 1;
 constexpr int kThreads = 32 * (kEpiWarp + kMaxSets);
 constexpr int kMaxTokens = 8 * kMaxTiles;  // and so the rows of an expert
 constexpr int kMaxExperts = 256;
@@ -58,9 +60,10 @@ constexpr int kMaxSize = 1 << 20;          // of K and F
 constexpr int kSegment = 512;              // elements of a row in a stage
 constexpr int kBlocks = kSegment / 64;
 constexpr int kBlockBytes = 16 * 128;      // 64 elements of 16 rows
+constexpr int kAtOnce = 4;                 // chunks of 32 elements whose pieces are read together
 constexpr int kPitch = kSegment * 2 + 64;  // bytes between token rows: eight lanes read different banks
 constexpr int kMaxStages = kWarps;
-constexpr int kSmem = 220 * 1024;          // ring and parts; the tables are static
+constexpr int kSmem = 217 * 1024;          // ring and parts; the tables are static
 
 struct Params {
     const void *x, *w13, *w2, *residual;
@@ -79,8 +82,10 @@ struct Params {
     KernelCtl ctl;
 };
 
-// Orders this thread's accesses to global memory with those of bulk copies.
-__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async;" ::: "memory"); }
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *tmap, uint32_t bar, int32_t x, int32_t y,
                                             int32_t z, int32_t w) {
     asm volatile(
@@ -118,22 +123,24 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t *smem = smem_raw + ((0u - smem_u32(smem_raw)) & 1023u);
     __shared__ int act_e[kMaxExperts], act_row[kMaxExperts], act_n[kMaxExperts];
     __shared__ uint16_t row_token[kMaxTokens * kMaxTopK];
+    __shared__ int16_t choice_row[kMaxTokens * kMaxTopK];
+    __shared__ float choice_weight[kMaxTokens * kMaxTopK];
     __shared__ int n_active;
-    __shared__ uint64_t bars[3 * kMaxStages + 2 * kMaxSets];
+    __shared__ uint64_t bars[2 * kMaxStages + 2 * kMaxSets];
     __shared__ int abort_word;
     volatile int *abort_flag = &abort_word;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, q = lane & 3;  // fragment row / column, and quarter of 32 elements
-    const uint32_t bar_weights = smem_u32(bars), bar_tokens = bar_weights + 8 * kMaxStages;
-    const uint32_t bar_empty = bar_tokens + 8 * kMaxStages;
+    const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * kMaxStages;
     const uint32_t bar_part = bar_empty + 8 * kMaxStages, bar_taken = bar_part + 8 * kMaxSets;
 
     // ---- active experts and the rows' tokens
     if (threadIdx.x == 0) {
+        prefetch_tmap(&map13);
+        prefetch_tmap(&map2);
         abort_word = 0;
         for (int i = 0; i < p.stages; i++) {
-            mbar_init(bar_weights + 8 * i, 1);
-            mbar_init(bar_tokens + 8 * i, kMaxTiles);
+            mbar_init(bar_full + 8 * i, 1);
             mbar_init(bar_empty + 8 * i, 1);
         }
         for (int i = 0; i < p.sets; i++) {
@@ -143,20 +150,22 @@ __global__ void __launch_bounds__(kThreads, 1)
         fence_barrier_init();
     }
     if (warp == 0) {
+        int at[kMaxExperts / 32 + 1];  // row offsets of experts lane, lane + 32, ...
+#pragma unroll
+        for (int i = 0; i < kMaxExperts / 32; i++) at[i] = p.m_offsets[min(i * 32 + lane, p.E)];
+        at[kMaxExperts / 32] = p.m_offsets[p.E];
         int n = 0;
-        for (int e0 = 0; e0 < p.E; e0 += 32) {
-            const int e = e0 + lane;
-            int r0 = 0, r1 = 0;
-            if (e < p.E) {
-                r0 = p.m_offsets[e];
-                r1 = p.m_offsets[e + 1];
-            }
-            const uint32_t live = __ballot_sync(0xffffffffu, r1 > r0);
-            if (r1 > r0) {
-                const int at = n + __popc(live & ((1u << lane) - 1u));
-                act_e[at] = e;
-                act_row[at] = r0;
-                act_n[at] = r1 - r0;
+#pragma unroll
+        for (int i = 0; i < kMaxExperts / 32; i++) {
+            int end = __shfl_down_sync(0xffffffffu, at[i], 1);
+            const int next = __shfl_sync(0xffffffffu, at[i + 1], 0);
+            if (lane == 31) end = next;
+            const uint32_t live = __ballot_sync(0xffffffffu, end > at[i]);
+            if (end > at[i]) {
+                const int slot = n + __popc(live & ((1u << lane) - 1u));
+                act_e[slot] = i * 32 + lane;
+                act_row[slot] = at[i];
+                act_n[slot] = end - at[i];
             }
             n += __popc(live);
         }
@@ -164,6 +173,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else {
         for (int i = threadIdx.x - 32; i < p.T * p.k; i += kThreads - 32) {
             const int r = p.rows[i];
+            choice_row[i] = (int16_t)r;
+            choice_weight[i] = p.weights[i];
             if (r >= 0) row_token[r] = (uint16_t)(i / p.k);
         }
     }
@@ -185,20 +196,48 @@ __global__ void __launch_bounds__(kThreads, 1)
         return k0 < whole ? min(kSegment, whole - k0) : red - k0;
     };
 
+    // The CTA's units one after another: u += stride, without a division for each.
     struct Unit {
+        int u;
         bool up;
         int a, idx, n, row0, red;  // active expert, unit of it, its rows, the reduction
     };
-    auto unit_at = [&](int u) {
-        Unit r;
-        r.up = u < total_up;
-        const int per = r.up ? units_up : units_down, v = r.up ? u : u - total_up;
+    const int up_a = stride / units_up, up_idx = stride - up_a * units_up;
+    const int down_a = stride / units_down, down_idx = stride - down_a * units_down;
+    auto open_unit = [&](Unit &r) {
+        r.up = r.u < total_up;
+        const int per = r.up ? units_up : units_down, v = r.up ? r.u : r.u - total_up;
         r.a = v / per;
         r.idx = v - r.a * per;
+        r.red = r.up ? p.K : p.F;
+    };
+    auto load_unit = [&](Unit &r) {
         r.n = act_n[r.a];
         r.row0 = act_row[r.a];
-        r.red = r.up ? p.K : p.F;
+    };
+    auto first_unit = [&]() {
+        Unit r;
+        r.u = first;
+        r.n = r.row0 = 0;
+        open_unit(r);
+        if (r.u < total) load_unit(r);
         return r;
+    };
+    auto next_unit = [&](Unit &r) {
+        r.u += stride;
+        if (r.u >= total) return;
+        if (r.up && r.u >= total_up) {
+            open_unit(r);
+        } else {
+            const int per = r.up ? units_up : units_down;
+            r.a += r.up ? up_a : down_a;
+            r.idx += r.up ? up_idx : down_idx;
+            if (r.idx >= per) {
+                r.idx -= per;
+                r.a++;
+            }
+        }
+        load_unit(r);
     };
 
     // y of 16 columns once all their parts are there (or none is to come)
@@ -209,15 +248,23 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (c >= cols) continue;
             const int64_t at = (int64_t)t * p.K + col0 + c * 4;
             float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int j = 0; j < p.k; j++) {
-                const int r = p.rows[t * p.k + j];
-                if (r < 0) continue;
-                const float w = p.weights[t * p.k + j];
-                const float4 v = __ldcg(reinterpret_cast<const float4 *>(p.part + (int64_t)r * p.K + col0 + c * 4));
-                s.x = fmaf(w, v.x, s.x);
-                s.y = fmaf(w, v.y, s.y);
-                s.z = fmaf(w, v.z, s.z);
-                s.w = fmaf(w, v.w, s.w);
+            for (int j0 = 0; j0 < p.k; j0 += 8) {
+                float4 v[8];
+                float w[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const int r = j0 + j < p.k ? choice_row[t * p.k + j0 + j] : -1;
+                    w[j] = r >= 0 ? choice_weight[t * p.k + j0 + j] : 0.0f;
+                    v[j] = r >= 0 ? __ldcg(reinterpret_cast<const float4 *>(p.part + (int64_t)r * p.K + col0 + c * 4))
+                                  : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    s.x = fmaf(w[j], v[j].x, s.x);
+                    s.y = fmaf(w[j], v[j].y, s.y);
+                    s.z = fmaf(w[j], v[j].z, s.z);
+                    s.w = fmaf(w[j], v[j].w, s.w);
+                }
             }
             if (p.residual) {
                 const uint2 r = *reinterpret_cast<const uint2 *>(static_cast<const T *>(p.residual) + at);
@@ -242,8 +289,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int set = warp - kEpiWarp;
         if (set >= p.sets) return;
         int phase = 0, from_warp = 0, turn = 0;
-        for (int u = first; u < total; u += stride, turn = turn + 1 == p.sets ? 0 : turn + 1) {
-            const Unit un = unit_at(u);
+        for (Unit un = first_unit(); un.u < total; next_unit(un), turn = turn + 1 == p.sets ? 0 : turn + 1) {
             const int stages = stages_of(un.red), parts = min(stages, p.stages), from0 = from_warp;
             from_warp = (from_warp + stages) % p.stages;
             if (turn != set) continue;
@@ -303,94 +349,56 @@ __global__ void __launch_bounds__(kThreads, 1)
         return;
     }
 
-    if (warp >= kWeightWarp) {
-        // ---- copies
-        const bool weights = warp == kWeightWarp;
-        const int tile = warp - kTokenWarp;
-        const uint32_t bar_full = weights ? bar_weights : bar_tokens;
-        int stage = 0, phase = 0, have = -1;
-        uint32_t issued = 0, issued_phase = 0;
-        bool ok = true;
-        for (int u = first; ok && u < total; u += stride) {
-            const Unit un = unit_at(u);
-            const int e = act_e[un.a], rows = weights ? 0 : min(8, un.n - tile * 8);  // a lane a token row
-            const T *from = nullptr;
-            if (!weights && !un.up && have != un.a) {
-                // the expert's hidden rows, by all CTAs of the grid
-                const int want = units_up;
-                int there = 1;
-                if (lane == 0 && load_acquire(p.up_done + e) < want) {
-                    const uint64_t t0 = global_timer_ns();
-                    while (load_acquire(p.up_done + e) < want) {
-                        if (*abort_flag || global_timer_ns() - t0 > tmo) {
-                            report_timeout(abort_flag, p.ctl.status);
-                            there = 0;
-                            break;
-                        }
+    if (warp == kWeightWarp) {
+        // ---- copies of weights, by one lane: a stage costs it less than its bytes take
+        if (lane == 0) {
+            int stage = 0, phase = 0;
+            uint32_t issued = 0, issued_phase = 0;
+            bool ok = true;
+            for (Unit un = first_unit(); ok && un.u < total; next_unit(un)) {
+                const int e = act_e[un.a], whole = un.red & ~63;
+                const int row = un.up ? e * 2 * p.F + (un.idx >> 1) * 32 + (un.idx & 1) * 8 : e * p.K + un.idx * 16;
+                for (int k0 = 0; k0 < un.red; k0 = k0 < whole ? min(k0 + kSegment, whole) : un.red) {
+                    if (!wait_parity(bar_empty + 8 * stage, phase ^ 1, tmo, abort_flag)) {
+                        report_timeout(abort_flag, p.ctl.status);
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t bar = bar_full + 8 * stage, dst = ring + stage * stage_bytes;
+                    issued |= 1u << stage;
+                    issued_phase = (issued_phase & ~(1u << stage)) | ((uint32_t)phase << stage);
+                    if (k0 < whole) {
+                        mbar_arrive_expect_tx(bar, kBlocks * kBlockBytes);  // blocks past the last are filled
+                        if (un.up) tma_load_4d(dst, &map13, bar, 0, row, 0, k0 / 64);
+                        else linear::tma_load_3d(dst, &map2, bar, 0, row, k0 / 64);
+                    } else {
+                        mbar_arrive_expect_tx(bar, kBlockBytes);
+                        if (un.up) linear::tma_load_3d(dst, &tail13, bar, k0, row, 0);
+                        else tma_load_2d(dst, &tail2, bar, k0, row);
+                    }
+                    if (++stage == p.stages) {
+                        stage = 0;
+                        phase ^= 1;
                     }
                 }
-                ok = __shfl_sync(0xffffffffu, there, 0) != 0;
-                if (!ok) break;
-                have = un.a;
-                fence_proxy_async();
             }
-            if (lane < rows) {
-                const int r = un.row0 + tile * 8 + lane;
-                from = un.up ? x + row_token[r] * p.ldx : h + (int64_t)r * p.hp;
-            }
-            const int row = un.up ? e * 2 * p.F + (un.idx >> 1) * 32 + (un.idx & 1) * 8 : e * p.K + un.idx * 16;
-            for (int k0 = 0, n; k0 < un.red; k0 += n) {
-                n = stage_elements(k0, un.red);
-                if (!linear::warp_wait_parity(bar_empty + 8 * stage, phase ^ 1, tmo, abort_flag, lane)) {
-                    if (lane == 0) report_timeout(abort_flag, p.ctl.status);
-                    ok = false;
-                    break;
-                }
-                const uint32_t bar = bar_full + 8 * stage, dst = ring + stage * stage_bytes;
-                issued |= 1u << stage;
-                issued_phase = (issued_phase & ~(1u << stage)) | ((uint32_t)phase << stage);
-                if (weights) {
-                    if (lane == 0) {
-                        if (k0 < (un.red & ~63)) {
-                            mbar_arrive_expect_tx(bar, kBlocks * kBlockBytes);  // blocks past the last are filled
-                            if (un.up) tma_load_4d(dst, &map13, bar, 0, row, 0, k0 / 64);
-                            else linear::tma_load_3d(dst, &map2, bar, 0, row, k0 / 64);
-                        } else {
-                            mbar_arrive_expect_tx(bar, kBlockBytes);
-                            if (un.up) linear::tma_load_3d(dst, &tail13, bar, k0, row, 0);
-                            else tma_load_2d(dst, &tail2, bar, k0, row);
-                        }
-                    }
-                } else if (rows > 0) {
-                    if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(rows * n) * 2);
-                    __syncwarp();
-                    if (lane < rows)
-                        bulk_load(dst + kBlocks * kBlockBytes + (tile * 8 + lane) * kPitch, from + k0, (uint32_t)n * 2, bar);
-                } else if (lane == 0) {
-                    mbar_arrive(bar);
-                }
-                __syncwarp();
-                if (++stage == p.stages) {
-                    stage = 0;
-                    phase ^= 1;
-                }
+            if (!ok) {  // let the copies in flight land before the memory goes
+                volatile int never = 0;
+                for (int i = 0; i < p.stages; i++)
+                    if (issued & (1u << i))
+                        wait_parity(bar_full + 8 * i, (issued_phase >> i) & 1, p.ctl.drain_timeout_ns, &never);
             }
         }
-        if (!ok && lane == 0) {  // let the copies in flight land before the memory goes
-            volatile int never = 0;
-            for (int i = 0; i < p.stages; i++)
-                if (issued & (1u << i))
-                    wait_parity(bar_full + 8 * i, (issued_phase >> i) & 1, p.ctl.drain_timeout_ns, &never);
-        }
-        __syncwarp();
         return;
     }
 
     // ---- the products: the stages in turn
     if (warp >= p.stages) return;
     int phase = 0, turn = 0, set = 0, set_phase = 0;  // turn: the warp of the unit's first stage
-    for (int u = first; u < total; u += stride) {
-        const Unit un = unit_at(u);
+    int have = -1;  // the active expert whose hidden rows are known to be there
+    const uint32_t base = ring + warp * stage_bytes, tokens = base + kBlocks * kBlockBytes;
+    const uint32_t wat = base + g * 128, tat = tokens + g * kPitch + q * 16;
+    for (Unit un = first_unit(); un.u < total; next_unit(un)) {
         const int stages = stages_of(un.red), mine = (warp - turn + p.stages) % p.stages;
         const bool low = un.up || un.idx * 16 + 8 < p.K;  // rows 8 .. 15 exist
         auto accumulate = [&](auto tiles_const) {
@@ -403,29 +411,53 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int st = mine; st < stages; st += p.stages) {
                 const int k0 = st * kSegment < (un.red & ~63) ? st * kSegment : un.red & ~63;
                 const int n = stage_elements(k0, un.red);
-                if (!linear::warp_wait_parity(bar_weights + 8 * warp, phase, tmo, abort_flag, lane) ||
-                    !linear::warp_wait_parity(bar_tokens + 8 * warp, phase, tmo, abort_flag, lane))
-                    return false;
-                const uint32_t base = ring + warp * stage_bytes;
-                const uint32_t wat = base + g * 128, tat = base + kBlocks * kBlockBytes + g * kPitch + q * 16;
-                const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll 4
-                for (int c = 0; c * 32 < n; c++) {
-                    const bool in = c * 32 + q * 8 < n;  // past the end the tokens' rows hold anything
-                    const uint32_t at = wat + (c >> 1) * kBlockBytes + ((((c & 1) * 4 + q) ^ g) << 4);
-                    uint4 wa, wb, b[NT];
-                    ld_shared_v4(at, wa.x, wa.y, wa.z, wa.w);
-                    ld_shared_v4(at + 1024, wb.x, wb.y, wb.z, wb.w);
-#pragma unroll
-                    for (int i = 0; i < NT; i++)
-                        ld_shared_v4(tat + i * 8 * kPitch + c * 64, b[i].x, b[i].y, b[i].z, b[i].w);
-                    if (!low) wb = zero;
-#pragma unroll
-                    for (int i = 0; i < NT; i++) {
-                        if (!in || i * 8 + g >= un.n) b[i] = zero;
-                        mma<T>(acc[i][0], wa.x, wb.x, wa.y, wb.y, b[i].x, b[i].y);
-                        mma<T>(acc[i][1], wa.z, wb.z, wa.w, wb.w, b[i].z, b[i].w);
+                if (!un.up && have != un.a) {
+                    // the expert's hidden rows, by all CTAs of the grid
+                    const int *done = p.up_done + act_e[un.a];
+                    int there = 1;
+                    if (lane == 0 && load_acquire(done) < units_up) {
+                        const uint64_t t0 = global_timer_ns();
+                        while (load_acquire(done) < units_up)
+                            if (*abort_flag || global_timer_ns() - t0 > tmo) {
+                                there = 0;
+                                break;
+                            }
                     }
+                    if (!__shfl_sync(0xffffffffu, there, 0)) return false;
+                    have = un.a;
+                }
+                for (int r = 0; r < un.n; r++) {
+                    const T *from = (un.up ? x + row_token[un.row0 + r] * p.ldx : h + (int64_t)(un.row0 + r) * p.hp) + k0;
+                    for (int i = lane; i * 8 < n; i += 32) copy16(tokens + r * kPitch + i * 16, from + i * 8);
+                }
+                if (!linear::warp_wait_parity(bar_full + 8 * warp, phase, tmo, abort_flag, lane)) return false;
+                copies_wait();
+                __syncwarp();
+                const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+                for (int c0 = 0; c0 * 32 < n; c0 += kAtOnce) {
+                    uint4 wa[kAtOnce], wb[kAtOnce], b[kAtOnce][NT];
+#pragma unroll
+                    for (int j = 0; j < kAtOnce; j++) {
+                        const int c = c0 + j;  // past the end the stage holds anything
+                        const bool in = c * 32 + q * 8 < n;
+                        const uint32_t at = wat + (c >> 1) * kBlockBytes + ((((c & 1) * 4 + q) ^ g) << 4);
+                        ld_shared_v4(at, wa[j].x, wa[j].y, wa[j].z, wa[j].w);
+                        ld_shared_v4(at + 1024, wb[j].x, wb[j].y, wb[j].z, wb[j].w);
+                        if (!in) wa[j] = zero;
+                        if (!in || !low) wb[j] = zero;
+#pragma unroll
+                        for (int i = 0; i < NT; i++) {
+                            ld_shared_v4(tat + i * 8 * kPitch + c * 64, b[j][i].x, b[j][i].y, b[j][i].z, b[j][i].w);
+                            if (!in || i * 8 + g >= un.n) b[j][i] = zero;
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < kAtOnce; j++)
+#pragma unroll
+                        for (int i = 0; i < NT; i++) {
+                            mma<T>(acc[i][0], wa[j].x, wb[j].x, wa[j].y, wb[j].y, b[j][i].x, b[j][i].y);
+                            mma<T>(acc[i][1], wa[j].z, wb[j].z, wa[j].w, wb[j].w, b[j][i].z, b[j][i].w);
+                        }
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar_empty + 8 * warp);
@@ -447,6 +479,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         };
         if (!(un.n > 8 ? accumulate(std::integral_constant<int, 2>()) : accumulate(std::integral_constant<int, 1>()))) {
             if (lane == 0) report_timeout(abort_flag, p.ctl.status);
+            copies_wait();
             break;
         }
         turn = (turn + stages) % p.stages;
