@@ -14,28 +14,27 @@
 // the warp that brings a block of 16 columns its last part forms the weighted sum there, in
 // the order of the choices: the same bits every time.
 //
-// Warps: 0-7 multiply, 8 copies weights, 9-12 add the parts up and hand them on, a unit each in
-// turn: the stores, the fence and the counter of one unit take 2 us, longer than the weights of
-// a short one.  A stage of the ring is 512 elements of 16 weight rows, one tensor copy; the
-// weights run on into W2 while its hidden rows are still being made.  The multiplying warps
-// bring the tokens' (hidden) rows of a stage themselves, by cp.async while its weights are on
-// their way: copies by another warp, or behind the weights in the same queue, came later than
-// the weights (64 experts of 2048 x 2048, 8 tokens: 225 us).  They take the stages in
-// turn, a warp a stage, so that its latencies run under the others' stages.  For each chunk of
-// 32 elements lanes 4g .. 4g + 3 read 64 bytes of row g, which is mma.m16n8k16's A fragment
-// with the chunk's elements permuted, and the tokens are read with the same permutation, so
-// nothing is shuffled.  The products are tiny (8 token columns a tile); the tensor core only
-// has to keep up with memory.  There are as many multiplying warps as stages, so that a warp
-// always has the same stage of the ring: what it waits for is the phase after its last one,
-// and a barrier tells no two phases apart that are further from each other.
+// Warps: 0-7 multiply, 8 says what each stage is, 9 watches the hidden rows' counters, 10-13 add
+// the parts up and hand them on, a unit each in turn (the stores and the counter of one unit
+// take longer than the weights of a short one).  A stage is 512 elements of 16 weight rows.
+// Each multiplying warp has one of its own: when it has read its stage it copies the next
+// weights there itself, one tensor copy, and brings the tokens' (hidden) rows by cp.async while
+// they are on their way, so its latencies run under the other warps' stages and nothing is
+// handed from warp to warp but sums.  The weights run on into W2 while its hidden rows are
+// still being made.  For each chunk of 32 elements lanes 4g .. 4g + 3 read 64 bytes of row g,
+// which is mma.m16n8k16's A fragment with the chunk's elements permuted, and the tokens are
+// read with the same permutation, so nothing is shuffled.  The products are tiny (8 token
+// columns a tile); the tensor core only has to keep up with memory.
 //
 // The weights are seen as [block of 64 elements][row][64] so that a box is eight whole swizzled
 // tiles of 8 rows by 128 bytes for each half of the rows.  Elements past the last whole block
-// are a stage of their own, from a second view that knows the row's end.
+// come beside the last stage's blocks, from a second view that knows the row's end.
 //
-// Measured on the way, E = 8 of 4096 x 14336, one token: pieces of 16 bytes by cp.async 3.6
-// TB/s whatever the depth; a bulk copy for each of the 16 rows 2.8 (82 cycles to issue one);
-// every warp a part of each stage 4.4.
+// Measured on the way, E = 8 of 4096 x 14336 (64 of 2048 x 2048, 8 tokens): pieces of 16 bytes
+// by cp.async 3.6 TB/s whatever the depth; a bulk copy for each of the 16 rows 2.8 (82 cycles to
+// issue one); every warp a part of each stage 4.4 (3.9); tokens by bulk copies of another warp
+// 4.6 (3.5), which then came after the weights; all weights copied by one lane, 0.4 us a stage, 5.5
+// (5.4).
 #include <algorithm>
 #include <climits>
 
@@ -50,9 +49,9 @@ namespace moe_layer {
 
 constexpr int kWarps = 8;                  // that multiply, at most: one a stage
 constexpr int kMaxTiles = 2;               // of 8 token columns
-constexpr int kMaxSets = 4;                // of parts: a warp each adds them up
-constexpr int kWeightWarp = kWarps, kEpiWarp = kWarps + 1;
-constexpr int kThreads = 32 * (kEpiWarp + kMaxSets);
+constexpr int kSets = 4;                   // of parts: a warp each adds them up
+constexpr int kPlanWarp = kWarps, kWatchWarp = kWarps + 1, kEpiWarp = kWarps + 2;
+constexpr int kThreads = 32 * (kEpiWarp + kSets);
 constexpr int kMaxTokens = 8 * kMaxTiles;  // and so the rows of an expert
 constexpr int kMaxExperts = 256;
 constexpr int kMaxTopK = 32;
@@ -60,10 +59,11 @@ constexpr int kMaxSize = 1 << 20;          // of K and F
 constexpr int kSegment = 512;              // elements of a row in a stage
 constexpr int kBlocks = kSegment / 64;
 constexpr int kBlockBytes = 16 * 128;      // 64 elements of 16 rows
-constexpr int kAtOnce = 4;                 // chunks of 32 elements whose pieces are read together
-constexpr int kPitch = kSegment * 2 + 64;  // bytes between token rows: eight lanes read different banks
+constexpr int kTokenRows = 8;              // of a stage: a second tile's rows take the first one's place
+constexpr int kPlans = 32;                 // stages that are described ahead, more than two for each warp
+constexpr int kUnits = 16;                 // units, likewise
 constexpr int kMaxStages = kWarps;
-constexpr int kSmem = 217 * 1024;          // ring and parts; the tables are static
+constexpr int kSmem = 223744;          // ring, parts, a row of zeros; the tables are static
 
 struct Params {
     const void *x, *w13, *w2, *residual;
@@ -78,7 +78,8 @@ struct Params {
     float *part;               // [T k, K]
     int T, E, k, K, F, hp;
     int stages, stage_bytes;   // of the ring
-    int sets;                  // of parts
+    int tail;                  // a stage has room for a block past its eight
+    int pitch;                 // bytes between token rows: eight lanes read different banks
     KernelCtl ctl;
 };
 
@@ -93,6 +94,38 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *tma
         " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
         "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
         : "memory");
+}
+// A counter in shared memory that only goes up, and the bounded wait for it to reach `want`.
+__device__ __forceinline__ void count_release(int *c, int n) {
+    asm volatile("red.release.cta.shared::cta.add.s32 [%0], %1;" ::"r"(smem_u32(c)), "r"(n) : "memory");
+}
+__device__ __forceinline__ bool count_wait(const int *c, int want, uint64_t timeout_ns, volatile int *abort) {
+    const uint32_t at = smem_u32(c);
+    auto there = [&] {
+        int v;
+        asm volatile("ld.acquire.cta.shared::cta.s32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+        return v - want >= 0;
+    };
+    if (there()) return true;
+    const uint64_t t0 = global_timer_ns();
+    for (uint32_t i = 1;; i++) {
+        if (there()) return true;
+        if ((i & 63) == 0 && (*abort || global_timer_ns() - t0 > timeout_ns)) return false;
+    }
+}
+__device__ __forceinline__ bool warp_count_wait(const int *c, int want, uint64_t timeout_ns, volatile int *abort,
+                                                int lane) {
+    int ok = 1;
+    if (lane == 0) ok = count_wait(c, want, timeout_ns, abort);
+    return __shfl_sync(0xffffffffu, ok, 0) != 0;
+}
+__device__ __forceinline__ void add_release(int *p) {
+    asm volatile("red.release.gpu.global.add.s32 [%0], 1;" ::"l"(p) : "memory");
+}
+__device__ __forceinline__ int add_acquire_release(int *p) {
+    int v;
+    asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(v) : "l"(p) : "memory");
+    return v;
 }
 __device__ __forceinline__ int load_acquire(const int *p) {
     int v;
@@ -115,38 +148,54 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
                      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// What a stage is.
+struct __align__(16) Plan {
+    int row, block, blocks, rest;  // weight: row, first block of 64 elements, whole blocks, elements past them
+    short up, n, row0, expert;     // of W13; the expert's rows; which of the active ones it is
+    short first, last;             // the warp's first and last stage in the unit
+    int unit;                      // of the CTA
+};
+// What a unit is, for those who add its parts up.
+struct __align__(16) UnitPlan {
+    short up, n, row0, expert;
+    int idx;
+    short warp, parts;  // the first stage's, and how many have one
+};
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 1)
     moe_layer_kernel(const __grid_constant__ CUtensorMap map13, const __grid_constant__ CUtensorMap tail13,
                      const __grid_constant__ CUtensorMap map2, const __grid_constant__ CUtensorMap tail2, const Params p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = smem_raw + ((0u - smem_u32(smem_raw)) & 1023u);
-    __shared__ int act_e[kMaxExperts], act_row[kMaxExperts], act_n[kMaxExperts];
+    __shared__ short act_e[kMaxExperts], act_row[kMaxExperts], act_n[kMaxExperts];
     __shared__ uint16_t row_token[kMaxTokens * kMaxTopK];
     __shared__ int16_t choice_row[kMaxTokens * kMaxTopK];
     __shared__ float choice_weight[kMaxTokens * kMaxTopK];
     __shared__ int n_active;
-    __shared__ uint64_t bars[2 * kMaxStages + 2 * kMaxSets];
+    __shared__ uint64_t bars[kMaxStages + 2 * kPlans];
+    __shared__ Plan plans[kPlans];
+    __shared__ UnitPlan units[kUnits];
+    __shared__ int planned_units, parted[kSets], taken[kSets], hidden;  // counters
     __shared__ int abort_word;
     volatile int *abort_flag = &abort_word;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, q = lane & 3;  // fragment row / column, and quarter of 32 elements
-    const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * kMaxStages;
-    const uint32_t bar_part = bar_empty + 8 * kMaxStages, bar_taken = bar_part + 8 * kMaxSets;
+    const uint32_t bar_full = smem_u32(bars), bar_plan = bar_full + 8 * kMaxStages;
+    const uint32_t bar_planned = bar_plan + 8 * kPlans;
 
     // ---- active experts and the rows' tokens
     if (threadIdx.x == 0) {
         prefetch_tmap(&map13);
         prefetch_tmap(&map2);
         abort_word = 0;
-        for (int i = 0; i < p.stages; i++) {
-            mbar_init(bar_full + 8 * i, 1);
-            mbar_init(bar_empty + 8 * i, 1);
+        for (int i = 0; i < p.stages; i++) mbar_init(bar_full + 8 * i, 1);
+        for (int i = 0; i < kPlans; i++) {
+            mbar_init(bar_plan + 8 * i, 1);
+            mbar_init(bar_planned + 8 * i, 1);
         }
-        for (int i = 0; i < p.sets; i++) {
-            mbar_init(bar_part + 8 * i, p.stages);
-            mbar_init(bar_taken + 8 * i, 1);
-        }
+        for (int i = 0; i < kSets; i++) parted[i] = taken[i] = 0;
+        hidden = planned_units = 0;
         fence_barrier_init();
     }
     if (warp == 0) {
@@ -163,9 +212,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t live = __ballot_sync(0xffffffffu, end > at[i]);
             if (end > at[i]) {
                 const int slot = n + __popc(live & ((1u << lane) - 1u));
-                act_e[slot] = i * 32 + lane;
-                act_row[slot] = at[i];
-                act_n[slot] = end - at[i];
+                act_e[slot] = (short)(i * 32 + lane);
+                act_row[slot] = (short)at[i];
+                act_n[slot] = (short)(end - at[i]);
             }
             n += __popc(live);
         }
@@ -178,6 +227,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (r >= 0) row_token[r] = (uint16_t)(i / p.k);
         }
     }
+    for (int i = threadIdx.x; i * 4 < p.pitch; i += kThreads)
+        reinterpret_cast<int *>(smem + p.stages * p.stage_bytes + kSets * kWarps * ((p.T + 7) / 8) * 512)[i] = 0;
     __syncthreads();
 
     const T *x = static_cast<const T *>(p.x);
@@ -189,12 +240,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int tiles_cap = (p.T + 7) / 8;
     const uint32_t stage_bytes = p.stage_bytes, ring = smem_u32(smem);
     float4 *sums = reinterpret_cast<float4 *>(smem + p.stages * stage_bytes);  // [set][warp][tile][lane]
-    auto stages_of = [](int red) { return ((red & ~63) + kSegment - 1) / kSegment + ((red & 63) != 0); };
-    // elements of the stage that begins at k0 of a reduction: whole blocks of 64, then the rest
-    auto stage_elements = [](int k0, int red) {
-        const int whole = red & ~63;
-        return k0 < whole ? min(kSegment, whole - k0) : red - k0;
-    };
+    // A reduction's stages, by their first element: up to eight whole blocks of 64, the last one
+    // with the elements past them
+    auto stages_of = [](int red) { return max(1, ((red & ~63) + kSegment - 1) / kSegment); };
 
     // The CTA's units one after another: u += stride, without a division for each.
     struct Unit {
@@ -284,28 +332,33 @@ __global__ void __launch_bounds__(kThreads, 1)
         return;
     }
 
+    // this CTA's units and stages
+    const int n_ups = first < total_up ? (total_up - first + stride - 1) / stride : 0;
+    const int n_units = first < total ? (total - first + stride - 1) / stride : 0;
+    const int n_stages = n_ups * stages_of(p.K) + (n_units - n_ups) * stages_of(p.F);
+
     if (warp >= kEpiWarp) {
         // ---- the parts of the units in turn
         const int set = warp - kEpiWarp;
-        if (set >= p.sets) return;
-        int phase = 0, from_warp = 0, turn = 0;
-        for (Unit un = first_unit(); un.u < total; next_unit(un), turn = turn + 1 == p.sets ? 0 : turn + 1) {
-            const int stages = stages_of(un.red), parts = min(stages, p.stages), from0 = from_warp;
-            from_warp = (from_warp + stages) % p.stages;
-            if (turn != set) continue;
-            if (!linear::warp_wait_parity(bar_part + 8 * set, phase, tmo, abort_flag, lane)) {
+        int want = 0;
+        for (int i = set; i < n_units; i += kSets) {
+            bool ok = warp_count_wait(&planned_units, i + 1, tmo, abort_flag, lane);
+            const UnitPlan un = units[i % kUnits];
+            want += un.parts;
+            if (ok) ok = warp_count_wait(&parted[set], want, tmo, abort_flag, lane);
+            if (!ok) {
                 if (lane == 0) report_timeout(abort_flag, p.ctl.status);
                 break;
             }
-            phase ^= 1;
             float4 sum[kMaxTiles];
 #pragma unroll
             for (int i = 0; i < kMaxTiles; i++) {
                 if (i * 8 >= un.n) break;
                 const float4 *from = sums + (set * kWarps * tiles_cap + i) * 32 + lane;
                 float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-                for (int w = 0; w < parts; w++) {  // in the order of the stages
-                    const float4 o = from[((from0 + w) % p.stages) * tiles_cap * 32];
+                for (int w = 0, at = un.warp; w < un.parts; w++) {  // in the order of the stages
+                    const float4 o = from[at * tiles_cap * 32];
+                    at = at + 1 == p.stages ? 0 : at + 1;
                     s.x += o.x;
                     s.y += o.y;
                     s.z += o.z;
@@ -314,7 +367,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 sum[i] = s;
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar_taken + 8 * set);  // other parts may take their place
+            if (lane == 0) count_release(&taken[set], 1);  // other parts may take their place
 #pragma unroll
             for (int i = 0; i < kMaxTiles; i++) {
                 if (i * 8 >= un.n) break;
@@ -336,157 +389,200 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
             int last = 0;
             if (lane == 0) {
-                __threadfence();
-                if (un.up) atomicAdd(p.up_done + act_e[un.a], 1);
-                else last = atomicAdd(p.col_done + un.idx, 1) == n_active - 1;
+                if (un.up) add_release(p.up_done + act_e[un.expert]);
+                else last = add_acquire_release(p.col_done + un.idx) == n_active - 1;
             }
-            if (__shfl_sync(0xffffffffu, last, 0)) {
-                __threadfence();
-                combine(un.idx * 16);
-            }
+            if (__shfl_sync(0xffffffffu, last, 0)) combine(un.idx * 16);
             __syncwarp();
         }
         return;
     }
 
-    if (warp == kWeightWarp) {
-        // ---- copies of weights, by one lane: a stage costs it less than its bytes take
+    if (warp == kPlanWarp) {
+        // ---- what the stages and the units are, one after another
         if (lane == 0) {
-            int stage = 0, phase = 0;
-            uint32_t issued = 0, issued_phase = 0;
-            bool ok = true;
-            for (Unit un = first_unit(); ok && un.u < total; next_unit(un)) {
-                const int e = act_e[un.a], whole = un.red & ~63;
-                const int row = un.up ? e * 2 * p.F + (un.idx >> 1) * 32 + (un.idx & 1) * 8 : e * p.K + un.idx * 16;
-                for (int k0 = 0; k0 < un.red; k0 = k0 < whole ? min(k0 + kSegment, whole) : un.red) {
-                    if (!wait_parity(bar_empty + 8 * stage, phase ^ 1, tmo, abort_flag)) {
+            int entry = 0, phase = 0, unit = 0, turn = 0;
+            for (Unit un = first_unit(); un.u < total; next_unit(un), unit++) {
+                const int e = act_e[un.a], stages = stages_of(un.red), whole = un.red / 64;
+                const int old = unit - kUnits;  // whose place this one takes
+                if (old >= 0 && !count_wait(&taken[old % kSets], old / kSets + 1, tmo, abort_flag)) {
+                    report_timeout(abort_flag, p.ctl.status);
+                    return;
+                }
+                units[unit % kUnits] = {(short)un.up, (short)un.n, (short)un.row0, (short)un.a, un.idx, (short)turn,
+                                        (short)min(stages, p.stages)};
+                count_release(&planned_units, 1);
+                Plan plan;
+                plan.row = un.up ? e * 2 * p.F + (un.idx >> 1) * 32 + (un.idx & 1) * 8 : e * p.K + un.idx * 16;
+                plan.up = un.up;
+                plan.n = (short)un.n;
+                plan.row0 = (short)un.row0;
+                plan.expert = (short)un.a;
+                plan.unit = unit;
+                for (int st = 0; st < stages; st++) {
+                    plan.block = st * kBlocks;
+                    plan.blocks = min(kBlocks, whole - plan.block);
+                    plan.rest = st == stages - 1 ? un.red & 63 : 0;
+                    plan.first = st < p.stages;
+                    plan.last = st + p.stages >= stages;
+                    if (!wait_parity(bar_planned + 8 * entry, phase ^ 1, tmo, abort_flag)) {
                         report_timeout(abort_flag, p.ctl.status);
-                        ok = false;
-                        break;
+                        return;
                     }
-                    const uint32_t bar = bar_full + 8 * stage, dst = ring + stage * stage_bytes;
-                    issued |= 1u << stage;
-                    issued_phase = (issued_phase & ~(1u << stage)) | ((uint32_t)phase << stage);
-                    if (k0 < whole) {
-                        mbar_arrive_expect_tx(bar, kBlocks * kBlockBytes);  // blocks past the last are filled
-                        if (un.up) tma_load_4d(dst, &map13, bar, 0, row, 0, k0 / 64);
-                        else linear::tma_load_3d(dst, &map2, bar, 0, row, k0 / 64);
-                    } else {
-                        mbar_arrive_expect_tx(bar, kBlockBytes);
-                        if (un.up) linear::tma_load_3d(dst, &tail13, bar, k0, row, 0);
-                        else tma_load_2d(dst, &tail2, bar, k0, row);
-                    }
-                    if (++stage == p.stages) {
-                        stage = 0;
+                    plans[entry] = plan;
+                    mbar_arrive(bar_plan + 8 * entry);
+                    if (++entry == kPlans) {
+                        entry = 0;
                         phase ^= 1;
                     }
+                    turn = turn + 1 == p.stages ? 0 : turn + 1;
                 }
-            }
-            if (!ok) {  // let the copies in flight land before the memory goes
-                volatile int never = 0;
-                for (int i = 0; i < p.stages; i++)
-                    if (issued & (1u << i))
-                        wait_parity(bar_full + 8 * i, (issued_phase >> i) & 1, p.ctl.drain_timeout_ns, &never);
             }
         }
         return;
     }
 
-    // ---- the products: the stages in turn
+    if (warp == kWatchWarp) {
+        // ---- which experts' hidden rows are there, by all CTAs of the grid
+        if (lane == 0 && n_stages > 0) {
+            const uint64_t t0 = global_timer_ns();
+            for (int a = 0; a < n_active; a++) {
+                const int *done = p.up_done + act_e[a];
+                while (load_acquire(done) < units_up)
+                    if (*abort_flag || global_timer_ns() - t0 > tmo) {
+                        report_timeout(abort_flag, p.ctl.status);
+                        return;
+                    }
+                count_release(&hidden, 1);
+            }
+        }
+        return;
+    }
+
+    // ---- the products: this warp's stages, first .. n_stages by p.stages
     if (warp >= p.stages) return;
-    int phase = 0, turn = 0, set = 0, set_phase = 0;  // turn: the warp of the unit's first stage
-    int have = -1;  // the active expert whose hidden rows are known to be there
-    const uint32_t base = ring + warp * stage_bytes, tokens = base + kBlocks * kBlockBytes;
-    const uint32_t wat = base + g * 128, tat = tokens + g * kPitch + q * 16;
-    for (Unit un = first_unit(); un.u < total; next_unit(un)) {
-        const int stages = stages_of(un.red), mine = (warp - turn + p.stages) % p.stages;
-        const bool low = un.up || un.idx * 16 + 8 < p.K;  // rows 8 .. 15 exist
-        auto accumulate = [&](auto tiles_const) {
-            constexpr int NT = decltype(tiles_const)::value;
-            float acc[NT][2][4];
-#pragma unroll
-            for (int i = 0; i < NT; i++)
-#pragma unroll
-                for (int j = 0; j < 8; j++) acc[i][j >> 2][j & 3] = 0.0f;
-            for (int st = mine; st < stages; st += p.stages) {
-                const int k0 = st * kSegment < (un.red & ~63) ? st * kSegment : un.red & ~63;
-                const int n = stage_elements(k0, un.red);
-                if (!un.up && have != un.a) {
-                    // the expert's hidden rows, by all CTAs of the grid
-                    const int *done = p.up_done + act_e[un.a];
-                    int there = 1;
-                    if (lane == 0 && load_acquire(done) < units_up) {
-                        const uint64_t t0 = global_timer_ns();
-                        while (load_acquire(done) < units_up)
-                            if (*abort_flag || global_timer_ns() - t0 > tmo) {
-                                there = 0;
-                                break;
-                            }
-                    }
-                    if (!__shfl_sync(0xffffffffu, there, 0)) return false;
-                    have = un.a;
-                }
-                for (int r = 0; r < un.n; r++) {
-                    const T *from = (un.up ? x + row_token[un.row0 + r] * p.ldx : h + (int64_t)(un.row0 + r) * p.hp) + k0;
-                    for (int i = lane; i * 8 < n; i += 32) copy16(tokens + r * kPitch + i * 16, from + i * 8);
-                }
-                if (!linear::warp_wait_parity(bar_full + 8 * warp, phase, tmo, abort_flag, lane)) return false;
-                copies_wait();
-                __syncwarp();
-                const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-                for (int c0 = 0; c0 * 32 < n; c0 += kAtOnce) {
-                    uint4 wa[kAtOnce], wb[kAtOnce], b[kAtOnce][NT];
-#pragma unroll
-                    for (int j = 0; j < kAtOnce; j++) {
-                        const int c = c0 + j;  // past the end the stage holds anything
-                        const bool in = c * 32 + q * 8 < n;
-                        const uint32_t at = wat + (c >> 1) * kBlockBytes + ((((c & 1) * 4 + q) ^ g) << 4);
-                        ld_shared_v4(at, wa[j].x, wa[j].y, wa[j].z, wa[j].w);
-                        ld_shared_v4(at + 1024, wb[j].x, wb[j].y, wb[j].z, wb[j].w);
-                        if (!in) wa[j] = zero;
-                        if (!in || !low) wb[j] = zero;
-#pragma unroll
-                        for (int i = 0; i < NT; i++) {
-                            ld_shared_v4(tat + i * 8 * kPitch + c * 64, b[j][i].x, b[j][i].y, b[j][i].z, b[j][i].w);
-                            if (!in || i * 8 + g >= un.n) b[j][i] = zero;
-                        }
-                    }
-#pragma unroll
-                    for (int j = 0; j < kAtOnce; j++)
-#pragma unroll
-                        for (int i = 0; i < NT; i++) {
-                            mma<T>(acc[i][0], wa[j].x, wb[j].x, wa[j].y, wb[j].y, b[j][i].x, b[j][i].y);
-                            mma<T>(acc[i][1], wa[j].z, wb[j].z, wa[j].w, wb[j].w, b[j][i].z, b[j][i].w);
-                        }
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar_empty + 8 * warp);
-                phase ^= 1;
+    uint8_t *weights = smem + warp * stage_bytes, *rows = weights + (kBlocks + p.tail) * kBlockBytes;
+    const uint8_t *zeros = smem + p.stages * stage_bytes + kSets * kWarps * tiles_cap * 512;  // a row of them
+    const uint8_t *even = weights + g * 128 + ((q ^ g) << 4), *odd = weights + g * 128 + (((4 + q) ^ g) << 4);
+    const uint32_t full = bar_full + 8 * warp;
+    // Takes the description of stage i and copies its weights (the warp has read those before).
+    auto open = [&](int i, Plan &plan) {
+        const int entry = i % kPlans;
+        const bool ok = linear::warp_wait_parity(bar_plan + 8 * entry, (i / kPlans) & 1, tmo, abort_flag, lane);
+        plan = plans[entry];
+        __syncwarp();
+        if (ok && lane == 0) {
+            const uint32_t dst = smem_u32(weights);
+            mbar_arrive(bar_planned + 8 * entry);
+            mbar_arrive_expect_tx(full, ((plan.blocks > 0 ? kBlocks : 0) + (plan.rest ? 1 : 0)) * kBlockBytes);
+            if (plan.blocks > 0) {  // blocks past the last are filled with zeros
+                if (plan.up) tma_load_4d(dst, &map13, full, 0, plan.row, 0, plan.block);
+                else linear::tma_load_3d(dst, &map2, full, 0, plan.row, plan.block);
             }
-            // the set's last parts have been taken
-            if (!linear::warp_wait_parity(bar_taken + 8 * set, set_phase ^ 1, tmo, abort_flag, lane)) return false;
-            if (mine < stages) {
-                float4 *to = sums + (set * kWarps + warp) * tiles_cap * 32 + lane;
-#pragma unroll
-                for (int i = 0; i < NT; i++)
-                    to[i * 32] = make_float4(acc[i][0][0] + acc[i][1][0], acc[i][0][1] + acc[i][1][1],
-                                             acc[i][0][2] + acc[i][1][2], acc[i][0][3] + acc[i][1][3]);
+            if (plan.rest) {
+                const int k = (plan.up ? p.K : p.F) & ~63;
+                if (plan.up) linear::tma_load_3d(dst + kBlocks * kBlockBytes, &tail13, full, k, plan.row, 0);
+                else tma_load_2d(dst + kBlocks * kBlockBytes, &tail2, full, k, plan.row);
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar_part + 8 * set);
-            __syncwarp();
-            return true;
+        }
+        __syncwarp();
+        return ok;
+    };
+    float acc[kMaxTiles][2][4];
+    Plan plan;
+    bool ok = true, flying = false;
+    int phase = 0;
+    if (warp < n_stages) ok = flying = open(warp, plan);
+    for (int i = warp; ok && i < n_stages; i += p.stages) {
+        if (!plan.up) {
+            ok = warp_count_wait(&hidden, plan.expert + 1, tmo, abort_flag, lane);
+            if (!ok) break;
+        }
+        const int k0 = plan.block * 64, n = plan.blocks * 64 + plan.rest;
+        auto bring = [&](int tile) {
+            uint32_t to = smem_u32(rows);
+            for (int r = tile * 8; r < min((int)plan.n, tile * 8 + 8); r++, to += p.pitch) {
+                const int row = plan.row0 + r;
+                const T *from = (plan.up ? x + row_token[row] * p.ldx : h + (int64_t)row * p.hp) + k0;
+                for (int c = lane; c * 8 < n; c += 32) copy16(to + c * 16, from + c * 8);
+            }
         };
-        if (!(un.n > 8 ? accumulate(std::integral_constant<int, 2>()) : accumulate(std::integral_constant<int, 1>()))) {
-            if (lane == 0) report_timeout(abort_flag, p.ctl.status);
+        bring(0);
+        if (plan.first)
+#pragma unroll
+            for (int t = 0; t < kMaxTiles; t++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) acc[t][j >> 2][j & 3] = 0.0f;
+        ok = linear::warp_wait_parity(full, phase, tmo, abort_flag, lane);
+        if (!ok) break;
+        phase ^= 1;
+        flying = false;
+#pragma unroll
+        for (int t = 0; t < kMaxTiles; t++) {
+            if (t * 8 >= plan.n) break;
+            if (t) {
+                __syncwarp();  // the first tile's rows have been read
+                bring(t);
+            }
             copies_wait();
-            break;
+            __syncwarp();
+            const uint8_t *column = (t * 8 + g < plan.n ? rows + g * p.pitch : zeros) + q * 16;
+            auto chunk = [&](const uint8_t *w, const uint8_t *b) {
+                const uint4 wa = *reinterpret_cast<const uint4 *>(w), wb = *reinterpret_cast<const uint4 *>(w + 1024);
+                const uint4 v = *reinterpret_cast<const uint4 *>(b);
+                mma<T>(acc[t][0], wa.x, wb.x, wa.y, wb.y, v.x, v.y);
+                mma<T>(acc[t][1], wa.z, wb.z, wa.w, wb.w, v.z, v.w);
+            };
+            if (plan.blocks == kBlocks) {
+#pragma unroll
+                for (int b = 0; b < kBlocks; b++) {
+                    chunk(even + b * kBlockBytes, column + b * 128);
+                    chunk(odd + b * kBlockBytes, column + b * 128 + 64);
+                }
+            } else {
+                for (int b = 0; b < plan.blocks; b++) {
+                    chunk(even + b * kBlockBytes, column + b * 128);
+                    chunk(odd + b * kBlockBytes, column + b * 128 + 64);
+                }
+            }
+            if (plan.rest)  // the weights past the row's end are zeros, the tokens' row is read no further
+#pragma unroll
+                for (int half = 0; half < 2; half++)
+                    if (half * 32 < plan.rest) {
+                        const bool in = half * 32 + q * 8 < plan.rest;
+                        chunk((half ? odd : even) + kBlocks * kBlockBytes,
+                              in ? column + plan.blocks * 128 + half * 64 : zeros);
+                    }
         }
-        turn = (turn + stages) % p.stages;
-        if (++set == p.sets) {
-            set = 0;
-            set_phase ^= 1;
+        __syncwarp();
+        const bool last = plan.last;
+        const int unit = plan.unit, columns = plan.n;
+        if (i + p.stages < n_stages) {
+            ok = flying = open(i + p.stages, plan);
+            if (!ok) break;
         }
+        if (last) {
+            const int set = unit % kSets;
+            ok = warp_count_wait(&taken[set], unit / kSets, tmo, abort_flag, lane);
+            if (!ok) break;
+            float4 *to = sums + (set * kWarps + warp) * tiles_cap * 32 + lane;
+#pragma unroll
+            for (int t = 0; t < kMaxTiles; t++)
+                if (t * 8 < columns)
+                    to[t * 32] = make_float4(acc[t][0][0] + acc[t][1][0], acc[t][0][1] + acc[t][1][1],
+                                             acc[t][0][2] + acc[t][1][2], acc[t][0][3] + acc[t][1][3]);
+            __syncwarp();
+            if (lane == 0) count_release(&parted[set], 1);
+        }
+    }
+    if (!ok) {  // let the copies in flight land before the memory goes
+        volatile int never = 0;
+        if (lane == 0) {
+            report_timeout(abort_flag, p.ctl.status);
+            if (flying) wait_parity(full, phase, p.ctl.drain_timeout_ns, &never);
+        }
+        copies_wait();
+        __syncwarp();
     }
 }
 
@@ -631,10 +727,12 @@ int nvfp4_moe_layer(const void *X, int64_t ldx, const void *logits, int logits_d
     p.F = F;
     p.hp = l.hp;
     const int tiles = (T + 7) / 8;
-    p.stage_bytes = (moe_layer::kBlocks * moe_layer::kBlockBytes + 8 * tiles * moe_layer::kPitch + 1023) & ~1023;
-    p.sets = tiles == 1 ? moe_layer::kMaxSets : 3;
+    p.tail = K % 64 || F % 64;
+    p.pitch = (moe_layer::kSegment + 64 * p.tail) * 2 + 64;
+    p.stage_bytes =
+        ((moe_layer::kBlocks + p.tail) * moe_layer::kBlockBytes + moe_layer::kTokenRows * p.pitch + 1023) & ~1023;
     p.stages = std::min(moe_layer::kMaxStages,
-                        (moe_layer::kSmem - 1024 - p.sets * moe_layer::kWarps * tiles * 512) / p.stage_bytes);
+                        (moe_layer::kSmem - 1024 - p.pitch - moe_layer::kSets * moe_layer::kWarps * tiles * 512) / p.stage_bytes);
     // the router's checks of its own arguments come before any launch
     st = moe::route_tokens(logits, logits_dtype, bias, T, E, top_k, scoring, renormalize, scale,
                            const_cast<float *>(p.weights), reinterpret_cast<int *>(ws + l.experts),
