@@ -14,9 +14,9 @@
 // the warp that brings a block of 16 columns its last part forms the weighted sum there, in
 // the order of the choices: the same bits every time.
 //
-// Warps: 0-7 multiply, 8 says what each stage is, 9 watches the hidden rows' counters, 10-13 add
+// Warps: 0-7 multiply, 8 says what each stage is, 9 watches the hidden rows' counters, 10-15 add
 // the parts up and hand them on, a unit each in turn (the stores and the counter of one unit
-// take longer than the weights of a short one).  A stage is 512 elements of 16 weight rows.
+// take 5 us under load, longer than the weights of a short one).  A stage is 512 elements of 16 weight rows.
 // Each multiplying warp has one of its own: when it has read its stage it copies the next
 // weights there itself, one tensor copy, and brings the tokens' (hidden) rows by cp.async while
 // they are on their way, so its latencies run under the other warps' stages and nothing is
@@ -49,9 +49,10 @@ namespace moe_layer {
 
 constexpr int kWarps = 8;                  // that multiply, at most: one a stage
 constexpr int kMaxTiles = 2;               // of 8 token columns
-constexpr int kSets = 4;                   // of parts: a warp each adds them up
+constexpr int kSets = 4;                   // of parts
+constexpr int kEpiWarps = 6;               // that add them up
 constexpr int kPlanWarp = kWarps, kWatchWarp = kWarps + 1, kEpiWarp = kWarps + 2;
-constexpr int kThreads = 32 * (kEpiWarp + kSets);
+constexpr int kThreads = 32 * (kEpiWarp + kEpiWarps);
 constexpr int kMaxTokens = 8 * kMaxTiles;  // and so the rows of an expert
 constexpr int kMaxExperts = 256;
 constexpr int kMaxTopK = 32;
@@ -99,17 +100,16 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *tma
 __device__ __forceinline__ void count_release(int *c, int n) {
     asm volatile("red.release.cta.shared::cta.add.s32 [%0], %1;" ::"r"(smem_u32(c)), "r"(n) : "memory");
 }
+__device__ __forceinline__ bool count_reached(const int *c, int want) {
+    int v;
+    asm volatile("ld.acquire.cta.shared::cta.s32 %0, [%1];" : "=r"(v) : "r"(smem_u32(c)) : "memory");
+    return v - want >= 0;
+}
 __device__ __forceinline__ bool count_wait(const int *c, int want, uint64_t timeout_ns, volatile int *abort) {
-    const uint32_t at = smem_u32(c);
-    auto there = [&] {
-        int v;
-        asm volatile("ld.acquire.cta.shared::cta.s32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
-        return v - want >= 0;
-    };
-    if (there()) return true;
+    if (count_reached(c, want)) return true;
     const uint64_t t0 = global_timer_ns();
     for (uint32_t i = 1;; i++) {
-        if (there()) return true;
+        if (count_reached(c, want)) return true;
         if ((i & 63) == 0 && (*abort || global_timer_ns() - t0 > timeout_ns)) return false;
     }
 }
@@ -160,6 +160,7 @@ struct __align__(16) UnitPlan {
     short up, n, row0, expert;
     int idx;
     short warp, parts;  // the first stage's, and how many have one
+    int set_parts;      // of the set so far, with these
 };
 
 template <typename T>
@@ -339,13 +340,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (warp >= kEpiWarp) {
         // ---- the parts of the units in turn
-        const int set = warp - kEpiWarp;
-        int want = 0;
-        for (int i = set; i < n_units; i += kSets) {
+        // which of a unit's rows a lane's fragments hold: the order in which eight lanes read two
+        // rows of a swizzled tile from different banks
+        const int r = (g >> 1) | ((g & 1) << 2);
+        for (int i = warp - kEpiWarp; i < n_units; i += kEpiWarps) {
+            const int set = i % kSets;
             bool ok = warp_count_wait(&planned_units, i + 1, tmo, abort_flag, lane);
             const UnitPlan un = units[i % kUnits];
-            want += un.parts;
-            if (ok) ok = warp_count_wait(&parted[set], want, tmo, abort_flag, lane);
+            if (ok) ok = warp_count_wait(&parted[set], un.set_parts, tmo, abort_flag, lane);
             if (!ok) {
                 if (lane == 0) report_timeout(abort_flag, p.ctl.status);
                 break;
@@ -372,13 +374,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int i = 0; i < kMaxTiles; i++) {
                 if (i * 8 >= un.n) break;
                 const float4 s = sum[i];
-                const int c = i * 8 + 2 * q;  // s.x, s.z: column c, rows g and g + 8; s.y, s.w: column c + 1
+                const int c = i * 8 + 2 * q;  // s.x, s.z: column c, rows r and r + 8; s.y, s.w: column c + 1
                 if (un.up) {
-                    T *to = h + (int64_t)(un.row0 + c) * p.hp + un.idx * 8 + g;
+                    T *to = h + (int64_t)(un.row0 + c) * p.hp + un.idx * 8 + r;
                     if (c < un.n) to[0] = Type16<T>::round(s.x * linear::sigma(s.x) * s.z);
                     if (c + 1 < un.n) to[p.hp] = Type16<T>::round(s.y * linear::sigma(s.y) * s.w);
                 } else {
-                    const int row = un.idx * 16 + g;
+                    const int row = un.idx * 16 + r;
                     float *to = p.part + (int64_t)(un.row0 + c) * p.K + row;
                     if (c < un.n && row < p.K) to[0] = s.x;
                     if (c < un.n && row + 8 < p.K) to[8] = s.z;
@@ -401,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == kPlanWarp) {
         // ---- what the stages and the units are, one after another
         if (lane == 0) {
-            int entry = 0, phase = 0, unit = 0, turn = 0;
+            int entry = 0, phase = 0, unit = 0, turn = 0, set_parts[kSets] = {};
             for (Unit un = first_unit(); un.u < total; next_unit(un), unit++) {
                 const int e = act_e[un.a], stages = stages_of(un.red), whole = un.red / 64;
                 const int old = unit - kUnits;  // whose place this one takes
@@ -409,8 +411,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                     report_timeout(abort_flag, p.ctl.status);
                     return;
                 }
+                const int parts = min(stages, p.stages);
+                int sum = 0;
+#pragma unroll
+                for (int i = 0; i < kSets; i++)
+                    if (i == unit % kSets) sum = set_parts[i] += parts;
                 units[unit % kUnits] = {(short)un.up, (short)un.n, (short)un.row0, (short)un.a, un.idx, (short)turn,
-                                        (short)min(stages, p.stages)};
+                                        (short)parts, sum};
                 count_release(&planned_units, 1);
                 Plan plan;
                 plan.row = un.up ? e * 2 * p.F + (un.idx >> 1) * 32 + (un.idx & 1) * 8 : e * p.K + un.idx * 16;
@@ -463,17 +470,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp >= p.stages) return;
     uint8_t *weights = smem + warp * stage_bytes, *rows = weights + (kBlocks + p.tail) * kBlockBytes;
     const uint8_t *zeros = smem + p.stages * stage_bytes + kSets * kWarps * tiles_cap * 512;  // a row of them
-    const uint8_t *even = weights + g * 128 + ((q ^ g) << 4), *odd = weights + g * 128 + (((4 + q) ^ g) << 4);
+    const int wr = (g >> 1) | ((g & 1) << 2);  // the weight row of this lane's fragments
+    const uint8_t *even = weights + wr * 128 + ((q ^ wr) << 4), *odd = weights + wr * 128 + (((4 + q) ^ wr) << 4);
     const uint32_t full = bar_full + 8 * warp;
-    // Takes the description of stage i and copies its weights (the warp has read those before).
-    auto open = [&](int i, Plan &plan) {
+    auto describe = [&](int i, Plan &plan) {
         const int entry = i % kPlans;
         const bool ok = linear::warp_wait_parity(bar_plan + 8 * entry, (i / kPlans) & 1, tmo, abort_flag, lane);
         plan = plans[entry];
         __syncwarp();
-        if (ok && lane == 0) {
+        if (lane == 0) mbar_arrive(bar_planned + 8 * entry);
+        return ok;
+    };
+    auto copy_weights = [&](const Plan &plan) {
+        if (lane == 0) {
             const uint32_t dst = smem_u32(weights);
-            mbar_arrive(bar_planned + 8 * entry);
             mbar_arrive_expect_tx(full, ((plan.blocks > 0 ? kBlocks : 0) + (plan.rest ? 1 : 0)) * kBlockBytes);
             if (plan.blocks > 0) {  // blocks past the last are filled with zeros
                 if (plan.up) tma_load_4d(dst, &map13, full, 0, plan.row, 0, plan.block);
@@ -486,28 +496,35 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
         __syncwarp();
-        return ok;
+    };
+    // eight of an expert's rows, the stage's elements of them
+    auto bring = [&](const Plan &plan, int tile) {
+        const int k0 = plan.block * 64, n = plan.blocks * 64 + plan.rest;
+        uint32_t to = smem_u32(rows);
+        for (int r = tile * 8; r < min((int)plan.n, tile * 8 + 8); r++, to += p.pitch) {
+            const int row = plan.row0 + r;
+            const T *from = (plan.up ? x + row_token[row] * p.ldx : h + (int64_t)row * p.hp) + k0;
+            for (int c = lane; c * 8 < n; c += 32) copy16(to + c * 16, from + c * 8);
+        }
     };
     float acc[kMaxTiles][2][4];
     Plan plan;
-    bool ok = true, flying = false;
+    bool ok = true, flying = false, brought = false;  // the weights, the rows of `plan`
     int phase = 0;
-    if (warp < n_stages) ok = flying = open(warp, plan);
+    if (warp < n_stages) {
+        ok = flying = describe(warp, plan);
+        if (ok) copy_weights(plan);
+    }
     for (int i = warp; ok && i < n_stages; i += p.stages) {
-        if (!plan.up) {
-            ok = warp_count_wait(&hidden, plan.expert + 1, tmo, abort_flag, lane);
+        if (!brought) {
+            if (!plan.up) ok = warp_count_wait(&hidden, plan.expert + 1, tmo, abort_flag, lane);
             if (!ok) break;
+            bring(plan, 0);
         }
-        const int k0 = plan.block * 64, n = plan.blocks * 64 + plan.rest;
-        auto bring = [&](int tile) {
-            uint32_t to = smem_u32(rows);
-            for (int r = tile * 8; r < min((int)plan.n, tile * 8 + 8); r++, to += p.pitch) {
-                const int row = plan.row0 + r;
-                const T *from = (plan.up ? x + row_token[row] * p.ldx : h + (int64_t)row * p.hp) + k0;
-                for (int c = lane; c * 8 < n; c += 32) copy16(to + c * 16, from + c * 8);
-            }
-        };
-        bring(0);
+        Plan next;
+        const bool more = i + p.stages < n_stages;
+        if (more) ok = describe(i + p.stages, next);
+        if (!ok) break;
         if (plan.first)
 #pragma unroll
             for (int t = 0; t < kMaxTiles; t++)
@@ -522,7 +539,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (t * 8 >= plan.n) break;
             if (t) {
                 __syncwarp();  // the first tile's rows have been read
-                bring(t);
+                bring(plan, t);
             }
             copies_wait();
             __syncwarp();
@@ -557,9 +574,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         const bool last = plan.last;
         const int unit = plan.unit, columns = plan.n;
-        if (i + p.stages < n_stages) {
-            ok = flying = open(i + p.stages, plan);
-            if (!ok) break;
+        brought = false;
+        if (more) {
+            plan = next;
+            copy_weights(plan);
+            flying = true;
+            // hidden rows that are not there yet wait for others, this warp's own parts among them
+            brought = plan.up || count_reached(&hidden, plan.expert + 1);
+            brought = __shfl_sync(0xffffffffu, (int)brought, 0) != 0;
+            if (brought) bring(plan, 0);
         }
         if (last) {
             const int set = unit % kSets;
@@ -577,6 +600,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (!ok) {  // let the copies in flight land before the memory goes
         volatile int never = 0;
+        __syncwarp();
         if (lane == 0) {
             report_timeout(abort_flag, p.ctl.status);
             if (flying) wait_parity(full, phase, p.ctl.drain_timeout_ns, &never);
