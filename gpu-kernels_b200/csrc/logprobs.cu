@@ -2,10 +2,18 @@
 // the most probable alternatives, and the gradient of the logits.
 //
 // One pass over a row.  With c = log2(e) / temperature and m the maximum so far, a thread keeps
-//   S0 = sum 2^(c (x - m)),  S1 = sum (x - m) 2^(c (x - m))
+//   S0 = sum 2^(c (x - m)),  S1 = sum c (x - m) 2^(c (x - m))
 // and rescales both when its maximum moves, once for a batch of vectors at most.  Parts are
 // joined the same way; then log p = (x - m) / temperature - ln S0 and the entropy is
-// ln S0 - S1 / S0 / temperature: nothing is subtracted that is large beside the result.
+// ln S0 - ln2 S1 / S0: nothing is subtracted that is large beside the result.
+//
+// At 8 instructions an element the pass was bound by their issue (2.8 TB/s).  So the exponents
+// come from one fused multiply-add on pairs, c x - r with r = c m rounded (what the rounding
+// leaves, c m - r, is known exactly and taken out of the sums at the end), and values far
+// below the maximum, -inf and NaN among them, are first raised to a finite one, in pairs of
+// 16-bit values, whose power of two is zero all the same.  Where that does not hold (nothing
+// but masked logits so far, or a maximum near the type's lowest value or past 2^60) the
+// exponents are taken one by one from the difference.
 //
 // Alternatives: a row's k-th highest value cannot be below the k-th highest of 32 disjoint
 // parts' maxima, which the pass has at hand; only threads whose own maximum reaches that
@@ -27,14 +35,14 @@
 namespace nvfp4 {
 namespace logprobs {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 384;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxTop = 32;
-constexpr int kCandidates = 512;   // one a thread when they are ranked
+constexpr int kCandidates = kThreads;  // one a thread when they are ranked
 constexpr int kMaxCluster = 8;
-constexpr float kCoolest = 1e-30f, kHottest = 1e30f;  // temperatures: c and kFar / c stay normal numbers
+constexpr float kCoolest = 1e-30f, kHottest = 1e30f;  // temperatures: c stays a normal number
 constexpr int kBatch = 4;          // vectors of a thread in flight
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kFar = -200.0f;    // 2^-200 is zero in fp32: where the exponents of masked logits are put
 
 __device__ __forceinline__ float ex2(float x) {
@@ -42,6 +50,84 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+
+// Pairs of fp32 values.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// The words of a vector.  floor: the finite value that -inf and NaN are raised to.
+template <typename T>
+struct Word {  // two 16-bit values
+    static constexpr float kFloor = std::is_same<T, __half>::value ? -65504.0f : -1e20f;
+    static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+        if constexpr (std::is_same<T, __half>::value) {
+            const __half2 r = __hmax2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b));
+            return *reinterpret_cast<const uint32_t *>(&r);
+        } else {
+            const __nv_bfloat162 r =
+                __hmax2(*reinterpret_cast<const __nv_bfloat162 *>(&a), *reinterpret_cast<const __nv_bfloat162 *>(&b));
+            return *reinterpret_cast<const uint32_t *>(&r);
+        }
+    }
+    // the maximum of a vector's values, NaN only if all are
+    static __device__ __forceinline__ uint32_t top(const uint4 &v) { return max2(max2(v.x, v.y), max2(v.z, v.w)); }
+    static __device__ __forceinline__ float top_value(uint32_t t) {
+        const float2 f = Type16<T>::unpack(t);
+        return fmaxf(f.x, f.y);
+    }
+    static __device__ __forceinline__ void raised(const uint4 &v, uint64_t (&p)[4]) {
+        const uint32_t floor = Type16<T>::pack(kFloor, kFloor), w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float2 f = Type16<T>::unpack(max2(w[i], floor));
+            p[i] = pair(f.x, f.y);
+        }
+    }
+    static constexpr int kPairs = 4;
+    static constexpr uint32_t kMasked = std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;  // -inf
+    static __device__ __forceinline__ uint32_t join(uint32_t a, uint32_t b) { return max2(a, b); }
+};
+template <>
+struct Word<float> {
+    static constexpr float kFloor = -1e20f;
+    static __device__ __forceinline__ uint32_t top(const uint4 &v) {
+        return __float_as_uint(fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)),
+                                     fmaxf(__uint_as_float(v.z), __uint_as_float(v.w))));
+    }
+    static __device__ __forceinline__ float top_value(uint32_t t) { return __uint_as_float(t); }
+    static __device__ __forceinline__ void raised(const uint4 &v, uint64_t (&p)[2]) {
+        p[0] = pair(fmaxf(__uint_as_float(v.x), kFloor), fmaxf(__uint_as_float(v.y), kFloor));
+        p[1] = pair(fmaxf(__uint_as_float(v.z), kFloor), fmaxf(__uint_as_float(v.w), kFloor));
+    }
+    static constexpr int kPairs = 2;
+    static constexpr uint32_t kMasked = 0xff800000u;
+    static __device__ __forceinline__ uint32_t join(uint32_t a, uint32_t b) {
+        return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+    }
+};
 
 template <typename T>
 constexpr int kVec = 16 / (int)sizeof(T);
@@ -67,6 +153,11 @@ __device__ __forceinline__ void unpack(const uint4 &v, float (&f)[kVec<T>]) {
     }
 }
 
+// Whether a value raised to `floor` has the power of two zero, and a finite exponent.
+__device__ __forceinline__ bool raises(float floor, float c, float r) {
+    return c < 1e6f && fmaf(floor, c, -r) < -150.0f;
+}
+
 // A row as 16-byte vectors at 16-byte addresses; the first and the last may reach past it.
 template <typename T>
 struct Row {
@@ -77,16 +168,30 @@ struct Row {
         : x(p), shift((int)((reinterpret_cast<uintptr_t>(p) & 15u) / sizeof(T))), n(len) {}
     __device__ __forceinline__ int vectors() const { return (int)(((int64_t)n + shift + kVec<T> - 1) / kVec<T>); }
     __device__ __forceinline__ int first(int v) const { return v * kVec<T> - shift; }  // may be negative
-    // -inf past the row's ends; its elements alone are read
-    __device__ __forceinline__ void load(int v, float (&f)[kVec<T>]) const {
-        const int e = first(v);
-        if (e >= 0 && e + kVec<T> <= n) {
-            unpack<T>(__ldg(reinterpret_cast<const uint4 *>(x + e)), f);
-        } else {
-#pragma unroll
-            for (int i = 0; i < kVec<T>; i++) f[i] = e + i >= 0 && e + i < n ? to_float<T>(x[e + i]) : -INFINITY;
-        }
+    // vectors [whole0(), whole1()) lie within the row
+    __device__ __forceinline__ int whole0() const { return shift ? 1 : 0; }
+    __device__ __forceinline__ int whole1() const { return (int)(((int64_t)n + shift) / kVec<T>); }
+    __device__ __forceinline__ uint4 whole(int v) const {
+        return __ldg(reinterpret_cast<const uint4 *>(x + first(v)));
     }
+    // -inf past the row's ends; its elements alone are read
+    __device__ __forceinline__ uint4 any(int v) const {
+        if (v >= whole0() && v < whole1()) return whole(v);
+        uint32_t w[4] = {Word<T>::kMasked, Word<T>::kMasked, Word<T>::kMasked, Word<T>::kMasked};
+        const int e = first(v);
+#pragma unroll
+        for (int i = 0; i < kVec<T>; i++)
+            if (e + i >= 0 && e + i < n) {
+                if constexpr (sizeof(T) == 4) {
+                    w[i] = __float_as_uint(x[e + i]);
+                } else {
+                    const uint32_t bits = reinterpret_cast<const uint16_t *>(x)[e + i];
+                    w[i / 2] = i & 1 ? (w[i / 2] & 0xffffu) | bits << 16 : (w[i / 2] & 0xffff0000u) | bits;
+                }
+            }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    __device__ __forceinline__ void load(int v, float (&f)[kVec<T>]) const { unpack<T>(any(v), f); }
 };
 
 struct Params {
@@ -94,7 +199,7 @@ struct Params {
     int64_t ld;
     int target8;       // targets are 64-bit
     int T, V, k;
-    float temperature, c, far;  // c = log2(e) / temperature, far = kFar / c
+    float temperature, c;  // c = log2(e) / temperature
     float *logprobs, *entropy, *top_logprobs, *lse;
     int *top_tokens;
 };
@@ -123,8 +228,8 @@ struct Stats {
 __device__ __forceinline__ Stats join(const Stats &a, const Stats &b, const Params &p) {
     Stats r;
     r.m = fmaxf(a.m, b.m);
-    const float da = fmaxf(a.m - r.m, p.far), db = fmaxf(b.m - r.m, p.far);
-    const float fa = ex2(da * p.c), fb = ex2(db * p.c);
+    const float da = fmaxf((a.m - r.m) * p.c, kFar), db = fmaxf((b.m - r.m) * p.c, kFar);
+    const float fa = ex2(da), fb = ex2(db);
     r.s0 = a.s0 * fa + b.s0 * fb;
     r.s1 = fmaf(a.s0, da, a.s1) * fa + fmaf(b.s0, db, b.s1) * fb;
     return r;
@@ -247,38 +352,97 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const Params p) {
             ignored = at < 0 || at >= p.V;
             if (!ignored) target = to_float<T>(row.x[at]);
         }
-        // ---- the pass
-        Stats a = {-INFINITY, 0.0f, 0.0f};
-        for (int64_t v = v0 + (int)threadIdx.x; v < v1; v += kBatch * kThreads) {
-            float f[kBatch][kVec<T>];
+        // ---- the pass: a batch of vectors in flight while the one before is added up
+        float m = -INFINITY, r = 0.0f, rest = 0.0f;  // r: c m rounded, rest: what that left
+        uint64_t s0[2] = {0, 0}, s1[2] = {0, 0};
+        bool paired = false;
+        auto add = [&](const uint4 (&raw)[kBatch]) {
+            uint32_t top = Word<T>::top(raw[0]);
 #pragma unroll
-            for (int b = 0; b < kBatch; b++) {
-                if (v + b * kThreads < v1) {
-                    row.load((int)(v + b * kThreads), f[b]);
+            for (int b = 1; b < kBatch; b++) top = Word<T>::join(top, Word<T>::top(raw[b]));
+            const float high = Word<T>::top_value(top);
+            if (high > m) {
+                const float r_next = high * p.c;
+                const bool pairs = raises(Word<T>::kFloor, p.c, r_next) && fabsf(r_next) < 0x1p60f;
+                const float rest_next = pairs ? fmaf(high, p.c, -r_next) : 0.0f;
+                const float d = fmaxf((m - high) * p.c, kFar) - rest + rest_next, scale = ex2(d);
+                const uint64_t dd = pair(d, d), ss = pair(scale, scale);
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    if (ENTROPY) s1[i] = mul2(fma2(s0[i], dd, s1[i]), ss);
+                    s0[i] = mul2(s0[i], ss);
+                }
+                m = high;
+                r = r_next;
+                rest = rest_next;
+                paired = pairs;
+            }
+            if (paired) {
+                const uint64_t cc = pair(p.c, p.c), rr = pair(-r, -r);
+#pragma unroll
+                for (int b = 0; b < kBatch; b++) {
+                    uint64_t x[Word<T>::kPairs];
+                    Word<T>::raised(raw[b], x);
+#pragma unroll
+                    for (int i = 0; i < Word<T>::kPairs; i++) {
+                        const uint64_t d = fma2(x[i], cc, rr);
+                        const float2 f = unpair(d);
+                        const uint64_t e = pair(ex2(f.x), ex2(f.y));
+                        s0[i & 1] = add2(s0[i & 1], e);
+                        if (ENTROPY) s1[i & 1] = fma2(d, e, s1[i & 1]);
+                    }
+                }
+            } else {
+                // fmaxf takes the bound where the difference is NaN, of two infinities or of a NaN
+                float t0 = 0.0f, t1 = 0.0f;
+#pragma unroll
+                for (int b = 0; b < kBatch; b++) {
+                    float f[kVec<T>];
+                    unpack<T>(raw[b], f);
+#pragma unroll
+                    for (int i = 0; i < kVec<T>; i++) {
+                        const float d = fmaxf((f[i] - m) * p.c, kFar), e = ex2(d);
+                        t0 += e;
+                        if (ENTROPY) t1 = fmaf(d, e, t1);
+                    }
+                }
+                s0[0] = add2(s0[0], pair(t0, 0.0f));
+                if (ENTROPY) s1[0] = add2(s1[0], pair(t1, 0.0f));
+            }
+        };
+        {
+            const int w0 = max(v0, row.whole0()), w1 = min(v1, row.whole1());
+            auto fetch = [&](int v, uint4 (&raw)[kBatch]) {
+                if (v >= w0 && v + (kBatch - 1) * kThreads < w1) {
+#pragma unroll
+                    for (int b = 0; b < kBatch; b++) raw[b] = row.whole(v + b * kThreads);
                 } else {
 #pragma unroll
-                    for (int i = 0; i < kVec<T>; i++) f[b][i] = -INFINITY;
+                    for (int b = 0; b < kBatch; b++)
+                        raw[b] = v + b * kThreads < v1 ? row.any(v + b * kThreads)
+                                                       : make_uint4(Word<T>::kMasked, Word<T>::kMasked,
+                                                                    Word<T>::kMasked, Word<T>::kMasked);
                 }
+            };
+            uint4 raw[kBatch], next[kBatch];
+            int v = v0 + (int)threadIdx.x;
+            if (v < v1) fetch(v, raw);
+            while (v < v1) {
+                const int after = v + kBatch * kThreads;  // below 2^31: a row has at most 2^29 vectors
+                if (after < v1) fetch(after, next);
+                add(raw);
+#pragma unroll
+                for (int b = 0; b < kBatch; b++) raw[b] = next[b];
+                v = after;
             }
-            float m = f[0][0];
-#pragma unroll
-            for (int b = 0; b < kBatch; b++)
-#pragma unroll
-                for (int i = 0; i < kVec<T>; i++) m = fmaxf(m, f[b][i]);
-            if (m > a.m) {
-                const float d = fmaxf(a.m - m, p.far), scale = ex2(d * p.c);
-                if (ENTROPY) a.s1 = fmaf(a.s0, d, a.s1) * scale;
-                a.s0 *= scale;
-                a.m = m;
-            }
-#pragma unroll
-            for (int b = 0; b < kBatch; b++)
-#pragma unroll
-                for (int i = 0; i < kVec<T>; i++) {
-                    const float d = fmaxf(f[b][i] - a.m, p.far), e = ex2(d * p.c);
-                    a.s0 += e;
-                    if (ENTROPY) a.s1 = fmaf(d, e, a.s1);
-                }
+        }
+        Stats a;
+        {
+            const float2 x = unpair(add2(s0[0], s0[1])), y = unpair(add2(s1[0], s1[1]));
+            const float sum0 = x.x + x.y, sum1 = y.x + y.y, back = ex2(-rest);
+            a.m = m;
+            a.s0 = sum0 * back;
+            a.s1 = ENTROPY ? fmaf(-rest, sum0, sum1) * back : 0.0f;
         }
         // ---- statistics of the CTA
         if (TOP) s.best[threadIdx.x] = a.m;
@@ -302,7 +466,20 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const Params p) {
                         const bool high = ((lane & o) == 0) == ((lane & size) == 0);  // descending overall
                         b = high ? fmaxf(b, other) : fminf(b, other);
                     }
+                float high = __shfl_sync(0xffffffffu, b, 0);
                 b = __shfl_sync(0xffffffffu, b, p.k - 1);
+                // of many alternatives the columns' bound is loose: halve the way up to the maximum while
+                // k threads' maxima still reach it
+                if (p.k > 8 && b > -INFINITY)
+                    for (int i = 0; i < 7; i++) {
+                        const float mid = 0.5f * b + 0.5f * high;
+                        int n = 0;
+#pragma unroll
+                        for (int w = 0; w < kWarps; w++) n += s.best[w * 32 + lane] >= mid;
+                        n = __reduce_add_sync(0xffffffffu, n);
+                        if (n >= p.k) b = mid;
+                        else high = mid;
+                    }
                 if (lane == 0) s.bound = b;
             }
             __syncthreads();
@@ -359,7 +536,7 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const Params p) {
                 const bool none = !(target > -INFINITY);
                 p.lse[t] = empty ? -INFINITY : all.m / p.temperature + l;
                 p.logprobs[t] = ignored ? 0.0f : empty || none ? -INFINITY : (target - all.m) / p.temperature - l;
-                if (ENTROPY) p.entropy[t] = empty ? 0.0f : l - all.s1 / all.s0 / p.temperature;
+                if (ENTROPY) p.entropy[t] = empty ? 0.0f : l - all.s1 / all.s0 * kLn2;
             }
             if (TOP) {
                 int n = s.n_top;
@@ -429,12 +606,23 @@ __global__ void __launch_bounds__(kGradThreads) logprobs_grad_kernel(const GradP
     const float H = p.dentropy ? p.entropy[t] : 0.0f;
     const float lse = p.lse[t];
     const float a = fmaf(h, H, g);  // d = -p (g + h H + h log p)
-    auto grad = [&](float v, int64_t e) {
+    // Away from the target in pairs, from log2 p = c x - c lse: -inf and NaN are raised as in the
+    // forward pass, where that leaves them at zero and log p is more than rounding.
+    const float c = p.inv_temperature * kLog2e, lse2 = lse * kLog2e, b = -h * kLn2;
+    const bool paired = fabsf(lse) < 1e4f && raises(Word<T>::kFloor, c, lse2);
+    const uint64_t cc = pair(c, c), ll = pair(-lse2, -lse2), aa = pair(-a, -a), bb = pair(b, b);
+    auto grad = [&](float v, int64_t e) {  // one element, the same bits
         if (e >= p.V || !(v > -INFINITY)) return 0.0f;
-        float l = fmaf(v, p.inv_temperature, -lse);
-        l = l > 0.0f ? 0.0f : l;  // of logits past 2^24 nothing but their rounding is left: p stays below 1
-        const float q = ex2(l * kLog2e);
-        const float y = q == 0.0f ? 0.0f : -q * fmaf(h, l, a);
+        float y;
+        if (paired) {
+            const float l = fmaf(fmaxf(v, Word<T>::kFloor), c, -lse2);
+            y = ex2(l) * fmaf(b, l, -a);
+        } else {
+            float l = fmaf(v, p.inv_temperature, -lse);
+            l = l > 0.0f ? 0.0f : l;  // of logits past 2^24 nothing but their rounding is left: p stays below 1
+            const float q = ex2(l * kLog2e);
+            y = q == 0.0f ? 0.0f : -q * fmaf(h, l, a);
+        }
         return e == target ? y + g : y;
     };
     auto put = [](float v) {
@@ -459,9 +647,22 @@ __global__ void __launch_bounds__(kGradThreads) logprobs_grad_kernel(const GradP
             const int64_t e = v * kVec<T> - row.shift;
             if (e >= 0 && e + kVec<T> <= p.W) {
                 float f[kVec<T>];
-                unpack<T>(raw[i], f);
+                if (paired && e + kVec<T> <= p.V && (target < e || target >= e + kVec<T>)) {
+                    uint64_t w[Word<T>::kPairs];
+                    Word<T>::raised(raw[i], w);
 #pragma unroll
-                for (int j = 0; j < kVec<T>; j++) f[j] = grad(f[j], e + j);
+                    for (int j = 0; j < Word<T>::kPairs; j++) {
+                        const uint64_t l = fma2(w[j], cc, ll);
+                        const float2 x = unpair(l);
+                        const float2 y = unpair(mul2(pair(ex2(x.x), ex2(x.y)), fma2(bb, l, aa)));
+                        f[2 * j] = y.x;
+                        f[2 * j + 1] = y.y;
+                    }
+                } else {
+                    unpack<T>(raw[i], f);
+#pragma unroll
+                    for (int j = 0; j < kVec<T>; j++) f[j] = grad(f[j], e + j);
+                }
                 uint4 o;
                 if constexpr (sizeof(T) == 4)
                     o = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
@@ -579,7 +780,6 @@ int nvfp4_token_logprobs(const void *logits, int64_t ld, int dtype, const void *
     p.k = top_k;
     p.temperature = temperature;
     p.c = logprobs::kLog2e / temperature;
-    p.far = logprobs::kFar / p.c;
     p.logprobs = logprobs;
     p.entropy = entropy;
     p.top_logprobs = top_logprobs;
