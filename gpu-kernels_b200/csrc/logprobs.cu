@@ -16,8 +16,8 @@
 // exponents are taken one by one from the difference.
 //
 // Alternatives: a row's k-th highest value cannot be below the k-th highest of 32 disjoint
-// parts' maxima, which the pass has at hand; only threads whose own maximum reaches that
-// bound can hold a candidate, so a few percent of the row are read again (from L2), and the
+// parts' maxima, which the pass has at hand; only quarters of a thread's vectors whose maximum
+// reaches that bound can hold a candidate, so a percent of the row is read again, and the
 // candidates are ranked by counting.  The rare row with more candidates than are kept (long
 // runs of equal logits) takes rounds of "highest value, lowest tokens first".
 //
@@ -35,11 +35,13 @@
 namespace nvfp4 {
 namespace logprobs {
 
-constexpr int kThreads = 384;
+constexpr int kThreads = 256;
+constexpr int kResident = 3;       // CTAs an SM
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxTop = 32;
 constexpr int kCandidates = kThreads;  // one a thread when they are ranked
 constexpr int kMaxCluster = 8;
+constexpr int kQuarters = 4;         // of a thread's vectors, each with its maximum
 constexpr float kCoolest = 1e-30f, kHottest = 1e30f;  // temperatures: c stays a normal number
 constexpr int kBatch = 4;          // vectors of a thread in flight
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -259,10 +261,9 @@ struct Shared {
     uint64_t cand[kCandidates];
     uint64_t top[kMaxTop];        // this CTA's alternatives, highest first
     Stats part[kWarps];
-    float best[kThreads];         // the threads' maxima
-    int winners[kThreads];
+    float best[kQuarters][kThreads];  // the maxima of quarters of the threads' vectors
+    int winners[kQuarters * kThreads];
     int count[kWarps + 1];
-    float bound;
     int n_winners, n_cand, n_top;
 };
 
@@ -271,6 +272,7 @@ __device__ __forceinline__ void rank_keys(const uint64_t *keys, int n, int k, ui
     if ((int)threadIdx.x < n) {
         const uint64_t mine = keys[threadIdx.x];
         int rank = 0;
+#pragma unroll 8
         for (int j = 0; j < n; j++) rank += keys[j] > mine;
         if (rank < k) out[rank] = mine;
     }
@@ -337,14 +339,37 @@ __device__ __noinline__ void select_rounds(const Row<T> &row, int v0, int v1, in
 }
 
 template <typename T, bool ENTROPY, bool TOP>
-__global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, kResident) logprobs_kernel(const Params p) {
     __shared__ Shared s;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int parts = (int)cluster_size(), part = (int)cluster_ctarank();
-    for (int64_t t = blockIdx.x / parts; t < p.T; t += gridDim.x / parts) {
-        const Row<T> row(static_cast<const T *>(p.logits) + t * p.ld, p.V);
-        const int nv = row.vectors();
-        const int v0 = (int)((int64_t)nv * part / parts), v1 = (int)((int64_t)nv * (part + 1) / parts);
+    auto row_at = [&](int64_t t) { return Row<T>(static_cast<const T *>(p.logits) + t * p.ld, p.V); };
+    auto from = [&](const Row<T> &row, int part) { return (int)((int64_t)row.vectors() * part / parts); };
+    // a batch from v on of the row's vectors v0 .. v1
+    auto fetch = [&](const Row<T> &row, int v0, int v1, int v, uint4 (&raw)[kBatch]) {
+        if (v >= max(v0, row.whole0()) && v + (kBatch - 1) * kThreads < min(v1, row.whole1())) {
+#pragma unroll
+            for (int b = 0; b < kBatch; b++) raw[b] = row.whole(v + b * kThreads);
+        } else {
+#pragma unroll
+            for (int b = 0; b < kBatch; b++)
+                raw[b] = v + b * kThreads < v1
+                             ? row.any(v + b * kThreads)
+                             : make_uint4(Word<T>::kMasked, Word<T>::kMasked, Word<T>::kMasked, Word<T>::kMasked);
+        }
+    };
+    uint4 raw[kBatch];  // the next batch; a row's first is fetched before the last one is finished
+    auto fetch_first = [&](int64_t t) {
+        if (t >= p.T) return;
+        const Row<T> row = row_at(t);
+        const int v0 = from(row, part), v1 = from(row, part + 1), v = v0 + (int)threadIdx.x;
+        if (v < v1) fetch(row, v0, v1, v, raw);
+    };
+    const int64_t step = gridDim.x / parts;
+    fetch_first(blockIdx.x / parts);
+    for (int64_t t = blockIdx.x / parts; t < p.T; t += step) {
+        const Row<T> row = row_at(t);
+        const int v0 = from(row, part), v1 = from(row, part + 1);
         float target = -INFINITY;
         bool ignored = true;
         if (part == 0 && threadIdx.x == 0) {
@@ -356,11 +381,14 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const Params p) {
         float m = -INFINITY, r = 0.0f, rest = 0.0f;  // r: c m rounded, rest: what that left
         uint64_t s0[2] = {0, 0}, s1[2] = {0, 0};
         bool paired = false;
+        const int quarter = max(1, ((v1 - v0 + kBatch * kThreads - 1) / (kBatch * kThreads) + kQuarters - 1) / kQuarters);
+        float high_quarter = -INFINITY;
         auto add = [&](const uint4 (&raw)[kBatch]) {
             uint32_t top = Word<T>::top(raw[0]);
 #pragma unroll
             for (int b = 1; b < kBatch; b++) top = Word<T>::join(top, Word<T>::top(raw[b]));
             const float high = Word<T>::top_value(top);
+            if (TOP) high_quarter = fmaxf(high_quarter, high);
             if (high > m) {
                 const float r_next = high * p.c;
                 const bool pairs = raises(Word<T>::kFloor, p.c, r_next) && fabsf(r_next) < 0x1p60f;
@@ -411,30 +439,26 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const Params p) {
             }
         };
         {
-            const int w0 = max(v0, row.whole0()), w1 = min(v1, row.whole1());
-            auto fetch = [&](int v, uint4 (&raw)[kBatch]) {
-                if (v >= w0 && v + (kBatch - 1) * kThreads < w1) {
-#pragma unroll
-                    for (int b = 0; b < kBatch; b++) raw[b] = row.whole(v + b * kThreads);
-                } else {
-#pragma unroll
-                    for (int b = 0; b < kBatch; b++)
-                        raw[b] = v + b * kThreads < v1 ? row.any(v + b * kThreads)
-                                                       : make_uint4(Word<T>::kMasked, Word<T>::kMasked,
-                                                                    Word<T>::kMasked, Word<T>::kMasked);
-                }
-            };
-            uint4 raw[kBatch], next[kBatch];
-            int v = v0 + (int)threadIdx.x;
-            if (v < v1) fetch(v, raw);
+            uint4 next[kBatch];
+            int v = v0 + (int)threadIdx.x, left = quarter;
+            float *best = &s.best[0][threadIdx.x];
             while (v < v1) {
                 const int after = v + kBatch * kThreads;  // below 2^31: a row has at most 2^29 vectors
-                if (after < v1) fetch(after, next);
+                if (after < v1) fetch(row, v0, v1, after, next);
                 add(raw);
+                if (TOP && (--left == 0 || after >= v1)) {
+                    *best = high_quarter;
+                    best += kThreads;
+                    high_quarter = -INFINITY;
+                    left = quarter;
+                }
 #pragma unroll
                 for (int b = 0; b < kBatch; b++) raw[b] = next[b];
                 v = after;
             }
+            if (TOP)
+                for (; best < &s.best[kQuarters][0]; best += kThreads) *best = -INFINITY;
+            fetch_first(t + step);
         }
         Stats a;
         {
@@ -445,7 +469,6 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const Params p) {
             a.s1 = ENTROPY ? fmaf(-rest, sum0, sum1) * back : 0.0f;
         }
         // ---- statistics of the CTA
-        if (TOP) s.best[threadIdx.x] = a.m;
         Stats w = a;
 #pragma unroll
         for (int o = 16; o; o >>= 1) w = join(w, shuffle(w, o), p);
@@ -454,42 +477,54 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const Params p) {
         __syncthreads();
         if (TOP) {
             // ---- candidates: the lanes' columns of maxima, sorted; the k-th is the bound
-            if (warp == 0) {
-                float b = -INFINITY;
+            float b = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < kWarps; i++) b = fmaxf(b, s.best[i * 32 + lane]);
+            for (int i = 0; i < kQuarters; i++)
 #pragma unroll
-                for (int size = 2; size <= 32; size <<= 1)
+                for (int w = 0; w < kWarps; w++) b = fmaxf(b, s.best[i][w * 32 + lane]);
 #pragma unroll
-                    for (int o = size >> 1; o; o >>= 1) {
-                        const float other = __shfl_xor_sync(0xffffffffu, b, o);
-                        const bool high = ((lane & o) == 0) == ((lane & size) == 0);  // descending overall
-                        b = high ? fmaxf(b, other) : fminf(b, other);
+            for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+                for (int o = size >> 1; o; o >>= 1) {
+                    const float other = __shfl_xor_sync(0xffffffffu, b, o);
+                    const bool high = ((lane & o) == 0) == ((lane & size) == 0);  // descending overall
+                    b = high ? fmaxf(b, other) : fminf(b, other);
+                }
+            float bound = __shfl_sync(0xffffffffu, b, p.k - 1), high = __shfl_sync(0xffffffffu, b, 0);
+            // of many alternatives the columns' bound is loose: while more than twice as many quarters as
+            // there are alternatives reach it, halve the way up to the maximum, as far as enough still do
+            auto reached = [&](float v) {
+                int n = 0;
+#pragma unroll
+                for (int j = 0; j < kQuarters; j++)
+#pragma unroll
+                    for (int w = 0; w < kWarps; w++) n += s.best[j][w * 32 + lane] >= v;
+                return __reduce_add_sync(0xffffffffu, n);
+            };
+            if (bound > -INFINITY) {
+                int n = p.k > 8 ? reached(bound) : 0;
+                for (int i = 0; i < 6 && n > 2 * p.k; i++) {
+                    const float mid = 0.5f * bound + 0.5f * high;
+                    const int at = reached(mid);
+                    if (at >= p.k) {
+                        bound = mid;
+                        n = at;
+                    } else {
+                        high = mid;
                     }
-                float high = __shfl_sync(0xffffffffu, b, 0);
-                b = __shfl_sync(0xffffffffu, b, p.k - 1);
-                // of many alternatives the columns' bound is loose: halve the way up to the maximum while
-                // k threads' maxima still reach it
-                if (p.k > 8 && b > -INFINITY)
-                    for (int i = 0; i < 7; i++) {
-                        const float mid = 0.5f * b + 0.5f * high;
-                        int n = 0;
+                }
+            }
 #pragma unroll
-                        for (int w = 0; w < kWarps; w++) n += s.best[w * 32 + lane] >= mid;
-                        n = __reduce_add_sync(0xffffffffu, n);
-                        if (n >= p.k) b = mid;
-                        else high = mid;
-                    }
-                if (lane == 0) s.bound = b;
+            for (int i = 0; i < kQuarters; i++) {
+                const float mine = s.best[i][threadIdx.x];
+                if (mine > -INFINITY && mine >= bound)
+                    s.winners[atomicAdd(&s.n_winners, 1)] = i * kThreads + (int)threadIdx.x;
             }
             __syncthreads();
-            const float bound = s.bound;
-            if (a.m > -INFINITY && a.m >= bound) s.winners[atomicAdd(&s.n_winners, 1)] = (int)threadIdx.x;
-            __syncthreads();
-            const int per = (v1 - v0 + kThreads - 1) / kThreads;  // vectors of a thread, at most
+            const int per = quarter * kBatch;  // vectors of a quarter, at most
             const int all = s.n_winners * per;
             for (int i = threadIdx.x; i < all; i += kThreads) {
-                const int v = v0 + s.winners[i / per] + i % per * kThreads;
+                const int w = s.winners[i / per], v = v0 + w % kThreads + (w / kThreads * per + i % per) * kThreads;
                 if (v >= v1) continue;
                 float f[kVec<T>];
                 row.load(v, f);
@@ -539,25 +574,35 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const Params p) {
                 if (ENTROPY) p.entropy[t] = empty ? 0.0f : l - all.s1 / all.s0 * kLn2;
             }
             if (TOP) {
-                int n = s.n_top;
+                int n = s.n_top;  // of this CTA
                 if (parts > 1) {
-                    // candidates have been ranked: their place takes the parts' alternatives
-                    if ((int)threadIdx.x < parts * kMaxTop) {
-                        const int q = threadIdx.x / kMaxTop, j = threadIdx.x % kMaxTop;
-                        const int have = (int)__float_as_int(ld_cluster_f32(map_to_cta(smem_u32(&s.n_top), q)));
-                        s.cand[threadIdx.x] = j < have ? ld_cluster_u64(map_to_cta(smem_u32(&s.top[j]), q))
-                                                       : (uint64_t)(kMaxCluster * kMaxTop - threadIdx.x - 1);  // below all
+                    // the candidates have been ranked: their place takes the parts' lists; a key's rank is
+                    // the number of keys above it in all of them
+                    const int q = threadIdx.x / kMaxTop, j = threadIdx.x % kMaxTop;
+                    uint64_t mine = 0;
+                    if (q < parts) {
+                        const int have = __float_as_int(ld_cluster_f32(map_to_cta(smem_u32(&s.n_top), q)));
+                        if (j == 0) s.winners[q] = have;
+                        if (j < have) s.cand[threadIdx.x] = mine = ld_cluster_u64(map_to_cta(smem_u32(&s.top[j]), q));
                     }
+                    __syncthreads();
                     n = 0;
-                    for (int q = 0; q < parts; q++)
-                        n += (int)__float_as_int(ld_cluster_f32(map_to_cta(smem_u32(&s.n_top), q)));
+                    for (int o = 0; o < parts; o++) n += s.winners[o];
                     n = min(n, p.k);
-                    __syncthreads();
-                    // ranked into the other half, since s.top may still be read as a part
-                    uint64_t *merged = s.cand + kMaxCluster * kMaxTop;
-                    rank_keys(s.cand, parts * kMaxTop, p.k, merged);
-                    __syncthreads();
-                    if ((int)threadIdx.x < n) s.top[threadIdx.x] = merged[threadIdx.x];
+                    int above[kMaxCluster] = {};  // in each list, by halving steps, the lists side by side
+                    if (mine)
+#pragma unroll
+                        for (int step = kMaxTop; step; step >>= 1)
+#pragma unroll
+                            for (int o = 0; o < kMaxCluster; o++)
+                                if (o < parts && above[o] + step <= s.winners[o] &&
+                                    s.cand[o * kMaxTop + above[o] + step - 1] > mine)
+                                    above[o] += step;
+                    int rank = 0;
+#pragma unroll
+                    for (int o = 0; o < kMaxCluster; o++) rank += above[o];
+                    __syncthreads();  // every list has been read
+                    if (mine && rank < p.k) s.top[rank] = mine;
                     __syncthreads();
                 }
                 if (warp == 0 && lane < p.k) {
@@ -703,7 +748,7 @@ static int launch(const Params &p, const DeviceInfo &di, cudaStream_t s) {
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = parts;
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.gridDim = dim3((unsigned)(parts == 1 ? std::min<int64_t>(p.T, 2 * di.sm_count) : p.T * parts));
+    cfg.gridDim = dim3((unsigned)(parts == 1 ? std::min<int64_t>(p.T, kResident * di.sm_count) : p.T * parts));
     cfg.blockDim = dim3(kThreads);
     cfg.stream = s;
     cfg.attrs = &attr;
