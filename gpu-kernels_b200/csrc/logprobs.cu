@@ -15,6 +15,9 @@
 // but masked logits so far, or a maximum near the type's lowest value or past 2^60) the
 // exponents are taken one by one from the difference.
 //
+// A warp of its own copies the rows through a ring in shared memory, in bulk copies of 16 KB, and
+// runs on into the next row while the others finish this one.
+//
 // Alternatives: a row's k-th highest value cannot be below the k-th highest of 32 disjoint
 // parts' maxima, which the pass has at hand; only quarters of a thread's vectors whose maximum
 // reaches that bound can hold a candidate, so a percent of the row is read again, and the
@@ -24,6 +27,7 @@
 // A row is one CTA's, or is cut between the CTAs of a cluster when there are few rows; the
 // parts meet in distributed shared memory.  Every sum has a fixed order.
 #include <algorithm>
+#include <atomic>
 #include <climits>
 #include <cmath>
 #include <type_traits>
@@ -37,13 +41,14 @@ namespace logprobs {
 
 constexpr int kThreads = 256;
 constexpr int kResident = 3;       // CTAs an SM
+constexpr int kRing = 4;           // chunks of kBatch vectors a thread
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxTop = 32;
 constexpr int kCandidates = kThreads;  // one a thread when they are ranked
 constexpr int kMaxCluster = 8;
 constexpr int kQuarters = 4;         // of a thread's vectors, each with its maximum
 constexpr float kCoolest = 1e-30f, kHottest = 1e30f;  // temperatures: c stays a normal number
-constexpr int kBatch = 4;          // vectors of a thread in flight
+constexpr int kBatch = 4;          // vectors of a thread added up together
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kFar = -200.0f;    // 2^-200 is zero in fp32: where the exponents of masked logits are put
 
@@ -204,6 +209,7 @@ struct Params {
     float temperature, c;  // c = log2(e) / temperature
     float *logprobs, *entropy, *top_logprobs, *lse;
     int *top_tokens;
+    KernelCtl ctl;
 };
 
 __device__ __forceinline__ int64_t target_of(const void *targets, int wide, int64_t t) {
@@ -239,6 +245,12 @@ __device__ __forceinline__ Stats join(const Stats &a, const Stats &b, const Para
 __device__ __forceinline__ Stats shuffle(const Stats &a, int o) {
     return {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s0, o),
             __shfl_xor_sync(0xffffffffu, a.s1, o)};
+}
+
+// Barrier of the threads that add up, without the one that copies.
+__device__ __forceinline__ void sync_adders() {
+    __syncwarp();  // .aligned
+    asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
 }
 
 __device__ __forceinline__ uint32_t cluster_size() {
@@ -296,9 +308,9 @@ __device__ __noinline__ void select_rounds(const Row<T> &row, int v0, int v1, in
             }
         }
         best = __reduce_max_sync(0xffffffffu, best);
-        __syncthreads();
+        sync_adders();
         if (lane == 0) s.count[warp] = best;
-        __syncthreads();
+        sync_adders();
         for (int w = 0; w < kWarps; w++) best = max(best, s.count[w]);
         if (best == INT_MIN) break;
         for (int base = v0; base < v1 && have < k; base += kThreads) {
@@ -316,9 +328,9 @@ __device__ __noinline__ void select_rounds(const Row<T> &row, int v0, int v1, in
                 const int u = __shfl_up_sync(0xffffffffu, before, o);
                 if (lane >= o) before += u;
             }
-            __syncthreads();  // the counts of the round before have been read
+            sync_adders();  // the counts of the round before have been read
             if (lane == 31) s.count[warp] = before;
-            __syncthreads();
+            sync_adders();
             int at = have + before - n, total = 0;
             for (int w = 0; w < kWarps; w++) {
                 if (w < warp) at += s.count[w];
@@ -339,35 +351,73 @@ __device__ __noinline__ void select_rounds(const Row<T> &row, int v0, int v1, in
 }
 
 template <typename T, bool ENTROPY, bool TOP>
-__global__ void __launch_bounds__(kThreads, kResident) logprobs_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads + 32, kResident) logprobs_kernel(const Params p) {
+    constexpr int kChunk = kBatch * kThreads;  // vectors
+    extern __shared__ __align__(16) uint4 ring[];  // [kRing][kChunk]
     __shared__ Shared s;
+    __shared__ uint64_t bars[2 * kRing];
+    __shared__ int abort_word;
+    volatile int *abort_flag = &abort_word;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int parts = (int)cluster_size(), part = (int)cluster_ctarank();
+    const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * kRing;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kRing; i++) {
+            mbar_init(bar_full + 8 * i, 1);
+            mbar_init(bar_empty + 8 * i, kWarps);
+        }
+        abort_word = 0;
+        fence_barrier_init();
+    }
+    __syncthreads();
     auto row_at = [&](int64_t t) { return Row<T>(static_cast<const T *>(p.logits) + t * p.ld, p.V); };
     auto from = [&](const Row<T> &row, int part) { return (int)((int64_t)row.vectors() * part / parts); };
-    // a batch from v on of the row's vectors v0 .. v1
-    auto fetch = [&](const Row<T> &row, int v0, int v1, int v, uint4 (&raw)[kBatch]) {
-        if (v >= max(v0, row.whole0()) && v + (kBatch - 1) * kThreads < min(v1, row.whole1())) {
-#pragma unroll
-            for (int b = 0; b < kBatch; b++) raw[b] = row.whole(v + b * kThreads);
-        } else {
-#pragma unroll
-            for (int b = 0; b < kBatch; b++)
-                raw[b] = v + b * kThreads < v1
-                             ? row.any(v + b * kThreads)
-                             : make_uint4(Word<T>::kMasked, Word<T>::kMasked, Word<T>::kMasked, Word<T>::kMasked);
+    const int64_t first = blockIdx.x / parts, step = gridDim.x / parts;
+    int slot = 0, phase = 0;  // of the ring
+    auto pass_slot = [&] {
+        if (++slot == kRing) {
+            slot = 0;
+            phase ^= 1;
         }
     };
-    uint4 raw[kBatch];  // the next batch; a row's first is fetched before the last one is finished
-    auto fetch_first = [&](int64_t t) {
-        if (t >= p.T) return;
-        const Row<T> row = row_at(t);
-        const int v0 = from(row, part), v1 = from(row, part + 1), v = v0 + (int)threadIdx.x;
-        if (v < v1) fetch(row, v0, v1, v, raw);
-    };
-    const int64_t step = gridDim.x / parts;
-    fetch_first(blockIdx.x / parts);
-    for (int64_t t = blockIdx.x / parts; t < p.T; t += step) {
+    if (warp == kWarps) {
+        // ---- copies: the whole vectors of the rows, chunk by chunk
+        if (lane == 0) {
+            uint32_t issued = 0, issued_phase = 0;
+            bool ok = true;
+            for (int64_t t = first; ok && t < p.T; t += step) {
+                const Row<T> row = row_at(t);
+                const int v0 = from(row, part), v1 = from(row, part + 1);
+                for (int v = v0; v < v1; v += kChunk) {
+                    if (!wait_parity(bar_empty + 8 * slot, phase ^ 1, p.ctl.wait_timeout_ns, abort_flag)) {
+                        report_timeout(abort_flag, p.ctl.status);
+                        ok = false;
+                        break;
+                    }
+                    const int a = max(v, row.whole0()), b = min(min(v + kChunk, v1), row.whole1());
+                    if (a < b) {
+                        const uint32_t bytes = (uint32_t)(b - a) * 16;
+                        mbar_arrive_expect_tx(bar_full + 8 * slot, bytes);
+                        issued |= 1u << slot;
+                        issued_phase = (issued_phase & ~(1u << slot)) | ((uint32_t)phase << slot);
+                        bulk_load(smem_u32(ring + slot * kChunk + (a - v)), row.x + row.first(a), bytes,
+                                  bar_full + 8 * slot);
+                    } else {
+                        mbar_arrive(bar_full + 8 * slot);
+                    }
+                    pass_slot();
+                }
+            }
+            if (!ok) {  // let the copies in flight land before the memory goes
+                volatile int never = 0;
+                for (int i = 0; i < kRing; i++)
+                    if (issued & (1u << i))
+                        wait_parity(bar_full + 8 * i, (issued_phase >> i) & 1, p.ctl.drain_timeout_ns, &never);
+            }
+        }
+        return;
+    }
+    for (int64_t t = first; t < p.T; t += step) {
         const Row<T> row = row_at(t);
         const int v0 = from(row, part), v1 = from(row, part + 1);
         float target = -INFINITY;
@@ -377,7 +427,7 @@ __global__ void __launch_bounds__(kThreads, kResident) logprobs_kernel(const Par
             ignored = at < 0 || at >= p.V;
             if (!ignored) target = to_float<T>(row.x[at]);
         }
-        // ---- the pass: a batch of vectors in flight while the one before is added up
+        // ---- the pass
         float m = -INFINITY, r = 0.0f, rest = 0.0f;  // r: c m rounded, rest: what that left
         uint64_t s0[2] = {0, 0}, s1[2] = {0, 0};
         bool paired = false;
@@ -439,26 +489,39 @@ __global__ void __launch_bounds__(kThreads, kResident) logprobs_kernel(const Par
             }
         };
         {
-            uint4 next[kBatch];
-            int v = v0 + (int)threadIdx.x, left = quarter;
+            int left = quarter;
             float *best = &s.best[0][threadIdx.x];
-            while (v < v1) {
-                const int after = v + kBatch * kThreads;  // below 2^31: a row has at most 2^29 vectors
-                if (after < v1) fetch(row, v0, v1, after, next);
+            const int w0 = row.whole0(), w1 = min(v1, row.whole1());
+            for (int v = v0 + (int)threadIdx.x; v - (int)threadIdx.x < v1; v += kChunk) {
+                // after a wait that gave up the sums are of anything, and the status says so
+                if (!wait_parity(bar_full + 8 * slot, phase, p.ctl.wait_timeout_ns, abort_flag))
+                    report_timeout(abort_flag, p.ctl.status);
+                uint4 raw[kBatch];
+                if (v >= w0 && v + (kBatch - 1) * kThreads < w1) {
+#pragma unroll
+                    for (int b = 0; b < kBatch; b++) raw[b] = ring[slot * kChunk + b * kThreads + threadIdx.x];
+                } else {
+#pragma unroll
+                    for (int b = 0; b < kBatch; b++) {
+                        const int at = v + b * kThreads;
+                        if (at >= w0 && at < w1) raw[b] = ring[slot * kChunk + b * kThreads + threadIdx.x];
+                        else if (at < v1) raw[b] = row.any(at);
+                        else raw[b] = make_uint4(Word<T>::kMasked, Word<T>::kMasked, Word<T>::kMasked, Word<T>::kMasked);
+                    }
+                }
                 add(raw);
-                if (TOP && (--left == 0 || after >= v1)) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar_empty + 8 * slot);
+                pass_slot();
+                if (TOP && (--left == 0 || v - (int)threadIdx.x + kChunk >= v1)) {
                     *best = high_quarter;
                     best += kThreads;
                     high_quarter = -INFINITY;
                     left = quarter;
                 }
-#pragma unroll
-                for (int b = 0; b < kBatch; b++) raw[b] = next[b];
-                v = after;
             }
             if (TOP)
                 for (; best < &s.best[kQuarters][0]; best += kThreads) *best = -INFINITY;
-            fetch_first(t + step);
         }
         Stats a;
         {
@@ -474,7 +537,7 @@ __global__ void __launch_bounds__(kThreads, kResident) logprobs_kernel(const Par
         for (int o = 16; o; o >>= 1) w = join(w, shuffle(w, o), p);
         if (lane == 0) s.part[warp] = w;
         if (threadIdx.x == 0) s.n_winners = s.n_cand = s.n_top = 0;
-        __syncthreads();
+        sync_adders();
         if (TOP) {
             // ---- candidates: the lanes' columns of maxima, sorted; the k-th is the bound
             float b = -INFINITY;
@@ -520,7 +583,7 @@ __global__ void __launch_bounds__(kThreads, kResident) logprobs_kernel(const Par
                 if (mine > -INFINITY && mine >= bound)
                     s.winners[atomicAdd(&s.n_winners, 1)] = i * kThreads + (int)threadIdx.x;
             }
-            __syncthreads();
+            sync_adders();
             const int per = quarter * kBatch;  // vectors of a quarter, at most
             const int all = s.n_winners * per;
             for (int i = threadIdx.x; i < all; i += kThreads) {
@@ -535,7 +598,7 @@ __global__ void __launch_bounds__(kThreads, kResident) logprobs_kernel(const Par
                         if (at < kCandidates) s.cand[at] = pair_key(f[e], row.first(v) + e);
                     }
             }
-            __syncthreads();
+            sync_adders();
             const int n = s.n_cand;
             if (n <= kCandidates) {
                 rank_keys(s.cand, n, p.k, s.top);
@@ -549,7 +612,7 @@ __global__ void __launch_bounds__(kThreads, kResident) logprobs_kernel(const Par
             __syncwarp();
             cluster_sync();
         } else if (TOP) {
-            __syncthreads();
+            sync_adders();
         }
         if (part == 0) {
             Stats all = {-INFINITY, 0.0f, 0.0f};
@@ -585,7 +648,7 @@ __global__ void __launch_bounds__(kThreads, kResident) logprobs_kernel(const Par
                         if (j == 0) s.winners[q] = have;
                         if (j < have) s.cand[threadIdx.x] = mine = ld_cluster_u64(map_to_cta(smem_u32(&s.top[j]), q));
                     }
-                    __syncthreads();
+                    sync_adders();
                     n = 0;
                     for (int o = 0; o < parts; o++) n += s.winners[o];
                     n = min(n, p.k);
@@ -601,9 +664,9 @@ __global__ void __launch_bounds__(kThreads, kResident) logprobs_kernel(const Par
                     int rank = 0;
 #pragma unroll
                     for (int o = 0; o < kMaxCluster; o++) rank += above[o];
-                    __syncthreads();  // every list has been read
+                    sync_adders();  // every list has been read
                     if (mine && rank < p.k) s.top[rank] = mine;
-                    __syncthreads();
+                    sync_adders();
                 }
                 if (warp == 0 && lane < p.k) {
                     const int64_t at = t * p.k + lane;
@@ -617,7 +680,7 @@ __global__ void __launch_bounds__(kThreads, kResident) logprobs_kernel(const Par
             __syncwarp();
             cluster_sync();  // the first CTA has read the others' parts
         } else {
-            __syncthreads();
+            sync_adders();
         }
     }
 }
@@ -743,13 +806,22 @@ static int parts_of(int T, int64_t vectors, int sm_count) {
 template <typename T, bool ENTROPY, bool TOP>
 static int launch(const Params &p, const DeviceInfo &di, cudaStream_t s) {
     const int parts = parts_of(p.T, p.V / kVec<T>, di.sm_count);
+    const int ring = kRing * kBatch * kThreads * (int)sizeof(uint4);
+    static std::atomic<bool> configured[64] = {};
+    if (!configured[di.device].load(std::memory_order_acquire)) {
+        if (cudaFuncSetAttribute(logprobs_kernel<T, ENTROPY, TOP>, cudaFuncAttributeMaxDynamicSharedMemorySize, ring) !=
+            cudaSuccess)
+            return NVFP4_ERR_CUDA;
+        configured[di.device].store(true, std::memory_order_release);
+    }
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = parts;
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.gridDim = dim3((unsigned)(parts == 1 ? std::min<int64_t>(p.T, kResident * di.sm_count) : p.T * parts));
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(kThreads + 32);
+    cfg.dynamicSmemBytes = ring;
     cfg.stream = s;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
@@ -830,6 +902,7 @@ int nvfp4_token_logprobs(const void *logits, int64_t ld, int dtype, const void *
     p.top_logprobs = top_logprobs;
     p.top_tokens = top_tokens;
     p.lse = lse;
+    if ((st = kernel_ctl(&p.ctl))) return st;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (dtype == NVFP4_BF16) return logprobs::forward<__nv_bfloat16>(p, di, s);
     if (dtype == NVFP4_F16) return logprobs::forward<__half>(p, di, s);
