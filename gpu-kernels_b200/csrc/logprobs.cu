@@ -15,8 +15,8 @@
 // but masked logits so far, or a maximum near the type's lowest value or past 2^60) the
 // exponents are taken one by one from the difference.
 //
-// A warp of its own copies the rows through a ring in shared memory, in bulk copies of 16 KB, and
-// runs on into the next row while the others finish this one.
+// A warp of its own copies the rows through a ring in shared memory, in bulk copies of 16 or 32 KB,
+// and runs on into the next row while the others finish this one.
 //
 // Alternatives: a row's k-th highest value cannot be below the k-th highest of 32 disjoint
 // parts' maxima, which the pass has at hand; only quarters of a thread's vectors whose maximum
@@ -41,14 +41,18 @@ namespace logprobs {
 
 constexpr int kThreads = 256;
 constexpr int kResident = 3;       // CTAs an SM
-constexpr int kRing = 4;           // chunks of kBatch vectors a thread
+constexpr int kRingBytes = 64 * 1024;  // a CTA's: chunks of a batch for each thread
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxTop = 32;
 constexpr int kCandidates = kThreads;  // one a thread when they are ranked
 constexpr int kMaxCluster = 8;
 constexpr int kQuarters = 4;         // of a thread's vectors, each with its maximum
 constexpr float kCoolest = 1e-30f, kHottest = 1e30f;  // temperatures: c stays a normal number
-constexpr int kBatch = 4;          // vectors of a thread added up together
+// Vectors of a thread that are added up together: what a batch costs beside its elements (the
+// wait, the maximum, the branches) is 2 instructions an element with 4, 4096 rows of 131072 in
+// 191 us, and 180 with 8; with alternatives, 8 do not fit into the registers (218 us and 498).
+template <bool TOP>
+constexpr int kBatchOf = TOP ? 4 : 8;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kFar = -200.0f;    // 2^-200 is zero in fp32: where the exponents of masked logits are put
 
@@ -298,6 +302,7 @@ __device__ __noinline__ void select_rounds(const Row<T> &row, int v0, int v1, in
     int have = 0, last = INT_MAX;  // order_key of +inf is below INT_MAX
     while (have < k) {
         int best = INT_MIN;
+#pragma unroll 4
         for (int v = v0 + (int)threadIdx.x; v < v1; v += kThreads) {
             float f[kVec<T>];
             row.load(v, f);
@@ -352,7 +357,8 @@ __device__ __noinline__ void select_rounds(const Row<T> &row, int v0, int v1, in
 
 template <typename T, bool ENTROPY, bool TOP>
 __global__ void __launch_bounds__(kThreads + 32, kResident) logprobs_kernel(const Params p) {
-    constexpr int kChunk = kBatch * kThreads;  // vectors
+    constexpr int kBatch = kBatchOf<TOP>, kChunk = kBatch * kThreads;  // vectors
+    constexpr int kRing = kRingBytes / (kChunk * 16);
     extern __shared__ __align__(16) uint4 ring[];  // [kRing][kChunk]
     __shared__ Shared s;
     __shared__ uint64_t bars[2 * kRing];
@@ -433,10 +439,11 @@ __global__ void __launch_bounds__(kThreads + 32, kResident) logprobs_kernel(cons
         bool paired = false;
         const int quarter = max(1, ((v1 - v0 + kBatch * kThreads - 1) / (kBatch * kThreads) + kQuarters - 1) / kQuarters);
         float high_quarter = -INFINITY;
-        auto add = [&](const uint4 (&raw)[kBatch]) {
+        auto add = [&](const auto &raw) {  // an array of vectors
+            constexpr int kN = (int)(sizeof(raw) / sizeof(uint4));
             uint32_t top = Word<T>::top(raw[0]);
 #pragma unroll
-            for (int b = 1; b < kBatch; b++) top = Word<T>::join(top, Word<T>::top(raw[b]));
+            for (int b = 1; b < kN; b++) top = Word<T>::join(top, Word<T>::top(raw[b]));
             const float high = Word<T>::top_value(top);
             if (TOP) high_quarter = fmaxf(high_quarter, high);
             if (high > m) {
@@ -458,7 +465,7 @@ __global__ void __launch_bounds__(kThreads + 32, kResident) logprobs_kernel(cons
             if (paired) {
                 const uint64_t cc = pair(p.c, p.c), rr = pair(-r, -r);
 #pragma unroll
-                for (int b = 0; b < kBatch; b++) {
+                for (int b = 0; b < kN; b++) {
                     uint64_t x[Word<T>::kPairs];
                     Word<T>::raised(raw[b], x);
 #pragma unroll
@@ -474,7 +481,7 @@ __global__ void __launch_bounds__(kThreads + 32, kResident) logprobs_kernel(cons
                 // fmaxf takes the bound where the difference is NaN, of two infinities or of a NaN
                 float t0 = 0.0f, t1 = 0.0f;
 #pragma unroll
-                for (int b = 0; b < kBatch; b++) {
+                for (int b = 0; b < kN; b++) {
                     float f[kVec<T>];
                     unpack<T>(raw[b], f);
 #pragma unroll
@@ -496,20 +503,20 @@ __global__ void __launch_bounds__(kThreads + 32, kResident) logprobs_kernel(cons
                 // after a wait that gave up the sums are of anything, and the status says so
                 if (!wait_parity(bar_full + 8 * slot, phase, p.ctl.wait_timeout_ns, abort_flag))
                     report_timeout(abort_flag, p.ctl.status);
-                uint4 raw[kBatch];
+                const uint4 *chunk = ring + slot * kChunk + threadIdx.x;
                 if (v >= w0 && v + (kBatch - 1) * kThreads < w1) {
+                    uint4 raw[kBatch];
 #pragma unroll
-                    for (int b = 0; b < kBatch; b++) raw[b] = ring[slot * kChunk + b * kThreads + threadIdx.x];
-                } else {
-#pragma unroll
-                    for (int b = 0; b < kBatch; b++) {
+                    for (int b = 0; b < kBatch; b++) raw[b] = chunk[b * kThreads];
+                    add(raw);
+                } else {  // the row's end: no more than its vectors
+                    for (int b = 0; b < kBatch && v + b * kThreads < v1; b++) {
                         const int at = v + b * kThreads;
-                        if (at >= w0 && at < w1) raw[b] = ring[slot * kChunk + b * kThreads + threadIdx.x];
-                        else if (at < v1) raw[b] = row.any(at);
-                        else raw[b] = make_uint4(Word<T>::kMasked, Word<T>::kMasked, Word<T>::kMasked, Word<T>::kMasked);
+                        uint4 raw[1];
+                        raw[0] = at >= w0 && at < w1 ? chunk[b * kThreads] : row.any(at);
+                        add(raw);
                     }
                 }
-                add(raw);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar_empty + 8 * slot);
                 pass_slot();
@@ -586,7 +593,8 @@ __global__ void __launch_bounds__(kThreads + 32, kResident) logprobs_kernel(cons
             sync_adders();
             const int per = quarter * kBatch;  // vectors of a quarter, at most
             const int all = s.n_winners * per;
-            for (int i = threadIdx.x; i < all; i += kThreads) {
+            // (more candidates than are kept, long runs of equal logits, are left to the rounds below)
+            for (int i = threadIdx.x; i < all && *(volatile int *)&s.n_cand <= kCandidates; i += kThreads) {
                 const int w = s.winners[i / per], v = v0 + w % kThreads + (w / kThreads * per + i % per) * kThreads;
                 if (v >= v1) continue;
                 float f[kVec<T>];
@@ -798,7 +806,7 @@ __global__ void __launch_bounds__(kGradThreads) logprobs_grad_kernel(const GradP
 // a batch of vectors for every thread.
 static int parts_of(int T, int64_t vectors, int sm_count) {
     int parts = 1;
-    while (parts < kMaxCluster && (int64_t)T * parts <= sm_count && vectors >= (int64_t)parts * 2 * kThreads)
+    while (parts < kMaxCluster && (int64_t)T * parts * 2 <= kResident * sm_count && vectors >= (int64_t)parts * 2 * kThreads)
         parts *= 2;
     return parts;
 }
@@ -806,10 +814,10 @@ static int parts_of(int T, int64_t vectors, int sm_count) {
 template <typename T, bool ENTROPY, bool TOP>
 static int launch(const Params &p, const DeviceInfo &di, cudaStream_t s) {
     const int parts = parts_of(p.T, p.V / kVec<T>, di.sm_count);
-    const int ring = kRing * kBatch * kThreads * (int)sizeof(uint4);
     static std::atomic<bool> configured[64] = {};
     if (!configured[di.device].load(std::memory_order_acquire)) {
-        if (cudaFuncSetAttribute(logprobs_kernel<T, ENTROPY, TOP>, cudaFuncAttributeMaxDynamicSharedMemorySize, ring) !=
+        if (cudaFuncSetAttribute(logprobs_kernel<T, ENTROPY, TOP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 kRingBytes) !=
             cudaSuccess)
             return NVFP4_ERR_CUDA;
         configured[di.device].store(true, std::memory_order_release);
@@ -821,7 +829,7 @@ static int launch(const Params &p, const DeviceInfo &di, cudaStream_t s) {
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.gridDim = dim3((unsigned)(parts == 1 ? std::min<int64_t>(p.T, kResident * di.sm_count) : p.T * parts));
     cfg.blockDim = dim3(kThreads + 32);
-    cfg.dynamicSmemBytes = ring;
+    cfg.dynamicSmemBytes = kRingBytes;
     cfg.stream = s;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
