@@ -1,10 +1,11 @@
 // embedding.cu — rows of a 16-bit table by token id, scaled, and the gradient of the table.
 //
-// The lookup is a copy: 16 bytes a thread, bound by memory.  The gradient adds up the rows of
-// equal tokens in the order of the tokens, so that the same inputs give the same bits: the
-// tokens are sorted first (stable), blocks of the sorted order are summed in fp32, and runs
-// that cross blocks are joined from the blocks' parts in order.  Each row of the gradient is
-// written once; most of a large table's rows are zeros, whose writing bounds the whole.
+// The lookup is a copy, bound by memory.  The gradient adds up the rows of equal tokens in the
+// order of the tokens, so that the same inputs give the same bits: the tokens are sorted first
+// (stable), blocks of the sorted order are summed in fp32, and runs that cross blocks are
+// joined from the blocks' parts in order.  Most of a large table's rows are zeros, whose
+// writing bounds the whole; the sort's launches, a few CTAs each, write zeros to a part of the
+// table besides, as many as go out in the time they take anyhow.
 //
 // Sorting: up to kSmallTokens tokens in one CTA (64-bit keys: token, then position).  More
 // take radix passes of up to 9 bits, each a count and a scatter over chunks of tokens; ranks
@@ -28,31 +29,41 @@ struct LookupParams {
     void *y;
     int64_t ld;  // elements
     float scale;
-    int T, V, vecs;       // 16-byte vectors of a row
-    int lanes, per_cta;   // threads of a row, rows of a CTA
-    int slabs;            // CTAs of a row
+    int V, vecs;  // 16-byte vectors of a row
+    int64_t n;    // vectors of the output
 };
 
-template <typename T, typename I, bool SCALE>
+// U vectors a thread, all in flight together: one where the output is small and latency counts,
+// four otherwise.  N: of the vectors' numbers.
+template <typename T, typename I, typename N, int U, bool SCALE>
 __global__ void __launch_bounds__(kLookupThreads) embedding_kernel(const LookupParams p) {
-    const int block = blockIdx.x / p.slabs, slab = blockIdx.x - block * p.slabs;
-    const int in_cta = threadIdx.x / p.lanes;
-    const int64_t t = (int64_t)block * p.per_cta + in_cta;
-    const int c = slab * p.lanes + threadIdx.x - in_cta * p.lanes;
-    if (in_cta >= p.per_cta || t >= p.T || c >= p.vecs) return;
-    const int64_t token = static_cast<const I *>(p.tokens)[t];
-    uint4 v = make_uint4(0u, 0u, 0u, 0u);
-    if (token >= 0 && token < p.V) {
-        v = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(p.table) + token * p.ld) + c);
-        if constexpr (SCALE) {
-            float f[8];
-            unpack8<T>(v, f);
+    const N first = (N)blockIdx.x * (kLookupThreads * U) + threadIdx.x;
+    uint4 v[U];
+    bool live[U] = {};
 #pragma unroll
-            for (int i = 0; i < 8; i++) f[i] *= p.scale;
-            v = pack8<T>(f);
+    for (int u = 0; u < U; u++) {
+        const N i = first + u * kLookupThreads;
+        v[u] = make_uint4(0u, 0u, 0u, 0u);
+        if (i < (N)p.n) {
+            const N t = i / (N)p.vecs, c = i - t * (N)p.vecs;
+            const int64_t token = static_cast<const I *>(p.tokens)[t];
+            live[u] = token >= 0 && token < p.V;
+            if (live[u])
+                v[u] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(p.table) + token * p.ld) + c);
         }
     }
-    static_cast<uint4 *>(p.y)[t * p.vecs + c] = v;
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const N i = first + u * kLookupThreads;
+        if (SCALE && live[u]) {
+            float f[8];
+            unpack8<T>(v[u], f);
+#pragma unroll
+            for (int e = 0; e < 8; e++) f[e] *= p.scale;
+            v[u] = pack8<T>(f);
+        }
+        if (i < (N)p.n) static_cast<uint4 *>(p.y)[i] = v[u];
+    }
 }
 
 // ------------------------------------------------------------------------- sorting
@@ -70,7 +81,21 @@ struct SortParams {
     int *counts;                 // [digits][chunks]
     int T, V, chunk, chunks;
     int shift, bits;
+    uint4 *zero;                 // written by the CTAs past the sort's own
+    int64_t zeros;
+    int sort_ctas;
 };
+
+// CTAs past the sort's own, kZeroVectors of the table each.
+constexpr int kZeroVectors = 16 * kSortThreads;
+__device__ __forceinline__ bool write_zeros(const SortParams &p) {
+    if ((int)blockIdx.x < p.sort_ctas) return false;
+    const int64_t i0 = (int64_t)((int)blockIdx.x - p.sort_ctas) * kZeroVectors + threadIdx.x;
+#pragma unroll
+    for (int u = 0; u < kZeroVectors / kSortThreads; u++)
+        if (i0 + u * kSortThreads < p.zeros) p.zero[i0 + u * kSortThreads] = make_uint4(0u, 0u, 0u, 0u);
+    return true;
+}
 
 __device__ __forceinline__ int key_of(const SortParams &p, int64_t t) {
     const int64_t token = p.wide ? static_cast<const int64_t *>(p.tokens)[t] : static_cast<const int *>(p.tokens)[t];
@@ -80,6 +105,7 @@ __device__ __forceinline__ int key_of(const SortParams &p, int64_t t) {
 // Bitonic sort of n (a power of two) keys that are all different, so it is stable.
 __global__ void __launch_bounds__(kSortThreads) sort_small_kernel(const SortParams p, int n) {
     extern __shared__ uint64_t key[];
+    if (write_zeros(p)) return;
     for (int i = threadIdx.x; i < n; i += kSortThreads)
         key[i] = i < p.T ? (uint64_t)(uint32_t)key_of(p, i) << 32 | (uint32_t)i : ~0ull;
     __syncthreads();
@@ -105,6 +131,7 @@ __device__ __forceinline__ int load_key(const SortParams &p, int64_t t) { return
 
 __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(const SortParams p) {
     __shared__ int count[kMaxDigits];
+    if (write_zeros(p)) return;
     const int digits = 1 << p.bits;
     for (int d = threadIdx.x; d < digits; d += kSortThreads) count[d] = 0;
     __syncthreads();
@@ -120,13 +147,18 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(const SortPa
     __shared__ int base[kMaxDigits];
     __shared__ uint16_t in_warp[kWarps][kMaxDigits];
     __shared__ int totals[kWarps];
+    if (write_zeros(p)) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int digits = 1 << p.bits;
+    const int64_t t0 = (int64_t)blockIdx.x * p.chunk, t1 = min((int64_t)p.T, t0 + p.chunk);
+    int64_t t = t0 + threadIdx.x;  // its token comes while the counts are added up
+    int key = t < t1 ? load_key(p, t) : 0, at = t < t1 ? (p.at_in ? p.at_in[t] : (int)t) : 0;
     // where this chunk's part of each digit starts: all counts of smaller digits, and the
     // digit's in earlier chunks
     const int threads_per_digit = kSortThreads / digits;  // at least two
     const int d = threadIdx.x / threads_per_digit, q = threadIdx.x % threads_per_digit;
     int all = 0, before = 0;
+#pragma unroll 8
     for (int c = q; c < p.chunks; c += threads_per_digit) {
         const int n = p.counts[(int64_t)d * p.chunks + c];
         all += n;
@@ -154,17 +186,23 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(const SortPa
     }
     if (lane == 31) totals[warp] = sum;
     __syncthreads();
-    for (int w = 0; w < warp; w++) sum += totals[w];
+    if (warp == 0) {
+        int w = totals[lane];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, w, o);
+            if (lane >= o) w += u;
+        }
+        totals[lane] = w;
+    }
+    __syncthreads();
+    if (warp) sum += totals[warp - 1];
     if ((int)threadIdx.x < digits) base[threadIdx.x] = sum - mine + digit_before[threadIdx.x];
 
-    const int64_t t0 = (int64_t)blockIdx.x * p.chunk, t1 = min((int64_t)p.T, t0 + p.chunk);
     for (int64_t tile = t0; tile < t1; tile += kSortThreads) {
         for (int i = lane; i < digits; i += 32) in_warp[warp][i] = 0;
         __syncwarp();
-        const int64_t t = tile + threadIdx.x;
         const bool live = t < t1;
-        const int key = live ? load_key(p, t) : 0;
-        const int at = live ? (p.at_in ? p.at_in[t] : (int)t) : 0;
         const int digit = live ? (key >> p.shift) & (digits - 1) : -1;
         const uint32_t same = __match_any_sync(0xffffffffu, digit);
         const int rank = __popc(same & ((1u << lane) - 1u));
@@ -190,6 +228,11 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(const SortPa
             p.keys[to] = key;
             p.at[to] = at;
         }
+        t += kSortThreads;
+        if (t < t1) {
+            key = load_key(p, t);
+            at = p.at_in ? p.at_in[t] : (int)t;
+        }
         __syncthreads();
     }
 }
@@ -197,7 +240,9 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(const SortPa
 // ------------------------------------------------------------------------- sums
 constexpr int kSumThreads = 256;
 constexpr int kSumCols = kSumThreads * 8;  // columns of a CTA
-constexpr int kAhead = 8;                  // rows of a thread in flight
+constexpr int kAhead = 8;                  // rows of a thread in flight, as many as are added up
+constexpr int kMaxBlock = 128;             // sorted tokens of a block
+constexpr int kJoinCols = 128 * 4;         // columns of a CTA that joins
 
 struct SumParams {
     const void *dy;
@@ -210,6 +255,7 @@ struct SumParams {
     int T, V, K, block, blocks, slabs;
     int sum_ctas;
     int fill_rows;         // rows of a CTA that writes zeros
+    int fill_from;         // the rows before it are zeros already
 };
 
 template <typename T>
@@ -242,7 +288,7 @@ __global__ void __launch_bounds__(kSumThreads) embedding_sum_kernel(const SumPar
     if ((int)blockIdx.x >= p.sum_ctas) {
         // rows that no token names
         __shared__ uint32_t named[8];  // a bit a row
-        const int64_t v0 = (int64_t)(blockIdx.x - p.sum_ctas) * p.fill_rows;
+        const int64_t v0 = p.fill_from + (int64_t)(blockIdx.x - p.sum_ctas) * p.fill_rows;
         const int n = (int)min((int64_t)p.fill_rows, p.V - v0);
         if (threadIdx.x < 8) named[threadIdx.x] = 0u;
         __syncthreads();
@@ -267,33 +313,42 @@ __global__ void __launch_bounds__(kSumThreads) embedding_sum_kernel(const SumPar
         }
         return;
     }
+    __shared__ int keys[kMaxBlock + 2], at[kMaxBlock];  // of the block, and the keys on both sides
     const int block = blockIdx.x / p.slabs, slab = blockIdx.x - block * p.slabs;
     const int c = slab * kSumCols + (int)threadIdx.x * 8;
+    const int64_t i0 = (int64_t)block * p.block;
+    const int n = (int)min((int64_t)p.block, p.T - i0);
+    if ((int)threadIdx.x < n + 2) {
+        const int64_t i = i0 - 1 + (int)threadIdx.x;
+        keys[threadIdx.x] = i >= 0 && i < p.T ? p.keys[i] : -1;
+    }
+    if ((int)threadIdx.x < n) at[threadIdx.x] = p.at[i0 + threadIdx.x];
+    __syncthreads();
     if (c >= p.K) return;
-    const int64_t i0 = (int64_t)block * p.block, i1 = min((int64_t)p.T, i0 + p.block);
-    const T *dy = static_cast<const T *>(p.dy);
-    const int before = i0 ? p.keys[i0 - 1] : -1;
-    const int after = i1 < p.T ? p.keys[i1] : -1;
+    const T *dy = static_cast<const T *>(p.dy) + c;
+    int run = keys[1];
+    if (run >= p.V) return;          // tokens outside the table sort last
+    bool began = run != keys[0];     // the current run starts in this block
     float sum[8] = {};
-    int run = p.keys[i0];
-    bool began = run != before;  // the current run starts in this block
-    if (run >= p.V) return;      // tokens outside the table sort last
-    for (int64_t i = i0; i < i1; i += kAhead) {
-        int key[kAhead];
-        uint4 row[kAhead];
+    auto fetch = [&](int i, uint4 (&row)[kAhead]) {
+#pragma unroll
+        for (int j = 0; j < kAhead; j++)
+            if (i + j < n && keys[1 + i + j] < p.V)
+                row[j] = __ldg(reinterpret_cast<const uint4 *>(dy + (int64_t)at[i + j] * p.ld));
+    };
+    uint4 row[kAhead], next[kAhead];
+    fetch(0, row);
+    for (int i = 0; i < n; i += kAhead) {
+        fetch(i + kAhead, next);
 #pragma unroll
         for (int j = 0; j < kAhead; j++) {
-            key[j] = i + j < i1 ? p.keys[i + j] : INT_MAX;
-            if (key[j] < p.V) row[j] = __ldg(reinterpret_cast<const uint4 *>(dy + (int64_t)p.at[i + j] * p.ld + c));
-        }
-#pragma unroll
-        for (int j = 0; j < kAhead; j++) {
-            if (i + j >= i1) break;
-            if (key[j] != run) {  // the run ends inside the block
+            if (i + j >= n) break;
+            const int key = keys[1 + i + j];
+            if (key != run) {  // the run ends inside the block
                 if (began) put_row<T>(p, run, c, sum);
                 else put_part(p, block, 0, c, sum);
-                if (key[j] >= p.V) return;
-                run = key[j];
+                if (key >= p.V) return;
+                run = key;
                 began = true;
 #pragma unroll
                 for (int e = 0; e < 8; e++) sum[e] = 0.0f;
@@ -303,46 +358,55 @@ __global__ void __launch_bounds__(kSumThreads) embedding_sum_kernel(const SumPar
 #pragma unroll
             for (int e = 0; e < 8; e++) sum[e] += f[e];
         }
+#pragma unroll
+        for (int j = 0; j < kAhead; j++) row[j] = next[j];
     }
     if (!began) put_part(p, block, 0, c, sum);        // ends here, or goes on: the join knows
-    else if (run == after) put_part(p, block, 1, c, sum);
+    else if (run == keys[1 + n]) put_part(p, block, 1, c, sum);
     else put_row<T>(p, run, c, sum);
 }
 
 // Runs of several blocks: the start in the block where the run begins, then the following
 // blocks' ends, in order.
 template <typename T>
-__global__ void __launch_bounds__(kSumThreads) embedding_join_kernel(const SumParams p) {
-    const int block = blockIdx.x / p.slabs, slab = blockIdx.x - block * p.slabs;
-    const int c = slab * kSumCols + (int)threadIdx.x * 8;
+__global__ void __launch_bounds__(kJoinCols / 4) embedding_join_kernel(const SumParams p) {
+    const int slabs = (p.K + kJoinCols - 1) / kJoinCols;
+    const int block = blockIdx.x / slabs, slab = blockIdx.x - block * slabs;
     const int64_t i0 = (int64_t)block * p.block, i1 = i0 + p.block;
     if (i1 >= p.T) return;
     const int run = p.keys[i1 - 1];
-    if (run >= p.V || p.keys[i1] != run) return;        // does not go on
+    if (run >= p.V || p.keys[i1] != run) return;                   // does not go on
     if (p.keys[i0] == run && i0 && p.keys[i0 - 1] == run) return;  // began in an earlier block
+    // The last block whose first token is the run's, by a warp: the steps of 32 that still are.
+    const int lane = threadIdx.x & 31;
+    int last = block + 1;
+    for (int64_t stride = (int64_t)1 << 25; stride; stride >>= 5) {
+        const int64_t q = last + (lane + 1) * stride;
+        const bool same = q < p.blocks && p.keys[q * p.block] == run;
+        last += (int)(__popc(__ballot_sync(0xffffffffu, same)) * stride);
+    }
+    const int c = slab * kJoinCols + (int)threadIdx.x * 4;
     if (c >= p.K) return;
-    const int last = (lower_bound(p.keys, p.T, run + 1) - 1) / p.block;
-    const float *from = p.parts + ((int64_t)block * 2 + 1) * p.K + c;
-    float sum[8];
-    {
-        const float4 a = reinterpret_cast<const float4 *>(from)[0], b = reinterpret_cast<const float4 *>(from)[1];
-        sum[0] = a.x, sum[1] = a.y, sum[2] = a.z, sum[3] = a.w;
-        sum[4] = b.x, sum[5] = b.y, sum[6] = b.z, sum[7] = b.w;
-    }
-#pragma unroll 4
+    auto part = [&](int q) {
+        return *reinterpret_cast<const float4 *>(p.parts + ((int64_t)q * 2 + (q == block ? 1 : 0)) * p.K + c);
+    };
+    float4 sum = part(block);
+#pragma unroll 8
     for (int q = block + 1; q <= last; q++) {
-        const float4 *f = reinterpret_cast<const float4 *>(p.parts + (int64_t)q * 2 * p.K + c);
-        const float4 a = f[0], b = f[1];
-        sum[0] += a.x, sum[1] += a.y, sum[2] += a.z, sum[3] += a.w;
-        sum[4] += b.x, sum[5] += b.y, sum[6] += b.z, sum[7] += b.w;
+        const float4 a = part(q);
+        sum.x += a.x;
+        sum.y += a.y;
+        sum.z += a.z;
+        sum.w += a.w;
     }
-    put_row<T>(p, run, c, sum);
+    *reinterpret_cast<uint2 *>(static_cast<T *>(p.d) + (int64_t)run * p.K + c) =
+        make_uint2(Type16<T>::pack(sum.x * p.scale, sum.y * p.scale), Type16<T>::pack(sum.z * p.scale, sum.w * p.scale));
 }
 
 // ------------------------------------------------------------------------- host side
 // Sorted tokens of a block of sums: the blocks' ends of crossing runs are written and read in
 // fp32, so longer blocks for more tokens.
-static int block_tokens(int T) { return T <= 32768 ? 32 : T <= 131072 ? 64 : 128; }
+static int block_tokens(int T) { return T <= 32768 ? 32 : T <= 131072 ? 64 : kMaxBlock; }
 
 // Radix chunks: one tile a CTA while there are no more than kMaxChunks.
 static int chunk_tokens(int T) {
@@ -382,14 +446,21 @@ static int sum(const SumParams &p, int64_t fill_ctas, cudaStream_t s) {
     embedding_sum_kernel<T><<<(unsigned)(p.sum_ctas + fill_ctas), kSumThreads, 0, s>>>(p);
     count_launch();
     if (p.blocks > 1) {
-        embedding_join_kernel<T><<<(unsigned)p.sum_ctas, kSumThreads, 0, s>>>(p);
+        const int64_t join_ctas = (int64_t)p.blocks * ((p.K + kJoinCols - 1) / kJoinCols);
+        embedding_join_kernel<T><<<(unsigned)join_ctas, kJoinCols / 4, 0, s>>>(p);
         count_launch();
     }
     return cuda_status(cudaGetLastError());
 }
 
+// Bytes of zeros that go out while a launch of the sort runs, about: a count takes 3.5 us, a
+// scatter 7, one CTA 10 for 4096 tokens and less for fewer.
+constexpr int64_t kCountZeros = 16 << 20, kScatterZeros = 36 << 20, kSmallZeros = 40 << 20;
+
 // Sorts the tokens; l.keys[0] and l.at[0] hold the result, or [1] if it returns 1 in *which.
-static int sort(const void *tokens, int wide, int T, int V, uint8_t *ws, const Layout &l, int *which, cudaStream_t s) {
+// The first *zero_rows rows of the table are zeros afterwards.
+static int sort(const void *tokens, int wide, int T, int V, int K, void *table, uint8_t *ws, const Layout &l, int *which,
+                int *zero_rows, cudaStream_t s) {
     SortParams p = {};
     p.tokens = tokens;
     p.wide = wide;
@@ -399,12 +470,24 @@ static int sort(const void *tokens, int wide, int T, int V, uint8_t *ws, const L
     p.chunks = l.chunks;
     p.counts = reinterpret_cast<int *>(ws + l.counts);
     *which = 0;
+    *zero_rows = 0;
+    const int64_t row = (int64_t)K * 2;
+    // the launch's share of zeros; the CTAs of all
+    auto zeros = [&](int64_t bytes, int sort_ctas) {
+        const int rows = (int)std::min<int64_t>(V - *zero_rows, bytes / row);
+        p.zero = static_cast<uint4 *>(table) + (int64_t)*zero_rows * K / 8;
+        p.zeros = (int64_t)rows * K / 8;
+        p.sort_ctas = sort_ctas;
+        *zero_rows += rows;
+        return (unsigned)(sort_ctas + (p.zeros + kZeroVectors - 1) / kZeroVectors);
+    };
     if (T <= kSmallTokens) {
         int n = 1;
         while (n < T) n *= 2;
         p.keys = reinterpret_cast<int *>(ws + l.keys[0]);
         p.at = reinterpret_cast<int *>(ws + l.at[0]);
-        sort_small_kernel<<<1, kSortThreads, n * sizeof(uint64_t), s>>>(p, n);
+        sort_small_kernel<<<zeros(kSmallZeros * (n + 512) / (kSmallTokens + 512), 1), kSortThreads,
+                            n * sizeof(uint64_t), s>>>(p, n);
         count_launch();
         return cuda_status(cudaGetLastError());
     }
@@ -420,8 +503,10 @@ static int sort(const void *tokens, int wide, int T, int V, uint8_t *ws, const L
         if (i) *which ^= 1;
         p.keys = reinterpret_cast<int *>(ws + l.keys[*which]);
         p.at = reinterpret_cast<int *>(ws + l.at[*which]);
-        sort_count_kernel<<<l.chunks, kSortThreads, 0, s>>>(p);
-        sort_scatter_kernel<<<l.chunks, kSortThreads, 0, s>>>(p);
+        const unsigned count_ctas = zeros(kCountZeros, l.chunks);
+        sort_count_kernel<<<count_ctas, kSortThreads, 0, s>>>(p);
+        const unsigned scatter_ctas = zeros(kScatterZeros, l.chunks);
+        sort_scatter_kernel<<<scatter_ctas, kSortThreads, 0, s>>>(p);
         count_launch();
         count_launch();
     }
@@ -440,15 +525,24 @@ static int check_sizes(const void *tokens, int token_bytes, int64_t ld, int T, i
     return misaligned(tokens, token_bytes) ? NVFP4_ERR_ALIGN : NVFP4_OK;
 }
 
+template <typename T, typename I, typename N, int U>
+static void lookup_u(const LookupParams &p, cudaStream_t s) {
+    const unsigned grid = (unsigned)((p.n + U * kLookupThreads - 1) / (U * kLookupThreads));
+    if (p.scale == 1.0f) embedding_kernel<T, I, N, U, false><<<grid, kLookupThreads, 0, s>>>(p);
+    else embedding_kernel<T, I, N, U, true><<<grid, kLookupThreads, 0, s>>>(p);
+}
+// One vector a thread as long as that makes no more CTAs than run at once.
+constexpr int64_t kFewVectors = 148 * 8 * kLookupThreads;
+template <typename T, typename I>
+static void lookup_i(const LookupParams &p, cudaStream_t s) {
+    if (p.n <= kFewVectors) lookup_u<T, I, uint32_t, 1>(p, s);
+    else if (p.n < ((int64_t)1 << 31)) lookup_u<T, I, uint32_t, 4>(p, s);
+    else lookup_u<T, I, uint64_t, 4>(p, s);
+}
 template <typename T>
-static void lookup(const LookupParams &p, int token_bytes, unsigned grid, cudaStream_t s) {
-    if (p.scale == 1.0f) {
-        if (token_bytes == 8) embedding_kernel<T, int64_t, false><<<grid, kLookupThreads, 0, s>>>(p);
-        else embedding_kernel<T, int, false><<<grid, kLookupThreads, 0, s>>>(p);
-    } else {
-        if (token_bytes == 8) embedding_kernel<T, int64_t, true><<<grid, kLookupThreads, 0, s>>>(p);
-        else embedding_kernel<T, int, true><<<grid, kLookupThreads, 0, s>>>(p);
-    }
+static void lookup(const LookupParams &p, int token_bytes, cudaStream_t s) {
+    if (token_bytes == 8) lookup_i<T, int64_t>(p, s);
+    else lookup_i<T, int>(p, s);
 }
 
 }  // namespace embedding
@@ -470,20 +564,16 @@ int nvfp4_embedding(const void *tokens, int token_bytes, const void *table, int6
     p.y = Y;
     p.ld = ld;
     p.scale = scale;
-    p.T = T;
     p.V = V;
     p.vecs = K / 8;
-    p.lanes = std::min(embedding::kLookupThreads, (p.vecs + 31) / 32 * 32);
-    p.per_cta = embedding::kLookupThreads / p.lanes;
-    p.slabs = (p.vecs + p.lanes - 1) / p.lanes;
-    const int64_t grid = ((int64_t)T + p.per_cta - 1) / p.per_cta * p.slabs;
-    if (grid > INT_MAX) return NVFP4_ERR_SHAPE;
+    p.n = (int64_t)T * p.vecs;
+    if (p.n / (4 * embedding::kLookupThreads) >= INT_MAX) return NVFP4_ERR_SHAPE;
     DeviceInfo di;
     if ((st = device_info(&di))) return st;
     if (T == 0) return NVFP4_OK;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (dtype == NVFP4_BF16) embedding::lookup<__nv_bfloat16>(p, token_bytes, (unsigned)grid, s);
-    else embedding::lookup<__half>(p, token_bytes, (unsigned)grid, s);
+    if (dtype == NVFP4_BF16) embedding::lookup<__nv_bfloat16>(p, token_bytes, s);
+    else embedding::lookup<__half>(p, token_bytes, s);
     count_launch();
     return cuda_status(cudaGetLastError());
 }
@@ -505,15 +595,16 @@ int nvfp4_embedding_backward(const void *dY, int64_t ldy, const void *tokens, in
         return NVFP4_ERR_WORKSPACE;
     const int slabs = (K + embedding::kSumCols - 1) / embedding::kSumCols;
     const embedding::Layout l = embedding::layout(T, K);
-    if ((int64_t)l.blocks * slabs > INT_MAX) return NVFP4_ERR_SHAPE;
+    if ((int64_t)l.blocks * std::max(slabs, (K + embedding::kJoinCols - 1) / embedding::kJoinCols) > INT_MAX)
+        return NVFP4_ERR_SHAPE;
     DeviceInfo di;
     if ((st = device_info(&di))) return st;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (T == 0)  // no token: the gradient is zero
         return cuda_status(cudaMemsetAsync(dTable, 0, (size_t)V * K * 2, s));
     uint8_t *ws = static_cast<uint8_t *>(workspace);
-    int which = 0;
-    if ((st = embedding::sort(tokens, token_bytes == 8, T, V, ws, l, &which, s))) return st;
+    int which = 0, zero_rows = 0;
+    if ((st = embedding::sort(tokens, token_bytes == 8, T, V, K, dTable, ws, l, &which, &zero_rows, s))) return st;
     embedding::SumParams p = {};
     p.dy = dY;
     p.ld = ldy;
@@ -530,7 +621,8 @@ int nvfp4_embedding_backward(const void *dY, int64_t ldy, const void *tokens, in
     p.slabs = slabs;
     p.sum_ctas = l.blocks * slabs;
     p.fill_rows = 64;
-    const int64_t fill = ((int64_t)V + p.fill_rows - 1) / p.fill_rows;
+    p.fill_from = zero_rows;
+    const int64_t fill = ((int64_t)V - zero_rows + p.fill_rows - 1) / p.fill_rows;
     return dtype == NVFP4_BF16 ? embedding::sum<__nv_bfloat16>(p, fill, s) : embedding::sum<__half>(p, fill, s);
 }
 
