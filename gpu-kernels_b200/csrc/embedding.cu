@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(const SortPa
 // ------------------------------------------------------------------------- sums
 constexpr int kSumThreads = 256;
 constexpr int kSumCols = kSumThreads * 8;  // columns of a CTA
-constexpr int kAhead = 8;                  // rows of a thread in flight, as many as are added up
+constexpr int kAhead = 4;                  // rows of a thread in flight, as many as are added up
 constexpr int kMaxBlock = 128;             // sorted tokens of a block
 constexpr int kJoinCols = 128 * 4;         // columns of a CTA that joins
 
@@ -253,9 +253,10 @@ struct SumParams {
     const int *keys, *at;  // sorted
     float scale;
     int T, V, K, block, blocks, slabs;
-    int sum_ctas;
-    int fill_rows;         // rows of a CTA that writes zeros
-    int fill_from;         // the rows before it are zeros already
+    int sum_ctas, fill_ctas, join_ctas;
+    int fill_rows, join_rows; // rows of a CTA that writes zeros, beside the sums and the joins
+    int fill_from, fill_end;  // rows that the sums' launch fills: the sort has filled those before,
+                              // the joins' fills those after
 };
 
 template <typename T>
@@ -272,49 +273,56 @@ __device__ __forceinline__ void put_part(const SumParams &p, int block, int whic
     to[1] = make_float4(sum[4], sum[5], sum[6], sum[7]);
 }
 
-// The first of the sorted tokens that is not below v.
-__device__ __forceinline__ int lower_bound(const int *keys, int n, int v) {
-    int lo = 0, hi = n;
-    while (lo < hi) {
-        const int mid = lo + (hi - lo) / 2;
-        if (keys[mid] < v) lo = mid + 1;
-        else hi = mid;
+// The first of the sorted tokens that is not below v, by a warp: 32 places at a time.
+__device__ __forceinline__ int lower_bound(const int *keys, int n, int v, int lane) {
+    int lo = 0;  // all before it are below
+    for (int64_t stride = (int64_t)1 << 30; stride; stride >>= 5) {
+        const int64_t i = lo + (lane + 1) * stride - 1;
+        const bool below = i < n && keys[i] < v;
+        lo += (int)(__popc(__ballot_sync(0xffffffffu, below)) * stride);
     }
     return lo;
 }
 
+// Zeros for those of `rows` rows (at most 256) from v0 on that no token names, by THREADS threads.
+template <typename T, int THREADS>
+__device__ __forceinline__ void fill(const SumParams &p, int64_t v0, int64_t end, int rows) {
+    __shared__ uint32_t named[8];  // a bit a row
+    const int n = (int)min((int64_t)rows, end - v0);
+    if (threadIdx.x < 8) named[threadIdx.x] = 0u;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        int i = lower_bound(p.keys, p.T, (int)v0, (int)threadIdx.x) + (int)threadIdx.x;
+        for (;; i += 32) {
+            const int key = i < p.T ? p.keys[i] : INT_MAX;
+            const bool mine = key - v0 < n;
+            if (mine) atomicOr(&named[(key - v0) >> 5], 1u << ((key - v0) & 31));
+            if (!__all_sync(0xffffffffu, mine)) break;
+        }
+    }
+    __syncthreads();
+    const int vecs = p.K / 8;
+    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+    for (int r = 0; r < n; r++) {
+        if ((named[r >> 5] >> (r & 31)) & 1u) continue;
+        uint4 *to = reinterpret_cast<uint4 *>(static_cast<T *>(p.d) + (v0 + r) * p.K);
+        for (int c = threadIdx.x; c < vecs; c += THREADS) to[c] = zero;
+    }
+}
+
+// Sums, and CTAs that write zeros between them, so that both are on every SM: the sums wait for
+// rows that lie anywhere, the zeros for nothing.
 template <typename T>
-__global__ void __launch_bounds__(kSumThreads) embedding_sum_kernel(const SumParams p) {
-    if ((int)blockIdx.x >= p.sum_ctas) {
-        // rows that no token names
-        __shared__ uint32_t named[8];  // a bit a row
-        const int64_t v0 = p.fill_from + (int64_t)(blockIdx.x - p.sum_ctas) * p.fill_rows;
-        const int n = (int)min((int64_t)p.fill_rows, p.V - v0);
-        if (threadIdx.x < 8) named[threadIdx.x] = 0u;
-        __syncthreads();
-        if (threadIdx.x < 32) {
-            int i = 0;
-            if (threadIdx.x == 0) i = lower_bound(p.keys, p.T, (int)v0);
-            i = __shfl_sync(0xffffffffu, i, 0) + (int)threadIdx.x;
-            for (;; i += 32) {
-                const int key = i < p.T ? p.keys[i] : INT_MAX;
-                const bool mine = key - v0 < n;
-                if (mine) atomicOr(&named[(key - v0) >> 5], 1u << ((key - v0) & 31));
-                if (!__all_sync(0xffffffffu, mine)) break;
-            }
-        }
-        __syncthreads();
-        const int vecs = p.K / 8;
-        const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-        for (int r = 0; r < n; r++) {
-            if ((named[r >> 5] >> (r & 31)) & 1u) continue;
-            uint4 *to = reinterpret_cast<uint4 *>(static_cast<T *>(p.d) + (v0 + r) * p.K);
-            for (int c = threadIdx.x; c < vecs; c += kSumThreads) to[c] = zero;
-        }
+__global__ void __launch_bounds__(kSumThreads, 4) embedding_sum_kernel(const SumParams p) {
+    // CTA i of sum_ctas + fill_ctas: how many of the first i are sums, and whether this one is
+    const int64_t all = (int64_t)p.sum_ctas + p.fill_ctas;
+    const int sums = (int)((int64_t)blockIdx.x * p.sum_ctas / all);
+    if ((int)(((int64_t)blockIdx.x + 1) * p.sum_ctas / all) == sums) {
+        fill<T, kSumThreads>(p, p.fill_from + (int64_t)((int)blockIdx.x - sums) * p.fill_rows, p.fill_end, p.fill_rows);
         return;
     }
     __shared__ int keys[kMaxBlock + 2], at[kMaxBlock];  // of the block, and the keys on both sides
-    const int block = blockIdx.x / p.slabs, slab = blockIdx.x - block * p.slabs;
+    const int block = sums / p.slabs, slab = sums - block * p.slabs;
     const int c = slab * kSumCols + (int)threadIdx.x * 8;
     const int64_t i0 = (int64_t)block * p.block;
     const int n = (int)min((int64_t)p.block, p.T - i0);
@@ -370,6 +378,10 @@ __global__ void __launch_bounds__(kSumThreads) embedding_sum_kernel(const SumPar
 // blocks' ends, in order.
 template <typename T>
 __global__ void __launch_bounds__(kJoinCols / 4) embedding_join_kernel(const SumParams p) {
+    if ((int)blockIdx.x >= p.join_ctas) {
+        fill<T, kJoinCols / 4>(p, p.fill_end + (int64_t)((int)blockIdx.x - p.join_ctas) * p.join_rows, p.V, p.join_rows);
+        return;
+    }
     const int slabs = (p.K + kJoinCols - 1) / kJoinCols;
     const int block = blockIdx.x / slabs, slab = blockIdx.x - block * slabs;
     const int64_t i0 = (int64_t)block * p.block, i1 = i0 + p.block;
@@ -441,21 +453,20 @@ static Layout layout(int T, int K) {
 }
 
 template <typename T>
-static int sum(const SumParams &p, int64_t fill_ctas, cudaStream_t s) {
-    if (p.sum_ctas + fill_ctas > INT_MAX) return NVFP4_ERR_SHAPE;
-    embedding_sum_kernel<T><<<(unsigned)(p.sum_ctas + fill_ctas), kSumThreads, 0, s>>>(p);
+static int sum(const SumParams &p, cudaStream_t s) {
+    embedding_sum_kernel<T><<<(unsigned)(p.sum_ctas + p.fill_ctas), kSumThreads, 0, s>>>(p);
     count_launch();
     if (p.blocks > 1) {
-        const int64_t join_ctas = (int64_t)p.blocks * ((p.K + kJoinCols - 1) / kJoinCols);
-        embedding_join_kernel<T><<<(unsigned)join_ctas, kJoinCols / 4, 0, s>>>(p);
+        const int ctas = (p.V - p.fill_end + p.join_rows - 1) / p.join_rows;
+        embedding_join_kernel<T><<<(unsigned)(p.join_ctas + ctas), kJoinCols / 4, 0, s>>>(p);
         count_launch();
     }
     return cuda_status(cudaGetLastError());
 }
 
-// Bytes of zeros that go out while a launch of the sort runs, about: a count takes 3.5 us, a
-// scatter 7, one CTA 10 for 4096 tokens and less for fewer.
-constexpr int64_t kCountZeros = 16 << 20, kScatterZeros = 36 << 20, kSmallZeros = 40 << 20;
+// Bytes of zeros that go out while a launch of the sort or the joins runs, about: a count takes
+// 3.5 us, a scatter 7, one CTA 10 for 4096 tokens and less for fewer, the joins 8.
+constexpr int64_t kCountZeros = 32 << 20, kScatterZeros = 56 << 20, kSmallZeros = 56 << 20, kJoinZeros = 40 << 20;
 
 // Sorts the tokens; l.keys[0] and l.at[0] hold the result, or [1] if it returns 1 in *which.
 // The first *zero_rows rows of the table are zeros afterwards.
@@ -620,10 +631,18 @@ int nvfp4_embedding_backward(const void *dY, int64_t ldy, const void *tokens, in
     p.blocks = l.blocks;
     p.slabs = slabs;
     p.sum_ctas = l.blocks * slabs;
-    p.fill_rows = 64;
+    p.join_ctas = l.blocks * ((K + embedding::kJoinCols - 1) / embedding::kJoinCols);
+    // about 256 KB a CTA, and 64 KB beside the joins
+    p.fill_rows = (int)std::max<int64_t>(1, std::min<int64_t>(256, (256 << 10) / ((int64_t)K * 2)));
+    p.join_rows = (p.fill_rows + 3) / 4;
     p.fill_from = zero_rows;
-    const int64_t fill = ((int64_t)V - zero_rows + p.fill_rows - 1) / p.fill_rows;
-    return dtype == NVFP4_BF16 ? embedding::sum<__nv_bfloat16>(p, fill, s) : embedding::sum<__half>(p, fill, s);
+    p.fill_end = V;
+    if (l.blocks > 1)  // the joins follow
+        p.fill_end -= (int)std::min<int64_t>(V - zero_rows, embedding::kJoinZeros / ((int64_t)K * 2));
+    p.fill_ctas = (p.fill_end - p.fill_from + p.fill_rows - 1) / p.fill_rows;
+    if ((int64_t)p.sum_ctas + p.fill_ctas > INT_MAX || (int64_t)p.join_ctas + V / p.join_rows >= INT_MAX)
+        return NVFP4_ERR_SHAPE;
+    return dtype == NVFP4_BF16 ? embedding::sum<__nv_bfloat16>(p, s) : embedding::sum<__half>(p, s);
 }
 
 }  // extern "C"
