@@ -8,8 +8,9 @@
 // table besides, as many as go out in the time they take anyhow.
 //
 // Sorting: up to kSmallTokens tokens in one CTA (64-bit keys: token, then position).  More
-// take radix passes of up to 9 bits, each a count and a scatter over chunks of tokens; ranks
-// within a chunk come from matching lanes and per-warp counts, never from atomics' order.
+// take radix passes of up to 9 bits over chunks of tokens; ranks within a chunk come from
+// matching lanes and per-warp counts, never from atomics' order.  A launch counts the first
+// digits by chunk; each pass counts the next ones as it puts the tokens into their new chunks.
 #include <algorithm>
 #include <climits>
 
@@ -68,17 +69,21 @@ __global__ void __launch_bounds__(kLookupThreads) embedding_kernel(const LookupP
 
 // ------------------------------------------------------------------------- sorting
 constexpr int kSortThreads = 1024;
-constexpr int kSmallTokens = 4096;
+constexpr int kSmallTokens = 1024;  // 55 steps of one CTA; 4096 would be 78 of four times the keys, 35 us
 constexpr int kMaxBits = 9;              // of a pass
 constexpr int kMaxDigits = 1 << kMaxBits;
 constexpr int kMaxChunks = 256;
+constexpr int kMaxPasses = 4;            // of 31 bits
 
 struct SortParams {
     const void *tokens;          // first pass
     int wide;                    // they are 64-bit
     const int *keys_in, *at_in;  // later passes
     int *keys, *at;              // sorted tokens (V for those outside the table) and their positions
-    int *counts;                 // [digits][chunks]
+    int *counts;                 // [digits][chunks], by pass
+    int *next;                   // the next pass's, or null; a count sets n_next of them to zero
+    int64_t n_next;
+    int next_shift, next_bits;
     int T, V, chunk, chunks;
     int shift, bits;
     uint4 *zero;                 // written by the CTAs past the sort's own
@@ -140,6 +145,8 @@ __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(const SortPara
         atomicAdd(&count[(load_key(p, t) >> p.shift) & (digits - 1)], 1);
     __syncthreads();
     for (int d = threadIdx.x; d < digits; d += kSortThreads) p.counts[(int64_t)d * p.chunks + blockIdx.x] = count[d];
+    for (int64_t i = (int64_t)blockIdx.x * kSortThreads + threadIdx.x; i < p.n_next; i += (int64_t)p.sort_ctas * kSortThreads)
+        p.next[i] = 0;
 }
 
 __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(const SortParams p) {
@@ -227,6 +234,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(const SortPa
             const int to = digit_before[digit] + in_warp[warp][digit] + rank;
             p.keys[to] = key;
             p.at[to] = at;
+            if (p.next) atomicAdd(&p.next[(int64_t)((key >> p.next_shift) & ((1 << p.next_bits) - 1)) * p.chunks + to / p.chunk], 1);
         }
         t += kSortThreads;
         if (t < t1) {
@@ -239,10 +247,12 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(const SortPa
 
 // ------------------------------------------------------------------------- sums
 constexpr int kSumThreads = 256;
-constexpr int kSumCols = kSumThreads * 8;  // columns of a CTA
+constexpr int kSumCols = kSumThreads * 8;  // columns of a CTA, for narrow rows several blocks' in one
 constexpr int kAhead = 4;                  // rows of a thread in flight, as many as are added up
 constexpr int kMaxBlock = 128;             // sorted tokens of a block
-constexpr int kJoinCols = 128 * 4;         // columns of a CTA that joins
+constexpr int kJoinCols = 32 * 4;          // columns of a warp that joins
+constexpr int kJoinBlocks = 8;             // blocks of a CTA that joins, a warp each: most have nothing to join
+constexpr int kJoinThreads = 32 * kJoinBlocks;
 
 struct SumParams {
     const void *dy;
@@ -253,6 +263,7 @@ struct SumParams {
     const int *keys, *at;  // sorted
     float scale;
     int T, V, K, block, blocks, slabs;
+    int lanes, per_cta;    // threads of a block in a CTA, blocks of a CTA
     int sum_ctas, fill_ctas, join_ctas;
     int fill_rows, join_rows; // rows of a CTA that writes zeros, beside the sums and the joins
     int fill_from, fill_end;  // rows that the sums' launch fills: the sort has filled those before,
@@ -321,18 +332,22 @@ __global__ void __launch_bounds__(kSumThreads, 4) embedding_sum_kernel(const Sum
         fill<T, kSumThreads>(p, p.fill_from + (int64_t)((int)blockIdx.x - sums) * p.fill_rows, p.fill_end, p.fill_rows);
         return;
     }
-    __shared__ int keys[kMaxBlock + 2], at[kMaxBlock];  // of the block, and the keys on both sides
-    const int block = sums / p.slabs, slab = sums - block * p.slabs;
-    const int c = slab * kSumCols + (int)threadIdx.x * 8;
+    // of the CTA's blocks: their keys and those on both sides, and where the rows are
+    __shared__ int block_keys[kSumThreads / 32][kMaxBlock + 2], block_at[kSumThreads / 32][kMaxBlock];
+    const int group = sums / p.slabs, slab = sums - group * p.slabs;
+    const int in_cta = threadIdx.x / p.lanes, x = threadIdx.x - in_cta * p.lanes;
+    const int block = group * p.per_cta + in_cta;
+    const int c = slab * kSumCols + x * 8;
     const int64_t i0 = (int64_t)block * p.block;
-    const int n = (int)min((int64_t)p.block, p.T - i0);
-    if ((int)threadIdx.x < n + 2) {
-        const int64_t i = i0 - 1 + (int)threadIdx.x;
-        keys[threadIdx.x] = i >= 0 && i < p.T ? p.keys[i] : -1;
+    const int n = in_cta < p.per_cta ? (int)max((int64_t)0, min((int64_t)p.block, p.T - i0)) : 0;
+    int *keys = block_keys[in_cta], *at = block_at[in_cta];
+    for (int j = x; n > 0 && j < n + 2; j += p.lanes) {
+        const int64_t i = i0 - 1 + j;
+        keys[j] = i >= 0 && i < p.T ? p.keys[i] : -1;
+        if (j < n) at[j] = p.at[i0 + j];
     }
-    if ((int)threadIdx.x < n) at[threadIdx.x] = p.at[i0 + threadIdx.x];
     __syncthreads();
-    if (c >= p.K) return;
+    if (n <= 0 || c >= p.K) return;
     const T *dy = static_cast<const T *>(p.dy) + c;
     int run = keys[1];
     if (run >= p.V) return;          // tokens outside the table sort last
@@ -374,42 +389,54 @@ __global__ void __launch_bounds__(kSumThreads, 4) embedding_sum_kernel(const Sum
     else put_row<T>(p, run, c, sum);
 }
 
+// volatile: the loads of a batch are issued before the first is waited for
+__device__ __forceinline__ float4 load_part(const float *from) {
+    float4 v;
+    asm volatile("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(from));
+    return v;
+}
+
 // Runs of several blocks: the start in the block where the run begins, then the following
 // blocks' ends, in order.
 template <typename T>
-__global__ void __launch_bounds__(kJoinCols / 4) embedding_join_kernel(const SumParams p) {
+__global__ void __launch_bounds__(kJoinThreads, 4) embedding_join_kernel(const SumParams p) {
     if ((int)blockIdx.x >= p.join_ctas) {
-        fill<T, kJoinCols / 4>(p, p.fill_end + (int64_t)((int)blockIdx.x - p.join_ctas) * p.join_rows, p.V, p.join_rows);
+        fill<T, kJoinThreads>(p, p.fill_end + (int64_t)((int)blockIdx.x - p.join_ctas) * p.join_rows, p.V, p.join_rows);
         return;
     }
-    const int slabs = (p.K + kJoinCols - 1) / kJoinCols;
-    const int block = blockIdx.x / slabs, slab = blockIdx.x - block * slabs;
-    const int64_t i0 = (int64_t)block * p.block, i1 = i0 + p.block;
+    const int slabs = (p.K + kJoinCols - 1) / kJoinCols, lane = threadIdx.x & 31;
+    const int eight = blockIdx.x / slabs, slab = blockIdx.x - eight * slabs;
+    const int64_t b = (int64_t)eight * kJoinBlocks + (threadIdx.x >> 5), i0 = b * p.block, i1 = i0 + p.block;
     if (i1 >= p.T) return;
-    const int run = p.keys[i1 - 1];
-    if (run >= p.V || p.keys[i1] != run) return;                   // does not go on
-    if (p.keys[i0] == run && i0 && p.keys[i0 - 1] == run) return;  // began in an earlier block
-    // The last block whose first token is the run's, by a warp: the steps of 32 that still are.
-    const int lane = threadIdx.x & 31;
+    const int block = (int)b;
+    const int run = p.keys[i1 - 1], after = p.keys[i1], first = p.keys[i0], before = i0 ? p.keys[i0 - 1] : -1;
+    if (run >= p.V || after != run) return;       // does not go on
+    if (first == run && before == run) return;    // began in an earlier block
+    // The last block whose first token is the run's: the steps of 32 that still are.
     int last = block + 1;
     for (int64_t stride = (int64_t)1 << 25; stride; stride >>= 5) {
         const int64_t q = last + (lane + 1) * stride;
         const bool same = q < p.blocks && p.keys[q * p.block] == run;
         last += (int)(__popc(__ballot_sync(0xffffffffu, same)) * stride);
     }
-    const int c = slab * kJoinCols + (int)threadIdx.x * 4;
+    const int c = slab * kJoinCols + lane * 4;
     if (c >= p.K) return;
-    auto part = [&](int q) {
-        return *reinterpret_cast<const float4 *>(p.parts + ((int64_t)q * 2 + (q == block ? 1 : 0)) * p.K + c);
-    };
-    float4 sum = part(block);
-#pragma unroll 8
-    for (int q = block + 1; q <= last; q++) {
-        const float4 a = part(q);
-        sum.x += a.x;
-        sum.y += a.y;
-        sum.z += a.z;
-        sum.w += a.w;
+    const float *start = p.parts + ((int64_t)block * 2 + 1) * p.K + c;
+    float4 sum = *reinterpret_cast<const float4 *>(start);
+    constexpr int kAtOnce = 8;  // parts on their way
+    for (int q0 = block + 1; q0 <= last; q0 += kAtOnce) {
+        float4 a[kAtOnce];
+#pragma unroll
+        for (int j = 0; j < kAtOnce; j++)
+            a[j] = load_part(p.parts + (int64_t)min(q0 + j, last) * 2 * p.K + c);
+#pragma unroll
+        for (int j = 0; j < kAtOnce; j++) {
+            const bool in = q0 + j <= last;
+            sum.x += in ? a[j].x : 0.0f;
+            sum.y += in ? a[j].y : 0.0f;
+            sum.z += in ? a[j].z : 0.0f;
+            sum.w += in ? a[j].w : 0.0f;
+        }
     }
     *reinterpret_cast<uint2 *>(static_cast<T *>(p.d) + (int64_t)run * p.K + c) =
         make_uint2(Type16<T>::pack(sum.x * p.scale, sum.y * p.scale), Type16<T>::pack(sum.z * p.scale, sum.w * p.scale));
@@ -418,7 +445,7 @@ __global__ void __launch_bounds__(kJoinCols / 4) embedding_join_kernel(const Sum
 // ------------------------------------------------------------------------- host side
 // Sorted tokens of a block of sums: the blocks' ends of crossing runs are written and read in
 // fp32, so longer blocks for more tokens.
-static int block_tokens(int T) { return T <= 32768 ? 32 : T <= 131072 ? 64 : kMaxBlock; }
+static int block_tokens(int T) { return T <= 16384 ? 32 : T <= 32768 ? 64 : kMaxBlock; }
 
 // Radix chunks: one tile a CTA while there are no more than kMaxChunks.
 static int chunk_tokens(int T) {
@@ -446,7 +473,7 @@ static Layout layout(int T, int K) {
         l.keys[i] = take((size_t)T * 4);
         l.at[i] = take((size_t)T * 4);
     }
-    l.counts = take((size_t)kMaxDigits * l.chunks * 4);
+    l.counts = take((size_t)kMaxPasses * kMaxDigits * l.chunks * 4);
     l.parts = take((size_t)l.blocks * 2 * K * 4);
     l.bytes = n;
     return l;
@@ -458,7 +485,7 @@ static int sum(const SumParams &p, cudaStream_t s) {
     count_launch();
     if (p.blocks > 1) {
         const int ctas = (p.V - p.fill_end + p.join_rows - 1) / p.join_rows;
-        embedding_join_kernel<T><<<(unsigned)(p.join_ctas + ctas), kJoinCols / 4, 0, s>>>(p);
+        embedding_join_kernel<T><<<(unsigned)(p.join_ctas + ctas), kJoinThreads, 0, s>>>(p);
         count_launch();
     }
     return cuda_status(cudaGetLastError());
@@ -505,21 +532,29 @@ static int sort(const void *tokens, int wide, int T, int V, int K, void *table, 
     int bits = 1;  // of the largest key, V
     while (bits < 31 && (V >> bits) != 0) bits++;
     const int passes = (bits + kMaxBits - 1) / kMaxBits;
-    for (int i = 0, done = 0; i < passes; i++) {
-        p.shift = done;
-        p.bits = (bits - done + passes - i - 1) / (passes - i);
-        done += p.bits;
+    const int64_t counts = (int64_t)kMaxDigits * l.chunks;  // of a pass
+    auto bits_of = [&](int pass) { return bits / passes + (pass < bits % passes ? 1 : 0); };
+    for (int i = 0; i < passes; i++) {
+        p.bits = bits_of(i);
+        p.next_shift = p.shift + p.bits;
+        p.next_bits = i + 1 < passes ? bits_of(i + 1) : 0;
+        p.next = i + 1 < passes ? p.counts + counts : nullptr;
+        if (i == 0) {
+            p.n_next = counts * (passes - 1);
+            const unsigned ctas = zeros(kCountZeros, l.chunks);
+            sort_count_kernel<<<ctas, kSortThreads, 0, s>>>(p);
+            count_launch();
+        }
         p.keys_in = i ? reinterpret_cast<int *>(ws + l.keys[*which]) : nullptr;
         p.at_in = i ? reinterpret_cast<int *>(ws + l.at[*which]) : nullptr;
         if (i) *which ^= 1;
         p.keys = reinterpret_cast<int *>(ws + l.keys[*which]);
         p.at = reinterpret_cast<int *>(ws + l.at[*which]);
-        const unsigned count_ctas = zeros(kCountZeros, l.chunks);
-        sort_count_kernel<<<count_ctas, kSortThreads, 0, s>>>(p);
-        const unsigned scatter_ctas = zeros(kScatterZeros, l.chunks);
-        sort_scatter_kernel<<<scatter_ctas, kSortThreads, 0, s>>>(p);
+        const unsigned ctas = zeros(kScatterZeros, l.chunks);
+        sort_scatter_kernel<<<ctas, kSortThreads, 0, s>>>(p);
         count_launch();
-        count_launch();
+        p.shift += p.bits;
+        p.counts += counts;
     }
     return cuda_status(cudaGetLastError());
 }
@@ -630,8 +665,11 @@ int nvfp4_embedding_backward(const void *dY, int64_t ldy, const void *tokens, in
     p.block = l.block;
     p.blocks = l.blocks;
     p.slabs = slabs;
-    p.sum_ctas = l.blocks * slabs;
-    p.join_ctas = l.blocks * ((K + embedding::kJoinCols - 1) / embedding::kJoinCols);
+    p.lanes = std::min(embedding::kSumThreads, (K / 8 + 31) / 32 * 32);
+    p.per_cta = embedding::kSumThreads / p.lanes;
+    p.sum_ctas = (l.blocks + p.per_cta - 1) / p.per_cta * slabs;
+    p.join_ctas = (l.blocks + embedding::kJoinBlocks - 1) / embedding::kJoinBlocks *
+                  ((K + embedding::kJoinCols - 1) / embedding::kJoinCols);
     // about 256 KB a CTA, and 64 KB beside the joins
     p.fill_rows = (int)std::max<int64_t>(1, std::min<int64_t>(256, (256 << 10) / ((int64_t)K * 2)));
     p.join_rows = (p.fill_rows + 3) / 4;
