@@ -9,13 +9,14 @@
 //
 // The work is a list of units of 16 weight rows: first all of W13 (8 gate rows with their 8 up
 // rows, so SwiGLU stays in a thread), then all of W2, each by active expert; experts without a
-// token are not in it.  CTAs take the units in turn.  A W2 unit waits for its expert's hidden
+// token are not in it, and one with more than 16 has each unit once for every 16 rows, side by
+// side, so that the weights come from memory once.  CTAs take the units in turn.  A W2 unit waits for its expert's hidden
 // rows alone (a counter an expert), not for the grid.  The rows' results are left in fp32, and
 // the warp that brings a block of 16 columns its last part forms the weighted sum there, in
 // the order of the choices: the same bits every time.
 //
-// Warps: 0-7 multiply, 8 says what each stage is, 9 watches the hidden rows' counters, 10-15 add
-// the parts up and hand them on, a unit each in turn (the stores and the counter of one unit
+// Warps: 0-7 multiply, 8 watches the hidden rows' counters, 9-14 add the parts up and hand them
+// on, a unit each in turn (the stores and the counter of one unit
 // take 5 us under load, longer than the weights of a short one).  A stage is 512 elements of 16 weight rows.
 // Each multiplying warp has one of its own: when it has read its stage it copies the next
 // weights there itself, one tensor copy, and brings the tokens' (hidden) rows by cp.async while
@@ -34,7 +35,8 @@
 // by cp.async 3.6 TB/s whatever the depth; a bulk copy for each of the 16 rows 2.8 (82 cycles to
 // issue one); every warp a part of each stage 4.4 (3.9); tokens by bulk copies of another warp
 // 4.6 (3.5), which then came after the weights; all weights copied by one lane, 0.4 us a stage, 5.5
-// (5.4).
+// (5.4).  Stages described by a warp of their own took 500 cycles each, more than the weights of
+// 768 elements; each warp finds its own while its weights are on their way.
 #include <algorithm>
 #include <climits>
 
@@ -51,9 +53,10 @@ constexpr int kWarps = 8;                  // that multiply, at most: one a stag
 constexpr int kMaxTiles = 2;               // of 8 token columns
 constexpr int kSets = 4;                   // of parts
 constexpr int kEpiWarps = 6;               // that add them up
-constexpr int kPlanWarp = kWarps, kWatchWarp = kWarps + 1, kEpiWarp = kWarps + 2;
+constexpr int kWatchWarp = kWarps, kEpiWarp = kWarps + 1;
 constexpr int kThreads = 32 * (kEpiWarp + kEpiWarps);
-constexpr int kMaxTokens = 8 * kMaxTiles;  // and so the rows of an expert
+constexpr int kMaxRows = 8 * kMaxTiles;    // of a unit
+constexpr int kMaxTokens = 64;             // one launch of the router
 constexpr int kMaxExperts = 256;
 constexpr int kMaxTopK = 32;
 constexpr int kMaxSize = 1 << 20;          // of K and F
@@ -61,10 +64,8 @@ constexpr int kSegment = 512;              // elements of a row in a stage
 constexpr int kBlocks = kSegment / 64;
 constexpr int kBlockBytes = 16 * 128;      // 64 elements of 16 rows
 constexpr int kTokenRows = 8;              // of a stage: a second tile's rows take the first one's place
-constexpr int kPlans = 32;                 // stages that are described ahead, more than two for each warp
-constexpr int kUnits = 16;                 // units, likewise
 constexpr int kMaxStages = kWarps;
-constexpr int kSmem = 223744;          // ring, parts, a row of zeros; the tables are static
+constexpr int kSmem = 228 * 1000;          // ring, parts, a row of zeros, the choices; the tables are static
 
 struct Params {
     const void *x, *w13, *w2, *residual;
@@ -148,19 +149,16 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
                      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// What a stage is.
-struct __align__(16) Plan {
-    int row, block, blocks, rest;  // weight: row, first block of 64 elements, whole blocks, elements past them
-    short up, n, row0, expert;     // of W13; the expert's rows; which of the active ones it is
-    short first, last;             // the warp's first and last stage in the unit
-    int unit;                      // of the CTA
+// What a unit is, and a stage of it.
+struct Unit {
+    bool up;                       // of W13
+    int a, idx, n, row0;           // active expert, its unit, the rows that take part and the first one
 };
-// What a unit is, for those who add its parts up.
-struct __align__(16) UnitPlan {
-    short up, n, row0, expert;
-    int idx;
-    short warp, parts;  // the first stage's, and how many have one
-    int set_parts;      // of the set so far, with these
+struct Stage {
+    Unit unit;
+    int number;                    // of the unit, among the CTA's
+    int row, block, blocks, rest;  // weight: row, first block of 64 elements, whole blocks, elements past them
+    bool first, last;              // the warp's first and last stage in the unit
 };
 
 template <typename T>
@@ -170,20 +168,23 @@ __global__ void __launch_bounds__(kThreads, 1)
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = smem_raw + ((0u - smem_u32(smem_raw)) & 1023u);
     __shared__ short act_e[kMaxExperts], act_row[kMaxExperts], act_n[kMaxExperts];
-    __shared__ uint16_t row_token[kMaxTokens * kMaxTopK];
-    __shared__ int16_t choice_row[kMaxTokens * kMaxTopK];
-    __shared__ float choice_weight[kMaxTokens * kMaxTopK];
-    __shared__ int n_active;
-    __shared__ uint64_t bars[kMaxStages + 2 * kPlans];
-    __shared__ Plan plans[kPlans];
-    __shared__ UnitPlan units[kUnits];
-    __shared__ int planned_units, parted[kSets], taken[kSets], hidden;  // counters
+    __shared__ int n_active, n_groups;  // experts, and sixteens of their rows
+    __shared__ short act_g[kMaxExperts + 1];  // sixteens of rows before
+    __shared__ uint64_t bars[kMaxStages];
+    __shared__ int parted[kSets], taken[kSets], hidden;  // counters
     __shared__ int abort_word;
     volatile int *abort_flag = &abort_word;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, q = lane & 3;  // fragment row / column, and quarter of 32 elements
-    const uint32_t bar_full = smem_u32(bars), bar_plan = bar_full + 8 * kMaxStages;
-    const uint32_t bar_planned = bar_plan + 8 * kPlans;
+    const uint32_t bar_full = smem_u32(bars);
+
+    // shared memory: the ring, the parts [set][warp][tile][lane], a row of zeros, the choices
+    const int tiles_cap = min(kMaxTiles, (p.T + 7) / 8), choices = p.T * p.k;
+    float4 *sums = reinterpret_cast<float4 *>(smem + p.stages * p.stage_bytes);
+    uint8_t *zeros = reinterpret_cast<uint8_t *>(sums + kSets * kWarps * tiles_cap * 32);
+    float *choice_weight = reinterpret_cast<float *>(zeros + p.pitch);
+    int16_t *choice_row = reinterpret_cast<int16_t *>(choice_weight + choices);
+    uint16_t *row_token = reinterpret_cast<uint16_t *>(choice_row + choices);
 
     // ---- active experts and the rows' tokens
     if (threadIdx.x == 0) {
@@ -191,12 +192,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         prefetch_tmap(&map2);
         abort_word = 0;
         for (int i = 0; i < p.stages; i++) mbar_init(bar_full + 8 * i, 1);
-        for (int i = 0; i < kPlans; i++) {
-            mbar_init(bar_plan + 8 * i, 1);
-            mbar_init(bar_planned + 8 * i, 1);
-        }
         for (int i = 0; i < kSets; i++) parted[i] = taken[i] = 0;
-        hidden = planned_units = 0;
+        hidden = 0;
         fence_barrier_init();
     }
     if (warp == 0) {
@@ -204,7 +201,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int i = 0; i < kMaxExperts / 32; i++) at[i] = p.m_offsets[min(i * 32 + lane, p.E)];
         at[kMaxExperts / 32] = p.m_offsets[p.E];
-        int n = 0;
+        int n = 0, sixteens = 0;
 #pragma unroll
         for (int i = 0; i < kMaxExperts / 32; i++) {
             int end = __shfl_down_sync(0xffffffffu, at[i], 1);
@@ -217,76 +214,61 @@ __global__ void __launch_bounds__(kThreads, 1)
                 act_row[slot] = (short)at[i];
                 act_n[slot] = (short)(end - at[i]);
             }
+            const int own = (end - at[i] + kMaxRows - 1) / kMaxRows;
+            int upto = own;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += v;
+            }
+            if (own) act_g[n + __popc(live & ((1u << lane) - 1u)) + 1] = (short)(sixteens + upto);
             n += __popc(live);
+            sixteens += __shfl_sync(0xffffffffu, upto, 31);
         }
-        if (lane == 0) n_active = n;
+        if (lane == 0) {
+            n_active = n;
+            n_groups = sixteens;
+            act_g[0] = 0;
+        }
     } else {
-        for (int i = threadIdx.x - 32; i < p.T * p.k; i += kThreads - 32) {
+        for (int i = threadIdx.x - 32; i < choices; i += kThreads - 32) {
             const int r = p.rows[i];
             choice_row[i] = (int16_t)r;
             choice_weight[i] = p.weights[i];
             if (r >= 0) row_token[r] = (uint16_t)(i / p.k);
         }
     }
-    for (int i = threadIdx.x; i * 4 < p.pitch; i += kThreads)
-        reinterpret_cast<int *>(smem + p.stages * p.stage_bytes + kSets * kWarps * ((p.T + 7) / 8) * 512)[i] = 0;
+    for (int i = threadIdx.x; i * 4 < p.pitch; i += kThreads) reinterpret_cast<int *>(zeros)[i] = 0;
     __syncthreads();
 
     const T *x = static_cast<const T *>(p.x);
     T *h = static_cast<T *>(p.h);
     const int units_up = p.F / 8, units_down = (p.K + 15) / 16;
-    const int total_up = n_active * units_up, total = total_up + n_active * units_down;
+    const int total_up = n_groups * units_up, total = total_up + n_groups * units_down;
     const int first = (int)blockIdx.x, stride = (int)gridDim.x;
     const uint64_t tmo = p.ctl.wait_timeout_ns;
-    const int tiles_cap = (p.T + 7) / 8;
-    const uint32_t stage_bytes = p.stage_bytes, ring = smem_u32(smem);
-    float4 *sums = reinterpret_cast<float4 *>(smem + p.stages * stage_bytes);  // [set][warp][tile][lane]
+    const uint32_t stage_bytes = p.stage_bytes;
     // A reduction's stages, by their first element: up to eight whole blocks of 64, the last one
     // with the elements past them
     auto stages_of = [](int red) { return max(1, ((red & ~63) + kSegment - 1) / kSegment); };
 
-    // The CTA's units one after another: u += stride, without a division for each.
-    struct Unit {
-        int u;
-        bool up;
-        int a, idx, n, row0, red;  // active expert, unit of it, its rows, the reduction
-    };
-    const int up_a = stride / units_up, up_idx = stride - up_a * units_up;
-    const int down_a = stride / units_down, down_idx = stride - down_a * units_down;
-    auto open_unit = [&](Unit &r) {
-        r.up = r.u < total_up;
-        const int per = r.up ? units_up : units_down, v = r.up ? r.u : r.u - total_up;
-        r.a = v / per;
-        r.idx = v - r.a * per;
-        r.red = r.up ? p.K : p.F;
-    };
-    auto load_unit = [&](Unit &r) {
-        r.n = act_n[r.a];
-        r.row0 = act_row[r.a];
-    };
-    auto first_unit = [&]() {
+    // The CTA's units, by number: of W13's and then of W2's, by expert, by the expert's unit, by
+    // sixteens of its rows.  a: the active expert of a unit before, or 0.
+    const int n_ups = first < total_up ? (total_up - first + stride - 1) / stride : 0;
+    const int n_units = first < total ? (total - first + stride - 1) / stride : 0;
+    const int stages_up = stages_of(p.K), stages_down = stages_of(p.F);
+    auto unit_at = [&](int number, int a) {
         Unit r;
-        r.u = first;
-        r.n = r.row0 = 0;
-        open_unit(r);
-        if (r.u < total) load_unit(r);
+        r.up = number < n_ups;
+        const int per = r.up ? units_up : units_down, v = first + number * stride - (r.up ? 0 : total_up);
+        while (act_g[a + 1] * per <= v) a++;
+        const int at = v - act_g[a] * per, sixteens = act_g[a + 1] - act_g[a];
+        r.a = a;
+        r.idx = sixteens == 1 ? at : at / sixteens;
+        const int part = at - r.idx * sixteens;
+        r.n = min(kMaxRows, act_n[a] - part * kMaxRows);
+        r.row0 = act_row[a] + part * kMaxRows;
         return r;
-    };
-    auto next_unit = [&](Unit &r) {
-        r.u += stride;
-        if (r.u >= total) return;
-        if (r.up && r.u >= total_up) {
-            open_unit(r);
-        } else {
-            const int per = r.up ? units_up : units_down;
-            r.a += r.up ? up_a : down_a;
-            r.idx += r.up ? up_idx : down_idx;
-            if (r.idx >= per) {
-                r.idx -= per;
-                r.a++;
-            }
-        }
-        load_unit(r);
     };
 
     // y of 16 columns once all their parts are there (or none is to come)
@@ -333,22 +315,25 @@ __global__ void __launch_bounds__(kThreads, 1)
         return;
     }
 
-    // this CTA's units and stages
-    const int n_ups = first < total_up ? (total_up - first + stride - 1) / stride : 0;
-    const int n_units = first < total ? (total - first + stride - 1) / stride : 0;
-    const int n_stages = n_ups * stages_of(p.K) + (n_units - n_ups) * stages_of(p.F);
-
     if (warp >= kEpiWarp) {
         // ---- the parts of the units in turn
         // which of a unit's rows a lane's fragments hold: the order in which eight lanes read two
         // rows of a swizzled tile from different banks
         const int r = (g >> 1) | ((g & 1) << 2);
+        const int parts_up = min(stages_up, p.stages), parts_down = min(stages_down, p.stages);
+        int a = 0;
         for (int i = warp - kEpiWarp; i < n_units; i += kEpiWarps) {
             const int set = i % kSets;
-            bool ok = warp_count_wait(&planned_units, i + 1, tmo, abort_flag, lane);
-            const UnitPlan un = units[i % kUnits];
-            if (ok) ok = warp_count_wait(&parted[set], un.set_parts, tmo, abort_flag, lane);
-            if (!ok) {
+            if (i >= n_ups && i - kEpiWarps < n_ups) a = 0;  // W2's units begin with the first expert
+            const Unit un = unit_at(i, a);
+            a = un.a;
+            // the unit's parts, its first stage's warp, and the parts that the set has got by then
+            const int parts = un.up ? parts_up : parts_down;
+            const int from_warp = (min(i, n_ups) * stages_up + max(0, i - n_ups) * stages_down) % p.stages;
+            auto of_set = [&](int n) { return n > set ? (n - 1 - set) / kSets + 1 : 0; };  // its units among n
+            const int ups = of_set(min(i + 1, n_ups));
+            const int want = ups * parts_up + (of_set(i + 1) - ups) * parts_down;
+            if (!warp_count_wait(&parted[set], want, tmo, abort_flag, lane)) {
                 if (lane == 0) report_timeout(abort_flag, p.ctl.status);
                 break;
             }
@@ -358,7 +343,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (i * 8 >= un.n) break;
                 const float4 *from = sums + (set * kWarps * tiles_cap + i) * 32 + lane;
                 float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-                for (int w = 0, at = un.warp; w < un.parts; w++) {  // in the order of the stages
+                for (int w = 0, at = from_warp; w < parts; w++) {  // in the order of the stages
                     const float4 o = from[at * tiles_cap * 32];
                     at = at + 1 == p.stages ? 0 : at + 1;
                     s.x += o.x;
@@ -391,8 +376,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
             int last = 0;
             if (lane == 0) {
-                if (un.up) add_release(p.up_done + act_e[un.expert]);
-                else last = add_acquire_release(p.col_done + un.idx) == n_active - 1;
+                if (un.up) add_release(p.up_done + act_e[un.a]);
+                else last = add_acquire_release(p.col_done + un.idx) == n_groups - 1;
             }
             if (__shfl_sync(0xffffffffu, last, 0)) combine(un.idx * 16);
             __syncwarp();
@@ -400,62 +385,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         return;
     }
 
-    if (warp == kPlanWarp) {
-        // ---- what the stages and the units are, one after another
-        if (lane == 0) {
-            int entry = 0, phase = 0, unit = 0, turn = 0, set_parts[kSets] = {};
-            for (Unit un = first_unit(); un.u < total; next_unit(un), unit++) {
-                const int e = act_e[un.a], stages = stages_of(un.red), whole = un.red / 64;
-                const int old = unit - kUnits;  // whose place this one takes
-                if (old >= 0 && !count_wait(&taken[old % kSets], old / kSets + 1, tmo, abort_flag)) {
-                    report_timeout(abort_flag, p.ctl.status);
-                    return;
-                }
-                const int parts = min(stages, p.stages);
-                int sum = 0;
-#pragma unroll
-                for (int i = 0; i < kSets; i++)
-                    if (i == unit % kSets) sum = set_parts[i] += parts;
-                units[unit % kUnits] = {(short)un.up, (short)un.n, (short)un.row0, (short)un.a, un.idx, (short)turn,
-                                        (short)parts, sum};
-                count_release(&planned_units, 1);
-                Plan plan;
-                plan.row = un.up ? e * 2 * p.F + (un.idx >> 1) * 32 + (un.idx & 1) * 8 : e * p.K + un.idx * 16;
-                plan.up = un.up;
-                plan.n = (short)un.n;
-                plan.row0 = (short)un.row0;
-                plan.expert = (short)un.a;
-                plan.unit = unit;
-                for (int st = 0; st < stages; st++) {
-                    plan.block = st * kBlocks;
-                    plan.blocks = min(kBlocks, whole - plan.block);
-                    plan.rest = st == stages - 1 ? un.red & 63 : 0;
-                    plan.first = st < p.stages;
-                    plan.last = st + p.stages >= stages;
-                    if (!wait_parity(bar_planned + 8 * entry, phase ^ 1, tmo, abort_flag)) {
-                        report_timeout(abort_flag, p.ctl.status);
-                        return;
-                    }
-                    plans[entry] = plan;
-                    mbar_arrive(bar_plan + 8 * entry);
-                    if (++entry == kPlans) {
-                        entry = 0;
-                        phase ^= 1;
-                    }
-                    turn = turn + 1 == p.stages ? 0 : turn + 1;
-                }
-            }
-        }
-        return;
-    }
-
     if (warp == kWatchWarp) {
         // ---- which experts' hidden rows are there, by all CTAs of the grid
-        if (lane == 0 && n_stages > 0) {
+        if (lane == 0 && n_units > 0) {
             const uint64_t t0 = global_timer_ns();
             for (int a = 0; a < n_active; a++) {
                 const int *done = p.up_done + act_e[a];
-                while (load_acquire(done) < units_up)
+                const int want = units_up * (act_g[a + 1] - act_g[a]);
+                while (load_acquire(done) < want)
                     if (*abort_flag || global_timer_ns() - t0 > tmo) {
                         report_timeout(abort_flag, p.ctl.status);
                         return;
@@ -466,66 +403,84 @@ __global__ void __launch_bounds__(kThreads, 1)
         return;
     }
 
-    // ---- the products: this warp's stages, first .. n_stages by p.stages
+    // ---- the products: every p.stages-th of the CTA's stages
     if (warp >= p.stages) return;
     uint8_t *weights = smem + warp * stage_bytes, *rows = weights + (kBlocks + p.tail) * kBlockBytes;
-    const uint8_t *zeros = smem + p.stages * stage_bytes + kSets * kWarps * tiles_cap * 512;  // a row of them
     const int wr = (g >> 1) | ((g & 1) << 2);  // the weight row of this lane's fragments
     const uint8_t *even = weights + wr * 128 + ((q ^ wr) << 4), *odd = weights + wr * 128 + (((4 + q) ^ wr) << 4);
     const uint32_t full = bar_full + 8 * warp;
-    auto describe = [&](int i, Plan &plan) {
-        const int entry = i % kPlans;
-        const bool ok = linear::warp_wait_parity(bar_plan + 8 * entry, (i / kPlans) & 1, tmo, abort_flag, lane);
-        plan = plans[entry];
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar_planned + 8 * entry);
-        return ok;
+    // The warp's next stage: unit `number`, stage `at` of it, which may be past the unit's.
+    int number = 0, at = warp, expert = 0;
+    auto next_stage = [&](Stage &s) {
+        for (;;) {
+            const int stages = number < n_ups ? stages_up : stages_down;
+            if (at < stages || number >= n_units) break;
+            at -= stages;
+            number++;
+            if (number == n_ups) expert = 0;
+        }
+        if (number >= n_units) return false;
+        s.unit = unit_at(number, expert);
+        expert = s.unit.a;
+        s.number = number;
+        const int e = act_e[s.unit.a], red = s.unit.up ? p.K : p.F, stages = s.unit.up ? stages_up : stages_down;
+        s.row = s.unit.up ? e * 2 * p.F + (s.unit.idx >> 1) * 32 + (s.unit.idx & 1) * 8 : e * p.K + s.unit.idx * 16;
+        s.block = at * kBlocks;
+        s.blocks = min(kBlocks, red / 64 - s.block);
+        s.rest = at == stages - 1 ? red & 63 : 0;
+        s.first = at < p.stages;
+        s.last = at + p.stages >= stages;
+        at += p.stages;
+        return true;
     };
-    auto copy_weights = [&](const Plan &plan) {
+    auto copy_weights = [&](const Stage &s) {
         if (lane == 0) {
             const uint32_t dst = smem_u32(weights);
-            mbar_arrive_expect_tx(full, ((plan.blocks > 0 ? kBlocks : 0) + (plan.rest ? 1 : 0)) * kBlockBytes);
-            if (plan.blocks > 0) {  // blocks past the last are filled with zeros
-                if (plan.up) tma_load_4d(dst, &map13, full, 0, plan.row, 0, plan.block);
-                else linear::tma_load_3d(dst, &map2, full, 0, plan.row, plan.block);
+            mbar_arrive_expect_tx(full, ((s.blocks > 0 ? kBlocks : 0) + (s.rest ? 1 : 0)) * kBlockBytes);
+            if (s.blocks > 0) {  // blocks past the last are filled with zeros
+                if (s.unit.up) tma_load_4d(dst, &map13, full, 0, s.row, 0, s.block);
+                else linear::tma_load_3d(dst, &map2, full, 0, s.row, s.block);
             }
-            if (plan.rest) {
-                const int k = (plan.up ? p.K : p.F) & ~63;
-                if (plan.up) linear::tma_load_3d(dst + kBlocks * kBlockBytes, &tail13, full, k, plan.row, 0);
-                else tma_load_2d(dst + kBlocks * kBlockBytes, &tail2, full, k, plan.row);
+            if (s.rest) {
+                const int k = (s.unit.up ? p.K : p.F) & ~63;
+                if (s.unit.up) linear::tma_load_3d(dst + kBlocks * kBlockBytes, &tail13, full, k, s.row, 0);
+                else tma_load_2d(dst + kBlocks * kBlockBytes, &tail2, full, k, s.row);
             }
         }
         __syncwarp();
     };
-    // eight of an expert's rows, the stage's elements of them
-    auto bring = [&](const Plan &plan, int tile) {
-        const int k0 = plan.block * 64, n = plan.blocks * 64 + plan.rest;
-        uint32_t to = smem_u32(rows);
-        for (int r = tile * 8; r < min((int)plan.n, tile * 8 + 8); r++, to += p.pitch) {
-            const int row = plan.row0 + r;
-            const T *from = (plan.up ? x + row_token[row] * p.ldx : h + (int64_t)row * p.hp) + k0;
-            for (int c = lane; c * 8 < n; c += 32) copy16(to + c * 16, from + c * 8);
+    // eight of the unit's rows, the stage's elements of them; lane r knows where row r is
+    auto bring = [&](const Stage &s, int tile) {
+        const int n = s.blocks * 64 + s.rest, rows_here = min(8, s.unit.n - tile * 8);
+        const T *mine = nullptr;
+        if (lane < rows_here) {
+            const int row = s.unit.row0 + tile * 8 + lane;
+            mine = (s.unit.up ? x + row_token[row] * p.ldx : h + (int64_t)row * p.hp) + s.block * 64;
+        }
+        const uint32_t to = smem_u32(rows) + lane * 16;
+#pragma unroll
+        for (int r = 0; r < 8; r++) {
+            const T *from = reinterpret_cast<const T *>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(mine), r));
+            if (r >= rows_here) break;
+#pragma unroll
+            for (int c = 0; c < 3; c++)  // at most 575 elements
+                if (c * 256 + lane * 8 < n) copy16(to + r * p.pitch + c * 512, from + c * 256 + lane * 8);
         }
     };
     float acc[kMaxTiles][2][4];
-    Plan plan;
-    bool ok = true, flying = false, brought = false;  // the weights, the rows of `plan`
+    Stage stage;
+    bool ok = true, brought = false, more = next_stage(stage), flying = more;  // the rows; the weights
     int phase = 0;
-    if (warp < n_stages) {
-        ok = flying = describe(warp, plan);
-        if (ok) copy_weights(plan);
-    }
-    for (int i = warp; ok && i < n_stages; i += p.stages) {
+    if (more) copy_weights(stage);
+    while (more) {
         if (!brought) {
-            if (!plan.up) ok = warp_count_wait(&hidden, plan.expert + 1, tmo, abort_flag, lane);
+            if (!stage.unit.up) ok = warp_count_wait(&hidden, stage.unit.a + 1, tmo, abort_flag, lane);
             if (!ok) break;
-            bring(plan, 0);
+            bring(stage, 0);
         }
-        Plan next;
-        const bool more = i + p.stages < n_stages;
-        if (more) ok = describe(i + p.stages, next);
-        if (!ok) break;
-        if (plan.first)
+        Stage next;
+        more = next_stage(next);
+        if (stage.first)
 #pragma unroll
             for (int t = 0; t < kMaxTiles; t++)
 #pragma unroll
@@ -536,53 +491,53 @@ __global__ void __launch_bounds__(kThreads, 1)
         flying = false;
 #pragma unroll
         for (int t = 0; t < kMaxTiles; t++) {
-            if (t * 8 >= plan.n) break;
+            if (t * 8 >= stage.unit.n) break;
             if (t) {
                 __syncwarp();  // the first tile's rows have been read
-                bring(plan, t);
+                bring(stage, t);
             }
             copies_wait();
             __syncwarp();
-            const uint8_t *column = (t * 8 + g < plan.n ? rows + g * p.pitch : zeros) + q * 16;
+            const uint8_t *column = (t * 8 + g < stage.unit.n ? rows + g * p.pitch : zeros) + q * 16;
             auto chunk = [&](const uint8_t *w, const uint8_t *b) {
                 const uint4 wa = *reinterpret_cast<const uint4 *>(w), wb = *reinterpret_cast<const uint4 *>(w + 1024);
                 const uint4 v = *reinterpret_cast<const uint4 *>(b);
                 mma<T>(acc[t][0], wa.x, wb.x, wa.y, wb.y, v.x, v.y);
                 mma<T>(acc[t][1], wa.z, wb.z, wa.w, wb.w, v.z, v.w);
             };
-            if (plan.blocks == kBlocks) {
+            if (stage.blocks == kBlocks) {
 #pragma unroll
                 for (int b = 0; b < kBlocks; b++) {
                     chunk(even + b * kBlockBytes, column + b * 128);
                     chunk(odd + b * kBlockBytes, column + b * 128 + 64);
                 }
             } else {
-                for (int b = 0; b < plan.blocks; b++) {
+                for (int b = 0; b < stage.blocks; b++) {
                     chunk(even + b * kBlockBytes, column + b * 128);
                     chunk(odd + b * kBlockBytes, column + b * 128 + 64);
                 }
             }
-            if (plan.rest)  // the weights past the row's end are zeros, the tokens' row is read no further
+            if (stage.rest)  // the weights past the row's end are zeros, the tokens' row is read no further
 #pragma unroll
                 for (int half = 0; half < 2; half++)
-                    if (half * 32 < plan.rest) {
-                        const bool in = half * 32 + q * 8 < plan.rest;
+                    if (half * 32 < stage.rest) {
+                        const bool in = half * 32 + q * 8 < stage.rest;
                         chunk((half ? odd : even) + kBlocks * kBlockBytes,
-                              in ? column + plan.blocks * 128 + half * 64 : zeros);
+                              in ? column + stage.blocks * 128 + half * 64 : zeros);
                     }
         }
         __syncwarp();
-        const bool last = plan.last;
-        const int unit = plan.unit, columns = plan.n;
+        const bool last = stage.last;
+        const int unit = stage.number, columns = stage.unit.n;
         brought = false;
         if (more) {
-            plan = next;
-            copy_weights(plan);
+            stage = next;
+            copy_weights(stage);
             flying = true;
             // hidden rows that are not there yet wait for others, this warp's own parts among them
-            brought = plan.up || count_reached(&hidden, plan.expert + 1);
+            brought = stage.unit.up || count_reached(&hidden, stage.unit.a + 1);
             brought = __shfl_sync(0xffffffffu, (int)brought, 0) != 0;
-            if (brought) bring(plan, 0);
+            if (brought) bring(stage, 0);
         }
         if (last) {
             const int set = unit % kSets;
@@ -750,13 +705,13 @@ int nvfp4_moe_layer(const void *X, int64_t ldx, const void *logits, int logits_d
     p.K = K;
     p.F = F;
     p.hp = l.hp;
-    const int tiles = (T + 7) / 8;
+    const int tiles = std::min(moe_layer::kMaxTiles, (T + 7) / 8);
     p.tail = K % 64 || F % 64;
     p.pitch = (moe_layer::kSegment + 64 * p.tail) * 2 + 64;
     p.stage_bytes =
         ((moe_layer::kBlocks + p.tail) * moe_layer::kBlockBytes + moe_layer::kTokenRows * p.pitch + 1023) & ~1023;
-    p.stages = std::min(moe_layer::kMaxStages,
-                        (moe_layer::kSmem - 1024 - p.pitch - moe_layer::kSets * moe_layer::kWarps * tiles * 512) / p.stage_bytes);
+    const int beside = 1024 + moe_layer::kSets * moe_layer::kWarps * tiles * 512 + p.pitch + 8 * T * top_k;
+    p.stages = std::min(moe_layer::kMaxStages, (moe_layer::kSmem - beside) / p.stage_bytes);
     // the router's checks of its own arguments come before any launch
     st = moe::route_tokens(logits, logits_dtype, bias, T, E, top_k, scoring, renormalize, scale,
                            const_cast<float *>(p.weights), reinterpret_cast<int *>(ws + l.experts),

@@ -17,7 +17,7 @@ import torch
 from ._bind import native
 from ._lib import ACTIVATIONS, SCORES
 
-FEW_TOKENS = 16  # tokens up to which moe_layer is the fused kernel
+FEW_TOKENS = 64  # tokens up to which moe_layer is the fused kernel
 
 
 class Routing(NamedTuple):

@@ -427,7 +427,7 @@ NVFP4_API int nvfp4_moe_combine_backward(const void *dY, const void *X_rows, int
  * [T, K]; Y may be the residual and shares memory with no other input.  The hidden state is
  * rounded to dtype, everything else is fp32 and rounded once; the weights of experts that no
  * token chose are not read.
- * T <= 16, top_k <= min(E, 32), E <= 256, K % 8 == 0, F % 16 == 0.  The second launch is
+ * T <= 64, top_k <= min(E, 32), E <= 256, K % 8 == 0, F % 16 == 0.  The second launch is
  * cooperative (its blocks wait for each other, bounded as every wait).  The workspace needs
  * no initial value; calls that may run at the same time need one each (256-byte aligned).
  */

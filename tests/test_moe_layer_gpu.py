@@ -67,9 +67,9 @@ def check(nv, d, k, scoring="softmax", bias=None, renormalize=True, scale=1.0):
 @pytest.mark.parametrize("T,E,k,K,F", [
     (1, 1, 1, 8, 16), (1, 8, 2, 64, 48), (2, 3, 1, 24, 1040), (3, 4, 4, 72, 16), (8, 128, 8, 2048, 768),
     (9, 5, 1, 2056, 2064), (12, 40, 32, 40, 32), (16, 1, 1, 2048, 2048), (14, 2, 2, 1032, 1024), (13, 64, 6, 264, 80), (16, 256, 8, 1024, 64), (17, 2, 2, 1032, 1024),
-    (25, 6, 3, 4104, 32), (32, 40, 32, 40, 32), (32, 1, 1, 2048, 2048), (32, 8, 2, 512, 1408), (31, 2, 2, 2048, 768)])
+    (25, 6, 3, 4104, 32), (64, 4, 2, 520, 96), (49, 256, 8, 1024, 48), (64, 40, 32, 40, 32), (33, 3, 3, 2056, 1040), (32, 40, 32, 40, 32), (32, 1, 1, 2048, 2048), (32, 8, 2, 512, 1408), (31, 2, 2, 2048, 768)])
 def test_moe_layer(nv, cuda_dev, T, E, k, K, F, dtype):
-    """One and two tiles of rows, sizes that fill no chunk or stage, more warps than chunks, experts
+    """One to eight tiles of rows, sizes that fill no chunk or stage, more warps than chunks, experts
     without a token; and more tokens than one launch takes."""
     check(nv, layer(T, E, K, F, dtype, T + E, residual=T % 2 == 1, logits=dtype if T % 3 else torch.float32), k)
 
@@ -119,7 +119,7 @@ def test_moe_layer_reads_chosen_experts_only(nv, cuda_dev):
 
 def test_moe_layer_one_expert_for_all(nv, cuda_dev):
     """Every token to the same expert: the most rows an expert can have."""
-    for T in (7, 8, 9, 15, 16):
+    for T in (7, 8, 9, 16, 17, 24, 33, 57, 64):
         d = layer(T, 5, 512, 96, torch.bfloat16, T)
         d["logits"][:, 3] = 50.0
         check(nv, d, 1)
@@ -139,7 +139,7 @@ def test_moe_layer_same_bits_and_agreement(nv, cuda_dev):
         assert torch.equal(one[0], y[t])
 
 
-@pytest.mark.parametrize("T", [0, 17, 64, 200])
+@pytest.mark.parametrize("T", [0, 65, 128, 200])
 def test_moe_layer_more_tokens(nv, cuda_dev, T):
     d = layer(T, 8, 256, 96, torch.bfloat16, 4)
     if T == 0:
