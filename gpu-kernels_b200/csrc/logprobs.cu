@@ -642,7 +642,10 @@ __global__ void __launch_bounds__(kThreads + 32, kResident) logprobs_kernel(cons
                 const bool none = !(target > -INFINITY);
                 p.lse[t] = empty ? -INFINITY : all.m / p.temperature + l;
                 p.logprobs[t] = ignored ? 0.0f : empty || none ? -INFINITY : (target - all.m) / p.temperature - l;
-                if (ENTROPY) p.entropy[t] = empty ? 0.0f : l - all.s1 / all.s0 * kLn2;
+                if (ENTROPY) {
+                    const float H = l - all.s1 / all.s0 * kLn2;
+                    p.entropy[t] = empty || H < 0.0f ? 0.0f : H;  // below zero it is rounding
+                }
             }
             if (TOP) {
                 int n = s.n_top;  // of this CTA

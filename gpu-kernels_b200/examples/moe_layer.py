@@ -1,8 +1,9 @@
 """A mixture-of-experts layer from the package's operators: bf16 forward, one training step,
-and the same routing over NVFP4 experts.
+and the same routing over NVFP4 experts; and between an embedding and its tied output
+projection, a decode step and a training step from token ids to log probabilities.
 
     python gpu-kernels_b200/examples/moe_layer.py [--tokens 4096] [--experts 8] [--top-k 2]
-        [--hidden 4096] [--ffn 14336] [--steps 3]
+        [--hidden 4096] [--ffn 14336] [--vocab 32000] [--steps 3]
 
     y = x + sum_j weight_j  W2_e ( silu(W1_e x) * (W3_e x) )      over the token's experts e
 
@@ -34,6 +35,22 @@ def train_forward(x, router, w13, w2, top_k):
     return ops.moe_combine(ops.linear_preact(h, w2, r[3])[0], *r, x)
 
 
+def decode(tokens, table, router, w13, w2, top_k, top=5):
+    """One decode step: the log probability of each next token is taken later, so here the five
+    most probable ones and the entropy.  Six kernels."""
+    x = nv.embedding(tokens, table, table.shape[1] ** 0.5)
+    y = nv.moe_layer(x, nv.linear(x, router), w13, w2, top_k, residual=x)
+    return nv.token_logprobs(nv.linear(y, table), tokens, top_k=top, entropy=True)
+
+
+def loss(tokens, targets, table, router, w13, w2, top_k):
+    """The training objective from token ids: the targets' mean log probability, negative."""
+    x = ops.embedding(tokens, table, table.shape[1] ** 0.5)
+    y = train_forward(x, router, w13, w2, top_k)
+    logits = ops.linear_preact(y, table)[0]
+    return -ops.token_logprobs(logits, targets)[0].mean()
+
+
 def quantize_weight(w, experts):
     """Per-expert NVFP4 weight: (codes, scales, global scales)."""
     rows = w.shape[0] // experts
@@ -60,6 +77,7 @@ def main():
     ap.add_argument("--top-k", type=int, default=2)
     ap.add_argument("--hidden", type=int, default=4096)
     ap.add_argument("--ffn", type=int, default=14336)
+    ap.add_argument("--vocab", type=int, default=32000)
     ap.add_argument("--steps", type=int, default=3)
     a = ap.parse_args()
     E, K, F = a.experts, a.hidden, a.ffn
@@ -93,11 +111,23 @@ def main():
     err = ((y4 - y).float().norm() / (y - x).float().norm()).item()
     print(f"NVFP4 experts         {ms:8.3f} ms   relative difference of the experts' part {err:.3f}")
 
+    table = weight(a.vocab, K)
+    tokens = torch.randint(0, a.vocab, (a.tokens + 1,), device="cuda", generator=g)
+    few = tokens[:16]
+    r16, ms = timed(lambda: decode(few, table, router, w13, w2, a.top_k))
+    print(f"decode, {len(few):2d} tokens     {ms:8.3f} ms   entropy {r16.entropy.mean().item():.2f}, "
+          f"most probable {r16.top_tokens[0].tolist()}")
+
     params = [t.requires_grad_() for t in (x, router, w13, w2)]
     dy = torch.randn(x.shape, device="cuda", generator=g).bfloat16()
     grads, ms = timed(lambda: torch.autograd.grad(train_forward(*params, a.top_k), params, dy))
     print(f"bf16 forward+backward {ms:8.3f} ms   gradient norms "
           + " ".join(f"{t.float().norm().item():.1f}" for t in grads))
+
+    params = [t.requires_grad_() for t in (table, router, w13, w2)]
+    value, ms = timed(lambda: torch.autograd.grad(loss(tokens[:-1], tokens[1:], *params, a.top_k), params))
+    print(f"tokens to gradients   {ms:8.3f} ms   gradient norms "
+          + " ".join(f"{t.float().norm().item():.3f}" for t in value))
 
 
 if __name__ == "__main__":

@@ -1,11 +1,15 @@
 """GPU: the whole mixture-of-experts layer of a few tokens against a plain 64-bit form, and as
 a part of a decode step."""
+import importlib.util
 import math
+import os
 
 import pytest
 import torch
 
 import ref16 as R
+from nvfp4_b200._bind import native
+from nvfp4_b200._lib import SCORES
 
 pytestmark = pytest.mark.gpu
 
@@ -53,24 +57,32 @@ def layer64(x, logits, w13, w2, k, scoring, bias, renormalize, scale, residual, 
 
 
 def check(nv, d, k, scoring="softmax", bias=None, renormalize=True, scale=1.0):
-    y = nv.moe_layer(d["x"], d["logits"], d["w13"], d["w2"], k, scoring=scoring, bias=bias, renormalize=renormalize,
-                     scale=scale, residual=d["residual"])
+    """moe_layer, and the kernel of a few tokens wherever it takes the call."""
+    args = d["x"], d["logits"], d["w13"], d["w2"], k
+    y = nv.moe_layer(*args, scoring=scoring, bias=bias, renormalize=renormalize, scale=scale, residual=d["residual"])
     torch.cuda.synchronize()
     nv.device_status()
-    ref, bound = layer64(d["x"], d["logits"], d["w13"], d["w2"], k, scoring, bias, renormalize, scale, d["residual"],
-                         rounded_rows=d["x"].shape[0] > nv.moe.FEW_TOKENS)
+    few = nv.moe._few(d["x"].shape[0], k, d["logits"].shape[1])
+    ref, bound = layer64(*args, scoring, bias, renormalize, scale, d["residual"], rounded_rows=not few)
     R.assert_close(y, ref, bound)
+    if not few and d["x"].shape[0] <= nv.moe.FEW_TOKENS:
+        z = native.moe_layer(*args, SCORES[scoring], bias, renormalize, scale, d["residual"])
+        torch.cuda.synchronize()
+        nv.device_status()
+        ref, bound = layer64(*args, scoring, bias, renormalize, scale, d["residual"])
+        R.assert_close(z, ref, bound)
     return y
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("T,E,k,K,F", [
     (1, 1, 1, 8, 16), (1, 8, 2, 64, 48), (2, 3, 1, 24, 1040), (3, 4, 4, 72, 16), (8, 128, 8, 2048, 768),
-    (9, 5, 1, 2056, 2064), (12, 40, 32, 40, 32), (16, 1, 1, 2048, 2048), (14, 2, 2, 1032, 1024), (13, 64, 6, 264, 80), (16, 256, 8, 1024, 64), (17, 2, 2, 1032, 1024),
-    (25, 6, 3, 4104, 32), (64, 4, 2, 520, 96), (49, 256, 8, 1024, 48), (64, 40, 32, 40, 32), (33, 3, 3, 2056, 1040), (32, 40, 32, 40, 32), (32, 1, 1, 2048, 2048), (32, 8, 2, 512, 1408), (31, 2, 2, 2048, 768)])
+    (9, 5, 1, 2056, 2064), (12, 40, 32, 40, 32), (16, 1, 1, 2048, 2048), (14, 2, 2, 1032, 1024), (13, 64, 6, 264, 80),
+    (16, 256, 8, 1024, 64), (17, 2, 2, 1032, 1024), (25, 6, 3, 4104, 32), (32, 8, 2, 512, 1408), (33, 3, 3, 2056, 1040),
+    (49, 256, 8, 1024, 48), (64, 1, 1, 2048, 512), (64, 4, 2, 520, 96), (64, 40, 32, 40, 32), (64, 256, 4, 512, 256)])
 def test_moe_layer(nv, cuda_dev, T, E, k, K, F, dtype):
-    """One to eight tiles of rows, sizes that fill no chunk or stage, more warps than chunks, experts
-    without a token; and more tokens than one launch takes."""
+    """One tile of rows to four units' sixteens, sizes that fill no chunk or stage, more warps than
+    chunks, experts without a token."""
     check(nv, layer(T, E, K, F, dtype, T + E, residual=T % 2 == 1, logits=dtype if T % 3 else torch.float32), k)
 
 
@@ -225,3 +237,38 @@ def test_decode_step(nv, cuda_dev):
     assert ((r.logprobs.double() - want[torch.arange(6), tokens.clamp_min(0)]).abs() <= limit)[live].all()
     op = torch.ops.nvfp4_b200.moe_layer(x, d["logits"], d["w13"], d["w2"], 2, "softmax", None, True, 1.0, x)
     assert torch.equal(op, y)
+
+
+def test_example(nv, cuda_dev):
+    """examples/moe_layer.py's decode step runs; its loss's gradients against 64 bits with the same
+    choice of experts.  Some ten results on the way are rounded by at most 2^-8 of themselves, so
+    a gradient is off by at most 10 2^-8 of its norm."""
+    path = os.path.join(os.path.dirname(nv.__file__), "..", "examples", "moe_layer.py")
+    spec = importlib.util.spec_from_file_location("example_moe_layer", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    V, K, F, E, T, k = 96, 64, 32, 8, 24, 2
+    g = gen(3)
+    table, router = (torch.randn(r, K, device="cuda", generator=g).mul(K ** -0.5).bfloat16() for r in (V, E))
+    w13 = (torch.randn(E * 2 * F, K, device="cuda", generator=g) * K ** -0.5).bfloat16()
+    w2 = (torch.randn(E * K, F, device="cuda", generator=g) * F ** -0.5).bfloat16()
+    tokens, targets = (torch.randint(0, V, (T,), device="cuda", generator=g) for _ in range(2))
+    targets[3] = -100
+    r = example.decode(tokens[:5], table, router, w13, w2, k)
+    assert r.top_tokens.shape == (5, 5) and torch.isfinite(r.entropy).all()
+    params = [t.requires_grad_() for t in (table, router, w13, w2)]
+    got = torch.autograd.grad(example.loss(tokens, targets, *params, k), params)
+
+    x = nv.embedding(tokens, table.detach(), K ** 0.5)
+    experts = nv.moe_route(nv.linear(x, router.detach()), k).experts.long()
+    p64 = [t.detach().double().requires_grad_() for t in params]
+    t64, r64, a64, b64 = p64
+    x = t64[tokens] * K ** 0.5
+    logits = x @ r64.t()
+    weights = torch.softmax(logits.gather(1, experts), 1)  # renormalised over the chosen ones
+    h = R.act64(torch.einsum("tk,tjfk->tjf", x, a64.view(E, 2 * F, K)[experts]).reshape(T * k, 2 * F), "swiglu")
+    y = x + (weights[:, :, None] * torch.einsum("tjf,tjkf->tjk", h.view(T, k, F), b64.view(E, K, F)[experts])).sum(1)
+    logp = torch.log_softmax(y @ t64.t(), 1).gather(1, targets.clamp_min(0)[:, None])[:, 0]
+    want = torch.autograd.grad(-(logp * (targets >= 0)).sum() / T, p64)
+    for name, a, b in zip(("table", "router", "w13", "w2"), got, want):
+        assert (a.double() - b).norm() <= 10 * 2.0 ** -8 * b.norm(), name
