@@ -10,33 +10,39 @@
 // The work is a list of units of 16 weight rows: first all of W13 (8 gate rows with their 8 up
 // rows, so SwiGLU stays in a thread), then all of W2, each by active expert; experts without a
 // token are not in it, and one with more than 16 has each unit once for every 16 rows, side by
-// side, so that the weights come from memory once.  CTAs take the units in turn.  A W2 unit waits for its expert's hidden
-// rows alone (a counter an expert), not for the grid.  The rows' results are left in fp32, and
-// the warp that brings a block of 16 columns its last part forms the weighted sum there, in
-// the order of the choices: the same bits every time.
+// side, so that the weights come from memory once.  CTAs take the units in turn.  A W2 unit
+// waits for its expert's hidden rows alone (a counter an expert), not for the grid.  The rows'
+// results are left in fp32, and the warp that brings a block of 16 columns its last part forms
+// the weighted sum there, in the order of the choices: the same bits every time.
 //
 // Warps: 0-7 multiply, 8 watches the hidden rows' counters, 9-14 add the parts up and hand them
-// on, a unit each in turn (the stores and the counter of one unit
-// take 5 us under load, longer than the weights of a short one).  A stage is 512 elements of 16 weight rows.
-// Each multiplying warp has one of its own: when it has read its stage it copies the next
-// weights there itself, one tensor copy, and brings the tokens' (hidden) rows by cp.async while
-// they are on their way, so its latencies run under the other warps' stages and nothing is
-// handed from warp to warp but sums.  The weights run on into W2 while its hidden rows are
-// still being made.  For each chunk of 32 elements lanes 4g .. 4g + 3 read 64 bytes of row g,
-// which is mma.m16n8k16's A fragment with the chunk's elements permuted, and the tokens are
-// read with the same permutation, so nothing is shuffled.  The products are tiny (8 token
-// columns a tile); the tensor core only has to keep up with memory.
+// on, a unit each in turn (the stores and the counter of one unit take 5 us under load, longer
+// than the weights of a short one).  A stage is 512 elements of 16 weight rows.  Each
+// multiplying warp has one of its own: when it has read its stage it copies the next weights
+// there itself, one tensor copy, and brings the tokens' (hidden) rows by cp.async while they
+// are on their way, so its latencies run under the other warps' stages and nothing is handed
+// from warp to warp but sums.  The weights run on into W2 while its hidden rows are still being
+// made.  For each chunk of 32 elements lanes 4g .. 4g + 3 read 64 bytes of row g, which is
+// mma.m16n8k16's A fragment with the chunk's elements permuted, and the tokens are read with
+// the same permutation, so nothing is shuffled.  The products are tiny (8 token columns a
+// tile); the tensor core only has to keep up with memory.
 //
 // The weights are seen as [block of 64 elements][row][64] so that a box is eight whole swizzled
 // tiles of 8 rows by 128 bytes for each half of the rows.  Elements past the last whole block
 // come beside the last stage's blocks, from a second view that knows the row's end.
 //
-// Measured on the way, E = 8 of 4096 x 14336 (64 of 2048 x 2048, 8 tokens): pieces of 16 bytes
-// by cp.async 3.6 TB/s whatever the depth; a bulk copy for each of the 16 rows 2.8 (82 cycles to
-// issue one); every warp a part of each stage 4.4 (3.9); tokens by bulk copies of another warp
-// 4.6 (3.5), which then came after the weights; all weights copied by one lane, 0.4 us a stage, 5.5
-// (5.4).  Stages described by a warp of their own took 500 cycles each, more than the weights of
-// 768 elements; each warp finds its own while its weights are on their way.
+// Measured, both launches, on the GPU: one token by 2 of 8 experts of 4096 x 14336 112 us (6.3
+// TB/s), 8 tokens by 6 of 64 of 2048 x 2048 124 us (6.3), 13 by 6 of 64 of 2056 x 1408, whose
+// rows begin anywhere in a 128-byte line, 136 us (5.4), one by 8 of 128 of 2048 x 768 28 us:
+// there it is bound by the router's launch (5 us), the first weights (3.5), the way from the
+// last W13 weights to the last hidden rows (4.5) and from the last W2 weights to the sum (4.5).
+//
+// On the way, the first two of these: pieces of 16 bytes by cp.async 3.6 TB/s whatever the
+// depth; a bulk copy for each of the 16 rows 2.8 and 2.8 (82 cycles to issue one); every warp a
+// part of each stage 4.4 and 3.9; tokens by bulk copies of another warp, which then came after
+// the weights, 4.6 and 3.5; all weights copied by one lane, 0.4 us a stage, 5.5 and 5.4; stages
+// described by a warp of their own, 500 cycles each, 6.2 and 6.3 but 4.6 instead of 5.8 for 256
+// experts of 2048 x 768.
 #include <algorithm>
 #include <climits>
 
@@ -118,7 +124,9 @@ __device__ __forceinline__ bool warp_count_wait(const int *c, int want, uint64_t
                                                 int lane) {
     int ok = 1;
     if (lane == 0) ok = count_wait(c, want, timeout_ns, abort);
-    return __shfl_sync(0xffffffffu, ok, 0) != 0;
+    ok = __shfl_sync(0xffffffffu, ok, 0);
+    __syncwarp();  // what lane 0 has acquired, for all
+    return ok != 0;
 }
 __device__ __forceinline__ void add_release(int *p) {
     asm volatile("red.release.gpu.global.add.s32 [%0], 1;" ::"l"(p) : "memory");
@@ -379,7 +387,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (un.up) add_release(p.up_done + act_e[un.a]);
                 else last = add_acquire_release(p.col_done + un.idx) == n_groups - 1;
             }
-            if (__shfl_sync(0xffffffffu, last, 0)) combine(un.idx * 16);
+            last = __shfl_sync(0xffffffffu, last, 0);
+            __syncwarp();  // what lane 0 has acquired, for all
+            if (last) combine(un.idx * 16);
             __syncwarp();
         }
         return;
@@ -537,6 +547,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             // hidden rows that are not there yet wait for others, this warp's own parts among them
             brought = stage.unit.up || count_reached(&hidden, stage.unit.a + 1);
             brought = __shfl_sync(0xffffffffu, (int)brought, 0) != 0;
+            __syncwarp();  // what lane 0 has acquired, for all
             if (brought) bring(stage, 0);
         }
         if (last) {
