@@ -46,6 +46,7 @@ PRODUCT_UNITS = [("runtime", os.path.join(CSRC, "runtime.cu"), []),
                  ("linear_grad", os.path.join(CSRC, "linear_grad.cu"), []),
                  ("moe", os.path.join(CSRC, "moe.cu"), []),
                  ("moe_layer", os.path.join(CSRC, "moe_layer.cu"), []),
+                 ("moe_products", os.path.join(CSRC, "moe_products.cu"), []),
                  ("embedding", os.path.join(CSRC, "embedding.cu"), []),
                  ("logprobs", os.path.join(CSRC, "logprobs.cu"), []),
                  ("host_pipeline", os.path.join(CSRC, "host_pipeline.cu"), []),

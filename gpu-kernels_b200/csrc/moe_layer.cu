@@ -49,6 +49,7 @@
 #include "common.cuh"
 #include "linear.cuh"
 #include "moe.cuh"
+#include "moe_products.cuh"
 #include "ptx.cuh"
 #include "types16.cuh"
 
@@ -577,8 +578,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // ------------------------------------------------------------------------- host side
+// Whether the kernel above takes the layer, or two products by row group (moe_products.cu).
+static bool streamed(int T, int E, int k) { return T <= 16 || T * k <= 4 * E; }
+
 struct Layout {
-    size_t weights, experts, rows, offsets, counters, h, part, bytes;
+    size_t weights, experts, rows, offsets, counters, h, part, x_rows, bytes;
     int n_counters, hp;
 };
 static Layout layout(int T, int E, int k, int K, int F) {
@@ -590,15 +594,17 @@ static Layout layout(int T, int E, int k, int K, int F) {
         return at;
     };
     const size_t R = (size_t)T * k;
-    l.hp = (F + 63) & ~63;  // whole 128-byte lines: no two rows share one
-    l.n_counters = E + (K + 15) / 16;
+    const bool one = streamed(T, E, k);
+    l.hp = one ? (F + 63) & ~63 : F;  // one kernel: whole 128-byte lines, no two rows share one
+    l.n_counters = one ? E + (K + 15) / 16 : 0;
     l.weights = take(R * 4);
     l.experts = take(R * 4);
     l.rows = take(R * 4);
     l.offsets = take((size_t)(E + 1) * 4);
     l.counters = take((size_t)l.n_counters * 4);
     l.h = take(R * l.hp * 2);
-    l.part = take(R * K * 4);
+    l.part = take(R * K * 4 * (one ? 1 : moe_products::kMaxParts));
+    l.x_rows = take(one ? 0 : R * K * 2);
     l.bytes = n;
     return l;
 }
@@ -710,12 +716,44 @@ int nvfp4_moe_layer(const void *X, int64_t ldx, const void *logits, int logits_d
     p.col_done = p.up_done + E;
     p.h = ws + l.h;
     p.part = reinterpret_cast<float *>(ws + l.part);
+    int *experts = reinterpret_cast<int *>(ws + l.experts);
     p.T = T;
     p.E = E;
     p.k = top_k;
     p.K = K;
     p.F = F;
     p.hp = l.hp;
+    // the router's checks of its own arguments come before any launch
+    st = moe::route_tokens(logits, logits_dtype, bias, T, E, top_k, scoring, renormalize, scale,
+                           const_cast<float *>(p.weights), experts, const_cast<int *>(p.rows),
+                           const_cast<int *>(p.m_offsets), nullptr, 0, p.up_done, l.n_counters, stream);
+    if (st) return st;
+    DeviceInfo di;
+    if ((st = device_info(&di))) return st;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (!moe_layer::streamed(T, E, top_k)) {
+        moe_products::Args a = {};
+        a.x = X;
+        a.w13 = W13;
+        a.w2 = W2;
+        a.residual = residual;
+        a.y = Y;
+        a.ldx = ldx;
+        a.weights = p.weights;
+        a.experts = experts;
+        a.rows = p.rows;
+        a.m_offsets = p.m_offsets;
+        a.x_rows = ws + l.x_rows;
+        a.h = p.h;
+        a.part = p.part;
+        a.T = T;
+        a.E = E;
+        a.k = top_k;
+        a.K = K;
+        a.F = F;
+        a.dtype = dtype;
+        return moe_products::run(a, di, s);
+    }
     const int tiles = std::min(moe_layer::kMaxTiles, (T + 7) / 8);
     p.tail = K % 64 || F % 64;
     p.pitch = (moe_layer::kSegment + 64 * p.tail) * 2 + 64;
@@ -723,16 +761,7 @@ int nvfp4_moe_layer(const void *X, int64_t ldx, const void *logits, int logits_d
         ((moe_layer::kBlocks + p.tail) * moe_layer::kBlockBytes + moe_layer::kTokenRows * p.pitch + 1023) & ~1023;
     const int beside = 1024 + moe_layer::kSets * moe_layer::kWarps * tiles * 512 + p.pitch + 8 * T * top_k;
     p.stages = std::min(moe_layer::kMaxStages, (moe_layer::kSmem - beside) / p.stage_bytes);
-    // the router's checks of its own arguments come before any launch
-    st = moe::route_tokens(logits, logits_dtype, bias, T, E, top_k, scoring, renormalize, scale,
-                           const_cast<float *>(p.weights), reinterpret_cast<int *>(ws + l.experts),
-                           const_cast<int *>(p.rows), const_cast<int *>(p.m_offsets), nullptr, 0,
-                           p.up_done, l.n_counters, stream);
-    if (st) return st;
-    DeviceInfo di;
-    if ((st = device_info(&di))) return st;
     if ((st = kernel_ctl(&p.ctl))) return st;
-    cudaStream_t s = static_cast<cudaStream_t>(stream);
     return dtype == NVFP4_BF16 ? moe_layer::launch<__nv_bfloat16>(p, di, s) : moe_layer::launch<__half>(p, di, s);
 }
 

@@ -17,16 +17,7 @@ import torch
 from ._bind import native
 from ._lib import ACTIVATIONS, SCORES
 
-FEW_TOKENS = 64  # the most that the fused kernel of moe_layer takes
-
-
-def _few(tokens: int, top_k: int, experts: int) -> bool:
-    """Whether moe_layer is the fused kernel: always up to 16 tokens, beyond them while an expert
-    has up to four rows on average.  Each expert's rows are brought to every unit of its weights,
-    and from eight rows on that takes longer than the weights: 32 tokens by 8 of 256 experts
-    (one row) 263 us fused and 263 by the operators, 64 by 6 of 64 (six) 300 and 262, 32 by 2 of
-    8 large experts (eight) 480 and 441, 64 by 4 of 16 (sixteen) 171 and 88."""
-    return tokens <= 16 or (tokens <= FEW_TOKENS and tokens * top_k <= 4 * experts)
+FEW_TOKENS = 64  # the most that nvfp4_moe_layer takes
 
 
 class Routing(NamedTuple):
@@ -93,13 +84,11 @@ def moe_layer(x: torch.Tensor, logits: torch.Tensor, w13: torch.Tensor, w2: torc
 
     with moe_route's choice (the same arguments) and SwiGLU experts: w13 [E * 2F, K], gate and
     up rows interleaved in blocks of 16 (swiglu_interleave by expert), w2 [E * K, F]; F a
-    multiple of 16.  A decode step's few tokens (up to 16; up to 64 that are few rows an expert)
-    are two kernels that read the chosen experts' weights once, and the experts' results are
-    summed in fp32.  More go through moe_route, moe_dispatch, linear_grouped and moe_combine,
-    which round each expert's result.  For inference: the differentiable form is those four
-    operators."""
-    matrices = all(isinstance(t, torch.Tensor) and t.dim() == 2 for t in (x, logits))
-    if matrices and not _few(x.shape[0], top_k, logits.shape[1]):
+    multiple of 16.  For up to 64 tokens, a decode step, kernels of its own read the chosen
+    experts' weights once and sum the experts' results in fp32.  More go through moe_route,
+    moe_dispatch, linear_grouped and moe_combine, which round each expert's result.  For
+    inference: the differentiable form is those four operators."""
+    if isinstance(x, torch.Tensor) and x.dim() == 2 and x.shape[0] > FEW_TOKENS:
         r = moe_route(logits, top_k, scoring, bias, renormalize, scale)
         rows = moe_dispatch(x.contiguous(), r)
         h = native.linear(rows, w13, r.m_offsets, None, ACTIVATIONS["swiglu"], None, None, False)
