@@ -291,6 +291,14 @@ __global__ void __launch_bounds__(kSumThreads) sum_kernel(const SumParams p) {
     __shared__ short parts[kExperts];  // of the tile, by expert
     __shared__ int before[kExperts / 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tile = blockIdx.x;
+    const int t = blockIdx.y * kSumTokens + warp, col = tile * 128 + lane * 4;
+    int row = -1, expert = 0;  // of the token's choice `lane`
+    float weight = 0.0f;
+    if (t < p.T && lane < p.k) {
+        row = p.rows[t * p.k + lane];
+        expert = p.experts[t * p.k + lane];
+        weight = p.weights[t * p.k + lane];
+    }
     bool live = false;
     if (threadIdx.x < p.E) {
         int r0, r1;
@@ -312,31 +320,31 @@ __global__ void __launch_bounds__(kSumThreads) sum_kernel(const SumParams p) {
         parts[threadIdx.x] = (short)(cut.piece_of(first + cut.per - 1) - cut.piece_of(first) + 1);
     }
     __syncthreads();
-    const int t = blockIdx.y * kSumTokens + warp, col = tile * 128 + lane * 4;
-    if (t >= p.T || col >= p.K) return;
-    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (t >= p.T) return;
+    const int count = row >= 0 && row < p.R ? parts[expert] : 0;
+    const bool in = col < p.K;
     const int64_t at = (int64_t)t * p.K + col;
-    for (int j0 = 0; j0 < p.k; j0 += 4) {
-        float4 v[4][2];
-        float w[4];
-        int n[4], row[4];
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int j0 = 0; j0 < p.k; j0 += 8) {
+        float4 v[8][2];
+        float w[8];
+        int n[8], r[8];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int c = t * p.k + j0 + j;
-            row[j] = j0 + j < p.k ? p.rows[c] : -1;
-            n[j] = row[j] >= 0 && row[j] < p.R ? parts[p.experts[c]] : 0;
-            w[j] = n[j] ? p.weights[c] : 0.0f;
+        for (int j = 0; j < 8; j++) {
+            r[j] = __shfl_sync(0xffffffffu, row, j0 + j);
+            n[j] = __shfl_sync(0xffffffffu, count, j0 + j);
+            w[j] = __shfl_sync(0xffffffffu, weight, j0 + j);
 #pragma unroll
             for (int i = 0; i < 2; i++)
-                v[j][i] = i < n[j] ? *reinterpret_cast<const float4 *>(p.part + ((int64_t)i * p.R + row[j]) * p.K + col)
-                                   : make_float4(0.f, 0.f, 0.f, 0.f);
+                v[j][i] = in && i < n[j] ? *reinterpret_cast<const float4 *>(p.part + ((int64_t)i * p.R + r[j]) * p.K + col)
+                                         : make_float4(0.f, 0.f, 0.f, 0.f);
         }
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
+        for (int j = 0; j < 8; j++) {
             float4 o = make_float4(v[j][0].x + v[j][1].x, v[j][0].y + v[j][1].y, v[j][0].z + v[j][1].z,
                                    v[j][0].w + v[j][1].w);
-            for (int i = 2; i < n[j]; i++) {
-                const float4 u = *reinterpret_cast<const float4 *>(p.part + ((int64_t)i * p.R + row[j]) * p.K + col);
+            for (int i = 2; in && i < n[j]; i++) {
+                const float4 u = *reinterpret_cast<const float4 *>(p.part + ((int64_t)i * p.R + r[j]) * p.K + col);
                 o.x += u.x;
                 o.y += u.y;
                 o.z += u.z;
@@ -350,6 +358,7 @@ __global__ void __launch_bounds__(kSumThreads) sum_kernel(const SumParams p) {
             }
         }
     }
+    if (!in) return;
     if (p.residual) {
         const uint2 r = *reinterpret_cast<const uint2 *>(static_cast<const T *>(p.residual) + at);
         const float2 lo = Type16<T>::unpack(r.x), hi = Type16<T>::unpack(r.y);
