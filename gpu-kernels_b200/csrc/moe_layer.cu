@@ -3,7 +3,8 @@
 //
 //   y[t] = residual[t] + sum_j w[t, j] W2_e ( silu(W1_e x[t]) * (W3_e x[t]) ),  e = e(t, j)
 //
-// Two launches: the router (moe.cu, which also clears this kernel's counters), and one
+// Several rows an expert are another file's (streamed(), below).  Here there are two launches:
+// the router (moe.cu, which also clears this kernel's counters), and one
 // cooperative kernel for the experts and the weighted sum, where six kernels and their gaps
 // took longer than the weights of small experts do.
 //
@@ -578,8 +579,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // ------------------------------------------------------------------------- host side
-// Whether the kernel above takes the layer, or two products by row group (moe_products.cu).
-static bool streamed(int T, int E, int k) { return T <= 16 || T * k <= 4 * E; }
+// Whether the kernel above takes the layer, or two products by row group (moe_products.cu): up
+// to 8 tokens, one tile of rows at most; beyond them while an expert has up to four rows on
+// average (its rows are brought to every unit) and a unit has two stages or more (its sums take
+// longer than one stage's weights).  us, this kernel and the products: 8 tokens by 8 of 8
+// experts of 2048 x 4096 76 and 85, 16 by 2 73 and 83, by 4 88 and 84, by 8 105 and 85; 32 by 8
+// of 256 of 2048 x 768 263 and 264; 64 by 4 of 256 of 768 x 512 114 and 98.
+static bool streamed(int T, int E, int k, int K, int F) { return T <= 8 || (T * k <= 4 * E && K + F >= 2048); }
 
 struct Layout {
     size_t weights, experts, rows, offsets, counters, h, part, x_rows, bytes;
@@ -594,7 +600,7 @@ static Layout layout(int T, int E, int k, int K, int F) {
         return at;
     };
     const size_t R = (size_t)T * k;
-    const bool one = streamed(T, E, k);
+    const bool one = streamed(T, E, k, K, F);
     l.hp = one ? (F + 63) & ~63 : F;  // one kernel: whole 128-byte lines, no two rows share one
     l.n_counters = one ? E + (K + 15) / 16 : 0;
     l.weights = take(R * 4);
@@ -731,7 +737,7 @@ int nvfp4_moe_layer(const void *X, int64_t ldx, const void *logits, int logits_d
     DeviceInfo di;
     if ((st = device_info(&di))) return st;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (!moe_layer::streamed(T, E, top_k)) {
+    if (!moe_layer::streamed(T, E, top_k, K, F)) {
         moe_products::Args a = {};
         a.x = X;
         a.w13 = W13;

@@ -419,7 +419,7 @@ NVFP4_API int nvfp4_moe_combine_backward(const void *dY, const void *X_rows, int
                                          int K, void *dX_rows, float *dweights, void *stream);
 
 /*
- * A whole mixture-of-experts layer for the few tokens of a decode step, in two launches:
+ * A whole mixture-of-experts layer for the few tokens of a decode step:
  *   Y[t] = residual[t] + sum_j weight[t, j] W2_e silu_mul(W13_e X[t]),  e the j-th expert of t
  * with the choice and the weights of nvfp4_moe_route from logits [T, E] (logits_dtype bf16,
  * fp16 or fp32) and SwiGLU experts: W13 [E * 2F, K] with gate and up rows interleaved in
@@ -427,9 +427,10 @@ NVFP4_API int nvfp4_moe_combine_backward(const void *dY, const void *X_rows, int
  * [T, K]; Y may be the residual and shares memory with no other input.  The hidden state is
  * rounded to dtype, everything else is fp32 and rounded once; the weights of experts that no
  * token chose are not read.
- * T <= 64, top_k <= min(E, 32), E <= 256, K % 8 == 0, F % 16 == 0.  The second launch is
- * cooperative (its blocks wait for each other, bounded as every wait).  The workspace needs
- * no initial value; calls that may run at the same time need one each (256-byte aligned).
+ * T <= 64, top_k <= min(E, 32), E <= 256, K % 8 == 0, F % 16 == 0.  Few rows an expert take
+ * two launches, the second cooperative (its blocks wait for each other, bounded as every
+ * wait); more take five, with products by row group.  The workspace needs no initial value;
+ * calls that may run at the same time need one each (256-byte aligned).
  */
 NVFP4_API size_t nvfp4_moe_layer_workspace_size(int T, int E, int top_k, int K, int F);
 NVFP4_API int nvfp4_moe_layer(const void *X, int64_t ldx, const void *logits, int logits_dtype, const float *bias,
