@@ -805,18 +805,24 @@ __global__ void __launch_bounds__(kGradThreads) logprobs_grad_kernel(const GradP
 }
 
 // ------------------------------------------------------------------------- host side
-// CTAs that share a row: as many as keep every row's on the GPU at once, while each still has
-// a batch of vectors for every thread.
-static int parts_of(int T, int64_t vectors, int sm_count) {
+// CTAs that share a row: as many as keep all rows' at two an SM, while each has a vector for
+// every thread, or, with alternatives, enough of them for the join of the lists (2-4 us).  us, by
+// 1, 2, 4 and 8 CTAs, bf16: 16 rows of 131072 13.4, 10.8, 8.8, 8.6, with 20 alternatives 19.2,
+// 15.8, 13.4, 13.2; 16 of 50257 with 5 13.0, 13.3, 12.8, 13.0, of 25600 10.8, 11.0, 10.9, 12.9; 55
+// of 131072 14.7, 11.6, 10.8, 14.8 (8 would be three an SM); 300 rows 25.4, 25.4, 29.6, 42.5.
+// A cluster has one row: its copies do not run on into a next one, for which its other warps
+// would have to give slots back before they meet the cluster.
+static int parts_of(int T, int64_t vectors, bool top, int sm_count) {
+    const int64_t least = top ? 1536 : kThreads;
     int parts = 1;
-    while (parts < kMaxCluster && (int64_t)T * parts * 2 <= kResident * sm_count && vectors >= (int64_t)parts * 2 * kThreads)
-        parts *= 2;
+    if (top && vectors < 4 * least) return parts;
+    while (parts < kMaxCluster && (int64_t)T * parts <= sm_count && vectors >= parts * 2 * least) parts *= 2;
     return parts;
 }
 
 template <typename T, bool ENTROPY, bool TOP>
 static int launch(const Params &p, const DeviceInfo &di, cudaStream_t s) {
-    const int parts = parts_of(p.T, p.V / kVec<T>, di.sm_count);
+    const int parts = parts_of(p.T, p.V / kVec<T>, TOP, di.sm_count);
     static std::atomic<bool> configured[64] = {};
     if (!configured[di.device].load(std::memory_order_acquire)) {
         if (cudaFuncSetAttribute(logprobs_kernel<T, ENTROPY, TOP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
