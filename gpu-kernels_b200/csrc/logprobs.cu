@@ -276,7 +276,7 @@ __device__ __forceinline__ uint64_t ld_cluster_u64(uint32_t addr) {
 struct Shared {
     uint64_t cand[kCandidates];
     uint64_t top[kMaxTop];        // this CTA's alternatives, highest first
-    Stats part[kWarps];
+    Stats part[2][kWarps];
     float best[kQuarters][kThreads];  // the maxima of quarters of the threads' vectors
     int winners[kQuarters * kThreads];
     int count[kWarps + 1];
@@ -423,15 +423,19 @@ __global__ void __launch_bounds__(kThreads + 32, kResident) logprobs_kernel(cons
         }
         return;
     }
+    // the row's target, read a row ahead: its logit is under way while the row is summed
+    const bool finishes = part == 0 && threadIdx.x == 0;
+    int64_t next = finishes && first < p.T ? target_of(p.targets, p.target8, first) : -1;
+    int turn = 0;  // of the statistics' two places
     for (int64_t t = first; t < p.T; t += step) {
         const Row<T> row = row_at(t);
         const int v0 = from(row, part), v1 = from(row, part + 1);
         float target = -INFINITY;
         bool ignored = true;
-        if (part == 0 && threadIdx.x == 0) {
-            const int64_t at = target_of(p.targets, p.target8, t);
-            ignored = at < 0 || at >= p.V;
-            if (!ignored) target = to_float<T>(row.x[at]);
+        if (finishes) {
+            ignored = next < 0 || next >= p.V;
+            if (!ignored) target = to_float<T>(row.x[next]);
+            if (t + step < p.T) next = target_of(p.targets, p.target8, t + step);
         }
         // ---- the pass
         float m = -INFINITY, r = 0.0f, rest = 0.0f;  // r: c m rounded, rest: what that left
@@ -509,7 +513,18 @@ __global__ void __launch_bounds__(kThreads + 32, kResident) logprobs_kernel(cons
 #pragma unroll
                     for (int b = 0; b < kBatch; b++) raw[b] = chunk[b * kThreads];
                     add(raw);
-                } else {  // the row's end: no more than its vectors
+                } else if (v >= w0 && v + kBatch / 2 * kThreads < w1) {  // the row's end, more than half a batch
+                    const uint4 masked = make_uint4(Word<T>::kMasked, Word<T>::kMasked, Word<T>::kMasked, Word<T>::kMasked);
+                    uint4 raw[kBatch];
+#pragma unroll
+                    for (int b = 0; b < kBatch; b++) raw[b] = v + b * kThreads < w1 ? chunk[b * kThreads] : masked;
+                    add(raw);
+                    for (int b = kBatch / 2; b < kBatch; b++)  // the vector that the row ends in
+                        if (v + b * kThreads >= w1 && v + b * kThreads < v1) {
+                            uint4 last[1] = {row.any(v + b * kThreads)};
+                            add(last);
+                        }
+                } else {  // no more than its vectors
                     for (int b = 0; b < kBatch && v + b * kThreads < v1; b++) {
                         const int at = v + b * kThreads;
                         uint4 raw[1];
@@ -542,7 +557,7 @@ __global__ void __launch_bounds__(kThreads + 32, kResident) logprobs_kernel(cons
         Stats w = a;
 #pragma unroll
         for (int o = 16; o; o >>= 1) w = join(w, shuffle(w, o), p);
-        if (lane == 0) s.part[warp] = w;
+        if (lane == 0) s.part[turn][warp] = w;
         if (threadIdx.x == 0) s.n_winners = s.n_cand = s.n_top = 0;
         sync_adders();
         if (TOP) {
@@ -626,7 +641,7 @@ __global__ void __launch_bounds__(kThreads + 32, kResident) logprobs_kernel(cons
             Stats all = {-INFINITY, 0.0f, 0.0f};
             if (warp == 0) {
                 for (int i = lane; i < parts * kWarps; i += 32) {
-                    const uint32_t at = map_to_cta(smem_u32(&s.part[i % kWarps]), i / kWarps);
+                    const uint32_t at = map_to_cta(smem_u32(&s.part[turn][i % kWarps]), i / kWarps);
                     all = join(all, {ld_cluster_f32(at), ld_cluster_f32(at + 4), ld_cluster_f32(at + 8)}, p);
                 }
 #pragma unroll
@@ -690,8 +705,10 @@ __global__ void __launch_bounds__(kThreads + 32, kResident) logprobs_kernel(cons
         if (parts > 1) {
             __syncwarp();
             cluster_sync();  // the first CTA has read the others' parts
-        } else {
+        } else if (TOP) {
             sync_adders();
+        } else {  // the first warp finishes this row while the others begin the next
+            turn ^= 1;
         }
     }
 }
