@@ -24,8 +24,17 @@
 // candidates are ranked by counting.  The rare row with more candidates than are kept (long
 // runs of equal logits) takes rounds of "highest value, lowest tokens first".
 //
-// A row is one CTA's, or is cut between the CTAs of a cluster when there are few rows; the
-// parts meet in distributed shared memory.  Every sum has a fixed order.
+// A row is one CTA's, or is cut between the CTAs of a cluster when there are few rows (the parts
+// meet in distributed shared memory), or a warp's when rows are short and many: a CTA's
+// barriers and its last steps take 2.5 us a row, 5 with alternatives.  Every sum has a fixed
+// order.
+//
+// Measured: 4096 rows of 131072 bf16, statistics 173 us (6.2 TB/s of a copy's 6.55), with the
+// entropy 179, and 8 alternatives 220 (their second reading and the ranking, 5 us a row of a
+// CTA), 32 262; the gradient 326 (6.6 TB/s).  16000 rows of 8000 52 us (4.9 TB/s).  Without
+// alternatives the pass is bound by memory and nearly by issue (61 % of cycles; the unit of
+// powers of two is 66 % busy).  One row of 50257 fp32 with 5 alternatives 9.1 us: launch, a pass of
+// 3 us, the join of a cluster and the ranking.
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -46,6 +55,7 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kMaxTop = 32;
 constexpr int kCandidates = kThreads;  // one a thread when they are ranked
 constexpr int kMaxCluster = 8;
+constexpr int kRowWarps = 8, kRowResident = 4, kRowBatch = 4;  // of the kernel of short rows
 constexpr int kQuarters = 4;         // of a thread's vectors, each with its maximum
 constexpr float kCoolest = 1e-30f, kHottest = 1e30f;  // temperatures: c stays a normal number
 // Vectors of a thread that are added up together: what a batch costs beside its elements (the
@@ -251,6 +261,77 @@ __device__ __forceinline__ Stats shuffle(const Stats &a, int o) {
             __shfl_xor_sync(0xffffffffu, a.s1, o)};
 }
 
+// The sums of a thread's part of a row so far.
+template <typename T, bool ENTROPY>
+struct Sums {
+    float m = -INFINITY, r = 0.0f, rest = 0.0f;  // r: c m rounded, rest: what that left
+    uint64_t s0[2] = {0, 0}, s1[2] = {0, 0};
+    bool paired = false;
+
+    // N vectors more; their maximum
+    template <int N>
+    __device__ __forceinline__ float add(const uint4 (&raw)[N], float c) {
+        uint32_t top = Word<T>::top(raw[0]);
+#pragma unroll
+        for (int b = 1; b < N; b++) top = Word<T>::join(top, Word<T>::top(raw[b]));
+        const float high = Word<T>::top_value(top);
+        if (high > m) {
+            const float r_next = high * c;
+            const bool pairs = raises(Word<T>::kFloor, c, r_next) && fabsf(r_next) < 0x1p60f;
+            const float rest_next = pairs ? fmaf(high, c, -r_next) : 0.0f;
+            const float d = fmaxf((m - high) * c, kFar) - rest + rest_next, scale = ex2(d);
+            const uint64_t dd = pair(d, d), ss = pair(scale, scale);
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                if (ENTROPY) s1[i] = mul2(fma2(s0[i], dd, s1[i]), ss);
+                s0[i] = mul2(s0[i], ss);
+            }
+            m = high;
+            r = r_next;
+            rest = rest_next;
+            paired = pairs;
+        }
+        if (paired) {
+            const uint64_t cc = pair(c, c), rr = pair(-r, -r);
+#pragma unroll
+            for (int b = 0; b < N; b++) {
+                uint64_t x[Word<T>::kPairs];
+                Word<T>::raised(raw[b], x);
+#pragma unroll
+                for (int i = 0; i < Word<T>::kPairs; i++) {
+                    const uint64_t d = fma2(x[i], cc, rr);
+                    const float2 f = unpair(d);
+                    const uint64_t e = pair(ex2(f.x), ex2(f.y));
+                    s0[i & 1] = add2(s0[i & 1], e);
+                    if (ENTROPY) s1[i & 1] = fma2(d, e, s1[i & 1]);
+                }
+            }
+        } else {
+            // fmaxf takes the bound where the difference is NaN, of two infinities or of a NaN
+            float t0 = 0.0f, t1 = 0.0f;
+#pragma unroll
+            for (int b = 0; b < N; b++) {
+                float f[kVec<T>];
+                unpack<T>(raw[b], f);
+#pragma unroll
+                for (int i = 0; i < kVec<T>; i++) {
+                    const float d = fmaxf((f[i] - m) * c, kFar), e = ex2(d);
+                    t0 += e;
+                    if (ENTROPY) t1 = fmaf(d, e, t1);
+                }
+            }
+            s0[0] = add2(s0[0], pair(t0, 0.0f));
+            if (ENTROPY) s1[0] = add2(s1[0], pair(t1, 0.0f));
+        }
+        return high;
+    }
+    __device__ __forceinline__ Stats stats() const {
+        const float2 x = unpair(add2(s0[0], s0[1])), y = unpair(add2(s1[0], s1[1]));
+        const float sum0 = x.x + x.y, sum1 = y.x + y.y, back = ex2(-rest);
+        return {m, sum0 * back, ENTROPY ? fmaf(-rest, sum0, sum1) * back : 0.0f};
+    }
+};
+
 // Barrier of the threads that add up, without the one that copies.
 __device__ __forceinline__ void sync_adders() {
     __syncwarp();  // .aligned
@@ -295,15 +376,17 @@ __device__ __forceinline__ void rank_keys(const uint64_t *keys, int n, int k, ui
 }
 
 // The alternatives of vectors [v0, v1) where equal values are too many to keep: the highest
-// value that is left, then its tokens from the lowest, until there are k.
-template <typename T>
-__device__ __noinline__ void select_rounds(const Row<T> &row, int v0, int v1, int k, Shared &s) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+// value that is left, then its tokens from the lowest, until there are k.  By the threads that
+// add up, whose warps' counts meet in `count`, or (WARP) by one warp.  Returns how many.
+template <typename T, bool WARP>
+__device__ __noinline__ int select_rounds(const Row<T> &row, int v0, int v1, int k, uint64_t *top, int *count) {
+    constexpr int kTeam = WARP ? 32 : kThreads;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, me = WARP ? lane : (int)threadIdx.x;
     int have = 0, last = INT_MAX;  // order_key of +inf is below INT_MAX
     while (have < k) {
         int best = INT_MIN;
 #pragma unroll 4
-        for (int v = v0 + (int)threadIdx.x; v < v1; v += kThreads) {
+        for (int v = v0 + me; v < v1; v += kTeam) {
             float f[kVec<T>];
             row.load(v, f);
 #pragma unroll
@@ -313,13 +396,15 @@ __device__ __noinline__ void select_rounds(const Row<T> &row, int v0, int v1, in
             }
         }
         best = __reduce_max_sync(0xffffffffu, best);
-        sync_adders();
-        if (lane == 0) s.count[warp] = best;
-        sync_adders();
-        for (int w = 0; w < kWarps; w++) best = max(best, s.count[w]);
+        if (!WARP) {
+            sync_adders();
+            if (lane == 0) count[warp] = best;
+            sync_adders();
+            for (int w = 0; w < kWarps; w++) best = max(best, count[w]);
+        }
         if (best == INT_MIN) break;
-        for (int base = v0; base < v1 && have < k; base += kThreads) {
-            const int v = base + (int)threadIdx.x;
+        for (int base = v0; base < v1 && have < k; base += kTeam) {
+            const int v = base + me;
             float f[kVec<T>];
             int n = 0;
             if (v < v1) {
@@ -333,26 +418,65 @@ __device__ __noinline__ void select_rounds(const Row<T> &row, int v0, int v1, in
                 const int u = __shfl_up_sync(0xffffffffu, before, o);
                 if (lane >= o) before += u;
             }
-            sync_adders();  // the counts of the round before have been read
-            if (lane == 31) s.count[warp] = before;
-            sync_adders();
-            int at = have + before - n, total = 0;
-            for (int w = 0; w < kWarps; w++) {
-                if (w < warp) at += s.count[w];
-                total += s.count[w];
+            int at = have + before - n, total = __shfl_sync(0xffffffffu, before, 31);
+            if (!WARP) {
+                sync_adders();  // the counts of the round before have been read
+                if (lane == 31) count[warp] = before;
+                sync_adders();
+                total = 0;
+                for (int w = 0; w < kWarps; w++) {
+                    if (w < warp) at += count[w];
+                    total += count[w];
+                }
             }
             if (n)
 #pragma unroll
                 for (int i = 0; i < kVec<T>; i++)
                     if (f[i] > -INFINITY && order_key(f[i]) == best) {
-                        if (at < k) s.top[at] = pair_key(f[i], row.first(v) + i);
+                        if (at < k) top[at] = pair_key(f[i], row.first(v) + i);
                         at++;
                     }
             have = min(k, have + total);
         }
         last = best;
     }
-    if (threadIdx.x == 0) s.n_top = have;
+    return have;
+}
+
+// A warp's values, the highest first.
+__device__ __forceinline__ float sort_lanes(float b, int lane) {
+#pragma unroll
+    for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+        for (int o = size >> 1; o; o >>= 1) {
+            const float other = __shfl_xor_sync(0xffffffffu, b, o);
+            const bool high = ((lane & o) == 0) == ((lane & size) == 0);  // descending overall
+            b = high ? fmaxf(b, other) : fminf(b, other);
+        }
+    return b;
+}
+
+// What a row's statistics say, by one thread; l = ln s0.
+template <bool ENTROPY>
+__device__ __forceinline__ void finish_row(const Params &p, int64_t t, const Stats &all, float l, bool ignored,
+                                           float target) {
+    const bool empty = all.m == -INFINITY;
+    const bool none = !(target > -INFINITY);
+    p.lse[t] = empty ? -INFINITY : all.m / p.temperature + l;
+    p.logprobs[t] = ignored ? 0.0f : empty || none ? -INFINITY : (target - all.m) / p.temperature - l;
+    if (ENTROPY) {
+        const float H = l - all.s1 / all.s0 * kLn2;
+        p.entropy[t] = empty || H < 0.0f ? 0.0f : H;  // below zero it is rounding
+    }
+}
+// An alternative, by a lane: the `lane`-th of n.
+__device__ __forceinline__ void put_top(const Params &p, int64_t t, const Stats &all, float l, const uint64_t *top,
+                                        int n, int lane) {
+    if (lane >= p.k) return;
+    const int64_t at = t * p.k + lane;
+    const float v = lane < n ? pair_value(top[lane]) : -INFINITY;
+    p.top_tokens[at] = lane < n ? pair_token(top[lane]) : -1;
+    p.top_logprobs[at] = lane < n ? (v - all.m) / p.temperature - l : -INFINITY;
 }
 
 template <typename T, bool ENTROPY, bool TOP>
@@ -438,66 +562,12 @@ __global__ void __launch_bounds__(kThreads + 32, kResident) logprobs_kernel(cons
             if (t + step < p.T) next = target_of(p.targets, p.target8, t + step);
         }
         // ---- the pass
-        float m = -INFINITY, r = 0.0f, rest = 0.0f;  // r: c m rounded, rest: what that left
-        uint64_t s0[2] = {0, 0}, s1[2] = {0, 0};
-        bool paired = false;
+        Sums<T, ENTROPY> sums;
         const int quarter = max(1, ((v1 - v0 + kBatch * kThreads - 1) / (kBatch * kThreads) + kQuarters - 1) / kQuarters);
         float high_quarter = -INFINITY;
-        auto add = [&](const auto &raw) {  // an array of vectors
-            constexpr int kN = (int)(sizeof(raw) / sizeof(uint4));
-            uint32_t top = Word<T>::top(raw[0]);
-#pragma unroll
-            for (int b = 1; b < kN; b++) top = Word<T>::join(top, Word<T>::top(raw[b]));
-            const float high = Word<T>::top_value(top);
+        auto add = [&](const auto &raw) {
+            const float high = sums.add(raw, p.c);
             if (TOP) high_quarter = fmaxf(high_quarter, high);
-            if (high > m) {
-                const float r_next = high * p.c;
-                const bool pairs = raises(Word<T>::kFloor, p.c, r_next) && fabsf(r_next) < 0x1p60f;
-                const float rest_next = pairs ? fmaf(high, p.c, -r_next) : 0.0f;
-                const float d = fmaxf((m - high) * p.c, kFar) - rest + rest_next, scale = ex2(d);
-                const uint64_t dd = pair(d, d), ss = pair(scale, scale);
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    if (ENTROPY) s1[i] = mul2(fma2(s0[i], dd, s1[i]), ss);
-                    s0[i] = mul2(s0[i], ss);
-                }
-                m = high;
-                r = r_next;
-                rest = rest_next;
-                paired = pairs;
-            }
-            if (paired) {
-                const uint64_t cc = pair(p.c, p.c), rr = pair(-r, -r);
-#pragma unroll
-                for (int b = 0; b < kN; b++) {
-                    uint64_t x[Word<T>::kPairs];
-                    Word<T>::raised(raw[b], x);
-#pragma unroll
-                    for (int i = 0; i < Word<T>::kPairs; i++) {
-                        const uint64_t d = fma2(x[i], cc, rr);
-                        const float2 f = unpair(d);
-                        const uint64_t e = pair(ex2(f.x), ex2(f.y));
-                        s0[i & 1] = add2(s0[i & 1], e);
-                        if (ENTROPY) s1[i & 1] = fma2(d, e, s1[i & 1]);
-                    }
-                }
-            } else {
-                // fmaxf takes the bound where the difference is NaN, of two infinities or of a NaN
-                float t0 = 0.0f, t1 = 0.0f;
-#pragma unroll
-                for (int b = 0; b < kN; b++) {
-                    float f[kVec<T>];
-                    unpack<T>(raw[b], f);
-#pragma unroll
-                    for (int i = 0; i < kVec<T>; i++) {
-                        const float d = fmaxf((f[i] - m) * p.c, kFar), e = ex2(d);
-                        t0 += e;
-                        if (ENTROPY) t1 = fmaf(d, e, t1);
-                    }
-                }
-                s0[0] = add2(s0[0], pair(t0, 0.0f));
-                if (ENTROPY) s1[0] = add2(s1[0], pair(t1, 0.0f));
-            }
         };
         {
             int left = quarter;
@@ -545,16 +615,8 @@ __global__ void __launch_bounds__(kThreads + 32, kResident) logprobs_kernel(cons
             if (TOP)
                 for (; best < &s.best[kQuarters][0]; best += kThreads) *best = -INFINITY;
         }
-        Stats a;
-        {
-            const float2 x = unpair(add2(s0[0], s0[1])), y = unpair(add2(s1[0], s1[1]));
-            const float sum0 = x.x + x.y, sum1 = y.x + y.y, back = ex2(-rest);
-            a.m = m;
-            a.s0 = sum0 * back;
-            a.s1 = ENTROPY ? fmaf(-rest, sum0, sum1) * back : 0.0f;
-        }
         // ---- statistics of the CTA
-        Stats w = a;
+        Stats w = sums.stats();
 #pragma unroll
         for (int o = 16; o; o >>= 1) w = join(w, shuffle(w, o), p);
         if (lane == 0) s.part[turn][warp] = w;
@@ -567,14 +629,7 @@ __global__ void __launch_bounds__(kThreads + 32, kResident) logprobs_kernel(cons
             for (int i = 0; i < kQuarters; i++)
 #pragma unroll
                 for (int w = 0; w < kWarps; w++) b = fmaxf(b, s.best[i][w * 32 + lane]);
-#pragma unroll
-            for (int size = 2; size <= 32; size <<= 1)
-#pragma unroll
-                for (int o = size >> 1; o; o >>= 1) {
-                    const float other = __shfl_xor_sync(0xffffffffu, b, o);
-                    const bool high = ((lane & o) == 0) == ((lane & size) == 0);  // descending overall
-                    b = high ? fmaxf(b, other) : fminf(b, other);
-                }
+            b = sort_lanes(b, lane);
             float bound = __shfl_sync(0xffffffffu, b, p.k - 1), high = __shfl_sync(0xffffffffu, b, 0);
             // of many alternatives the columns' bound is loose: while more than twice as many quarters as
             // there are alternatives reach it, halve the way up to the maximum, as far as enough still do
@@ -627,7 +682,8 @@ __global__ void __launch_bounds__(kThreads + 32, kResident) logprobs_kernel(cons
                 rank_keys(s.cand, n, p.k, s.top);
                 if (threadIdx.x == 0) s.n_top = min(n, p.k);
             } else {
-                select_rounds<T>(row, v0, v1, p.k, s);
+                const int n = select_rounds<T, false>(row, v0, v1, p.k, s.top, s.count);
+                if (threadIdx.x == 0) s.n_top = n;
             }
         }
         // ---- join the CTAs' parts, finish the row
@@ -652,16 +708,7 @@ __global__ void __launch_bounds__(kThreads + 32, kResident) logprobs_kernel(cons
                 all.s1 = __shfl_sync(0xffffffffu, all.s1, 0);
             }
             const float l = logf(all.s0);
-            if (threadIdx.x == 0) {
-                const bool empty = all.m == -INFINITY;
-                const bool none = !(target > -INFINITY);
-                p.lse[t] = empty ? -INFINITY : all.m / p.temperature + l;
-                p.logprobs[t] = ignored ? 0.0f : empty || none ? -INFINITY : (target - all.m) / p.temperature - l;
-                if (ENTROPY) {
-                    const float H = l - all.s1 / all.s0 * kLn2;
-                    p.entropy[t] = empty || H < 0.0f ? 0.0f : H;  // below zero it is rounding
-                }
-            }
+            if (threadIdx.x == 0) finish_row<ENTROPY>(p, t, all, l, ignored, target);
             if (TOP) {
                 int n = s.n_top;  // of this CTA
                 if (parts > 1) {
@@ -694,12 +741,7 @@ __global__ void __launch_bounds__(kThreads + 32, kResident) logprobs_kernel(cons
                     if (mine && rank < p.k) s.top[rank] = mine;
                     sync_adders();
                 }
-                if (warp == 0 && lane < p.k) {
-                    const int64_t at = t * p.k + lane;
-                    const float v = lane < n ? pair_value(s.top[lane]) : -INFINITY;
-                    p.top_tokens[at] = lane < n ? pair_token(s.top[lane]) : -1;
-                    p.top_logprobs[at] = lane < n ? (v - all.m) / p.temperature - l : -INFINITY;
-                }
+                if (warp == 0) put_top(p, t, all, l, s.top, n, lane);
             }
         }
         if (parts > 1) {
@@ -713,6 +755,131 @@ __global__ void __launch_bounds__(kThreads + 32, kResident) logprobs_kernel(cons
     }
 }
 
+// Short rows, a warp each, in the same steps: nothing waits for a CTA.
+template <typename T, bool ENTROPY, bool TOP>
+__global__ void __launch_bounds__(32 * kRowWarps, kRowResident) logprobs_rows_kernel(const Params p) {
+    __shared__ uint64_t cands[TOP ? kRowWarps : 1][kCandidates], tops[TOP ? kRowWarps : 1][kMaxTop];
+    __shared__ int counts[kRowWarps];
+    __shared__ uint8_t lists[kRowWarps][32 * kRowBatch];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t t = (int64_t)blockIdx.x * kRowWarps + warp;
+    if (t >= p.T) return;
+    const Row<T> row(static_cast<const T *>(p.logits) + t * p.ld, p.V);
+    const int nv = row.vectors(), w0 = row.whole0(), w1 = row.whole1();
+    const uint4 masked = make_uint4(Word<T>::kMasked, Word<T>::kMasked, Word<T>::kMasked, Word<T>::kMasked);
+    auto load = [&](int v, uint4 (&raw)[kRowBatch]) {
+#pragma unroll
+        for (int b = 0; b < kRowBatch; b++) raw[b] = v + b * 32 < w1 ? row.whole(v + b * 32) : masked;
+    };
+    uint4 next[kRowBatch];
+    load(w0 + lane, next);
+    const int64_t at = lane == 0 ? target_of(p.targets, p.target8, t) : -1;
+    // the vectors that the row begins and ends in
+    const int edge = lane == 0 && w0 ? 0 : lane == 1 && w1 < nv && nv > w0 ? nv - 1 : -1;
+    uint4 ends[1] = {edge >= 0 ? row.any(edge) : masked};
+    const bool ignored = at < 0 || at >= p.V;
+    const float target = ignored ? -INFINITY : to_float<T>(row.x[at]);
+    Sums<T, ENTROPY> sums;
+    uint32_t best[kRowBatch];  // maxima of the lane's vectors, by their place in the batch
+#pragma unroll
+    for (int b = 0; b < kRowBatch; b++) best[b] = Word<T>::kMasked;
+    for (int v = w0; v < w1; v += 32 * kRowBatch) {
+        uint4 raw[kRowBatch];
+#pragma unroll
+        for (int b = 0; b < kRowBatch; b++) raw[b] = next[b];
+        if (v + 32 * kRowBatch < w1) load(v + 32 * kRowBatch + lane, next);
+        sums.add(raw, p.c);
+        if (TOP)
+#pragma unroll
+            for (int b = 0; b < kRowBatch; b++) best[b] = Word<T>::join(best[b], Word<T>::top(raw[b]));
+    }
+    if (w0 || w1 < nv) sums.add(ends, p.c);
+    Stats all = sums.stats();
+#pragma unroll
+    for (int o = 16; o; o >>= 1) all = join(all, shuffle(all, o), p);
+    // lane 0's for all: a join's two sides round differently
+    all.m = __shfl_sync(0xffffffffu, all.m, 0);
+    all.s0 = __shfl_sync(0xffffffffu, all.s0, 0);
+    const float l = logf(all.s0);
+    if (lane == 0) finish_row<ENTROPY>(p, t, all, l, ignored, target);
+    if constexpr (TOP) {
+        uint64_t *cand = cands[warp], *top = tops[warp];
+        int *n_cand = &counts[warp];
+        uint8_t *list = lists[warp];
+        // the k-th highest of the lanes' maxima, then, while more than twice as many of their four
+        // parts each as there are alternatives reach it, halfway up to the highest
+        float part[kRowBatch], b = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kRowBatch; i++) b = fmaxf(b, part[i] = Word<T>::top_value(best[i]));
+        b = sort_lanes(b, lane);
+        float bound = __shfl_sync(0xffffffffu, b, p.k - 1), high = __shfl_sync(0xffffffffu, b, 0);
+        auto reached = [&](float v) {
+            int n = 0;
+#pragma unroll
+            for (int i = 0; i < kRowBatch; i++) n += part[i] >= v;
+            return __reduce_add_sync(0xffffffffu, n);
+        };
+        if (bound > -INFINITY) {
+            int n = reached(bound);
+            for (int i = 0; i < 6 && n > 2 * p.k; i++) {
+                const float mid = 0.5f * bound + 0.5f * high;
+                const int at = reached(mid);
+                if (at >= p.k) {
+                    bound = mid;
+                    n = at;
+                } else {
+                    high = mid;
+                }
+            }
+        }
+        int winners = 0;
+#pragma unroll
+        for (int i = 0; i < kRowBatch; i++) {
+            const bool wins = part[i] > -INFINITY && part[i] >= bound;
+            const uint32_t all = __ballot_sync(0xffffffffu, wins);
+            if (wins) list[winners + __popc(all & ((1u << lane) - 1u))] = (uint8_t)(i * 32 + lane);
+            winners += __popc(all);
+        }
+        if (lane == 0) *n_cand = 0;
+        __syncwarp();
+        auto take = [&](const uint4 &raw, int v) {
+            float f[kVec<T>];
+            unpack<T>(raw, f);
+#pragma unroll
+            for (int e = 0; e < kVec<T>; e++)
+                if (f[e] > -INFINITY && f[e] >= bound) {
+                    const int i = atomicAdd(n_cand, 1);
+                    if (i < kCandidates) cand[i] = pair_key(f[e], row.first(v) + e);
+                }
+        };
+        if (edge >= 0) take(ends[0], edge);
+        const int per = (w1 - w0 + 32 * kRowBatch - 1) / (32 * kRowBatch), items = per * winners;
+#pragma unroll 4
+        for (int i = lane; i < items; i += 32) {
+            const int which = i / per, v = w0 + list[which] + (i - which * per) * 32 * kRowBatch;
+            if (v >= w1) continue;
+            const uint4 raw = row.whole(v);
+            if (Word<T>::top_value(Word<T>::top(raw)) >= bound) take(raw, v);
+        }
+        __syncwarp();
+        int n = *(volatile int *)n_cand;
+        if (n <= kCandidates) {
+            for (int i = lane; i < n; i += 32) {
+                const uint64_t mine = cand[i];
+                int rank = 0;
+#pragma unroll 8
+                for (int j = 0; j < n; j++) rank += cand[j] > mine;
+                if (rank < p.k) top[rank] = mine;
+            }
+            n = min(n, p.k);
+        } else {
+            n = select_rounds<T, true>(row, 0, nv, p.k, top, nullptr);
+        }
+        __syncwarp();
+        put_top(p, t, all, l, top, n, lane);
+    }
+}
+
 // ------------------------------------------------------------------------- gradient
 struct GradParams {
     const float *dlogprobs, *dentropy, *lse, *entropy;
@@ -721,7 +888,9 @@ struct GradParams {
     int64_t ld, ldd;
     int target8;
     int V, W;
+    int64_t n_rows;
     int chunks;  // CTAs of a row
+    int wide;    // log2 of a row's threads in a CTA, which has several short rows
     float inv_temperature;
 };
 
@@ -729,11 +898,20 @@ constexpr int kGradThreads = 256;
 constexpr int kGradBatch = 4;
 
 // Elementwise, with the row's scalars in registers: bound by reading and writing the logits.
-// SAME: the gradient's rows have the logits' alignment, so whole vectors go out.
-template <typename T, bool SAME>
+// SAME: the gradient's rows have the logits' alignment, so whole vectors go out.  SHORT: a CTA
+// has several rows (16000 of 1500 50 -> 30 us; with long ones in the same code 326 -> 381).
+template <typename T, bool SAME, bool SHORT>
 __global__ void __launch_bounds__(kGradThreads) logprobs_grad_kernel(const GradParams p) {
-    const int64_t t = blockIdx.x / p.chunks;
-    const int chunk = (int)(blockIdx.x - t * p.chunks);
+    const int team = SHORT ? 1 << p.wide : kGradThreads, me = SHORT ? threadIdx.x & (team - 1) : threadIdx.x;
+    int64_t t;
+    int chunk = 0;
+    if constexpr (SHORT) {
+        t = (int64_t)blockIdx.x * (kGradThreads >> p.wide) + (threadIdx.x >> p.wide);
+        if (t >= p.n_rows) return;
+    } else {
+        t = blockIdx.x / p.chunks;
+        chunk = (int)(blockIdx.x - t * p.chunks);
+    }
     const T *x = static_cast<const T *>(p.logits) + t * p.ld;
     T *d = static_cast<T *>(p.dlogits) + t * p.ldd;
     const int64_t target = target_of(p.targets, p.target8, t);
@@ -768,17 +946,17 @@ __global__ void __launch_bounds__(kGradThreads) logprobs_grad_kernel(const GradP
     if constexpr (SAME) {
         const Row<T> row(x, p.W);
         const int nv = row.vectors();
-        const int64_t v0 = (int64_t)chunk * kGradBatch * kGradThreads + threadIdx.x;
+        const int64_t v0 = (int64_t)chunk * kGradBatch * kGradThreads + me;
         uint4 raw[kGradBatch];
 #pragma unroll
         for (int i = 0; i < kGradBatch; i++) {
-            const int64_t v = v0 + i * kGradThreads;
+            const int64_t v = v0 + i * team;
             const int64_t e = v * kVec<T> - row.shift;
             if (v < nv && e >= 0 && e + kVec<T> <= p.W) raw[i] = *reinterpret_cast<const uint4 *>(x + e);
         }
 #pragma unroll
         for (int i = 0; i < kGradBatch; i++) {
-            const int64_t v = v0 + i * kGradThreads;
+            const int64_t v = v0 + i * team;
             if (v >= nv) break;
             const int64_t e = v * kVec<T> - row.shift;
             if (e >= 0 && e + kVec<T> <= p.W) {
@@ -812,10 +990,10 @@ __global__ void __launch_bounds__(kGradThreads) logprobs_grad_kernel(const GradP
             }
         }
     } else {
-        const int64_t e0 = (int64_t)chunk * kGradBatch * kGradThreads * kVec<T> + threadIdx.x;
+        const int64_t e0 = (int64_t)chunk * kGradBatch * kGradThreads * kVec<T> + me;
 #pragma unroll 4
         for (int i = 0; i < kGradBatch * kVec<T>; i++) {
-            const int64_t e = e0 + i * kGradThreads;
+            const int64_t e = e0 + i * team;
             if (e < p.W) d[e] = put(grad(to_float<T>(x[e]), e));
         }
     }
@@ -837,8 +1015,21 @@ static int parts_of(int T, int64_t vectors, bool top, int sm_count) {
     return parts;
 }
 
+// Whether a row is a warp's: short ones of which there are many.  us, a CTA a row and a warp a
+// row, bf16 with entropy: 16000 rows of 1000 90 and 15, with 8 alternatives 195 and 25; of 8000
+// 136 and 52, 231 and 75; 592 rows of 4000 8.8 and 7.4, 15 and 11; 1200 of 8000 16 and 13, 23 and
+// 17; 2400 of 16000 29 and 25, 46 and 35; but 256 of 8000 8.8 and 10.6, 2400 of 32000 39 and 45.
+static bool short_rows(int T, int64_t bytes, int sm_count) {
+    return bytes <= 32768 && T > kResident * sm_count * std::max<int64_t>(1, bytes / 8192);
+}
+
 template <typename T, bool ENTROPY, bool TOP>
 static int launch(const Params &p, const DeviceInfo &di, cudaStream_t s) {
+    if (short_rows(p.T, p.V * (int64_t)sizeof(T), di.sm_count)) {
+        logprobs_rows_kernel<T, ENTROPY, TOP><<<(unsigned)((p.T + kRowWarps - 1) / kRowWarps), 32 * kRowWarps, 0, s>>>(p);
+        count_launch();
+        return cuda_status(cudaGetLastError());
+    }
     const int parts = parts_of(p.T, p.V / kVec<T>, TOP, di.sm_count);
     static std::atomic<bool> configured[64] = {};
     if (!configured[di.device].load(std::memory_order_acquire)) {
@@ -881,9 +1072,19 @@ static int backward(GradParams p, int64_t n_rows, cudaStream_t s) {
     const uintptr_t from = reinterpret_cast<uintptr_t>(p.logits), to = reinterpret_cast<uintptr_t>(p.dlogits);
     const bool same = ((from - to) & 15u) == 0 && ((p.ld - p.ldd) * (int64_t)sizeof(T)) % 16 == 0;
     p.chunks = grad_chunks(p.W, sizeof(T));
-    const unsigned grid = (unsigned)(n_rows * p.chunks);
-    if (same) logprobs_grad_kernel<T, true><<<grid, kGradThreads, 0, s>>>(p);
-    else logprobs_grad_kernel<T, false><<<grid, kGradThreads, 0, s>>>(p);
+    // a short row's threads: as many as have four vectors each, 32 at least
+    const int64_t vectors = ((int64_t)p.W + 2 * kVec<T> - 2) / kVec<T>;
+    for (p.wide = 5; (kGradBatch << p.wide) < vectors && (1 << p.wide) < kGradThreads;) p.wide++;
+    p.n_rows = n_rows;
+    const int64_t rows = kGradThreads >> p.wide;
+    const unsigned grid = (unsigned)(rows > 1 ? (n_rows + rows - 1) / rows : n_rows * p.chunks);
+    if (rows > 1) {
+        if (same) logprobs_grad_kernel<T, true, true><<<grid, kGradThreads, 0, s>>>(p);
+        else logprobs_grad_kernel<T, false, true><<<grid, kGradThreads, 0, s>>>(p);
+    } else {
+        if (same) logprobs_grad_kernel<T, true, false><<<grid, kGradThreads, 0, s>>>(p);
+        else logprobs_grad_kernel<T, false, false><<<grid, kGradThreads, 0, s>>>(p);
+    }
     count_launch();
     return cuda_status(cudaGetLastError());
 }

@@ -264,6 +264,49 @@ def test_logprobs_ties(nv, cuda_dev, dtype, T):
         check_logprobs(nv, x, t, None, k, grad=False)
 
 
+@pytest.mark.parametrize("dtype", DT + [torch.float32])
+@pytest.mark.parametrize("T,vocab,W", [(600, 1, 1), (641, 7, 7), (600, 40, 40), (700, 1000, 1003), (650, 2040, 2056),
+                                       (1300, 4001, 4001), (2500, 8100, 8104)])
+def test_logprobs_many_short_rows(nv, cuda_dev, dtype, T, vocab, W):
+    """Rows that a warp takes each, and gradients of several rows a CTA."""
+    x = logits_of(T, W, dtype, vocab)
+    for k, entropy, temperature in ((0, False, 1.0), (8, True, 0.7), (32, True, 1.0)):
+        check_logprobs(nv, x, targets_of(T, vocab, k), vocab, k, temperature, entropy)
+
+
+@pytest.mark.parametrize("dtype", DT + [torch.float32])
+@pytest.mark.parametrize("n", [9, 300, 3001])
+def test_logprobs_many_short_rows_forms(nv, cuda_dev, dtype, n):
+    """The same with masks, ties, rows of any alignment, maxima that move at every step."""
+    T = 1000
+    low = torch.finfo(dtype).min
+    wide = logits_of(T, n + 20, dtype, 3, masked=0.4)
+    for first in (0, 1, 5, 8):
+        x = wide[:, first:first + n]
+        x[0] = -math.inf
+        x[1] = math.nan
+        x[2] = low
+        x[3] = -math.inf
+        x[3, 7] = 1.5
+        x[4, ::3] = math.nan
+        x[5] = 2.5
+        x[6] = torch.randint(0, 3, (n,), device="cuda", generator=gen(1)).to(dtype)
+        x[7] = (torch.arange(n, device="cuda") / 8).to(dtype)
+        x[8] = (-torch.arange(n, device="cuda") / 8).to(dtype)
+        x[9] = torch.linspace(-3e4, 3e4, n).to(dtype)
+        t = targets_of(T, n, first)
+        t[0], t[3], t[4], t[9] = 2, 7, 3, n - 1
+        for k in (0, 1, 8, 20, 32):
+            r = check_logprobs(nv, x, t, None, k)
+            assert r.logprobs[0] == -math.inf and r.entropy[0] == 0
+        check_logprobs(nv, x, t, None, 0, out=torch.empty_like(wide)[:, first + 1:first + n + 1])
+        d = nv.token_logprobs_backward(torch.ones(T, device="cuda"), x, t, r, torch.ones(T, device="cuda"))
+        assert not d[~(x > -math.inf)].any() and torch.isfinite(d).all()
+        own = x.clone()
+        assert torch.equal(nv.token_logprobs_backward(torch.ones(T, device="cuda"), own, t, r,
+                                                      torch.ones(T, device="cuda"), out=own), d)
+
+
 def test_logprobs_far_values(nv, cuda_dev):
     """Probabilities that underflow, and maxima that move at every step."""
     n = 9000
