@@ -12,6 +12,7 @@
 // matching lanes and per-warp counts, never from atomics' order.  A launch counts the first
 // digits by chunk; each pass counts the next ones as it puts the tokens into their new chunks.
 #include <algorithm>
+#include <atomic>
 #include <climits>
 
 #include "common.cuh"
@@ -69,7 +70,6 @@ __global__ void __launch_bounds__(kLookupThreads) embedding_kernel(const LookupP
 
 // ------------------------------------------------------------------------- sorting
 constexpr int kSortThreads = 1024;
-constexpr int kSmallTokens = 1024;  // 55 steps of one CTA; 4096 would be 78 of four times the keys, 35 us
 constexpr int kMaxBits = 9;              // of a pass
 constexpr int kMaxDigits = 1 << kMaxBits;
 constexpr int kMaxChunks = 256;
@@ -105,31 +105,6 @@ __device__ __forceinline__ bool write_zeros(const SortParams &p) {
 __device__ __forceinline__ int key_of(const SortParams &p, int64_t t) {
     const int64_t token = p.wide ? static_cast<const int64_t *>(p.tokens)[t] : static_cast<const int *>(p.tokens)[t];
     return token >= 0 && token < p.V ? (int)token : p.V;
-}
-
-// Bitonic sort of n (a power of two) keys that are all different, so it is stable.
-__global__ void __launch_bounds__(kSortThreads) sort_small_kernel(const SortParams p, int n) {
-    extern __shared__ uint64_t key[];
-    if (write_zeros(p)) return;
-    for (int i = threadIdx.x; i < n; i += kSortThreads)
-        key[i] = i < p.T ? (uint64_t)(uint32_t)key_of(p, i) << 32 | (uint32_t)i : ~0ull;
-    __syncthreads();
-    for (int size = 2; size <= n; size <<= 1)
-        for (int o = size >> 1; o; o >>= 1) {
-            for (int i = threadIdx.x; i < n / 2; i += kSortThreads) {
-                const int a = 2 * i - (i & (o - 1)), b = a + o;
-                const uint64_t x = key[a], y = key[b];
-                if ((x > y) == ((a & size) == 0)) {
-                    key[a] = y;
-                    key[b] = x;
-                }
-            }
-            __syncthreads();
-        }
-    for (int i = threadIdx.x; i < p.T; i += kSortThreads) {
-        p.keys[i] = (int)(key[i] >> 32);
-        p.at[i] = (int)(uint32_t)key[i];
-    }
 }
 
 __device__ __forceinline__ int load_key(const SortParams &p, int64_t t) { return p.keys_in ? p.keys_in[t] : key_of(p, t); }
@@ -245,6 +220,155 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(const SortPa
     }
 }
 
+// ------------------------------------------------------------------------- zeros
+// Zeros for those of n rows of `vecs` vectors whose bit is not set, by THREADS threads.
+template <typename T, int THREADS>
+__device__ __forceinline__ void zero_rows(T *d, const uint32_t *named, int n, int vecs) {
+    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+    uint4 *to = reinterpret_cast<uint4 *>(d);
+    if (vecs >= THREADS) {
+        for (int r = 0; r < n; r++, to += vecs)
+            if (!((named[r >> 5] >> (r & 31)) & 1u))
+                for (int c = threadIdx.x; c < vecs; c += THREADS) to[c] = zero;
+    } else {  // threads over the rows too
+        for (int i = threadIdx.x; i < n * vecs; i += THREADS) {
+            const int r = i / vecs;
+            if (!((named[r >> 5] >> (r & 31)) & 1u)) to[i] = zero;
+        }
+    }
+}
+
+// ------------------------------------------------------------------------- few tokens
+// One launch: every CTA has all tokens in shared memory.  A warp looks for the places of its
+// token, gives up if there is one before its own, and sums the rows; runs longer than kLongRun
+// are cut between the CTA's warps.  CTAs between them write zeros to the rows that no token names.
+constexpr int kFewThreads = 256, kFewWarps = kFewThreads / 32;
+constexpr int kFewTokens = 2048;
+constexpr int kLongRun = 32;
+constexpr int kFewCols = 32 * 8;     // columns of a warp at a time
+constexpr int kFewAhead = 8;         // rows on their way
+constexpr int kFewFill = 256;        // most rows of a CTA that writes zeros
+
+struct FewParams {
+    const void *dy, *tokens;
+    int64_t ld;
+    void *d;
+    float scale;
+    int T, V, K, cols, slabs;  // columns of a CTA; CTAs for a token
+    int sum_ctas, fill_ctas, fill_rows;
+};
+
+template <typename T, typename I>
+__global__ void __launch_bounds__(kFewThreads) embedding_few_kernel(const FewParams p) {
+    extern __shared__ int4 key4[];  // [padded tokens / 4], and then each warp's places
+    int *key = reinterpret_cast<int *>(key4);
+    const int padded = (p.T + 127) & ~127, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int i = threadIdx.x; i < padded; i += kFewThreads) {
+        const int64_t token = i < p.T ? (int64_t)static_cast<const I *>(p.tokens)[i] : -1;
+        key[i] = token >= 0 && token < p.V ? (int)token : -1;
+    }
+    __syncthreads();
+    // CTA i of sum_ctas + fill_ctas: how many of the first i are sums, and whether this one is
+    const int64_t all = (int64_t)p.sum_ctas + p.fill_ctas;
+    const int sums = (int)((int64_t)blockIdx.x * p.sum_ctas / all);
+    if ((int)(((int64_t)blockIdx.x + 1) * p.sum_ctas / all) == sums) {
+        __shared__ uint32_t named[kFewFill / 32];  // a bit a row
+        const int64_t v0 = (int64_t)((int)blockIdx.x - sums) * p.fill_rows;
+        const int n = (int)min((int64_t)p.fill_rows, p.V - v0);
+        if (threadIdx.x < kFewFill / 32) named[threadIdx.x] = 0u;
+        __syncthreads();
+        for (int i = threadIdx.x; i < p.T; i += kFewThreads) {
+            const int64_t at = key[i] - v0;
+            if (at >= 0 && at < n) atomicOr(&named[at >> 5], 1u << (at & 31));
+        }
+        __syncthreads();
+        zero_rows<T, kFewThreads>(static_cast<T *>(p.d) + v0 * p.K, named, n, p.K / 8);
+        return;
+    }
+    __shared__ int runs[kFewWarps];
+    __shared__ float part[kFewWarps][kFewCols];
+    const int group = sums / p.slabs, slab = sums - group * p.slabs, t = group * kFewWarps + warp;
+    uint16_t *places = reinterpret_cast<uint16_t *>(key + padded), *mine = places + warp * padded;
+    const int token = t < p.T ? key[t] : -1;
+    int n = 0;
+    if (token >= 0)
+        for (int j = 0; j < padded; j += 128) {
+            const int4 k = key4[j / 4 + lane];
+            const int hits = (k.x == token) | (k.y == token) << 1 | (k.z == token) << 2 | (k.w == token) << 3;
+            const uint32_t any = __ballot_sync(0xffffffffu, hits != 0);
+            if (!any) continue;
+            const int here = j + 4 * lane;
+            if (n == 0) {
+                const int first = __shfl_sync(0xffffffffu, here + __ffs(hits) - 1, __ffs(any) - 1);
+                if (first < t) break;  // another warp's
+            }
+            int upto = __popc(hits);
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += u;
+            }
+            int at = n + upto - __popc(hits);
+#pragma unroll
+            for (int b = 0; b < 4; b++)
+                if (hits >> b & 1) mine[at++] = (uint16_t)(here + b);
+            n += __shfl_sync(0xffffffffu, upto, 31);
+        }
+    if (lane == 0) runs[warp] = n;
+    __syncthreads();
+    const T *dy = static_cast<const T *>(p.dy);
+    const int c0 = slab * p.cols, c1 = min(p.K, c0 + p.cols);
+    // rows list[i0] to list[i1 - 1], eight columns from c on, in order
+    auto add_rows = [&](const uint16_t *list, int i0, int i1, int c, float (&sum)[8]) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) sum[e] = 0.0f;
+        for (int i = i0; i < i1; i += kFewAhead) {
+            uint4 row[kFewAhead];
+#pragma unroll
+            for (int j = 0; j < kFewAhead; j++)
+                if (i + j < i1) row[j] = __ldg(reinterpret_cast<const uint4 *>(dy + list[i + j] * p.ld + c));
+#pragma unroll
+            for (int j = 0; j < kFewAhead; j++)
+                if (i + j < i1) {
+                    float f[8];
+                    unpack8<T>(row[j], f);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) sum[e] += f[e];
+                }
+        }
+    };
+    if (n > 0 && n <= kLongRun)
+        for (int c = c0 + lane * 8; c < c1; c += kFewCols) {
+            float sum[8];
+            add_rows(mine, 0, n, c, sum);
+#pragma unroll
+            for (int e = 0; e < 8; e++) sum[e] *= p.scale;
+            *reinterpret_cast<uint4 *>(static_cast<T *>(p.d) + (int64_t)token * p.K + c) = pack8<T>(sum);
+        }
+    for (int w = 0; w < kFewWarps; w++) {
+        const int run = runs[w];
+        if (run <= kLongRun) continue;  // the same for all
+        T *to = static_cast<T *>(p.d) + (int64_t)key[group * kFewWarps + w] * p.K;
+        for (int base = c0; base < c1; base += kFewCols) {
+            const int c = base + lane * 8;
+            if (c < c1) {
+                float sum[8];
+                add_rows(places + w * padded, run * warp / kFewWarps, run * (warp + 1) / kFewWarps, c, sum);
+#pragma unroll
+                for (int e = 0; e < 8; e++) part[warp][lane * 8 + e] = sum[e];
+            }
+            __syncthreads();
+            if (base + (int)threadIdx.x < c1) {
+                float sum = part[0][threadIdx.x];
+#pragma unroll
+                for (int i = 1; i < kFewWarps; i++) sum += part[i][threadIdx.x];
+                to[base + threadIdx.x] = Type16<T>::round(sum * p.scale);
+            }
+            __syncthreads();
+        }
+    }
+}
+
 // ------------------------------------------------------------------------- sums
 constexpr int kSumThreads = 256;
 constexpr int kSumCols = kSumThreads * 8;  // columns of a CTA, for narrow rows several blocks' in one
@@ -312,13 +436,7 @@ __device__ __forceinline__ void fill(const SumParams &p, int64_t v0, int64_t end
         }
     }
     __syncthreads();
-    const int vecs = p.K / 8;
-    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-    for (int r = 0; r < n; r++) {
-        if ((named[r >> 5] >> (r & 31)) & 1u) continue;
-        uint4 *to = reinterpret_cast<uint4 *>(static_cast<T *>(p.d) + (v0 + r) * p.K);
-        for (int c = threadIdx.x; c < vecs; c += THREADS) to[c] = zero;
-    }
+    zero_rows<T, THREADS>(static_cast<T *>(p.d) + v0 * p.K, named, n, p.K / 8);
 }
 
 // Sums, and CTAs that write zeros between them, so that both are on every SM: the sums wait for
@@ -479,6 +597,21 @@ static Layout layout(int T, int K) {
     return l;
 }
 
+template <typename T, typename I>
+static int few(const FewParams &p, const DeviceInfo &di, cudaStream_t s) {
+    const int padded = (p.T + 127) & ~127;
+    static std::atomic<bool> configured[64] = {};
+    if (!configured[di.device]) {
+        if (cudaFuncSetAttribute(embedding_few_kernel<T, I>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 kFewTokens * (4 + 2 * kFewWarps)) != cudaSuccess)
+            return NVFP4_ERR_CUDA;
+        configured[di.device] = true;
+    }
+    embedding_few_kernel<T, I><<<(unsigned)(p.sum_ctas + p.fill_ctas), kFewThreads, padded * (4 + 2 * kFewWarps), s>>>(p);
+    count_launch();
+    return cuda_status(cudaGetLastError());
+}
+
 template <typename T>
 static int sum(const SumParams &p, cudaStream_t s) {
     embedding_sum_kernel<T><<<(unsigned)(p.sum_ctas + p.fill_ctas), kSumThreads, 0, s>>>(p);
@@ -493,7 +626,7 @@ static int sum(const SumParams &p, cudaStream_t s) {
 
 // Bytes of zeros that go out while a launch of the sort or the joins runs, about: a count takes
 // 3.5 us, a scatter 7, one CTA 10 for 4096 tokens and less for fewer, the joins 8.
-constexpr int64_t kCountZeros = 32 << 20, kScatterZeros = 56 << 20, kSmallZeros = 56 << 20, kJoinZeros = 40 << 20;
+constexpr int64_t kCountZeros = 32 << 20, kScatterZeros = 56 << 20, kJoinZeros = 40 << 20;
 
 // Sorts the tokens; l.keys[0] and l.at[0] hold the result, or [1] if it returns 1 in *which.
 // The first *zero_rows rows of the table are zeros afterwards.
@@ -519,16 +652,6 @@ static int sort(const void *tokens, int wide, int T, int V, int K, void *table, 
         *zero_rows += rows;
         return (unsigned)(sort_ctas + (p.zeros + kZeroVectors - 1) / kZeroVectors);
     };
-    if (T <= kSmallTokens) {
-        int n = 1;
-        while (n < T) n *= 2;
-        p.keys = reinterpret_cast<int *>(ws + l.keys[0]);
-        p.at = reinterpret_cast<int *>(ws + l.at[0]);
-        sort_small_kernel<<<zeros(kSmallZeros * (n + 512) / (kSmallTokens + 512), 1), kSortThreads,
-                            n * sizeof(uint64_t), s>>>(p, n);
-        count_launch();
-        return cuda_status(cudaGetLastError());
-    }
     int bits = 1;  // of the largest key, V
     while (bits < 31 && (V >> bits) != 0) bits++;
     const int passes = (bits + kMaxBits - 1) / kMaxBits;
@@ -627,7 +750,7 @@ int nvfp4_embedding(const void *tokens, int token_bytes, const void *table, int6
 size_t nvfp4_embedding_backward_workspace_size(int T, int V, int K) {
     if (T < 1 || V < 1 || K < 8 || T > embedding::kMaxRows || V > embedding::kMaxRows || K > embedding::kMaxRows)
         return 0;
-    return embedding::layout(T, K).bytes;
+    return T <= embedding::kFewTokens ? 0 : embedding::layout(T, K).bytes;
 }
 
 int nvfp4_embedding_backward(const void *dY, int64_t ldy, const void *tokens, int token_bytes, float scale,
@@ -637,8 +760,8 @@ int nvfp4_embedding_backward(const void *dY, int64_t ldy, const void *tokens, in
     if (st) return st;
     if (!dTable || (T && !dY)) return NVFP4_ERR_INVALID;
     if (!aligned16(dY) || !aligned16(dTable) || !aligned16(workspace)) return NVFP4_ERR_ALIGN;
-    if (T && (!workspace || workspace_bytes < nvfp4_embedding_backward_workspace_size(T, V, K)))
-        return NVFP4_ERR_WORKSPACE;
+    const size_t need = nvfp4_embedding_backward_workspace_size(T, V, K);
+    if (need && (!workspace || workspace_bytes < need)) return NVFP4_ERR_WORKSPACE;
     const int slabs = (K + embedding::kSumCols - 1) / embedding::kSumCols;
     const embedding::Layout l = embedding::layout(T, K);
     if ((int64_t)l.blocks * std::max(slabs, (K + embedding::kJoinCols - 1) / embedding::kJoinCols) > INT_MAX)
@@ -648,6 +771,32 @@ int nvfp4_embedding_backward(const void *dY, int64_t ldy, const void *tokens, in
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (T == 0)  // no token: the gradient is zero
         return cuda_status(cudaMemsetAsync(dTable, 0, (size_t)V * K * 2, s));
+    // rows of zeros: about 256 KB a CTA, and 64 KB beside the joins
+    const int fill_rows = (int)std::max<int64_t>(1, std::min<int64_t>(256, (256 << 10) / ((int64_t)K * 2)));
+    if (T <= embedding::kFewTokens) {
+        embedding::FewParams p = {};
+        p.dy = dY;
+        p.tokens = tokens;
+        p.ld = ldy;
+        p.d = dTable;
+        p.scale = scale;
+        p.T = T;
+        p.V = V;
+        p.K = K;
+        // the narrowest CTAs, for latency, that still run all at once
+        const int64_t groups = (T + embedding::kFewWarps - 1) / embedding::kFewWarps;
+        p.cols = embedding::kFewCols;
+        while (groups * ((K + p.cols - 1) / p.cols) > 4 * di.sm_count && p.cols < K) p.cols *= 2;
+        p.slabs = (K + p.cols - 1) / p.cols;
+        p.fill_rows = fill_rows;
+        p.fill_ctas = (V + fill_rows - 1) / fill_rows;
+        if (groups * p.slabs + p.fill_ctas > INT_MAX) return NVFP4_ERR_SHAPE;
+        p.sum_ctas = (int)(groups * p.slabs);
+        if (dtype == NVFP4_BF16)
+            return token_bytes == 8 ? embedding::few<__nv_bfloat16, int64_t>(p, di, s)
+                                    : embedding::few<__nv_bfloat16, int>(p, di, s);
+        return token_bytes == 8 ? embedding::few<__half, int64_t>(p, di, s) : embedding::few<__half, int>(p, di, s);
+    }
     uint8_t *ws = static_cast<uint8_t *>(workspace);
     int which = 0, zero_rows = 0;
     if ((st = embedding::sort(tokens, token_bytes == 8, T, V, K, dTable, ws, l, &which, &zero_rows, s))) return st;
@@ -670,8 +819,7 @@ int nvfp4_embedding_backward(const void *dY, int64_t ldy, const void *tokens, in
     p.sum_ctas = (l.blocks + p.per_cta - 1) / p.per_cta * slabs;
     p.join_ctas = (l.blocks + embedding::kJoinBlocks - 1) / embedding::kJoinBlocks *
                   ((K + embedding::kJoinCols - 1) / embedding::kJoinCols);
-    // about 256 KB a CTA, and 64 KB beside the joins
-    p.fill_rows = (int)std::max<int64_t>(1, std::min<int64_t>(256, (256 << 10) / ((int64_t)K * 2)));
+    p.fill_rows = fill_rows;
     p.join_rows = (p.fill_rows + 3) / 4;
     p.fill_from = zero_rows;
     p.fill_end = V;

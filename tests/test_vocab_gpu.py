@@ -65,7 +65,9 @@ def check_embedding_backward(nv, dy, t, rows, scale=1.0):
 
 @pytest.mark.parametrize("dtype", DT)
 @pytest.mark.parametrize("T,rows,K", [(1, 1, 8), (1, 70, 4096), (31, 5, 64), (32, 5, 64), (33, 5, 72), (64, 1, 2056),
-                                      (65, 1000, 128), (1000, 63, 264), (4096, 64, 40), (4096, 5000, 256)])
+                                      (65, 1000, 128), (1000, 63, 264), (4096, 64, 40), (4096, 5000, 256),
+                                      (7, 300, 8200), (900, 40, 1032), (1024, 3000, 520), (1025, 9, 8), (2047, 700, 2056),
+                                      (2048, 30, 16), (2049, 30, 64), (129, 2000, 4104)])
 def test_embedding_backward_small(nv, cuda_dev, dtype, T, rows, K):
     dy = torch.randn(T, K, device="cuda", generator=gen(T)).to(dtype)
     for seed, (common, padded) in enumerate([(0.0, 0.0), (0.5, 0.2), (1.0, 0.0), (0.0, 1.0)]):
