@@ -579,16 +579,22 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // ------------------------------------------------------------------------- host side
-// Whether the kernel above takes the layer, or two products by row group (moe_products.cu): up
-// to 8 tokens, one tile of rows at most; beyond them while an expert has up to four rows on
-// average (its rows are brought to every unit) and a unit has two stages or more (its sums take
-// longer than one stage's weights).  us, this kernel and the products: 8 tokens by 8 of 8
-// experts of 2048 x 4096 76 and 85, 16 by 2 73 and 83, by 4 88 and 84, by 8 105 and 85; 32 by 8
-// of 256 of 2048 x 768 263 and 264; 64 by 4 of 256 of 768 x 512 114 and 98.
-static bool streamed(int T, int E, int k, int K, int F) { return T <= 8 || (T * k <= 4 * E && K + F >= 2048); }
+// Whether the kernel above takes the layer, or two products by row group (moe_products.cu).  An
+// expert's rows are brought to every unit, so few of them: up to 8 tokens, one tile at most, or
+// four rows on average.  Beyond 8 tokens units of two stages and more, since a unit's sums take
+// longer than one stage's weights.  us, this kernel and the products: 1 token by 2 of 8 experts
+// of 512 x 1024 16 and 20, 7 by 2 of 16 of 648 x 288 20 and 21, 8 by 8 of 8 of 2048 x 4096 76 and
+// 89; 16 by 2 73 and 83, by 4 88 and 87, by 8 105 and 89; 32 by 8 of 256 of 2048 x 768 (2.9
+// stages a unit) 263 and 264, 40 by 4 of 60 of 1024 x 704 (2.0) 72 and 66, 64 by 4 of 256 of 768 x
+// 512 (1.6) 114 and 98.
+static bool streamed(int T, int E, int k, int K, int F) {
+    const int64_t ups = F / 8, downs = (K + 15) / 16, units = ups + downs;
+    const int64_t stages = ups * ((K + kSegment - 1) / kSegment) + downs * ((F + kSegment - 1) / kSegment);
+    return T <= 8 || (T * k <= 4 * E && 4 * stages >= 9 * units);
+}
 
 struct Layout {
-    size_t weights, experts, rows, offsets, counters, h, part, x_rows, bytes;
+    size_t weights, experts, rows, offsets, counters, h, part, parts, x_rows, bytes;
     int n_counters, hp;
 };
 static Layout layout(int T, int E, int k, int K, int F) {
@@ -610,6 +616,7 @@ static Layout layout(int T, int E, int k, int K, int F) {
     l.counters = take((size_t)l.n_counters * 4);
     l.h = take(R * l.hp * 2);
     l.part = take(R * K * 4 * (one ? 1 : moe_products::kMaxParts));
+    l.parts = take(one ? 0 : (size_t)E * ((K + moe_products::kTile - 1) / moe_products::kTile));
     l.x_rows = take(one ? 0 : R * K * 2);
     l.bytes = n;
     return l;
@@ -752,6 +759,7 @@ int nvfp4_moe_layer(const void *X, int64_t ldx, const void *logits, int logits_d
         a.x_rows = ws + l.x_rows;
         a.h = p.h;
         a.part = p.part;
+        a.parts = ws + l.parts;
         a.T = T;
         a.E = E;
         a.k = top_k;

@@ -41,13 +41,20 @@ constexpr int kSumTokens = kSumThreads / 32;  // of a CTA: 32 threads of 4 colum
 // pieces than 3 a tile are made, none of less than kMinSlots.
 struct Cut {
     int64_t slots, pieces;
-    int per;  // slots of a tile
+    int per;     // slots of a tile
+    bool small;  // products of slots and pieces are 32-bit numbers, whose division is short
     __device__ __forceinline__ Cut(int active, int tiles, int per_tile, int ctas) : per(per_tile) {
         slots = (int64_t)active * tiles * per;
         pieces = max((int64_t)1, min(min((int64_t)ctas, slots / kMinSlots), (int64_t)active * tiles * 3));
+        small = (slots + 1) * pieces < ((int64_t)1 << 32);
     }
-    __device__ __forceinline__ int64_t begin(int64_t piece) const { return slots * piece / pieces; }
-    __device__ __forceinline__ int piece_of(int64_t slot) const { return (int)(((slot + 1) * pieces - 1) / slots); }
+    __device__ __forceinline__ int64_t begin(int64_t piece) const {
+        return small ? (uint32_t)(slots * piece) / (uint32_t)pieces : slots * piece / pieces;
+    }
+    __device__ __forceinline__ int piece_of(int64_t slot) const {
+        const int64_t n = (slot + 1) * pieces - 1;
+        return (int)(small ? (uint32_t)n / (uint32_t)slots : n / slots);
+    }
 };
 
 __global__ void __launch_bounds__(kGatherThreads)
@@ -60,6 +67,7 @@ __global__ void __launch_bounds__(kGatherThreads)
 struct DownParams {
     const int *m_offsets;
     float *part;
+    uint8_t *parts;  // [E][tiles]: how many a tile has
     int E, R, K, F;
     int stages, ncap, ctas;
     KernelCtl ctl;
@@ -128,7 +136,7 @@ __global__ void __launch_bounds__(kThreads, kResident)
     const bool mine = cut.slots > 0 && blockIdx.x < cut.pieces;
     const int64_t i0 = mine ? cut.begin(blockIdx.x) : 0, i1 = mine ? cut.begin((int64_t)blockIdx.x + 1) : 0;
     // the tile that a slot belongs to, by active expert and tile, and the slot in it
-    const int64_t tile0 = mine ? i0 / cut.per : 0;
+    const int64_t tile0 = !mine ? 0 : i0 >> 31 ? i0 / cut.per : (uint32_t)i0 / (uint32_t)cut.per;
     const int a0 = (int)(tile0 / tiles), f0 = (int)(tile0 - (int64_t)a0 * tiles);
     const int s0 = (int)(i0 - tile0 * cut.per);
 
@@ -244,6 +252,7 @@ __global__ void __launch_bounds__(kThreads, kResident)
             }
             tc_fence_after();
             const int part = (int)blockIdx.x - cut.piece_of(i - s), feature = f * 128 + quarter * 32 + lane;
+            if (s + n == cut.per && quarter == 0 && lane == 0) p.parts[act_e[a] * tiles + f] = (uint8_t)(part + 1);
             float *to = p.part + ((int64_t)part * p.R + act_row[a]) * p.K + feature;
             const int rows = act_n[a];
             const uint32_t from = tmem + acc * p.ncap + ((uint32_t)(quarter * 32) << 16);
@@ -279,49 +288,27 @@ __global__ void __launch_bounds__(kThreads, kResident)
 
 struct SumParams {
     const float *part, *weights;
-    const int *experts, *rows, *m_offsets;
+    const uint8_t *parts;
+    const int *experts, *rows;
     const void *residual;
     void *y;
-    int T, k, E, R, K, F, ctas;
+    int T, k, R, K;
 };
 
 // 128 columns (a tile's) of kSumTokens tokens.
 template <typename T>
 __global__ void __launch_bounds__(kSumThreads) sum_kernel(const SumParams p) {
-    __shared__ short parts[kExperts];  // of the tile, by expert
-    __shared__ int before[kExperts / 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tile = blockIdx.x;
     const int t = blockIdx.y * kSumTokens + warp, col = tile * 128 + lane * 4;
-    int row = -1, expert = 0;  // of the token's choice `lane`
-    float weight = 0.0f;
-    if (t < p.T && lane < p.k) {
-        row = p.rows[t * p.k + lane];
-        expert = p.experts[t * p.k + lane];
-        weight = p.weights[t * p.k + lane];
-    }
-    bool live = false;
-    if (threadIdx.x < p.E) {
-        int r0, r1;
-        linear::group_rows(p.m_offsets, threadIdx.x, p.R, r0, r1);
-        live = r1 > r0;
-    }
-    const uint32_t alive = __ballot_sync(0xffffffffu, live);
-    if (lane == 0) before[warp] = __popc(alive);
-    __syncthreads();
-    int a = __popc(alive & ((1u << lane) - 1u)), active = 0;
-    for (int w = 0; w < kExperts / 32; w++) {
-        if (w < warp) a += before[w];
-        active += before[w];
-    }
-    const int tiles = (p.K + 127) / 128;
-    const Cut cut(active, tiles, (p.F + kBlockK - 1) / kBlockK, p.ctas);
-    if (live) {
-        const int64_t first = ((int64_t)a * tiles + tile) * cut.per;
-        parts[threadIdx.x] = (short)(cut.piece_of(first + cut.per - 1) - cut.piece_of(first) + 1);
-    }
-    __syncthreads();
     if (t >= p.T) return;
-    const int count = row >= 0 && row < p.R ? parts[expert] : 0;
+    int row = -1, count = 0;  // of the token's choice `lane`
+    float weight = 0.0f;
+    if (lane < p.k) {
+        row = p.rows[t * p.k + lane];
+        weight = p.weights[t * p.k + lane];
+        const int expert = p.experts[t * p.k + lane];
+        if (row >= 0 && row < p.R) count = p.parts[expert * (int)gridDim.x + tile];
+    }
     const bool in = col < p.K;
     const int64_t at = (int64_t)t * p.K + col;
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -386,6 +373,7 @@ static int run_t(const Args &a, const DeviceInfo &di, cudaStream_t s) {
     DownParams d = {};
     d.m_offsets = a.m_offsets;
     d.part = a.part;
+    d.parts = a.parts;
     d.E = a.E;
     d.R = R;
     d.K = a.K;
@@ -410,19 +398,16 @@ static int run_t(const Args &a, const DeviceInfo &di, cudaStream_t s) {
 
     SumParams m = {};
     m.part = a.part;
+    m.parts = a.parts;
     m.weights = a.weights;
     m.experts = a.experts;
     m.rows = a.rows;
-    m.m_offsets = a.m_offsets;
     m.residual = a.residual;
     m.y = a.y;
     m.T = a.T;
     m.k = a.k;
-    m.E = a.E;
     m.R = R;
     m.K = a.K;
-    m.F = a.F;
-    m.ctas = d.ctas;
     sum_kernel<T><<<dim3((unsigned)((a.K + 127) / 128), (unsigned)((a.T + kSumTokens - 1) / kSumTokens)), kSumThreads, 0,
                     s>>>(m);
     count_launch();

@@ -11,6 +11,7 @@ namespace moe_products {
 
 constexpr int kMaxTokens = 64;  // an expert's rows are the MMA's N
 constexpr int kMaxParts = 5;    // that a W2 tile's reduction is cut into
+constexpr int kTile = 128;      // W2 rows, columns of the output
 
 struct Args {
     const void *x, *w13, *w2, *residual;
@@ -21,6 +22,7 @@ struct Args {
     const int *m_offsets;            // [E + 1]
     void *x_rows, *h;                // workspace: [T k, K] and [T k, F] 16-bit
     float *part;                     // workspace: [kMaxParts][T k, K]
+    uint8_t *parts;                  // workspace: [E][tiles of 128 columns]
     int T, E, k, K, F, dtype;
 };
 

@@ -146,7 +146,7 @@ def test_moe_layer_same_bits(nv, cuda_dev):
 
 
 def test_moe_layer_same_bits_and_agreement(nv, cuda_dev):
-    d = layer(16, 32, 1024, 1024, torch.bfloat16, 1)
+    d = layer(16, 32, 2048, 1024, torch.bfloat16, 1)
     args = d["x"], d["logits"], d["w13"], d["w2"], 4
     y = nv.moe_layer(*args, residual=d["residual"])
     for _ in range(20):
