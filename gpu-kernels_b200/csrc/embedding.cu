@@ -251,7 +251,7 @@ constexpr int kFewTokens = 4096;
 constexpr int kLongRun = 16;
 constexpr int kFewCols = 32 * 8;     // columns of a warp at a time
 constexpr int kFewAhead = 8;         // rows on their way
-constexpr int kFewFill = 256;        // most rows of a CTA that writes zeros
+constexpr int kFewFill = 2048;       // most rows of a CTA that writes zeros
 
 struct FewParams {
     const void *dy, *tokens;
@@ -789,7 +789,7 @@ int nvfp4_embedding_backward(const void *dY, int64_t ldy, const void *tokens, in
     if (T == 0)  // no token: the gradient is zero
         return cuda_status(cudaMemsetAsync(dTable, 0, (size_t)V * K * 2, s));
     // rows of zeros: about 256 KB a CTA, and 64 KB beside the joins
-    const int fill_rows = (int)std::max<int64_t>(1, std::min<int64_t>(256, (256 << 10) / ((int64_t)K * 2)));
+    const int fill_rows = (int)std::max<int64_t>(1, (256 << 10) / ((int64_t)K * 2));
     if (embedding::unsorted(T, K)) {
         embedding::FewParams p = {};
         p.dy = dY;
@@ -805,8 +805,8 @@ int nvfp4_embedding_backward(const void *dY, int64_t ldy, const void *tokens, in
         p.cols = embedding::kFewCols;
         while (groups * ((K + p.cols - 1) / p.cols) > 4 * di.sm_count && p.cols < K) p.cols *= 2;
         p.slabs = (K + p.cols - 1) / p.cols;
-        p.fill_rows = fill_rows;
-        p.fill_ctas = (V + fill_rows - 1) / fill_rows;
+        p.fill_rows = std::min(embedding::kFewFill, fill_rows);
+        p.fill_ctas = (V + p.fill_rows - 1) / p.fill_rows;
         if (groups * p.slabs + p.fill_ctas > INT_MAX) return NVFP4_ERR_SHAPE;
         p.sum_ctas = (int)(groups * p.slabs);
         if (dtype == NVFP4_BF16)
@@ -836,7 +836,7 @@ int nvfp4_embedding_backward(const void *dY, int64_t ldy, const void *tokens, in
     p.sum_ctas = (l.blocks + p.per_cta - 1) / p.per_cta * slabs;
     p.join_ctas = (l.blocks + embedding::kJoinBlocks - 1) / embedding::kJoinBlocks *
                   ((K + embedding::kJoinCols - 1) / embedding::kJoinCols);
-    p.fill_rows = fill_rows;
+    p.fill_rows = std::min(256, fill_rows);
     p.join_rows = (p.fill_rows + 3) / 4;
     p.fill_from = zero_rows;
     p.fill_end = V;
