@@ -137,6 +137,17 @@ def test_moe_layer_one_expert_for_all(nv, cuda_dev):
         check(nv, d, 2)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_moe_layer_uneven_rows(nv, cuda_dev, dtype):
+    """Few rows an expert on average and most of them one expert's: units of up to four sixteens,
+    beside experts of one row, with whole and partial stages."""
+    for T in (9, 16, 17, 32, 33, 50, 64):
+        d = layer(T, 64, 1032, 1040, dtype, T, residual=T % 2 == 0)
+        d["logits"][:, 3] = 50.0
+        check(nv, d, 1)
+        check(nv, d, 3)
+
+
 def test_moe_layer_same_bits(nv, cuda_dev):
     d = layer(50, 10, 1032, 528, torch.bfloat16, 1)
     args = d["x"], d["logits"], d["w13"], d["w2"], 4
