@@ -12,8 +12,9 @@
 // leaves, c m - r, is known exactly and taken out of the sums at the end), and values far
 // below the maximum, -inf and NaN among them, are first raised to a finite one, in pairs of
 // 16-bit values, whose power of two is zero all the same.  Where that does not hold (nothing
-// but masked logits so far, or a maximum near the type's lowest value or past 2^60) the
-// exponents are taken one by one from the difference.
+// but masked logits so far, or a maximum near the type's lowest value), or c m is so large that
+// its rounding is no small part of an exponent (past 2^24: masks of -1e9 and the like, in the
+// parts of a row that hold nothing else), the exponents are taken one by one from the difference.
 //
 // A warp of its own copies the rows through a ring in shared memory, in bulk copies of 16 or 32 KB,
 // and runs on into the next row while the others finish this one.
@@ -174,6 +175,10 @@ __device__ __forceinline__ void unpack(const uint4 &v, float (&f)[kVec<T>]) {
     }
 }
 
+// c m up to which the exponents are c x - r: what r's rounding leaves of c m is then half a unit
+// at most.  It is a factor of all sums until they are handed on, which 2^128 and more would end.
+constexpr float kMostPaired = 0x1p24f;
+
 // Whether a value raised to `floor` has the power of two zero, and a finite exponent.
 __device__ __forceinline__ bool raises(float floor, float c, float r) {
     return c < 1e6f && fmaf(floor, c, -r) < -150.0f;
@@ -277,7 +282,7 @@ struct Sums {
         const float high = Word<T>::top_value(top);
         if (high > m) {
             const float r_next = high * c;
-            const bool pairs = raises(Word<T>::kFloor, c, r_next) && fabsf(r_next) < 0x1p60f;
+            const bool pairs = raises(Word<T>::kFloor, c, r_next) && fabsf(r_next) < kMostPaired;
             const float rest_next = pairs ? fmaf(high, c, -r_next) : 0.0f;
             const float d = fmaxf((m - high) * c, kFar) - rest + rest_next, scale = ex2(d);
             const uint64_t dd = pair(d, d), ss = pair(scale, scale);
