@@ -32,7 +32,7 @@
 //
 // Measured: 4096 rows of 131072 bf16, statistics 173 us (6.2 TB/s of a copy's 6.55), with the
 // entropy 179, and 8 alternatives 220 (their second reading and the ranking, 5 us a row of a
-// CTA), 32 262; the gradient 326 (6.6 TB/s).  16000 rows of 8000 52 us (4.9 TB/s).  Without
+// CTA), 32 262; the gradient 329 (6.5 TB/s).  16000 rows of 8000 52 us (4.9 TB/s).  Without
 // alternatives the pass is bound by memory and nearly by issue (61 % of cycles; the unit of
 // powers of two is 66 % busy).  One row of 50257 fp32 with 5 alternatives 9.1 us: launch, a pass of
 // 3 us, the join of a cluster and the ranking.
@@ -184,6 +184,20 @@ __device__ __forceinline__ bool raises(float floor, float c, float r) {
     return c < 1e6f && fmaf(floor, c, -r) < -150.0f;
 }
 
+// The same the other way.
+template <typename T>
+__device__ __forceinline__ T value_of(float v) {
+    if constexpr (sizeof(T) == 4) return v;
+    else return Type16<T>::round(v);
+}
+template <typename T>
+__device__ __forceinline__ uint4 vector_of(const float (&f)[kVec<T>]) {
+    if constexpr (sizeof(T) == 4)
+        return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+    else
+        return pack8<T>(f);
+}
+
 // A row as 16-byte vectors at 16-byte addresses; the first and the last may reach past it.
 template <typename T>
 struct Row {
@@ -252,10 +266,10 @@ struct Stats {
     float m, s0, s1;  // maximum (of the logits themselves), and the sums relative to it
 };
 // fmaxf takes the bound where the difference is NaN: of two infinities, or of a masked NaN.
-__device__ __forceinline__ Stats join(const Stats &a, const Stats &b, const Params &p) {
+__device__ __forceinline__ Stats join(const Stats &a, const Stats &b, float c) {
     Stats r;
     r.m = fmaxf(a.m, b.m);
-    const float da = fmaxf((a.m - r.m) * p.c, kFar), db = fmaxf((b.m - r.m) * p.c, kFar);
+    const float da = fmaxf((a.m - r.m) * c, kFar), db = fmaxf((b.m - r.m) * c, kFar);
     const float fa = ex2(da), fb = ex2(db);
     r.s0 = a.s0 * fa + b.s0 * fb;
     r.s1 = fmaf(a.s0, da, a.s1) * fa + fmaf(b.s0, db, b.s1) * fb;
@@ -623,7 +637,7 @@ __global__ void __launch_bounds__(kThreads + 32, kResident) logprobs_kernel(cons
         // ---- statistics of the CTA
         Stats w = sums.stats();
 #pragma unroll
-        for (int o = 16; o; o >>= 1) w = join(w, shuffle(w, o), p);
+        for (int o = 16; o; o >>= 1) w = join(w, shuffle(w, o), p.c);
         if (lane == 0) s.part[turn][warp] = w;
         if (threadIdx.x == 0) s.n_winners = s.n_cand = s.n_top = 0;
         sync_adders();
@@ -703,10 +717,10 @@ __global__ void __launch_bounds__(kThreads + 32, kResident) logprobs_kernel(cons
             if (warp == 0) {
                 for (int i = lane; i < parts * kWarps; i += 32) {
                     const uint32_t at = map_to_cta(smem_u32(&s.part[turn][i % kWarps]), i / kWarps);
-                    all = join(all, {ld_cluster_f32(at), ld_cluster_f32(at + 4), ld_cluster_f32(at + 8)}, p);
+                    all = join(all, {ld_cluster_f32(at), ld_cluster_f32(at + 4), ld_cluster_f32(at + 8)}, p.c);
                 }
 #pragma unroll
-                for (int o = 16; o; o >>= 1) all = join(all, shuffle(all, o), p);
+                for (int o = 16; o; o >>= 1) all = join(all, shuffle(all, o), p.c);
                 // lane 0's for all: a join's two sides round differently
                 all.m = __shfl_sync(0xffffffffu, all.m, 0);
                 all.s0 = __shfl_sync(0xffffffffu, all.s0, 0);
@@ -801,7 +815,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, kRowResident) logprobs_rows_ke
     if (w0 || w1 < nv) sums.add(ends, p.c);
     Stats all = sums.stats();
 #pragma unroll
-    for (int o = 16; o; o >>= 1) all = join(all, shuffle(all, o), p);
+    for (int o = 16; o; o >>= 1) all = join(all, shuffle(all, o), p.c);
     // lane 0's for all: a join's two sides round differently
     all.m = __shfl_sync(0xffffffffu, all.m, 0);
     all.s0 = __shfl_sync(0xffffffffu, all.s0, 0);
@@ -902,11 +916,98 @@ struct GradParams {
 constexpr int kGradThreads = 256;
 constexpr int kGradBatch = 4;
 
+// |lse| up to which the probabilities come from it.  It is one rounded number, so log p is off by up
+// to 4e-7 of it: 1e-4 for 16-bit results, 3e-5 for fp32.  Beyond that it says too little (past 2^29
+// nothing of ln s is left in it), and the row is summed again.
+template <typename T>
+constexpr float kMostLse = sizeof(T) == 4 ? 64.0f : 256.0f;
+
+// A row whose lse says too little, by one CTA, or (WARP) one warp: its maximum m and sum s once
+// more, then d from 2^(c (x - m)) / s, as the log probabilities' own kernel has it.  One reader of
+// the whole row, which writes behind its last read: in place too.  Not inlined and with one load in
+// flight, so that the kernel's registers are those of the other rows; 4096 rows of 131072 bf16 that
+// are all of this sort take 875 us where the others take 329.
+template <typename T, bool WARP>
+__device__ __noinline__ void far_row(const GradParams &p, int64_t t) {
+    constexpr int kTeam = WARP ? 32 : kGradThreads;
+    const int me = threadIdx.x & (kTeam - 1), lane = threadIdx.x & 31;
+    const float c = p.inv_temperature * kLog2e;
+    const T *x = static_cast<const T *>(p.logits) + t * p.ld;
+    T *d = static_cast<T *>(p.dlogits) + t * p.ldd;
+    const bool whole = (reinterpret_cast<uintptr_t>(x) & 15u) == 0, whole_out = (reinterpret_cast<uintptr_t>(d) & 15u) == 0;
+    const uint32_t V = p.V, W = p.W;  // a place past them by a team's elements is no negative number
+    // kVec elements from e on, -inf past the row's n.  Pieces count from the row's start, whatever
+    // its alignment, for the same bits
+    auto load = [&](uint32_t e, uint32_t n, float (&f)[kVec<T>]) {
+        if (whole && e + kVec<T> <= n) {
+            unpack<T>(*reinterpret_cast<const uint4 *>(x + e), f);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kVec<T>; i++) f[i] = e + i < n ? to_float<T>(x[e + i]) : -INFINITY;
+        }
+    };
+    Stats all = {-INFINITY, 0.0f, 0.0f};
+#pragma unroll 1
+    for (uint32_t e = me * kVec<T>; e < V; e += kTeam * kVec<T>) {
+        float f[kVec<T>], high = -INFINITY, sum = 0.0f;
+        load(e, V, f);
+#pragma unroll
+        for (int i = 0; i < kVec<T>; i++) high = fmaxf(high, f[i]);
+        if (high > all.m) {
+            all.s0 *= ex2(fmaxf((all.m - high) * c, kFar));
+            all.m = high;
+        }
+#pragma unroll
+        for (int i = 0; i < kVec<T>; i++) sum += ex2(fmaxf((f[i] - all.m) * c, kFar));
+        all.s0 += sum;
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) all = join(all, shuffle(all, o), c);
+    if constexpr (!WARP) {
+        __shared__ Stats part[kGradThreads / 32];
+        if (lane == 0) part[threadIdx.x >> 5] = all;
+        __syncthreads();
+        all = part[0];
+        for (int w = 1; w < kGradThreads / 32; w++) all = join(all, part[w], c);
+    } else {  // lane 0's for all: a join's two sides round differently
+        all.m = __shfl_sync(0xffffffffu, all.m, 0);
+        all.s0 = __shfl_sync(0xffffffffu, all.s0, 0);
+    }
+    const float ln_s = logf(all.s0), inv_s = 1.0f / all.s0;
+    const int64_t target = target_of(p.targets, p.target8, t);
+    const float g = target >= 0 && target < p.V ? p.dlogprobs[t] * p.inv_temperature : 0.0f;
+    const float h = p.dentropy ? p.dentropy[t] * p.inv_temperature : 0.0f;
+    const float a = p.dentropy ? fmaf(h, p.entropy[t], g) : g;
+#pragma unroll 1
+    for (uint32_t e = me * kVec<T>; e < W; e += kTeam * kVec<T>) {
+        float f[kVec<T>];
+        load(e, W, f);
+#pragma unroll
+        for (int i = 0; i < kVec<T>; i++) {
+            float y = 0.0f;
+            if (e + i < V && f[i] > -INFINITY) {
+                const float off = f[i] - all.m, q = ex2(off * c) * inv_s;
+                y = q == 0.0f ? 0.0f : -q * fmaf(h, fmaf(off, p.inv_temperature, -ln_s), a);
+                if (e + i == target) y += g;
+            }
+            f[i] = y;
+        }
+        if (whole_out && e + kVec<T> <= W) {
+            *reinterpret_cast<uint4 *>(d + e) = vector_of<T>(f);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kVec<T>; i++)
+                if (e + i < W) d[e + i] = value_of<T>(f[i]);
+        }
+    }
+}
+
 // Elementwise, with the row's scalars in registers: bound by reading and writing the logits.
 // SAME: the gradient's rows have the logits' alignment, so whole vectors go out.  SHORT: a CTA
-// has several rows (16000 of 1500 50 -> 30 us; with long ones in the same code 326 -> 381).
+// has several rows (16000 of 1500 50 -> 28 us; with long ones in the same code 326 -> 381).
 template <typename T, bool SAME, bool SHORT>
-__global__ void __launch_bounds__(kGradThreads) logprobs_grad_kernel(const GradParams p) {
+__global__ void __launch_bounds__(kGradThreads, SHORT && SAME ? 4 : SAME ? 5 : 8)
+    logprobs_grad_kernel(const __grid_constant__ GradParams p) {
     const int team = SHORT ? 1 << p.wide : kGradThreads, me = SHORT ? threadIdx.x & (team - 1) : threadIdx.x;
     int64_t t;
     int chunk = 0;
@@ -924,11 +1025,12 @@ __global__ void __launch_bounds__(kGradThreads) logprobs_grad_kernel(const GradP
     const float h = p.dentropy ? p.dentropy[t] * p.inv_temperature : 0.0f;
     const float H = p.dentropy ? p.entropy[t] : 0.0f;
     const float lse = p.lse[t];
+    const bool far = !(fabsf(lse) <= kMostLse<T>);
     const float a = fmaf(h, H, g);  // d = -p (g + h H + h log p)
     // Away from the target in pairs, from log2 p = c x - c lse: -inf and NaN are raised as in the
-    // forward pass, where that leaves them at zero and log p is more than rounding.
+    // forward pass, where that leaves them at zero.
     const float c = p.inv_temperature * kLog2e, lse2 = lse * kLog2e, b = -h * kLn2;
-    const bool paired = fabsf(lse) < 1e4f && raises(Word<T>::kFloor, c, lse2);
+    const bool paired = raises(Word<T>::kFloor, c, lse2);
     const uint64_t cc = pair(c, c), ll = pair(-lse2, -lse2), aa = pair(-a, -a), bb = pair(b, b);
     auto grad = [&](float v, int64_t e) {  // one element, the same bits
         if (e >= p.V || !(v > -INFINITY)) return 0.0f;
@@ -937,16 +1039,10 @@ __global__ void __launch_bounds__(kGradThreads) logprobs_grad_kernel(const GradP
             const float l = fmaf(fmaxf(v, Word<T>::kFloor), c, -lse2);
             y = ex2(l) * fmaf(b, l, -a);
         } else {
-            float l = fmaf(v, p.inv_temperature, -lse);
-            l = l > 0.0f ? 0.0f : l;  // of logits past 2^24 nothing but their rounding is left: p stays below 1
-            const float q = ex2(l * kLog2e);
+            const float l = fmaf(v, p.inv_temperature, -lse), q = ex2(l * kLog2e);
             y = q == 0.0f ? 0.0f : -q * fmaf(h, l, a);
         }
         return e == target ? y + g : y;
-    };
-    auto put = [](float v) {
-        if constexpr (sizeof(T) == 4) return v;
-        else return Type16<T>::round(v);
     };
     if constexpr (SAME) {
         const Row<T> row(x, p.W);
@@ -959,10 +1055,11 @@ __global__ void __launch_bounds__(kGradThreads) logprobs_grad_kernel(const GradP
             const int64_t e = v * kVec<T> - row.shift;
             if (v < nv && e >= 0 && e + kVec<T> <= p.W) raw[i] = *reinterpret_cast<const uint4 *>(x + e);
         }
+        const int n_out = far ? 0 : nv;  // asked once the logits are on their way
 #pragma unroll
         for (int i = 0; i < kGradBatch; i++) {
             const int64_t v = v0 + i * team;
-            if (v >= nv) break;
+            if (v >= n_out) break;
             const int64_t e = v * kVec<T> - row.shift;
             if (e >= 0 && e + kVec<T> <= p.W) {
                 float f[kVec<T>];
@@ -982,26 +1079,19 @@ __global__ void __launch_bounds__(kGradThreads) logprobs_grad_kernel(const GradP
 #pragma unroll
                     for (int j = 0; j < kVec<T>; j++) f[j] = grad(f[j], e + j);
                 }
-                uint4 o;
-                if constexpr (sizeof(T) == 4)
-                    o = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
-                                   __float_as_uint(f[3]));
-                else
-                    o = pack8<T>(f);
-                *reinterpret_cast<uint4 *>(d + e) = o;
+                *reinterpret_cast<uint4 *>(d + e) = vector_of<T>(f);
             } else {
                 for (int j = 0; j < kVec<T>; j++)
-                    if (e + j >= 0 && e + j < p.W) d[e + j] = put(grad(to_float<T>(x[e + j]), e + j));
+                    if (e + j >= 0 && e + j < p.W) d[e + j] = value_of<T>(grad(to_float<T>(x[e + j]), e + j));
             }
         }
     } else {
         const int64_t e0 = (int64_t)chunk * kGradBatch * kGradThreads * kVec<T> + me;
+        const int64_t n_out = far ? 0 : min((int64_t)p.W, e0 + kGradBatch * kVec<T> * team);
 #pragma unroll 4
-        for (int i = 0; i < kGradBatch * kVec<T>; i++) {
-            const int64_t e = e0 + i * team;
-            if (e < p.W) d[e] = put(grad(to_float<T>(x[e]), e));
-        }
+        for (int64_t e = e0; e < n_out; e += team) d[e] = value_of<T>(grad(to_float<T>(x[e]), e));
     }
+    if (far && chunk == 0 && (!SHORT || me < 32)) far_row<T, SHORT>(p, t);
 }
 
 // ------------------------------------------------------------------------- host side

@@ -479,7 +479,9 @@ NVFP4_API int nvfp4_token_logprobs(const void *logits, int64_t ld, int dtype, co
  * entropies (which then are needed too): with p the probabilities,
  *   dlogits = (g ([v = target] - p) - h p (log p + entropy)) / temperature
  * in the logits' type, rows ldd apart; masked columns and columns V to W - 1 are zero.  The
- * alternatives carry no gradient.  dlogits may be the logits themselves (same rows).
+ * alternatives carry no gradient.  dlogits may be the logits themselves (same rows).  p comes
+ * from lse while that is at most 256 in size (64 for fp32 logits), and beyond it, where one
+ * number holds too little of it, from the row's own maximum and sum, taken once more.
  */
 NVFP4_API int nvfp4_token_logprobs_backward(const float *dlogprobs, const float *dentropy, const void *logits,
                                             int64_t ld, int dtype, const void *targets, int target_bytes,
