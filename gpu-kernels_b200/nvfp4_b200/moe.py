@@ -90,6 +90,8 @@ def moe_layer(x: torch.Tensor, logits: torch.Tensor, w13: torch.Tensor, w2: torc
     inference: the differentiable form is those four operators."""
     if isinstance(x, torch.Tensor) and x.dim() == 2 and x.shape[0] > FEW_TOKENS:
         r = moe_route(logits, top_k, scoring, bias, renormalize, scale)
+        if not isinstance(w2, torch.Tensor) or w2.dim() != 2 or w2.shape[0] != logits.shape[1] * x.shape[1]:
+            raise ValueError(f"w2 must be [E * {x.shape[1]}, F]")  # the product by itself takes any
         rows = moe_dispatch(x.contiguous(), r)
         h = native.linear(rows, w13, r.m_offsets, None, ACTIVATIONS["swiglu"], None, None, False)
         return moe_combine(native.linear(h, w2, r.m_offsets, None, 0, None, None, False), r, residual)
