@@ -806,7 +806,7 @@ int nvfp4_embedding_backward(const void *dY, int64_t ldy, const void *tokens, in
         while (groups * ((K + p.cols - 1) / p.cols) > 4 * di.sm_count && p.cols < K) p.cols *= 2;
         p.slabs = (K + p.cols - 1) / p.cols;
         p.fill_rows = std::min(embedding::kFewFill, fill_rows);
-        p.fill_ctas = (V + p.fill_rows - 1) / p.fill_rows;
+        p.fill_ctas = (int)(((int64_t)V + p.fill_rows - 1) / p.fill_rows);
         if (groups * p.slabs + p.fill_ctas > INT_MAX) return NVFP4_ERR_SHAPE;
         p.sum_ctas = (int)(groups * p.slabs);
         if (dtype == NVFP4_BF16)
