@@ -25,6 +25,7 @@ namespace nvfp4 {
 namespace embedding {
 
 constexpr int kMaxRows = INT_MAX - 1023;
+constexpr int kMaxCols = 1 << 30;  // of the gradient, whose columns and a slab more are 32-bit numbers
 
 // ------------------------------------------------------------------------- lookup
 constexpr int kLookupThreads = 256;
@@ -765,7 +766,7 @@ int nvfp4_embedding(const void *tokens, int token_bytes, const void *table, int6
 }
 
 size_t nvfp4_embedding_backward_workspace_size(int T, int V, int K) {
-    if (T < 1 || V < 1 || K < 8 || T > embedding::kMaxRows || V > embedding::kMaxRows || K > embedding::kMaxRows)
+    if (T < 1 || V < 1 || K < 8 || T > embedding::kMaxRows || V > embedding::kMaxRows || K > embedding::kMaxCols)
         return 0;
     return embedding::unsorted(T, K) ? 0 : embedding::layout(T, K).bytes;
 }
@@ -775,6 +776,7 @@ int nvfp4_embedding_backward(const void *dY, int64_t ldy, const void *tokens, in
                              void *stream) {
     int st = embedding::check_sizes(tokens, token_bytes, ldy, T, V, K, dtype);
     if (st) return st;
+    if (K > embedding::kMaxCols) return NVFP4_ERR_SHAPE;
     if (!dTable || (T && !dY)) return NVFP4_ERR_INVALID;
     if (!aligned16(dY) || !aligned16(dTable) || !aligned16(workspace)) return NVFP4_ERR_ALIGN;
     const size_t need = nvfp4_embedding_backward_workspace_size(T, V, K);
