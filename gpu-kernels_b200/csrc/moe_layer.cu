@@ -45,6 +45,7 @@
 // described by a warp of their own, 500 cycles each, 6.2 and 6.3 but 4.6 instead of 5.8 for 256
 // experts of 2048 x 768.
 #include <algorithm>
+#include <atomic>
 #include <climits>
 
 #include "common.cuh"
@@ -659,11 +660,11 @@ static int launch(const Params &p, const DeviceInfo &di, cudaStream_t s) {
     int st = map_weights<T>(&map13, &tail13, p.w13, (int64_t)p.E * 2 * p.F, p.K, true);
     if (!st) st = map_weights<T>(&map2, &tail2, p.w2, (int64_t)p.E * p.K, p.F, false);
     if (st) return st;
-    static int configured[64] = {};
-    if (!configured[di.device]) {
+    static std::atomic<bool> configured[64] = {};
+    if (!configured[di.device].load(std::memory_order_acquire)) {
         if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
             return NVFP4_ERR_CUDA;
-        configured[di.device] = 1;
+        configured[di.device].store(true, std::memory_order_release);
     }
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr;

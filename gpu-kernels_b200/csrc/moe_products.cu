@@ -21,6 +21,7 @@
 // Warps: 0 TMA producer, 1 MMA issue and TMEM owner, 2-5 write the accumulators out, under the
 // next tile's loads and products.
 #include <algorithm>
+#include <atomic>
 #include <climits>
 
 #include "linear.cuh"
@@ -391,11 +392,11 @@ static int run_t(const Args &a, const DeviceInfo &di, cudaStream_t s) {
     if ((st = map_weight<T>(&w, a.w2, a.E, a.K, a.F, 128))) return st;
     if ((st = map_rows<T>(&h, a.h, R, a.F, a.F, 16))) return st;
     auto kern = down_kernel<T>;
-    static int configured[64] = {};
-    if (!configured[di.device]) {
+    static std::atomic<bool> configured[64] = {};
+    if (!configured[di.device].load(std::memory_order_acquire)) {
         if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing + 1024) != cudaSuccess)
             return NVFP4_ERR_CUDA;
-        configured[di.device] = 1;
+        configured[di.device].store(true, std::memory_order_release);
     }
     kern<<<(unsigned)d.ctas, kThreads, d.stages * (kTileBytes + d.ncap * 128) + 1024, s>>>(w, h, d);
     count_launch();
