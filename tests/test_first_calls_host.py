@@ -11,5 +11,5 @@ CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
 @pytest.mark.parametrize("name", ["embedding", "logprobs", "moe", "moe_layer", "moe_products"])
 def test_first_call_flags_are_atomic(name):
     with open(os.path.join(CSRC, name + ".cu")) as f:
-        flags = re.findall(r"^ +static (?!constexpr|const )(.*?)[;=]", f.read(), re.M)
+        flags = re.findall(r"^ +static (?!constexpr|const |__device__)(.*?)[;=]", f.read(), re.M)
     assert flags and all(flag.startswith("std::atomic<") for flag in flags), flags
