@@ -718,18 +718,17 @@ static void lookup_u(const LookupParams &p, cudaStream_t s) {
     if (p.scale == 1.0f) embedding_kernel<T, I, N, U, false><<<grid, kLookupThreads, 0, s>>>(p);
     else embedding_kernel<T, I, N, U, true><<<grid, kLookupThreads, 0, s>>>(p);
 }
-// One vector a thread as long as that makes no more CTAs than run at once.
-constexpr int64_t kFewVectors = 148 * 8 * kLookupThreads;
+// One vector a thread as long as that makes no more CTAs than run at once, eight an SM.
 template <typename T, typename I>
-static void lookup_i(const LookupParams &p, cudaStream_t s) {
-    if (p.n <= kFewVectors) lookup_u<T, I, uint32_t, 1>(p, s);
+static void lookup_i(const LookupParams &p, int sm_count, cudaStream_t s) {
+    if (p.n <= (int64_t)sm_count * 8 * kLookupThreads) lookup_u<T, I, uint32_t, 1>(p, s);
     else if (p.n < ((int64_t)1 << 31)) lookup_u<T, I, uint32_t, 4>(p, s);
     else lookup_u<T, I, uint64_t, 4>(p, s);
 }
 template <typename T>
-static void lookup(const LookupParams &p, int token_bytes, cudaStream_t s) {
-    if (token_bytes == 8) lookup_i<T, int64_t>(p, s);
-    else lookup_i<T, int>(p, s);
+static void lookup(const LookupParams &p, int token_bytes, int sm_count, cudaStream_t s) {
+    if (token_bytes == 8) lookup_i<T, int64_t>(p, sm_count, s);
+    else lookup_i<T, int>(p, sm_count, s);
 }
 
 }  // namespace embedding
@@ -759,8 +758,8 @@ int nvfp4_embedding(const void *tokens, int token_bytes, const void *table, int6
     if ((st = device_info(&di))) return st;
     if (T == 0) return NVFP4_OK;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (dtype == NVFP4_BF16) embedding::lookup<__nv_bfloat16>(p, token_bytes, s);
-    else embedding::lookup<__half>(p, token_bytes, s);
+    if (dtype == NVFP4_BF16) embedding::lookup<__nv_bfloat16>(p, token_bytes, di.sm_count, s);
+    else embedding::lookup<__half>(p, token_bytes, di.sm_count, s);
     count_launch();
     return cuda_status(cudaGetLastError());
 }
