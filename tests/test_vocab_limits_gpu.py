@@ -2,6 +2,8 @@
 import pytest
 import torch
 
+import ref_vocab as V
+
 pytestmark = pytest.mark.gpu
 ROWS = 2 ** 31 - 1 - 1023  # the most there may be
 
@@ -32,4 +34,56 @@ def test_embedding_of_the_most_rows(nv, cuda_dev, T):
     finally:
         del d
         words = None
+        torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("T,n,dtype", [(17000, 131072, torch.bfloat16), (300000, 8000, torch.float16),
+                                       (17000, 131075, torch.float32)])
+def test_logprobs_past_32_bits(nv, cuda_dev, T, n, dtype):
+    """More logits than 2^31: the last rows are their own, and nothing else is written."""
+    g = torch.Generator(device="cuda").manual_seed(2)
+    block = (torch.randn(1000, n, device="cuda", generator=g) * 3).to(dtype)
+    x = block.repeat(T // 1000, 1)
+    x[-2:] = block[:2] + 1
+    t = torch.randint(0, n, (T,), device="cuda", generator=g)
+    dl, dh = torch.randn(T, device="cuda", generator=g), torch.randn(T, device="cuda", generator=g)
+    try:
+        r = nv.token_logprobs(x, t, None, 4, 0.7, True)
+        pick = torch.tensor([0, 1, T // 2, (1 << 31) // n - 1, (1 << 31) // n, (1 << 31) // n + 1, T - 2, T - 1],
+                            device="cuda")
+        rows, at = x[pick].clone(), t[pick]
+        ref = V.Logprobs(rows, at, n, 4, 0.7)
+        V.assert_near(r.logprobs[pick], ref.logprobs, ref.logprobs_bound, "logprobs")
+        V.assert_near(r.entropy[pick], ref.entropy, ref.entropy_bound, "entropy")
+        assert torch.equal(r.top_tokens[pick].long(), ref.top_tokens)
+        d = nv.token_logprobs_backward(dl, x, t, r, dh, None, 0.7, out=x)
+        want, bound = ref.grad(dl[pick], dh[pick], n)
+        V.assert_grad(d[pick], want, bound, "dlogits")
+        nv.device_status()
+    finally:
+        x = d = None
+        torch.cuda.empty_cache()
+
+
+def test_embedding_past_32_bits(nv, cuda_dev):
+    """More elements than 2^31 in the output, and in the gradient that comes in."""
+    T, rows, K = 300000, 37, 8192
+    g = torch.Generator(device="cuda").manual_seed(3)
+    table = torch.randn(rows, K, device="cuda", generator=g).bfloat16()
+    t = torch.arange(T, device="cuda") % (rows + 1)  # the last is outside
+    try:
+        y = nv.embedding(t, table)
+        for i in range(0, T, 50000):
+            at = t[i:i + 50000]
+            want = torch.where((at < rows)[:, None], table[at.clamp(max=rows - 1)], torch.zeros((), device="cuda").bfloat16())
+            assert torch.equal(y[i:i + 50000], want)
+        y[:-rows] = 0  # the last tokens alone count
+        d = nv.embedding_backward(y, t, rows)
+        last = t[-rows:]
+        want = torch.zeros_like(table)
+        want[last[last < rows]] = table[last[last < rows]]
+        assert torch.equal(d, want)
+        nv.device_status()
+    finally:
+        y = None
         torch.cuda.empty_cache()
