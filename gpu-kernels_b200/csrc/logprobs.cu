@@ -31,8 +31,9 @@
 // order.
 //
 // Measured: 4096 rows of 131072 bf16, statistics 173 us (6.2 TB/s of a copy's 6.55), with the
-// entropy 179, and 8 alternatives 220 (their second reading and the ranking, 5 us a row of a
-// CTA), 32 262; the gradient 329 (6.5 TB/s).  16000 rows of 8000 52 us (4.9 TB/s).  Without
+// entropy 179, and 8 alternatives 221 (their second reading and the ranking, 5 us a row of a
+// CTA; 238 where the logits are others in every call), 32 263; the gradient 329 (6.5 TB/s).  16000
+// rows of 8000 52 us (4.9 TB/s).  Without
 // alternatives the pass is bound by memory and nearly by issue (61 % of cycles; the unit of
 // powers of two is 66 % busy).  One row of 50257 fp32 with 5 alternatives 9.1 us: launch, a pass of
 // 3 us, the join of a cluster and the ranking.

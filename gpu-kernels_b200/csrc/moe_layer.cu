@@ -34,7 +34,7 @@
 //
 // Measured, both launches, on the GPU: one token by 2 of 8 experts of 4096 x 14336 112 us (6.3
 // TB/s), 8 tokens by 6 of 64 of 2048 x 2048 124 us (6.3), 13 by 6 of 64 of 2056 x 1408, whose
-// rows begin anywhere in a 128-byte line, 136 us (5.4), one by 8 of 128 of 2048 x 768 28 us:
+// rows begin anywhere in a 128-byte line, 132 to 139 us (5.4), one by 8 of 128 of 2048 x 768 28 us:
 // there it is bound by the router's launch (5 us), the first weights (3.5), the way from the
 // last W13 weights to the last hidden rows (4.5) and from the last W2 weights to the sum (4.5).
 //

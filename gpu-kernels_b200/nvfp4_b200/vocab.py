@@ -22,7 +22,7 @@ from ._bind import native
 def embedding(tokens: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
     """scale * table[tokens], rounded once (scale 1 copies the bits).
 
-    tokens int32 or int64 of any shape, table [V, K] bf16 or fp16 (rows may be a slice of wider
+    tokens int32 or int64 of any shape, contiguous; table [V, K] bf16 or fp16 (rows may be a slice of wider
     ones, 16-byte aligned; K a multiple of 8); the result is tokens.shape + [K].  A token
     outside [0, V), such as the -1 of padding, gives zeros."""
     return native.embedding(tokens, table, scale)
@@ -30,7 +30,7 @@ def embedding(tokens: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> 
 
 def embedding_backward(dy: torch.Tensor, tokens: torch.Tensor, rows: int, scale: float = 1.0) -> torch.Tensor:
     """Gradient [rows, K] of the table: scale * the sum of dy over equal tokens, in fp32 and in
-    an order that the tokens alone decide, rounded once; zero for rows that no token names."""
+    an order that the tokens and the sizes decide, rounded once; zero for rows that no token names."""
     return native.embedding_backward(dy, tokens, rows, scale)
 
 
@@ -51,7 +51,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, vocab: Optional[
     vocab: the first so many columns are tokens, the others padding.  top_k <= 32: also the
     most probable tokens, the lowest first among equals.  entropy: also each row's entropy.
     A target outside [0, vocab) is ignored: log probability 0.  A logit of -inf or NaN masks
-    its token (probability 0, no alternative); a row with nothing left has log probability
+    its token (probability 0, no alternative), finite ones of any size are ordinary; a row with nothing left has log probability
     -inf and entropy 0; a logit of +inf makes its row's results NaN."""
     return TokenLogprobs._make(native.token_logprobs(logits, targets, vocab, top_k, temperature, entropy))
 
@@ -63,7 +63,9 @@ def token_logprobs_backward(dlogprobs: torch.Tensor, logits: torch.Tensor, targe
     """Gradient of the logits [T, W] from those of the log probabilities (fp32 [T]; no effect
     where the target is ignored) and, with dentropy, of the entropies: result is
     token_logprobs(..., the same vocab and temperature), with entropy=True for dentropy.
-    Masked tokens and padding columns get zero; the alternatives carry no gradient.
+    Masked tokens and padding columns get zero; the alternatives carry no gradient.  Rows whose
+    log sum exp is past 256 in size (64 for fp32 logits) are summed again, for which lse alone
+    says too little.
     out: where it goes; it may be the logits themselves."""
     return native.token_logprobs_backward(dlogprobs, dentropy, logits, targets, result[4], result[1], vocab,
                                           temperature, out)

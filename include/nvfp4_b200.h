@@ -448,9 +448,9 @@ NVFP4_API int nvfp4_embedding(const void *tokens, int token_bytes, const void *t
                               int T, int V, int K, int dtype, void *stream);
 /*
  * Gradient of the table: dTable[v] = scale * the sum of dY[t] (rows ldy apart) over the
- * tokens t equal to v, in fp32 and an order that the tokens alone decide, rounded once; rows
- * that no token names are zero.  Every row of dTable [V, K] is written; K <= 2^30.  Few tokens need no
- * workspace (0 bytes, which may be NULL); it needs no initial value.
+ * tokens t equal to v, in fp32 an order that the tokens and the sizes decide, rounded once; rows
+ * that no token names are zero.  Every row of dTable [V, K] is written.  K <= 2^30.  Few tokens
+ * need no workspace (0 bytes, which may be NULL); it needs no initial value.
  */
 NVFP4_API size_t nvfp4_embedding_backward_workspace_size(int T, int V, int K);
 NVFP4_API int nvfp4_embedding_backward(const void *dY, int64_t ldy, const void *tokens, int token_bytes, float scale,
